@@ -32,6 +32,7 @@ EXPORTS = (
     "cute_b200_ipc_export", "cute_b200_ipc_open", "cute_b200_ipc_close", "cute_b200_copy_async", "cute_b200_gemm_tn_multi",
     "cute_b200_gemm_layout_info", "cute_b200_gemm_plan", "cute_b200_comm_create", "cute_b200_comm_destroy", "cute_b200_comm_info",
     "cute_b200_gemm_tn_sharded", "cute_b200_gemm_tn_sharded_host", "cute_b200_gemm_tn_multi_signal", "cute_b200_wait_signal",
+    "cute_b200_lora_workspace", "cute_b200_lora_tn", "cute_b200_lora_tn_backward", "cute_b200_moe_workspace", "cute_b200_moe_tn",
 )
 
 REPLICATE_NONE, REPLICATE_AUTO, REPLICATE_FUSED, REPLICATE_COLLECTIVE, REPLICATE_COPIES = range(5)
@@ -52,6 +53,16 @@ class GemmLayout(ctypes.Structure):
         "epilogue_warps", "full_arrivals", "empty_arrivals", "tmem_full_arrivals", "tmem_empty_arrivals",
         "full_expect_tx_bytes_per_k_block", "push_chunk_bytes", "push_chunk_rows", "push_chunks_per_tile", "shared_memory_bytes",
         "descriptor_k_step")] + [("smem_descriptor", ctypes.c_uint64)]
+
+
+class LoraDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("m", "n", "k", "rank", "adapters", "ab_dtype", "c_dtype", "ldx", "ldy")] + [
+        ("tuning", ctypes.c_int32 * 2)]
+
+
+class MoeDesc(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("tokens", "experts", "top", "d", "f", "dtype", "renormalise")] + [
+        ("tuning", ctypes.c_int32 * 2)]
 
 
 class Arg(ctypes.Structure):
@@ -121,6 +132,11 @@ def load() -> ctypes.CDLL:
                                             ctypes.POINTER(u64), i32]
     L.cute_b200_gemm_tn_sharded_host.argtypes = [vp, ctypes.POINTER(GemmDesc), vp, vp, vp, ctypes.POINTER(ctypes.c_double)]
     L.cute_b200_gemm_plan.argtypes = [ctypes.POINTER(GemmDesc), i32, ctypes.POINTER(i32 * 4)]
+    L.cute_b200_lora_workspace.argtypes = [ctypes.POINTER(LoraDesc), ctypes.POINTER(u64), ctypes.POINTER(u64)]
+    L.cute_b200_lora_tn.argtypes = [ctypes.POINTER(LoraDesc)] + [u64] * 8 + [vp]
+    L.cute_b200_lora_tn_backward.argtypes = [ctypes.POINTER(LoraDesc)] + [u64] * 12 + [vp]
+    L.cute_b200_moe_workspace.argtypes = [ctypes.POINTER(MoeDesc), ctypes.POINTER(u64)]
+    L.cute_b200_moe_tn.argtypes = [ctypes.POINTER(MoeDesc)] + [u64] * 7 + [vp]
     L.cute_b200_launch_count.argtypes = []
     L.cute_b200_launch_count.restype = u64
     for name in EXPORTS:
@@ -202,6 +218,52 @@ def shard_rows(m: int, world: int, rank: int) -> tuple[int, int]:
     b, r = ctypes.c_int32(), ctypes.c_int32()
     check(load().cute_b200_shard_rows(m, world, rank, ctypes.byref(b), ctypes.byref(r)))
     return b.value, r.value
+
+
+def lora_desc(m, n, k, rank, adapters, ab_dtype, c_dtype, ldx=0, ldy=0) -> LoraDesc:
+    return LoraDesc(m, n, k, rank, adapters, ab_dtype, c_dtype, ldx, ldy, (ctypes.c_int32 * 2)(0, 0))
+
+
+def lora_workspace(desc: LoraDesc) -> int:
+    """Bytes of lora_tn's workspace."""
+    fwd, bwd = ctypes.c_uint64(), ctypes.c_uint64()
+    check(load().cute_b200_lora_workspace(ctypes.byref(desc), ctypes.byref(fwd), ctypes.byref(bwd)))
+    return fwd.value
+
+
+def lora_backward_workspace(desc: LoraDesc) -> int:
+    """Bytes of lora_tn_backward's workspace."""
+    fwd, bwd = ctypes.c_uint64(), ctypes.c_uint64()
+    check(load().cute_b200_lora_workspace(ctypes.byref(desc), ctypes.byref(fwd), ctypes.byref(bwd)))
+    return bwd.value
+
+
+def lora_tn(desc: LoraDesc, dX: int, dW: int, dA: int, dB: int, dIds: int, dScale: int, dY: int, dWorkspace: int,
+            stream: int = 0) -> None:
+    """y[i] = W x[i] + scale[a] B[a] (A[a] x[i]), a = ids[i]."""
+    check(load().cute_b200_lora_tn(ctypes.byref(desc), dX, dW, dA, dB, dIds, dScale, dY, dWorkspace, stream))
+
+
+def lora_tn_backward(desc: LoraDesc, dX: int, dWt: int, dA: int, dB: int, dIds: int, dScale: int, dGradY: int, dForward: int,
+                     dGradX: int, dGradA: int, dGradB: int, dWorkspace: int, stream: int = 0) -> None:
+    """Gradients of lora_tn for the input and the adapters; dForward is the forward call's workspace, dWt W transposed."""
+    check(load().cute_b200_lora_tn_backward(ctypes.byref(desc), dX, dWt, dA, dB, dIds, dScale, dGradY, dForward, dGradX, dGradA,
+                                            dGradB, dWorkspace, stream))
+
+
+def moe_desc(tokens, experts, top, d, f, dtype, renormalise=True) -> MoeDesc:
+    return MoeDesc(tokens, experts, top, d, f, dtype, int(renormalise), (ctypes.c_int32 * 2)(0, 0))
+
+
+def moe_workspace(desc: MoeDesc) -> int:
+    out = ctypes.c_uint64()
+    check(load().cute_b200_moe_workspace(ctypes.byref(desc), ctypes.byref(out)))
+    return out.value
+
+
+def moe_tn(desc: MoeDesc, dX: int, dRouter: int, dGate: int, dUp: int, dDown: int, dY: int, dWorkspace: int, stream: int = 0) -> None:
+    """A mixture-of-experts layer: router, softmax, top-k, gated experts, weighted sum."""
+    check(load().cute_b200_moe_tn(ctypes.byref(desc), dX, dRouter, dGate, dUp, dDown, dY, dWorkspace, stream))
 
 
 def sgemm_nt(m, n, k, alpha, beta, dA: int, dB: int, dC: int, stream: int = 0) -> None:

@@ -67,6 +67,8 @@ static cute_b200_status init_device(int ordinal) {
     CB_CUDA(cudaMemset(d.status_word, 0, 64));
     CB_TRY(gemm_tn_init(d));
     CB_TRY(sgemm_nt_init(d));
+    CB_TRY(lora_init(d));
+    CB_TRY(moe_init(d));
     d.ready = true;
     return CUTE_B200_OK;
 }
@@ -595,6 +597,49 @@ cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint6
     uint32_t *shared = nullptr;
     if (cudaGetDevice(&device) == cudaSuccess) shared = status_word_if_ready(device);
     return gemm_tn_static(*desc, dA, dB, dC, static_cast<cudaStream_t>(stream), shared);
+}
+
+// The arguments are checked before the device is looked for, so that a refusal reads the same without one.
+cute_b200_status cute_b200_lora_workspace(const cute_b200_lora_desc *desc, uint64_t *forward, uint64_t *backward) {
+    if (!desc || !forward || !backward) return fail(CUTE_B200_ERR_NULL_POINTER, "lora_workspace: null argument");
+    return lora_workspace(*desc, forward, backward);
+}
+
+cute_b200_status cute_b200_lora_tn(const cute_b200_lora_desc *desc, uint64_t dX, uint64_t dW, uint64_t dA, uint64_t dB,
+                                   uint64_t dIds, uint64_t dScale, uint64_t dY, uint64_t dWorkspace, void *stream) {
+    if (!desc) return fail(CUTE_B200_ERR_NULL_POINTER, "lora_tn: desc is null");
+    const uint64_t ptr[8] = {dX, dW, dA, dB, dIds, dScale, dY, dWorkspace};
+    CB_TRY(lora_tn_check(*desc, ptr));
+    DeviceState *dev;
+    CB_TRY(current_device(&dev));
+    return lora_tn(*desc, ptr, static_cast<cudaStream_t>(stream), *dev);
+}
+
+cute_b200_status cute_b200_lora_tn_backward(const cute_b200_lora_desc *desc, uint64_t dX, uint64_t dWt, uint64_t dA,
+                                            uint64_t dB, uint64_t dIds, uint64_t dScale, uint64_t dGradY, uint64_t dForward,
+                                            uint64_t dGradX, uint64_t dGradA, uint64_t dGradB, uint64_t dWorkspace,
+                                            void *stream) {
+    if (!desc) return fail(CUTE_B200_ERR_NULL_POINTER, "lora_tn_backward: desc is null");
+    const uint64_t ptr[12] = {dX, dWt, dA, dB, dIds, dScale, dGradY, dForward, dGradX, dGradA, dGradB, dWorkspace};
+    CB_TRY(lora_tn_backward_check(*desc, ptr));
+    DeviceState *dev;
+    CB_TRY(current_device(&dev));
+    return lora_tn_backward(*desc, ptr, static_cast<cudaStream_t>(stream), *dev);
+}
+
+cute_b200_status cute_b200_moe_workspace(const cute_b200_moe_desc *desc, uint64_t *bytes) {
+    if (!desc || !bytes) return fail(CUTE_B200_ERR_NULL_POINTER, "moe_workspace: null argument");
+    return moe_workspace(*desc, bytes);
+}
+
+cute_b200_status cute_b200_moe_tn(const cute_b200_moe_desc *desc, uint64_t dX, uint64_t dRouter, uint64_t dGate, uint64_t dUp,
+                                  uint64_t dDown, uint64_t dY, uint64_t dWorkspace, void *stream) {
+    if (!desc) return fail(CUTE_B200_ERR_NULL_POINTER, "moe_tn: desc is null");
+    const uint64_t ptr[7] = {dX, dRouter, dGate, dUp, dDown, dY, dWorkspace};
+    CB_TRY(moe_tn_check(*desc, ptr));
+    DeviceState *dev;
+    CB_TRY(current_device(&dev));
+    return moe_tn(*desc, ptr, static_cast<cudaStream_t>(stream), *dev);
 }
 
 cute_b200_status cute_b200_sgemm_nt(int32_t m, int32_t n, int32_t k, float alpha, float beta, uint64_t dA, uint64_t dB,

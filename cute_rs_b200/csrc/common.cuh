@@ -71,6 +71,17 @@ uint32_t *gemm_tn_static_status_words(int device);
 cute_b200_status sgemm_nt_init(const DeviceState &dev);
 // Waits for the current device and turns a kernel's bounded-wait report into CUTE_B200_ERR_DEVICE_TIMEOUT.
 cute_b200_status sync_and_check();
+// Products whose weights are chosen row by row (lora_sm100.cu, moe_sm100.cu).
+cute_b200_status lora_workspace(const cute_b200_lora_desc &desc, uint64_t *forward, uint64_t *backward);
+cute_b200_status lora_tn_check(const cute_b200_lora_desc &desc, const uint64_t ptr[8]);
+cute_b200_status lora_tn(const cute_b200_lora_desc &desc, const uint64_t ptr[8], cudaStream_t stream, const DeviceState &dev);
+cute_b200_status lora_tn_backward_check(const cute_b200_lora_desc &desc, const uint64_t ptr[12]);
+cute_b200_status lora_tn_backward(const cute_b200_lora_desc &desc, const uint64_t ptr[12], cudaStream_t stream, const DeviceState &dev);
+cute_b200_status lora_init(const DeviceState &dev);
+cute_b200_status moe_workspace(const cute_b200_moe_desc &desc, uint64_t *bytes);
+cute_b200_status moe_tn_check(const cute_b200_moe_desc &desc, const uint64_t ptr[7]);
+cute_b200_status moe_tn(const cute_b200_moe_desc &desc, const uint64_t ptr[7], cudaStream_t stream, const DeviceState &dev);
+cute_b200_status moe_init(const DeviceState &dev);
 // The launcher for several GPUs (multi_gpu.cu).
 cute_b200_status comm_create(int ngpus, const int *ordinals, void **comm_out);
 cute_b200_status comm_destroy(void *comm);

@@ -165,6 +165,93 @@ cute_b200_status cute_b200_release_workspace(void);
 cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint64_t dA, uint64_t dB, uint64_t dC,
                                           void *stream);
 
+/* ---- products whose weights are chosen row by row ----------------------------
+ * Two operators of language models beside the GEMM: a projection shared by all
+ * rows with a low-rank adapter chosen row by row (forward and backward), and a
+ * mixture-of-experts layer for a few tokens.  No counterpart in the reference,
+ * whose examples end at one product of two matrices.
+ *
+ * Conventions beyond those at the top of this file: 16-bit operands are f16 or
+ * bf16, all of one type, K-major and 16-byte aligned, like the GEMM's; sums are
+ * held in f32.  Workspaces belong to the caller (256-byte aligned, sizes from
+ * the *_workspace calls, contents undefined before the call): nothing is
+ * allocated, nothing is kept between calls, and calls with workspaces of their
+ * own may run at the same time on different streams.  Every call may be
+ * captured into a CUDA graph, provided the device was set up before
+ * (cute_b200_init or any earlier call).  The tables that choose the weights
+ * (ids, the router's choice) are read on the device: a replayed graph follows
+ * their current contents.
+ *
+ * cute_b200_lora_tn:  with a = ids[i],
+ *     y[i] = W x[i] + scale[a] * B[a] (A[a] x[i])      0 <= a < adapters
+ *     y[i] = W x[i]                                    any other a: no adapter
+ *   X: (m, k), rows ldx apart; W: (n, k); A: (adapters, rank, k);
+ *   B: (adapters, n, rank); ids: (m) i32; scale: (adapters) f32;
+ *   Y: (m, n) f32, f16 or bf16, rows ldy apart.
+ *   Rows may come in any order: packed sequences, single tokens of many
+ *   requests, both mixed.  A row's result depends on its own X row and its own
+ *   adapter alone, whatever infinities or NaNs other rows or adapters hold.
+ *   m >= 0; n >= 1; k >= 8 and a multiple of 8; rank a multiple of 8 in 8..128
+ *   (an adapter of a smaller rank is padded with zeros); adapters >= 1 with
+ *   adapters * n, adapters * k and adapters * rank below 2^31.
+ *   A[a] x is rounded to the sum of two 16-bit numbers (16 significant bits for
+ *   bf16, 22 for f16 where it lies inside f16's range; past +-65504 an f16
+ *   product is infinite) before it is multiplied by B.
+ *   The workspace begins with these numbers, which the backward pass reads.
+ *
+ * cute_b200_lora_tn_backward: the gradients for dY (m, n) in the operands' type
+ *   with the pitch of Y (which then has to be a multiple of 8, as n has), the
+ *   shared weight frozen:
+ *     dX[i] = W^T dY[i] + scale[a] * A[a]^T (B[a]^T dY[i])          (m, k) in c_dtype, pitch of X
+ *     dA[a] = scale[a] * sum over rows i with ids[i] == a of (B[a]^T dY[i]) x[i]^T     f32, overwritten
+ *     dB[a] = scale[a] * sum over rows i with ids[i] == a of dY[i] (A[a] x[i])^T       f32, overwritten
+ *   dWt is W transposed, (k, n) row-major, which a program whose weight is
+ *   frozen lays out once.  dForward is the workspace of the forward call on the
+ *   same X, A, ids and scale, unchanged since.  dX may be null (no gradient of
+ *   the input wanted), dA and dB may both be null; adapters no row names get
+ *   zeros.  The sums run in a fixed order: the same call gives the same bits.
+ *
+ * No buffer that a call writes may overlap another of its buffers. */
+typedef struct {
+    int32_t m, n, k;
+    int32_t rank, adapters;
+    int32_t ab_dtype;  /* CUTE_B200_F16 or CUTE_B200_BF16: X, W, A, B, dY */
+    int32_t c_dtype;   /* CUTE_B200_F32, CUTE_B200_F16 or CUTE_B200_BF16: Y, dX */
+    int32_t ldx, ldy;  /* elements between rows of X (a multiple of 8) and of Y; 0 = dense (k, n) */
+    int32_t tuning[2]; /* zero.  Measurement and test knobs: [0] 1 = the kernels for few rows (m <= 128), 2 = the tiled kernels;
+                          [1] bits 2 + 3 make every in-kernel wait run out after 20 ms, as in cute_b200_gemm_desc */
+} cute_b200_lora_desc;
+
+/* Bytes of the forward and of the backward call's workspace. */
+cute_b200_status cute_b200_lora_workspace(const cute_b200_lora_desc *desc, uint64_t *forward, uint64_t *backward);
+cute_b200_status cute_b200_lora_tn(const cute_b200_lora_desc *desc, uint64_t dX, uint64_t dW, uint64_t dA, uint64_t dB,
+                                   uint64_t dIds, uint64_t dScale, uint64_t dY, uint64_t dWorkspace, void *stream);
+cute_b200_status cute_b200_lora_tn_backward(const cute_b200_lora_desc *desc, uint64_t dX, uint64_t dWt, uint64_t dA,
+                                            uint64_t dB, uint64_t dIds, uint64_t dScale, uint64_t dGradY, uint64_t dForward,
+                                            uint64_t dGradX, uint64_t dGradA, uint64_t dGradB, uint64_t dWorkspace,
+                                            void *stream);
+
+/* cute_b200_moe_tn: a mixture-of-experts layer for up to 64 tokens,
+ *     p = softmax(R x[t]);  the `top` largest p are chosen, equal ones by the lower index
+ *     w_e = p_e, divided by the sum of the chosen p where `renormalise` is not 0
+ *     y[t] = sum over chosen e of w_e D[e] (silu(G[e] x[t]) * (U[e] x[t])),   silu(v) = v / (1 + exp(-v))
+ *   X, Y: (tokens, d); R: (experts, d); G, U: (experts, f, d); D: (experts, d, f); all in one 16-bit type.
+ *   0 <= tokens <= 64; 1 <= top <= 16, top <= experts <= 512; d and f multiples of 8, experts * f and experts * d
+ *   below 2^31.  The router's product, the softmax and the choice are f32; w_e * silu * up is rounded to the operands'
+ *   type once, before the last product.  A token whose logits are not all finite gets a valid but unspecified choice
+ *   and NaNs; other tokens are not affected. */
+typedef struct {
+    int32_t tokens, experts, top;
+    int32_t d, f;
+    int32_t dtype;       /* CUTE_B200_F16 or CUTE_B200_BF16 */
+    int32_t renormalise;
+    int32_t tuning[2];   /* zero; [1] as in cute_b200_lora_desc */
+} cute_b200_moe_desc;
+
+cute_b200_status cute_b200_moe_workspace(const cute_b200_moe_desc *desc, uint64_t *bytes);
+cute_b200_status cute_b200_moe_tn(const cute_b200_moe_desc *desc, uint64_t dX, uint64_t dRouter, uint64_t dGate, uint64_t dUp,
+                                  uint64_t dDown, uint64_t dY, uint64_t dWorkspace, void *stream);
+
 /* ---- SIMT sgemm ------------------------------------------------------------
  * C = alpha * (A * B^T) + beta * C, all f32 and column-major: a[i + l*m],
  * b[j + l*n], c[i + j*m].  fma.rn.f32 accumulation with l ascending and a
