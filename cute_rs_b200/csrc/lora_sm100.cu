@@ -4,89 +4,10 @@
 // values per row) goes to the workspace as two 16-bit numbers per value, their
 // sum: the second product can then run on 16-bit operands and still carry 16
 // (bf16) or 22 (f16) bits of T.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "common.cuh"
-#include "ptx_sm100.cuh"
+#include "lora_sm100.cuh"
 
 namespace cb {
 namespace {
-
-template <bool BF16>
-__device__ __forceinline__ float to_f32(uint16_t v) {
-    if constexpr (BF16) return __uint_as_float(uint32_t(v) << 16);
-    else return __half2float(__ushort_as_half(v));
-}
-template <bool BF16>
-__device__ __forceinline__ uint16_t from_f32(float v) {
-    if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
-    else return __half_as_ushort(__float2half_rn(v));
-}
-__device__ __forceinline__ void store_c(void *c, int dtype, size_t i, float v) {
-    if (dtype == CUTE_B200_F32) static_cast<float *>(c)[i] = v;
-    else if (dtype == CUTE_B200_BF16) static_cast<__nv_bfloat16 *>(c)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half *>(c)[i] = __float2half_rn(v);
-}
-
-// Width of the rank in T: 16, 32, 64 or 128.
-__host__ __device__ constexpr int padded_rank(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
-
-struct LoraParams {
-    const uint16_t *x, *w, *a, *b;
-    const int32_t *ids;
-    const float *scale;
-    void *y;
-    uint16_t *t;
-    int m, n, k, rank, rp, adapters, c_dtype;
-    int64_t ldx, ldy;
-};
-
-template <bool BF16>
-__global__ void shrink_simple(const LoraParams p) {
-    const int row = blockIdx.x, lane = threadIdx.x & 31;
-    const int id = p.ids[row];
-    const bool has = id >= 0 && id < p.adapters;
-    for (int j = threadIdx.x >> 5; j < p.rp; j += blockDim.x >> 5) {
-        float acc = 0.0f;
-        if (has && j < p.rank) {
-            const uint16_t *a = p.a + (int64_t(id) * p.rank + j) * p.k;
-            for (int l = lane; l < p.k; l += 32) acc = fmaf(to_f32<BF16>(a[l]), to_f32<BF16>(p.x[row * p.ldx + l]), acc);
-            for (int s = 16; s > 0; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
-            acc *= p.scale[id];
-        }
-        if (lane == 0) {
-            const uint16_t hi = from_f32<BF16>(acc);
-            const float rest = acc - to_f32<BF16>(hi);
-            p.t[int64_t(row) * 2 * p.rp + j] = hi;
-            p.t[int64_t(row) * 2 * p.rp + p.rp + j] = from_f32<BF16>(rest);
-        }
-    }
-}
-
-template <bool BF16>
-__global__ void product_simple(const LoraParams p) {
-    __shared__ float xs[16][17], ws[16][17];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t row = int64_t(blockIdx.y) * 16 + ty;
-    const int64_t col = int64_t(blockIdx.x) * 16 + tx, wrow = int64_t(blockIdx.x) * 16 + ty;
-    float acc = 0.0f;
-    for (int l = 0; l < p.k; l += 16) {
-        xs[ty][tx] = row < p.m && l + tx < p.k ? to_f32<BF16>(p.x[row * p.ldx + l + tx]) : 0.0f;
-        ws[ty][tx] = wrow < p.n && l + tx < p.k ? to_f32<BF16>(p.w[wrow * p.k + l + tx]) : 0.0f;
-        __syncthreads();
-        for (int i = 0; i < 16; i++) acc = fmaf(xs[ty][i], ws[tx][i], acc);
-        __syncthreads();
-    }
-    if (row >= p.m || col >= p.n) return;
-    const int id = p.ids[row];
-    if (id >= 0 && id < p.adapters)
-        for (int j = 0; j < p.rank; j++) {
-            const float t = to_f32<BF16>(p.t[row * 2 * p.rp + j]) + to_f32<BF16>(p.t[row * 2 * p.rp + p.rp + j]);
-            acc = fmaf(t, to_f32<BF16>(p.b[(int64_t(id) * p.n + col) * p.rank + j]), acc);
-        }
-    store_c(p.y, p.c_dtype, row * p.ldy + col, acc);
-}
 
 // (rows, cols) -> (cols, rows) of each of `count` 16-bit matrices.
 __global__ void transpose_simple(const uint16_t *in, uint16_t *out, int rows, int cols) {
@@ -110,13 +31,392 @@ __global__ void grad_simple(const uint16_t *t, const uint16_t *v, int64_t ldv, c
     out[int64_t(a) * rank * cols + j * sj + c * sc] = acc;
 }
 
+// ---- few rows (m <= 128) ------------------------------------------------------
+// T: a CTA takes one row and four of its adapter's `rank` rows; its 256 threads
+// walk k in 16-byte pieces.  It is over before the weights have streamed past
+// (below), so it is kept simple.
+constexpr int SHRINK_THREADS = 256, SHRINK_J = 4;
+
+template <bool BF16>
+__global__ void __launch_bounds__(SHRINK_THREADS) shrink_rows_kernel(const LoraParams p) {
+    __shared__ float part[SHRINK_THREADS / 32][SHRINK_J];
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const int row = blockIdx.x, j0 = blockIdx.y * SHRINK_J, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int id = p.ids[row];
+    const bool has = id >= 0 && id < p.adapters && j0 < p.rank;
+    float acc[SHRINK_J] = {};
+    if (has) {
+        const uint16_t *x = p.x + row * p.ldx;
+        const uint16_t *a = p.a + (int64_t(id) * p.rank + j0) * p.k;
+        const int vecs = p.k / 8;
+#pragma unroll 2
+        for (int c = threadIdx.x; c < vecs; c += SHRINK_THREADS) {
+            const uint4 xv = *reinterpret_cast<const uint4 *>(x + 8 * c);
+            uint4 av[SHRINK_J];
+#pragma unroll
+            for (int j = 0; j < SHRINK_J; j++) av[j] = __ldg(reinterpret_cast<const uint4 *>(a + int64_t(j) * p.k + 8 * c));
+            const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 xf = pair_f32<BF16>(xw[i]);
+#pragma unroll
+                for (int j = 0; j < SHRINK_J; j++) {
+                    const uint32_t w = i == 0 ? av[j].x : (i == 1 ? av[j].y : (i == 2 ? av[j].z : av[j].w));
+                    const float2 af = pair_f32<BF16>(w);
+                    acc[j] = fmaf(af.y, xf.y, fmaf(af.x, xf.x, acc[j]));
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < SHRINK_J; j++) {
+        acc[j] = warp_sum(acc[j]);
+        if (lane == 0) part[warp][j] = acc[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < SHRINK_J) {
+        float sum = 0.0f;
+        for (int w = 0; w < SHRINK_THREADS / 32; w++) sum += part[w][threadIdx.x];
+        if (has) sum *= p.scale[id];
+        const uint16_t hi = from_f32<BF16>(sum);
+        uint16_t *t = p.t + int64_t(row) * 2 * p.rp + j0 + threadIdx.x;
+        t[0] = hi;
+        t[p.rp] = from_f32<BF16>(sum - to_f32<BF16>(hi));
+    }
+}
+
+// Y: the weight streams past the rows.  The (up to 128) rows of X are the M = 128
+// lanes of one accumulator, `bn` rows of W its columns; a cluster of `kc` CTAs
+// shares a tile's k blocks and, after them, the adapters its rows name, and adds
+// its partial sums through shared memory.  Bound by HBM: every byte of W is
+// read once, the ring keeps ~190 KB of it in flight per SM.
+//   warp 0  TMA: per stage a (xr x 64) block of X and a (bn x 64) block of W;
+//           then, per adapter, blocks of T and of B[a].
+//   warp 1  MMA: M 128, N bn.  The MMA always reads 128 rows of X; those past
+//           the loaded xr rows are whatever lies behind them in the ring (in
+//           bounds, see few_smem), and end up in lanes that nothing reads.  An
+//           adapter's product is masked to the lanes of the rows that name it,
+//           so that nothing of it reaches another row.
+//   warps 2-5  which adapters the rows name, while the weights stream; then
+//           the accumulator's rows to shared memory, the sum over the cluster
+//           and the stores.
+// W and X do not depend on the kernel that computes T, which has waited for all
+// before it: they are loaded before griddepcontrol.wait, T and the ids after.
+constexpr int FEW_THREADS = 192, FEW_MAX_STAGES = 16, FEW_ROWS = 128;
+constexpr uint32_t FEW_HEAD = 4096;  // barriers, masks and ids, ahead of the ring
+
+struct FewParams {
+    const int32_t *ids;
+    void *y;
+    int64_t ldy;
+    int m, n, rank, rp, adapters, c_dtype, vec;
+    int k_blocks, bn, kc, xr, stages;
+    uint32_t stage_bytes, w_offset, idesc, tmem_cols;
+    uint32_t *status;
+    int debug;
+};
+
+struct FewHead {
+    uint64_t full[FEW_MAX_STAGES], empty[FEW_MAX_STAGES], plan, done, drain;
+    uint32_t tmem, abort;
+    int32_t entries, entry_id[FEW_ROWS];
+    uint32_t off[FEW_ROWS][4];  // lanes of entry e that keep their sums: bit set = not a row of this adapter
+    int32_t id[FEW_ROWS], before[4];
+};
+static_assert(sizeof(FewHead) <= FEW_HEAD, "head");
+
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+    lora_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT,
+                    const __grid_constant__ CUtensorMap tmB, const FewParams p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    FewHead &h = *reinterpret_cast<FewHead *>(smem_raw + (base - raw));
+    const uint32_t ring = base + FEW_HEAD;
+    auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
+    volatile uint32_t *abort_flag = &h.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = p.kc > 1 ? ptx::cluster_ctarank() : 0u;
+    const int n0 = int(blockIdx.x) / p.kc * p.bn;
+    const int kb0 = int(int64_t(p.k_blocks) * rank / p.kc), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / p.kc);
+    const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            ptx::mbar_init(bar(h.full[s]), 1);
+            ptx::mbar_init(bar(h.empty[s]), 1);
+        }
+        ptx::mbar_init(bar(h.plan), 1);
+        ptx::mbar_init(bar(h.done), 1);
+        ptx::mbar_init(bar(h.drain), 1);
+        h.abort = 0u;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), p.tmem_cols);
+        ptx::tmem_relinquish<1>();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&h.tmem);
+    const int q_blocks = ext_blocks(p.rp);
+    if (threadIdx.x == 0) ptx::griddep_launch_dependents();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            ptx::prefetch_tensormap(&tmX);
+            ptx::prefetch_tensormap(&tmW);
+            ptx::prefetch_tensormap(&tmT);
+            ptx::prefetch_tensormap(&tmB);
+            int s = 0;
+            uint32_t ph = 0, filled = 0, filled_parity = 0;
+            const uint32_t bytes = uint32_t(p.xr + p.bn) * 128u;
+            bool ok = !(p.debug & 4);
+            auto load = [&](const CUtensorMap *rows, int rx, const CUtensorMap *weights, int wx, int wy) {
+                if (!wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit)) return false;
+                const uint32_t dst = ring + uint32_t(s) * p.stage_bytes;
+                ptx::mbar_arrive_expect_tx(bar(h.full[s]), bytes);
+                ptx::tma_load_2d(dst + p.w_offset, weights, bar(h.full[s]), wx, wy);
+                ptx::tma_load_2d(dst, rows, bar(h.full[s]), rx, 0);
+                filled |= 1u << s;
+                filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
+                if (++s == p.stages) s = 0, ph ^= 1u;
+                return true;
+            };
+            for (int kb = kb0; kb < kb1 && ok; kb++) ok = load(&tmX, kb * 64, &tmW, kb * 64, n0);
+            if (ok) {
+                ptx::griddep_wait();
+                ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit);
+            }
+            for (int e = int(rank); ok && e < h.entries; e += p.kc)
+                for (int q = 0; q < q_blocks && ok; q++) {
+                    const ExtBlock b = ext_block(q, p.rp, p.rank);
+                    if (b.steps > 0) ok = load(&tmT, b.t_col, &tmB, b.b_col, h.entry_id[e] * p.n + n0);
+                }
+            if (!ok)  // giving up: let the copies in flight land (bounded) before the shared memory is handed back
+                for (int i = 0; i < p.stages; i++)
+                    if (filled & (1u << i)) {
+                        const uint64_t t0 = ptx::globaltimer_ns();
+                        while (!ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
+                            if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+                    }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true, issued = false;
+            auto ready = [&] {
+                if (!wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit)) return false;
+                ptx::tc_fence_after();
+                return true;
+            };
+            auto free_stage = [&] {
+                issued = true;
+                ptx::umma_commit<1>(bar(h.empty[s]));
+                if (++s == p.stages) s = 0, ph ^= 1u;
+            };
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!(ok = ready())) break;
+                const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+                const uint64_t a = sw128_desc(src), b = sw128_desc(src + p.w_offset);
+#pragma unroll
+                for (int j = 0; j < 4; j++) ptx::umma_f16<1>(tmem, a + 2u * j, b + 2u * j, p.idesc, (kb > kb0 || j > 0) ? 1u : 0u);
+                free_stage();
+            }
+            if (ok) ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit);
+            for (int e = int(rank); ok && e < h.entries; e += p.kc) {
+                const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
+                for (int q = 0; q < q_blocks; q++) {
+                    const ExtBlock x = ext_block(q, p.rp, p.rank);
+                    if (x.steps <= 0) continue;
+                    if (!(ok = ready())) break;
+                    const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+                    const uint64_t a = sw128_desc(src), b = sw128_desc(src + p.w_offset);
+                    for (int j = 0; j < x.steps; j++)
+                        ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * (j & x.b_mask), p.idesc, 1u, o0, o1, o2, o3);
+                    free_stage();
+                }
+            }
+            if (ok) {
+                ptx::umma_commit<1>(bar(h.done));
+            } else if (issued) {  // giving up: wait (bounded) until the tensor core is done with shared memory and TMEM
+                ptx::umma_commit<1>(bar(h.drain));
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while (!ptx::mbar_try_wait(bar(h.drain), 0u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        // The adapters the rows name, in the order of their first row.
+        const int row = threadIdx.x - 64, w = warp - 2;
+        ptx::griddep_wait();
+        int id = row < p.m ? p.ids[row] : -1;
+        if (id < 0 || id >= p.adapters) id = -1;
+        h.id[row] = id;
+        ptx::named_barrier(1, 128);
+        const uint32_t same = __match_any_sync(0xffffffffu, id);  // every lane takes part, those without an adapter too
+        bool first = id >= 0 && __ffs(same) - 1 == lane;
+        if (first)
+            for (int i = 0; i < 32 * w; i++)
+                if (h.id[i] == id) {
+                    first = false;
+                    break;
+                }
+        __syncwarp();
+        const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+        if (lane == 0) h.before[w] = __popc(firsts);
+        ptx::named_barrier(1, 128);
+        int at = __popc(firsts & ((1u << lane) - 1u)), total = 0;
+        for (int i = 0; i < 4; i++) {
+            if (i < w) at += h.before[i];
+            total += h.before[i];
+        }
+        if (first) h.entry_id[at] = id;
+        if (threadIdx.x == 64) h.entries = total;
+        ptx::named_barrier(1, 128);
+        for (int e = 0; e < total; e++) {
+            const uint32_t mine = __ballot_sync(0xffffffffu, id == h.entry_id[e]);
+            if (lane == 0) h.off[e][w] = ~mine;
+        }
+        ptx::named_barrier(1, 128);
+        if (threadIdx.x == 64) ptx::mbar_arrive(bar(h.plan));
+
+        // The accumulator's rows to shared memory (the ring is idle: every load has been consumed).
+        const bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.done), 0, abort_flag, p.status, WHERE_EPILOGUE, 0u, limit));
+        const int q = warp & 3;  // the TMEM lanes this warp may read: rows 32 q ..
+        const uint32_t pitch = uint32_t(p.bn + 4) * 4u;
+        if (ok && 32 * q < p.m) {
+            ptx::tc_fence_after();
+            ptx::fence_proxy_async_shared();
+            for (int c = 0; c < p.bn; c += 32) {
+                uint32_t v[32];
+                ptx::tmem_ld_32x32(tmem + (uint32_t(32 * q) << 16) + uint32_t(c), v);
+                ptx::tmem_ld_wait(v);
+                if (32 * q + lane < p.m) {
+                    const uint32_t dst = ring + uint32_t(32 * q + lane) * pitch + uint32_t(c) * 4u;
+#pragma unroll
+                    for (int g = 0; g < 8; g++)
+                        if (c + 4 * g < p.bn) ptx::st_shared_v4(dst + 16u * g, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+                }
+            }
+        }
+        __syncwarp();
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (p.kc > 1) {  // every CTA of the cluster has its partial sums in shared memory (or has given up)
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    if (!*abort_flag) {
+        const int quads = p.bn / 4, items = p.m * quads;
+        const uint32_t pitch = uint32_t(p.bn + 4) * 4u;
+        for (int i = int(rank) * FEW_THREADS + int(threadIdx.x); i < items; i += p.kc * FEW_THREADS) {
+            const int row = i / quads, col = (i - row * quads) * 4;
+            const uint32_t at = ring + uint32_t(row) * pitch + uint32_t(col) * 4u;
+            float4 v = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(at, 0) : at);
+            for (int c = 1; c < p.kc; c++) {  // in ascending order of the k ranges
+                const float4 o = ptx::ld_shared_cluster_v4(ptx::mapa(at, uint32_t(c)));
+                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+            }
+            const int64_t gcol = n0 + col, out = int64_t(row) * p.ldy + gcol;
+            if (p.vec && gcol + 4 <= p.n) {
+                if (p.c_dtype == CUTE_B200_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.y) + out) = v;
+                else {
+                    const bool bf16 = p.c_dtype == CUTE_B200_BF16;
+                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + out) = make_uint2(pack_16(v.x, v.y, bf16), pack_16(v.z, v.w, bf16));
+                }
+            } else {
+                const float f[4] = {v.x, v.y, v.z, v.w};
+                for (int j = 0; j < 4; j++)
+                    if (gcol + j < p.n) store_c(p.y, p.c_dtype, size_t(out + j), f[j]);
+            }
+        }
+    }
+    __syncthreads();
+    if (p.kc > 1) {  // until every CTA has read its peers' shared memory
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, p.tmem_cols);
+}
+
+constexpr uint32_t FEW_SMEM = 227 * 1024;
+
+// How the few-row kernel is cut: bn columns of Y per tile, a cluster of kc CTAs per tile.  The launch is one wave
+// where it can be; the cut with the least time for the slowest CTA wins.  A CTA streams at most what an even share of
+// HBM gives it, and no faster than its MMAs take (four per k block, a fixed ~60 clocks or bn / 2 each).
+int g_few_clusters[64][4];  // clusters of 1, 2, 4, 8 CTAs of the few-row kernel that fit each device at once
+
+void few_cut(int n, int k, const int (&max_clusters)[4], int *bn, int *kc) {
+    const int k_blocks = (k + 63) / 64;
+    double best = 1e300;
+    for (int c = 0; c < 4; c++) {
+        const int parts = 1 << c, ctas_at_once = max_clusters[c] * parts;
+        if (parts > k_blocks || max_clusters[c] < 1) continue;
+        for (int b = 16; b <= 256; b += 16) {
+            const int64_t ctas = int64_t((n + b - 1) / b) * parts;
+            const int64_t waves = (ctas + ctas_at_once - 1) / ctas_at_once;
+            const double share = 6.5e12 / double(ctas < ctas_at_once ? ctas : ctas_at_once);
+            const double rate = share < 7.0e10 ? share : 7.0e10;
+            const double load = b * 128.0 / rate, math = 4.0 * (b / 2 > 60 ? b / 2 : 60) / 1.7e9;
+            const double t = double(waves) * (((k_blocks + parts - 1) / parts) * (load > math ? load : math) + 2.0e-6) + (parts > 1 ? 1.0e-6 : 0.0);
+            if (t < best * 0.999) best = t, *bn = b, *kc = parts;
+        }
+    }
+}
+
+template <bool BF16>
+cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int debug, cudaStream_t stream) {
+    CB_TRY(launch_dependent(shrink_rows_kernel<BF16>, dim3(unsigned(p.m), unsigned(p.rp / SHRINK_J)), SHRINK_THREADS, 0, 1, stream, p));
+    if (!p.y) return CUTE_B200_OK;
+    FewParams f = {};
+    f.ids = p.ids, f.y = p.y, f.ldy = p.ldy;
+    f.m = p.m, f.n = p.n, f.rank = p.rank, f.rp = p.rp, f.adapters = p.adapters, f.c_dtype = p.c_dtype;
+    const uint64_t esize = p.c_dtype == CUTE_B200_F32 ? 4 : 2;
+    f.vec = reinterpret_cast<uint64_t>(p.y) % (4 * esize) == 0 && p.ldy % 4 == 0;
+    f.k_blocks = (p.k + 63) / 64;
+    f.bn = 16, f.kc = 1;
+    int device = 0;
+    CB_CUDA(cudaGetDevice(&device));
+    few_cut(p.n, p.k, g_few_clusters[device], &f.bn, &f.kc);
+    f.xr = (p.m + 7) / 8 * 8;
+    f.w_offset = uint32_t(f.xr) * 128u;
+    f.stage_bytes = uint32_t(f.xr + f.bn) * 128u;
+    // The head, the ring, and behind the last stage as much as an MMA reads past its rows of X.
+    const uint32_t ring = FEW_SMEM - FEW_HEAD - 1024;
+    const uint32_t over = f.stage_bytes < 16384 ? 16384 - f.stage_bytes : 0;
+    f.stages = int((ring - over) / f.stage_bytes);
+    if (f.stages > FEW_MAX_STAGES) f.stages = FEW_MAX_STAGES;
+    f.idesc = make_idesc(BF16, 128, f.bn);
+    f.tmem_cols = f.bn <= 32 ? 32 : (f.bn <= 64 ? 64 : (f.bn <= 128 ? 128 : 256));
+    f.status = dev.status_word;
+    f.debug = debug;
+    CUtensorMap tmX, tmW, tmT, tmB;
+    CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), BF16, p.m, p.k, p.ldx, f.xr));
+    CB_TRY(rows_tensor_map(&tmW, reinterpret_cast<uint64_t>(p.w), BF16, p.n, p.k, p.k, f.bn));
+    CB_TRY(rows_tensor_map(&tmT, reinterpret_cast<uint64_t>(p.t), BF16, p.m, 2 * p.rp, 2 * p.rp, f.xr));
+    CB_TRY(rows_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), BF16, uint64_t(p.adapters) * p.n, p.rank, p.rank, f.bn));
+    const unsigned grid = unsigned((p.n + f.bn - 1) / f.bn) * unsigned(f.kc);
+    return launch_dependent(lora_few_kernel, dim3(grid), FEW_THREADS, FEW_SMEM, f.kc, stream, tmX, tmW, tmT, tmB, f);
+}
+
 constexpr uint64_t kAlign = 256;
 uint64_t round_up(uint64_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
 uint64_t t_bytes(const cute_b200_lora_desc &d) { return round_up(uint64_t(d.m) * padded_rank(d.rank) * 4); }
 
+uint64_t plan_bytes(const cute_b200_lora_desc &d) { return round_up(lora_plan_bytes(d.m, d.adapters)) + kAlign; }
+
 cute_b200_status check_desc(const cute_b200_lora_desc &d, const char *who) {
     if (d.m < 0 || d.n < 1 || d.k < 8)
         return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: invalid size %dx%dx%d", who, d.m, d.n, d.k);
+    if (d.m > (1 << 30) || d.n > (1 << 30) || d.k > (1 << 30))
+        return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: m, n and k may be at most 2^30, got %dx%dx%d", who, d.m, d.n, d.k);
     if (d.k % 8) return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: k must be a multiple of 8, got %d", who, d.k);
     if (d.rank < 8 || d.rank > 128 || d.rank % 8)
         return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: rank must be a multiple of 8 in 8..128, got %d", who, d.rank);
@@ -133,8 +433,8 @@ cute_b200_status check_desc(const cute_b200_lora_desc &d, const char *who) {
         return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: ldx must be 0 or a multiple of 8 of at least k = %d, got %d", who, d.k, d.ldx);
     if (d.ldy != 0 && d.ldy < d.n)
         return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: ldy must be 0 or at least n = %d, got %d", who, d.n, d.ldy);
-    if (d.tuning[0] < 0 || d.tuning[0] > 2 || (d.tuning[0] == 1 && d.m > 128))
-        return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: tuning[0] must be 0, 1 (with m <= 128) or 2, got %d", who, d.tuning[0]);
+    if (d.tuning[0] < 0 || d.tuning[0] > 5 || (d.tuning[0] == 1 && d.m > 128))
+        return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: tuning[0] must be 0, 1 (with m <= 128) or 2 to 5, got %d", who, d.tuning[0]);
     return CUTE_B200_OK;
 }
 
@@ -146,23 +446,19 @@ cute_b200_status check_ptr(const char *who, const char *name, uint64_t p, uint64
 
 uint64_t elem_bytes(int dtype) { return dtype == CUTE_B200_F32 ? 4 : 2; }
 
-template <bool BF16>
-cute_b200_status forward(const LoraParams &p, cudaStream_t stream) {
+cute_b200_status forward(const LoraParams &p, bool bf16, const int32_t (&tuning)[2], const DeviceState &dev, cudaStream_t stream) {
     if (p.m == 0) return CUTE_B200_OK;
-    shrink_simple<BF16><<<p.m, 128, 0, stream>>>(p);
-    CB_CUDA(cudaGetLastError());
-    product_simple<BF16><<<dim3(unsigned((p.n + 15) / 16), unsigned((p.m + 15) / 16)), 256, 0, stream>>>(p);
-    CB_CUDA(cudaGetLastError());
-    count_launch(2);
-    return CUTE_B200_OK;
+    if (tuning[0] == 1 || (tuning[0] == 0 && p.m <= FEW_ROWS))
+        return bf16 ? forward_few<true>(p, dev, tuning[1], stream) : forward_few<false>(p, dev, tuning[1], stream);
+    return lora_tiled(p, bf16, tuning[0] - 3, tuning[1], dev, stream);
 }
 
 }  // namespace
 
 cute_b200_status lora_workspace(const cute_b200_lora_desc &d, uint64_t *forward, uint64_t *backward) {
     CB_TRY(check_desc(d, "lora_workspace"));
-    *forward = t_bytes(d) + kAlign;
-    *backward = t_bytes(d) + round_up(uint64_t(d.adapters) * d.rank * d.k * 2) + round_up(uint64_t(d.adapters) * d.rank * d.n * 2) + kAlign;
+    *forward = t_bytes(d) + plan_bytes(d);
+    *backward = t_bytes(d) + plan_bytes(d) + round_up(uint64_t(d.adapters) * d.rank * d.k * 2) + round_up(uint64_t(d.adapters) * d.rank * d.n * 2);
     return CUTE_B200_OK;
 }
 
@@ -182,7 +478,7 @@ cute_b200_status lora_tn_check(const cute_b200_lora_desc &d, const uint64_t ptr[
     return CUTE_B200_OK;
 }
 
-cute_b200_status lora_tn(const cute_b200_lora_desc &d, const uint64_t ptr[8], cudaStream_t stream, const DeviceState &) {
+cute_b200_status lora_tn(const cute_b200_lora_desc &d, const uint64_t ptr[8], cudaStream_t stream, const DeviceState &dev) {
     LoraParams p = {};
     p.x = reinterpret_cast<const uint16_t *>(ptr[0]);
     p.w = reinterpret_cast<const uint16_t *>(ptr[1]);
@@ -192,10 +488,11 @@ cute_b200_status lora_tn(const cute_b200_lora_desc &d, const uint64_t ptr[8], cu
     p.scale = reinterpret_cast<const float *>(ptr[5]);
     p.y = reinterpret_cast<void *>(ptr[6]);
     p.t = reinterpret_cast<uint16_t *>(ptr[7]);
+    p.plan = reinterpret_cast<uint32_t *>(ptr[7] + t_bytes(d));
     p.m = d.m, p.n = d.n, p.k = d.k, p.rank = d.rank, p.rp = padded_rank(d.rank), p.adapters = d.adapters, p.c_dtype = d.c_dtype;
     p.ldx = d.ldx ? d.ldx : d.k;
     p.ldy = d.ldy ? d.ldy : d.n;
-    return d.ab_dtype == CUTE_B200_BF16 ? forward<true>(p, stream) : forward<false>(p, stream);
+    return forward(p, d.ab_dtype == CUTE_B200_BF16, d.tuning, dev, stream);
 }
 
 // ptr: X, W transposed, A, B, ids, scale, dY, forward workspace, dX, dA, dB, workspace
@@ -220,7 +517,7 @@ cute_b200_status lora_tn_backward_check(const cute_b200_lora_desc &d, const uint
     return CUTE_B200_OK;
 }
 
-cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t ptr[12], cudaStream_t stream, const DeviceState &) {
+cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t ptr[12], cudaStream_t stream, const DeviceState &dev) {
     const int64_t ldx = d.ldx ? d.ldx : d.k, ldy = d.ldy ? d.ldy : d.n;
     const bool bf16 = d.ab_dtype == CUTE_B200_BF16;
     float *da = reinterpret_cast<float *>(ptr[9]), *db = reinterpret_cast<float *>(ptr[10]);
@@ -230,8 +527,9 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
         return CUTE_B200_OK;
     }
     uint16_t *u = reinterpret_cast<uint16_t *>(ptr[11]);
-    uint16_t *at = reinterpret_cast<uint16_t *>(ptr[11] + t_bytes(d));
-    uint16_t *bt = reinterpret_cast<uint16_t *>(ptr[11] + t_bytes(d) + round_up(uint64_t(d.adapters) * d.rank * d.k * 2));
+    const uint64_t copies = ptr[11] + t_bytes(d) + plan_bytes(d);
+    uint16_t *at = reinterpret_cast<uint16_t *>(copies);
+    uint16_t *bt = reinterpret_cast<uint16_t *>(copies + round_up(uint64_t(d.adapters) * d.rank * d.k * 2));
     transpose_simple<<<dim3(unsigned((int64_t(d.rank) * d.k + 255) / 256), unsigned(d.adapters)), 256, 0, stream>>>(
         reinterpret_cast<const uint16_t *>(ptr[2]), at, d.rank, d.k);
     transpose_simple<<<dim3(unsigned((int64_t(d.rank) * d.n + 255) / 256), unsigned(d.adapters)), 256, 0, stream>>>(
@@ -247,17 +545,11 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
     p.scale = reinterpret_cast<const float *>(ptr[5]);
     p.y = reinterpret_cast<void *>(ptr[8]);
     p.t = u;
+    p.plan = reinterpret_cast<uint32_t *>(ptr[11] + t_bytes(d));
     p.m = d.m, p.n = d.k, p.k = d.n, p.rank = d.rank, p.rp = padded_rank(d.rank), p.adapters = d.adapters, p.c_dtype = d.c_dtype;
     p.ldx = ldy;
     p.ldy = ldx;
-    if (p.y) {
-        CB_TRY(bf16 ? forward<true>(p, stream) : forward<false>(p, stream));
-    } else {
-        if (bf16) shrink_simple<true><<<p.m, 128, 0, stream>>>(p);
-        else shrink_simple<false><<<p.m, 128, 0, stream>>>(p);
-        CB_CUDA(cudaGetLastError());
-        count_launch();
-    }
+    CB_TRY(forward(p, bf16, d.tuning, dev, stream));
     if (da) {
         const uint16_t *x = reinterpret_cast<const uint16_t *>(ptr[0]), *dy = p.x, *t = reinterpret_cast<const uint16_t *>(ptr[7]);
         const dim3 ga(unsigned((d.k + 127) / 128), unsigned(d.rank), unsigned(d.adapters));
@@ -275,6 +567,13 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
     return CUTE_B200_OK;
 }
 
-cute_b200_status lora_init(const DeviceState &) { return CUTE_B200_OK; }
+cute_b200_status lora_init(const DeviceState &) {
+    int device = 0;
+    CB_CUDA(cudaGetDevice(&device));
+    CB_CUDA(cudaFuncSetAttribute(lora_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
+    for (int c = 0; c < 4; c++) CB_TRY(max_clusters(lora_few_kernel, FEW_THREADS, FEW_SMEM, 1 << c, &g_few_clusters[device][c]));
+    CB_TRY(lora_tiled_init());
+    return CUTE_B200_OK;
+}
 
 }  // namespace cb

@@ -1,0 +1,50 @@
+// Shared by the translation units of lora_tn and its gradients.  Internal.
+#pragma once
+
+#include "rows_sm100.cuh"
+
+namespace cb {
+
+struct LoraParams {
+    const uint16_t *x, *w, *a, *b;
+    const int32_t *ids;
+    const float *scale;
+    void *y;
+    uint16_t *t;    // (m, 2 rp): the rounded inner products, then their remainders
+    uint32_t *plan; // which adapters each tile of rows names (tiled kernels)
+    int m, n, k, rank, rp, adapters, c_dtype;
+    int64_t ldx, ldy;
+};
+
+// The tiled forward product (any m; cut 0..2 names a tile, a negative one chooses) and the bytes of its plan.
+cute_b200_status lora_tiled(const LoraParams &p, bool bf16, int cut, int debug, const DeviceState &dev, cudaStream_t stream);
+uint64_t lora_plan_bytes(int m, int adapters);
+cute_b200_status lora_tiled_init();
+
+namespace {
+
+__device__ __forceinline__ void store_c(void *c, int dtype, size_t i, float v) {
+    if (dtype == CUTE_B200_F32) static_cast<float *>(c)[i] = v;
+    else if (dtype == CUTE_B200_BF16) static_cast<__nv_bfloat16 *>(c)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half *>(c)[i] = __float2half_rn(v);
+}
+
+// Width of the rank in T: 16, 32, 64 or 128.
+__host__ __device__ constexpr int padded_rank(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
+
+// An adapter's part of the product runs over the 2 rp columns of T in blocks of
+// 64: block q pairs columns t_col.. of T with columns b_col.. of B; `steps` MMAs
+// of 16, whose step of B is s & b_mask (with rp <= 32 the numbers and their
+// remainders lie in one block and B's columns are used for both).
+struct ExtBlock {
+    int t_col, b_col, steps, b_mask;
+};
+__device__ __forceinline__ int ext_blocks(int rp) { return rp <= 32 ? 1 : rp / 32; }
+__device__ __forceinline__ ExtBlock ext_block(int q, int rp, int rank) {
+    if (rp <= 32) return {0, 0, rp / 8, rp / 16 - 1};
+    const int half = q >> 1, left = (rank - 64 * half + 15) / 16;  // at least 1: rank > rp / 2
+    return {(q & 1) * rp + 64 * half, 64 * half, left < 4 ? left : 4, 3};
+}
+
+}  // namespace
+}  // namespace cb

@@ -181,6 +181,25 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
             "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
             : "memory");
 }
+// The same with a mask over the accumulator's 128 lanes (rows of A): a lane whose bit is set keeps what it holds.
+__device__ __forceinline__ void umma_f16_lanes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate,
+                                               uint32_t off0, uint32_t off1, uint32_t off2, uint32_t off3) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(off0), "r"(off1), "r"(off2), "r"(off3)
+        : "memory");
+}
+// ... over the 2 x 128 lanes of a CTA pair: off[0..3] this (the leader's) CTA, off[4..7] its peer.
+__device__ __forceinline__ void umma_f16_lanes_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate,
+                                                    const uint32_t (&off)[8]) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]),
+        "r"(off[5]), "r"(off[6]), "r"(off[7])
+        : "memory");
+}
 // Make `cluster_bar` (shared::cluster address, own or peer CTA) receive one
 // arrival when every tcgen05.mma issued so far by this thread has finished.
 template <int CTA_GROUP>
@@ -206,6 +225,21 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&v)[32])
           "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr)
         : "memory");
+}
+// Zeros into 32 lanes x 32 consecutive columns, complete on return.
+__device__ __forceinline__ void tmem_zero_32x32(uint32_t taddr) {
+    const uint32_t z = 0;
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, "
+        "%1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1, %1};\n\t"
+        "tcgen05.wait::st.sync.aligned;" ::"r"(taddr), "r"(z)
+        : "memory");
+}
+// Barrier of `threads` threads of the CTA (whole warps), `id` 1..15.
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 // Wait for this thread's tcgen05.ld reads.  The loaded registers are passed
 // through the statement so that the compiler cannot schedule a use of them

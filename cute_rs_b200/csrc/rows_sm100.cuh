@@ -1,0 +1,105 @@
+// Shared by the products whose weights are chosen row by row: 16-bit
+// conversions, tensor maps of row-major 16-bit matrices, small device helpers.
+// Internal.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "pipe_sm100.cuh"
+
+namespace cb {
+namespace {
+
+template <bool BF16>
+__device__ __forceinline__ float to_f32(uint16_t v) {
+    if constexpr (BF16) return __uint_as_float(uint32_t(v) << 16);
+    else return __half2float(__ushort_as_half(v));
+}
+template <bool BF16>
+__device__ __forceinline__ uint16_t from_f32(float v) {
+    if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    else return __half_as_ushort(__float2half_rn(v));
+}
+// The two values of a 32-bit word, the lower address first.
+template <bool BF16>
+__device__ __forceinline__ float2 pair_f32(uint32_t w) {
+    if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    else return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ uint32_t pack_16(float a, float b, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+    return v;
+}
+
+// Tensor map of a row-major 16-bit matrix of `rows` x `cols`, `pitch` elements between rows, in boxes of 64 columns
+// (one 128-byte swizzled row) by box_rows; what lies outside reads as zero.  Encoded anew for every call: it takes
+// a fraction of a microsecond on the host, and nothing is kept by an operand's address.
+inline cute_b200_status rows_tensor_map(CUtensorMap *tm, uint64_t base, bool bf16, uint64_t rows, uint64_t cols, uint64_t pitch, int box_rows) {
+    EncodeTiledFn encode;
+    CB_TRY(encode_fn(&encode));
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {pitch * 2};
+    const cuuint32_t box[2] = {64, cuuint32_t(box_rows)};
+    const cuuint32_t elem[2] = {1, 1};
+    const CUresult r = encode(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                              reinterpret_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(CUTE_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed: CUresult %d (rows %llu, columns %llu, box %d)", int(r),
+                    (unsigned long long)rows, (unsigned long long)cols, box_rows);
+    return CUTE_B200_OK;
+}
+
+// Launch as a programmatic dependent of the kernel before it in the stream, in clusters of `cluster` CTAs.
+template <typename... P, typename... A>
+cute_b200_status launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
+                                  const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    CB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    count_launch();
+    return CUTE_B200_OK;
+}
+
+// How many clusters of `size` CTAs of a kernel the current device can hold at once.
+template <typename... P>
+cute_b200_status max_clusters(void (*kernel)(P...), int threads, size_t smem, int size, int *out) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(size));
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(size);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CB_CUDA(cudaOccupancyMaxActiveClusters(out, kernel, &cfg));
+    return CUTE_B200_OK;
+}
+
+}  // namespace
+}  // namespace cb

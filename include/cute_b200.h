@@ -191,7 +191,7 @@ cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint6
  *   Rows may come in any order: packed sequences, single tokens of many
  *   requests, both mixed.  A row's result depends on its own X row and its own
  *   adapter alone, whatever infinities or NaNs other rows or adapters hold.
- *   m >= 0; n >= 1; k >= 8 and a multiple of 8; rank a multiple of 8 in 8..128
+ *   m >= 0; n >= 1; k >= 8 and a multiple of 8; none above 2^30; rank a multiple of 8 in 8..128
  *   (an adapter of a smaller rank is padded with zeros); adapters >= 1 with
  *   adapters * n, adapters * k and adapters * rank below 2^31.
  *   A[a] x is rounded to the sum of two 16-bit numbers (16 significant bits for
@@ -218,7 +218,8 @@ typedef struct {
     int32_t ab_dtype;  /* CUTE_B200_F16 or CUTE_B200_BF16: X, W, A, B, dY */
     int32_t c_dtype;   /* CUTE_B200_F32, CUTE_B200_F16 or CUTE_B200_BF16: Y, dX */
     int32_t ldx, ldy;  /* elements between rows of X (a multiple of 8) and of Y; 0 = dense (k, n) */
-    int32_t tuning[2]; /* zero.  Measurement and test knobs: [0] 1 = the kernels for few rows (m <= 128), 2 = the tiled kernels;
+    int32_t tuning[2]; /* zero.  Measurement and test knobs: [0] 1 = the kernels for few rows (m <= 128), 2 = the tiled kernels,
+                          3, 4, 5 = those with a tile of 512 x 256, 128 x 256, 128 x 128;
                           [1] bits 2 + 3 make every in-kernel wait run out after 20 ms, as in cute_b200_gemm_desc */
 } cute_b200_lora_desc;
 

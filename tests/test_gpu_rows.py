@@ -149,7 +149,7 @@ class Lora:
 
 
 def variants(m):
-    return [(0, 0), (2, 0)] + ([(1, 0)] if m <= 128 else [])
+    return [(0, 0), (2, 0), (3, 0), (4, 0), (5, 0)] + ([(1, 0)] if m <= 128 else [])
 
 
 SHAPES = [  # m, n, k, rank, adapters, ids
