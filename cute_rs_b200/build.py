@@ -13,7 +13,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcute_b200.so")
-SOURCES = ["api.cu", "elementwise_sm100.cu", "sgemm_sm100.cu", "gemm_sm100.cu", "multi_gpu.cu", "lora_sm100.cu", "lora_tile_sm100.cu", "moe_sm100.cu"]
+SOURCES = ["api.cu", "elementwise_sm100.cu", "sgemm_sm100.cu", "gemm_sm100.cu", "multi_gpu.cu", "lora_sm100.cu", "lora_tile_sm100.cu", "lora_grad_sm100.cu", "moe_sm100.cu"]
 HEADERS = ["common.cuh", "ptx_sm100.cuh", "pipe_sm100.cuh", "rows_sm100.cuh", "lora_sm100.cuh", os.path.join("..", "..", "include", "cute_b200.h")]
 
 

@@ -1,0 +1,339 @@
+// Gradients of the adapters:
+//     dA[a] = sum over rows i of adapter a of U[i] x[i]^T        (rank, k)
+//     dB[a] = sum over rows i of adapter a of dY[i] T[i]^T       (n, rank)
+// Both are products over the rows of one adapter of a wide matrix V (X or dY)
+// with a narrow one L (U or T, each value the sum of two 16-bit numbers).
+//
+// A row list per adapter comes first (rows in ascending order).  Then one CTA
+// takes 128 columns of V for one adapter: M = the columns, N = the 2 rp columns
+// of L, the rows are the k of the MMA, so both operands lie in shared memory
+// with k slow ("MN-major").  64 rows make a block: a plain TMA box where the
+// list's next 64 rows follow one another, else gathered four rows at a time;
+// rows past the end of the list read as zero in both operands, so nothing of
+// another adapter's row, not even a NaN, takes part.  A cluster shares the rows
+// of a tile and adds its partial sums in order: the result does not depend on
+// timing.  Bound by reading X and dY once.
+#include "lora_sm100.cuh"
+
+namespace cb {
+namespace {
+
+constexpr int LIST_THREADS = 1024;
+
+// list[first[a] .. first[a + 1]) = the rows that name adapter a.  A CTA per adapter counts the rows of lower adapters (its
+// place in the list) and its own, then writes its own: no CTA waits for another.
+__global__ void __launch_bounds__(LIST_THREADS) row_list_kernel(const int32_t *ids, int m, int adapters, int32_t *first, int32_t *list) {
+    __shared__ int lower_sum[LIST_THREADS / 32], own_sum[LIST_THREADS / 32];
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const int a = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int lower = 0, own = 0;
+    for (int i = threadIdx.x; i < m; i += LIST_THREADS) {
+        const int id = ids[i];
+        lower += id >= 0 && id < a;
+        own += id == a;
+    }
+    lower = __reduce_add_sync(0xffffffffu, lower);
+    own = __reduce_add_sync(0xffffffffu, own);
+    if (lane == 0) lower_sum[warp] = lower, own_sum[warp] = own;
+    __syncthreads();
+    int begin = 0, count = 0;
+    for (int w = 0; w < LIST_THREADS / 32; w++) begin += lower_sum[w], count += own_sum[w];
+    if (threadIdx.x == 0) {
+        first[a] = begin;
+        if (a == adapters - 1) first[adapters] = begin + count;
+    }
+    __syncthreads();
+    int at = begin;
+    for (int i0 = 0; i0 < m && at < begin + count; i0 += LIST_THREADS) {
+        const int i = i0 + int(threadIdx.x);
+        const bool mine = i < m && ids[i] == a;
+        const uint32_t votes = __ballot_sync(0xffffffffu, mine);
+        if (lane == 0) own_sum[warp] = __popc(votes);
+        __syncthreads();
+        int before = __popc(votes & ((1u << lane) - 1u)), total = 0;
+        for (int w = 0; w < LIST_THREADS / 32; w++) {
+            if (w < warp) before += own_sum[w];
+            total += own_sum[w];
+        }
+        if (mine) list[at + before] = i;
+        at += total;
+        __syncthreads();
+    }
+}
+
+// (rows, cols) -> (cols, rows) of each adapter's 16-bit matrix, 64 x 64 values per CTA; adapters without a row are left out.
+__global__ void __launch_bounds__(256) transpose_kernel(const uint16_t *in, uint16_t *out, int rows, int cols, const int32_t *first) {
+    __shared__ uint16_t tile[64][66];
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const int per_col = (cols + 63) / 64, per_row = (rows + 63) / 64;
+    const int64_t block = blockIdx.x;
+    const int a = int(block / (per_col * per_row)), left = int(block % (per_col * per_row));
+    if (first[a] == first[a + 1]) return;
+    const int r0 = left / per_col * 64, c0 = left % per_col * 64;
+    const int64_t base = int64_t(a) * rows * cols;
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int r = i >> 6, c = i & 63;
+        if (r0 + r < rows && c0 + c < cols) tile[r][c] = in[base + int64_t(r0 + r) * cols + c0 + c];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int c = i >> 6, r = i & 63;
+        if (r0 + r < rows && c0 + c < cols) out[base + int64_t(c0 + c) * rows + r0 + r] = tile[r][c];
+    }
+}
+
+constexpr int GRAD_THREADS = 192, GRAD_M = 128, GRAD_ROWS = 64, GRAD_STAGES = 4;
+constexpr uint32_t GRAD_BOX = GRAD_ROWS * 128, GRAD_RING = 96 * 1024, GRAD_HEAD = 1024;
+constexpr uint32_t GRAD_SMEM = 1024 + GRAD_HEAD + GRAD_RING;
+
+struct GradMaps {
+    CUtensorMap wide[2], wide_rows[2], low[2], low_rows[2];  // [0] for dA: X and U, [1] for dB: dY and T; boxes of 64 rows, and of one
+};
+
+struct GradParams {
+    float *out[2];
+    const int32_t *first, *list;
+    int cols[2], tiles[2], m, rank, rp, kc, stages;
+    uint32_t stage_bytes, idesc, tmem_cols;
+    uint32_t *status;
+    int debug;
+};
+
+struct GradHead {
+    uint64_t full[GRAD_STAGES], empty[GRAD_STAGES], done, drain;
+    uint32_t tmem, abort;
+};
+
+// Shared-memory matrix descriptor of an MN-major tile in 128-byte rows with the 128B swizzle: 64 values of M or N per
+// row, the rows are k.  Leading byte offset: from 64 values to the next 64 (one box); stride byte offset: from eight k
+// to the next eight.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
+    return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(GRAD_BOX >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+           (uint64_t(2) << 61);
+}
+
+__global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    GradHead &h = *reinterpret_cast<GradHead *>(smem_raw + (base - raw));
+    const uint32_t ring = base + GRAD_HEAD;
+    auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
+    volatile uint32_t *abort_flag = &h.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = p.kc > 1 ? ptx::cluster_ctarank() : 0u;
+    const int unit = int(blockIdx.x) / p.kc, per = p.tiles[0] + p.tiles[1], a = unit / per;
+    int tile = unit - a * per;
+    const int job = tile >= p.tiles[0] ? 1 : 0;
+    if (job) tile -= p.tiles[0];
+    const int c0 = tile * GRAD_M, low_boxes = (2 * p.rp + 63) / 64;
+    const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < GRAD_STAGES; s++) {
+            ptx::mbar_init(bar(h.full[s]), 1);
+            ptx::mbar_init(bar(h.empty[s]), 1);
+        }
+        ptx::mbar_init(bar(h.done), 1);
+        ptx::mbar_init(bar(h.drain), 1);
+        h.abort = 0u;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), p.tmem_cols);
+        ptx::tmem_relinquish<1>();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&h.tmem);
+    ptx::griddep_wait();
+    if (threadIdx.x == 0) ptx::griddep_launch_dependents();
+    const int begin = p.first[a], count = p.first[a + 1] - begin, blocks = (count + GRAD_ROWS - 1) / GRAD_ROWS;
+    const int b0 = int(int64_t(blocks) * rank / p.kc), b1 = int(int64_t(blocks) * (rank + 1) / p.kc);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            ptx::prefetch_tensormap(&maps.wide[job]);
+            ptx::prefetch_tensormap(&maps.low[job]);
+        }
+        int s = 0;
+        uint32_t ph = 0, filled = 0, filled_parity = 0;
+        bool ok = !(p.debug & 4);
+        const uint32_t bytes = uint32_t(2 + low_boxes) * GRAD_BOX;
+        for (int b = b0; b < b1 && ok; b++) {
+            // Lanes 0-15 hold four rows of the block each; past the end of the list a row that no matrix has.
+            int row[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = b * GRAD_ROWS + 4 * (lane & 15) + i;
+                row[i] = at < count ? p.list[begin + at] : p.m;
+            }
+            const int first_row = __shfl_sync(0xffffffffu, row[0], 0), last_row = __shfl_sync(0xffffffffu, row[3], 15);
+            const bool run = last_row < p.m && last_row - first_row == GRAD_ROWS - 1;
+            ok = wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint32_t dst = ring + uint32_t(s) * p.stage_bytes, full = bar(h.full[s]);
+            if (lane == 0) ptx::mbar_arrive_expect_tx(full, bytes);
+            __syncwarp();
+            if (run) {
+                if (lane == 0) {
+                    for (int x = 0; x < 2; x++) ptx::tma_load_2d(dst + x * GRAD_BOX, &maps.wide[job], full, c0 + 64 * x, first_row);
+                    for (int x = 0; x < low_boxes; x++) ptx::tma_load_2d(dst + (2 + x) * GRAD_BOX, &maps.low[job], full, 64 * x, first_row);
+                }
+            } else if (lane < 16) {
+                for (int x = 0; x < 2; x++)
+                    ptx::tma_gather4(dst + x * GRAD_BOX + 512u * lane, &maps.wide_rows[job], full, c0 + 64 * x, row[0], row[1], row[2], row[3]);
+                for (int x = 0; x < low_boxes; x++)
+                    ptx::tma_gather4(dst + (2 + x) * GRAD_BOX + 512u * lane, &maps.low_rows[job], full, 64 * x, row[0], row[1], row[2], row[3]);
+            }
+            __syncwarp();
+            filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
+            if (++s == p.stages) s = 0, ph ^= 1u;
+        }
+        if (!ok && lane == 0) {  // giving up: let the copies in flight land (bounded)
+            const uint64_t t0 = ptx::globaltimer_ns();
+            for (int i = 0; i < GRAD_STAGES; i++)
+                while ((filled >> i & 1u) && !ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true, issued = false;
+            for (int b = b0; b < b1; b++) {
+                if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) break;
+                ptx::tc_fence_after();
+                const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+                const uint64_t wide = mn_desc(src), low = mn_desc(src + 2 * GRAD_BOX);
+#pragma unroll
+                for (int j = 0; j < 4; j++)  // 16 rows of 128 bytes further
+                    ptx::umma_f16<1>(tmem, wide + 128u * j, low + 128u * j, p.idesc, (b > b0 || j > 0) ? 1u : 0u);
+                issued = true;
+                ptx::umma_commit<1>(bar(h.empty[s]));
+                if (++s == p.stages) s = 0, ph ^= 1u;
+            }
+            if (ok) {
+                ptx::umma_commit<1>(bar(h.done));
+            } else if (issued) {
+                ptx::umma_commit<1>(bar(h.drain));
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while (!ptx::mbar_try_wait(bar(h.drain), 0u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        const bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.done), 0, abort_flag, p.status, WHERE_EPILOGUE, 0u, limit));
+        const int q = warp & 3;
+        const uint32_t pitch = uint32_t(p.rp + 4) * 4u, dst = ring + uint32_t(32 * q + lane) * pitch;
+        if (ok) {
+            ptx::tc_fence_after();
+            ptx::fence_proxy_async_shared();
+            // Columns j and rp + j belong to the two numbers of value j: their sum is the gradient's part.
+            for (int c = 0; c < p.rp; c += 16) {
+                float v[16];
+                if (b0 < b1) {
+                    uint32_t hi[16], lo[16];
+                    ptx::tmem_ld_32x16(tmem + (uint32_t(32 * q) << 16) + uint32_t(c), hi);
+                    ptx::tmem_ld_32x16(tmem + (uint32_t(32 * q) << 16) + uint32_t(p.rp + c), lo);
+                    ptx::tmem_ld_wait_all();
+                    ptx::pin16(hi);
+                    ptx::pin16(lo);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = __uint_as_float(hi[j]) + __uint_as_float(lo[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = 0.0f;
+                }
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    ptx::st_shared_v4(dst + uint32_t(c + 4 * g) * 4u, __float_as_uint(v[4 * g]), __float_as_uint(v[4 * g + 1]),
+                                      __float_as_uint(v[4 * g + 2]), __float_as_uint(v[4 * g + 3]));
+            }
+        }
+        __syncwarp();
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (p.kc > 1) {
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    if (!*abort_flag) {
+        const uint32_t pitch = uint32_t(p.rp + 4) * 4u;
+        const int cols = p.cols[job], wide = min(GRAD_M, cols - c0), items = GRAD_M * p.rank;
+        float *out = p.out[job] + int64_t(a) * p.rank * cols;
+        for (int i = int(rank) * GRAD_THREADS + int(threadIdx.x); i < items; i += p.kc * GRAD_THREADS) {
+            // Neighbouring threads write neighbouring addresses: columns of dA, ranks of dB.
+            const int c = job ? i / p.rank : i % GRAD_M, j = job ? i % p.rank : i / GRAD_M;
+            if (c >= wide) continue;
+            const uint32_t at = ring + uint32_t(c) * pitch + uint32_t(j) * 4u;
+            float v = ptx::ld_shared_cluster(p.kc > 1 ? ptx::mapa(at, 0) : at);
+            for (int x = 1; x < p.kc; x++) v += ptx::ld_shared_cluster(ptx::mapa(at, uint32_t(x)));
+            out[job ? int64_t(c0 + c) * p.rank + j : int64_t(j) * cols + c0 + c] = v;
+        }
+    }
+    __syncthreads();
+    if (p.kc > 1) {
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, p.tmem_cols);
+}
+
+}  // namespace
+
+cute_b200_status lora_row_lists(const int32_t *ids, int m, int adapters, int32_t *first, int32_t *list, cudaStream_t stream) {
+    return launch_dependent(row_list_kernel, dim3(unsigned(adapters)), LIST_THREADS, 0, 1, stream, ids, m, adapters, first, list);
+}
+
+cute_b200_status lora_transpose(const uint16_t *in, uint16_t *out, int adapters, int rows, int cols, const int32_t *first,
+                                cudaStream_t stream) {
+    const int64_t blocks = int64_t(adapters) * ((rows + 63) / 64) * ((cols + 63) / 64);
+    if (blocks > 0x7fffffff) return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "lora_tn_backward: the adapters are too large");
+    return launch_dependent(transpose_kernel, dim3(unsigned(blocks)), 256, 0, 1, stream, in, out, rows, cols, first);
+}
+
+cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream) {
+    GradParams p = {};
+    GradMaps maps;
+    for (int i = 0; i < 2; i++) {
+        p.out[i] = g.out[i];
+        p.cols[i] = g.cols[i];
+        p.tiles[i] = (g.cols[i] + GRAD_M - 1) / GRAD_M;
+        const uint64_t wide = reinterpret_cast<uint64_t>(g.wide[i]), low = reinterpret_cast<uint64_t>(g.low[i]);
+        CB_TRY(rows_tensor_map(&maps.wide[i], wide, bf16, g.m, g.cols[i], g.pitch[i], GRAD_ROWS));
+        CB_TRY(rows_tensor_map(&maps.wide_rows[i], wide, bf16, g.m, g.cols[i], g.pitch[i], 1));
+        CB_TRY(rows_tensor_map(&maps.low[i], low, bf16, g.m, 2 * g.rp, 2 * g.rp, GRAD_ROWS));
+        CB_TRY(rows_tensor_map(&maps.low_rows[i], low, bf16, g.m, 2 * g.rp, 2 * g.rp, 1));
+    }
+    p.first = g.first, p.list = g.list;
+    p.m = g.m, p.rank = g.rank, p.rp = g.rp;
+    p.stage_bytes = uint32_t(2 + (2 * g.rp + 63) / 64) * GRAD_BOX;
+    p.stages = int(GRAD_RING / p.stage_bytes);
+    if (p.stages > GRAD_STAGES) p.stages = GRAD_STAGES;
+    p.idesc = make_idesc(bf16, GRAD_M, 2 * g.rp) | (1u << 15) | (1u << 16);  // both operands MN-major
+    p.tmem_cols = uint32_t(2 * g.rp);
+    p.status = dev.status_word;
+    p.debug = debug;
+    // The rows of a tile are shared by a cluster while that fills the GPU (two CTAs per SM) and leaves each CTA of an
+    // adapter of average size at least four blocks.
+    const int64_t units = int64_t(p.tiles[0] + p.tiles[1]) * g.adapters;
+    p.kc = 1;
+    while (p.kc < 8 && units * p.kc < 2 * dev.sm_count && int64_t(g.m) >= int64_t(8 * GRAD_ROWS) * p.kc * g.adapters) p.kc *= 2;
+    if (units * p.kc > 0x7fffffff) return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "lora_tn_backward: the adapters are too large");
+    return launch_dependent(lora_grad_kernel, dim3(unsigned(units * p.kc)), GRAD_THREADS, GRAD_SMEM, p.kc, stream, maps, p);
+}
+
+cute_b200_status lora_grad_init() {
+    CB_CUDA(cudaFuncSetAttribute(lora_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM));
+    return CUTE_B200_OK;
+}
+
+}  // namespace cb

@@ -9,28 +9,6 @@
 namespace cb {
 namespace {
 
-// (rows, cols) -> (cols, rows) of each of `count` 16-bit matrices.
-__global__ void transpose_simple(const uint16_t *in, uint16_t *out, int rows, int cols) {
-    const int64_t base = int64_t(blockIdx.y) * rows * cols;
-    const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i >= int64_t(rows) * cols) return;
-    out[base + (i % cols) * rows + i / cols] = in[base + i];
-}
-
-// out[a][j * sj + c * sc] = sum over rows i with ids[i] == a of (hi + lo of t[i][j]) * v[i][c]
-template <bool BF16>
-__global__ void grad_simple(const uint16_t *t, const uint16_t *v, int64_t ldv, const int32_t *ids, float *out, int m, int cols, int rank,
-                            int rp, int64_t sj, int64_t sc) {
-    const int a = blockIdx.z, j = blockIdx.y;
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= cols) return;
-    float acc = 0.0f;
-    for (int64_t i = 0; i < m; i++)
-        if (ids[i] == a)
-            acc = fmaf(to_f32<BF16>(t[i * 2 * rp + j]) + to_f32<BF16>(t[i * 2 * rp + rp + j]), to_f32<BF16>(v[i * ldv + c]), acc);
-    out[int64_t(a) * rank * cols + j * sj + c * sc] = acc;
-}
-
 // ---- few rows (m <= 128) ------------------------------------------------------
 // T: a CTA takes one row and four of its adapter's `rank` rows; its 256 threads
 // walk k in 16-byte pieces.  It is over before the weights have streamed past
@@ -412,6 +390,20 @@ uint64_t t_bytes(const cute_b200_lora_desc &d) { return round_up(uint64_t(d.m) *
 
 uint64_t plan_bytes(const cute_b200_lora_desc &d) { return round_up(lora_plan_bytes(d.m, d.adapters)) + kAlign; }
 
+// The backward call's workspace: U and the plan of its product, the adapters transposed, the row lists.
+struct BackLayout {
+    uint64_t at, bt, first, list, total;
+};
+BackLayout back_layout(const cute_b200_lora_desc &d) {
+    BackLayout l;
+    l.at = t_bytes(d) + plan_bytes(d);
+    l.bt = l.at + round_up(uint64_t(d.adapters) * d.rank * d.k * 2);
+    l.first = l.bt + round_up(uint64_t(d.adapters) * d.rank * d.n * 2);
+    l.list = l.first + round_up((uint64_t(d.adapters) + 1) * 4);
+    l.total = l.list + round_up(uint64_t(d.m) * 4) + kAlign;
+    return l;
+}
+
 cute_b200_status check_desc(const cute_b200_lora_desc &d, const char *who) {
     if (d.m < 0 || d.n < 1 || d.k < 8)
         return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: invalid size %dx%dx%d", who, d.m, d.n, d.k);
@@ -458,7 +450,7 @@ cute_b200_status forward(const LoraParams &p, bool bf16, const int32_t (&tuning)
 cute_b200_status lora_workspace(const cute_b200_lora_desc &d, uint64_t *forward, uint64_t *backward) {
     CB_TRY(check_desc(d, "lora_workspace"));
     *forward = t_bytes(d) + plan_bytes(d);
-    *backward = t_bytes(d) + plan_bytes(d) + round_up(uint64_t(d.adapters) * d.rank * d.k * 2) + round_up(uint64_t(d.adapters) * d.rank * d.n * 2);
+    *backward = back_layout(d).total;
     return CUTE_B200_OK;
 }
 
@@ -527,15 +519,12 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
         return CUTE_B200_OK;
     }
     uint16_t *u = reinterpret_cast<uint16_t *>(ptr[11]);
-    const uint64_t copies = ptr[11] + t_bytes(d) + plan_bytes(d);
-    uint16_t *at = reinterpret_cast<uint16_t *>(copies);
-    uint16_t *bt = reinterpret_cast<uint16_t *>(copies + round_up(uint64_t(d.adapters) * d.rank * d.k * 2));
-    transpose_simple<<<dim3(unsigned((int64_t(d.rank) * d.k + 255) / 256), unsigned(d.adapters)), 256, 0, stream>>>(
-        reinterpret_cast<const uint16_t *>(ptr[2]), at, d.rank, d.k);
-    transpose_simple<<<dim3(unsigned((int64_t(d.rank) * d.n + 255) / 256), unsigned(d.adapters)), 256, 0, stream>>>(
-        reinterpret_cast<const uint16_t *>(ptr[3]), bt, d.n, d.rank);
-    CB_CUDA(cudaGetLastError());
-    count_launch(2);
+    const BackLayout l = back_layout(d);
+    uint16_t *at = reinterpret_cast<uint16_t *>(ptr[11] + l.at), *bt = reinterpret_cast<uint16_t *>(ptr[11] + l.bt);
+    int32_t *first = reinterpret_cast<int32_t *>(ptr[11] + l.first), *list = reinterpret_cast<int32_t *>(ptr[11] + l.list);
+    CB_TRY(lora_row_lists(reinterpret_cast<const int32_t *>(ptr[4]), d.m, d.adapters, first, list, stream));
+    if (ptr[8]) CB_TRY(lora_transpose(reinterpret_cast<const uint16_t *>(ptr[2]), at, d.adapters, d.rank, d.k, first, stream));
+    CB_TRY(lora_transpose(reinterpret_cast<const uint16_t *>(ptr[3]), bt, d.adapters, d.n, d.rank, first, stream));
     LoraParams p = {};
     p.x = reinterpret_cast<const uint16_t *>(ptr[6]);
     p.w = reinterpret_cast<const uint16_t *>(ptr[1]);
@@ -551,18 +540,15 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
     p.ldy = ldx;
     CB_TRY(forward(p, bf16, d.tuning, dev, stream));
     if (da) {
-        const uint16_t *x = reinterpret_cast<const uint16_t *>(ptr[0]), *dy = p.x, *t = reinterpret_cast<const uint16_t *>(ptr[7]);
-        const dim3 ga(unsigned((d.k + 127) / 128), unsigned(d.rank), unsigned(d.adapters));
-        const dim3 gb(unsigned((d.n + 127) / 128), unsigned(d.rank), unsigned(d.adapters));
-        if (bf16) {
-            grad_simple<true><<<ga, 128, 0, stream>>>(u, x, ldx, p.ids, da, d.m, d.k, d.rank, p.rp, d.k, 1);
-            grad_simple<true><<<gb, 128, 0, stream>>>(t, dy, ldy, p.ids, db, d.m, d.n, d.rank, p.rp, 1, d.rank);
-        } else {
-            grad_simple<false><<<ga, 128, 0, stream>>>(u, x, ldx, p.ids, da, d.m, d.k, d.rank, p.rp, d.k, 1);
-            grad_simple<false><<<gb, 128, 0, stream>>>(t, dy, ldy, p.ids, db, d.m, d.n, d.rank, p.rp, 1, d.rank);
-        }
-        CB_CUDA(cudaGetLastError());
-        count_launch(2);
+        LoraGrads g = {};
+        g.out[0] = da, g.out[1] = db;
+        g.wide[0] = reinterpret_cast<const uint16_t *>(ptr[0]), g.wide[1] = p.x;
+        g.low[0] = u, g.low[1] = reinterpret_cast<const uint16_t *>(ptr[7]);
+        g.pitch[0] = ldx, g.pitch[1] = ldy;
+        g.cols[0] = d.k, g.cols[1] = d.n;
+        g.m = d.m, g.rank = d.rank, g.rp = p.rp, g.adapters = d.adapters;
+        g.first = first, g.list = list;
+        CB_TRY(lora_grads(g, bf16, d.tuning[1], dev, stream));
     }
     return CUTE_B200_OK;
 }
@@ -573,6 +559,7 @@ cute_b200_status lora_init(const DeviceState &) {
     CB_CUDA(cudaFuncSetAttribute(lora_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
     for (int c = 0; c < 4; c++) CB_TRY(max_clusters(lora_few_kernel, FEW_THREADS, FEW_SMEM, 1 << c, &g_few_clusters[device][c]));
     CB_TRY(lora_tiled_init());
+    CB_TRY(lora_grad_init());
     return CUTE_B200_OK;
 }
 

@@ -21,6 +21,20 @@ cute_b200_status lora_tiled(const LoraParams &p, bool bf16, int cut, int debug, 
 uint64_t lora_plan_bytes(int m, int adapters);
 cute_b200_status lora_tiled_init();
 
+// The adapters' gradients: [0] dA from X and U, [1] dB from dY and T.  `first` (adapters + 1) and `list` (m) are the row lists.
+struct LoraGrads {
+    float *out[2];
+    const uint16_t *wide[2], *low[2];
+    int64_t pitch[2];
+    int cols[2], m, rank, rp, adapters;
+    const int32_t *first, *list;
+};
+cute_b200_status lora_row_lists(const int32_t *ids, int m, int adapters, int32_t *first, int32_t *list, cudaStream_t stream);
+cute_b200_status lora_transpose(const uint16_t *in, uint16_t *out, int adapters, int rows, int cols, const int32_t *first,
+                                cudaStream_t stream);
+cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream);
+cute_b200_status lora_grad_init();
+
 namespace {
 
 __device__ __forceinline__ void store_c(void *c, int dtype, size_t i, float v) {
