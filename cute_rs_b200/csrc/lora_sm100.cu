@@ -326,28 +326,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 
 constexpr uint32_t FEW_SMEM = 227 * 1024;
 
-// How the few-row kernel is cut: bn columns of Y per tile, a cluster of kc CTAs per tile.  The launch is one wave
-// where it can be; the cut with the least time for the slowest CTA wins.  A CTA streams at most what an even share of
-// HBM gives it, and no faster than its MMAs take (four per k block, a fixed ~60 clocks or bn / 2 each).
 int g_few_clusters[64][4];  // clusters of 1, 2, 4, 8 CTAs of the few-row kernel that fit each device at once
-
-void few_cut(int n, int k, const int (&max_clusters)[4], int *bn, int *kc) {
-    const int k_blocks = (k + 63) / 64;
-    double best = 1e300;
-    for (int c = 0; c < 4; c++) {
-        const int parts = 1 << c, ctas_at_once = max_clusters[c] * parts;
-        if (parts > k_blocks || max_clusters[c] < 1) continue;
-        for (int b = 16; b <= 256; b += 16) {
-            const int64_t ctas = int64_t((n + b - 1) / b) * parts;
-            const int64_t waves = (ctas + ctas_at_once - 1) / ctas_at_once;
-            const double share = 6.5e12 / double(ctas < ctas_at_once ? ctas : ctas_at_once);
-            const double rate = share < 7.0e10 ? share : 7.0e10;
-            const double load = b * 128.0 / rate, math = 4.0 * (b / 2 > 60 ? b / 2 : 60) / 1.7e9;
-            const double t = double(waves) * (((k_blocks + parts - 1) / parts) * (load > math ? load : math) + 2.0e-6) + (parts > 1 ? 1.0e-6 : 0.0);
-            if (t < best * 0.999) best = t, *bn = b, *kc = parts;
-        }
-    }
-}
 
 template <bool BF16>
 cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int debug, cudaStream_t stream) {
@@ -362,7 +341,7 @@ cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int de
     f.bn = 16, f.kc = 1;
     int device = 0;
     CB_CUDA(cudaGetDevice(&device));
-    few_cut(p.n, p.k, g_few_clusters[device], &f.bn, &f.kc);
+    stream_cut(p.n, (p.k + 63) / 64, g_few_clusters[device], &f.bn, &f.kc);
     f.xr = (p.m + 7) / 8 * 8;
     f.w_offset = uint32_t(f.xr) * 128u;
     f.stage_bytes = uint32_t(f.xr + f.bn) * 128u;

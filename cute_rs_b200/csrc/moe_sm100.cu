@@ -1,74 +1,118 @@
-// A mixture-of-experts layer for a few tokens: router, softmax, top-k, gated
-// experts, weighted sum.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "common.cuh"
-#include "ptx_sm100.cuh"
+// A mixture-of-experts layer for a few tokens, in three kernels:
+//   router   logits, softmax, top-k: a cluster of eight CTAs for four tokens;
+//   up       the gate and up weights of the experts that anybody chose stream past all the tokens, each byte once;
+//   down     the down weights likewise, summed over the experts in the accumulator.
+// Bound by HBM: 6 d f bytes per chosen expert.  The tokens (at most 64 of the M = 128 rows of an MMA) are the lanes of
+// the accumulators, the weights' rows its columns, so that nothing is gathered or sorted: an expert's product is
+// computed for all tokens - the tensor core has time to spare, an MMA of N columns costs the same for 1 and for 128 rows -
+// and used, or added, only in the lanes of the tokens that chose it.
+#include "rows_sm100.cuh"
 
 namespace cb {
 namespace {
 
-template <bool BF16>
-__device__ __forceinline__ float to_f32(uint16_t v) {
-    if constexpr (BF16) return __uint_as_float(uint32_t(v) << 16);
-    else return __half2float(__ushort_as_half(v));
-}
-template <bool BF16>
-__device__ __forceinline__ uint16_t from_f32(float v) {
-    if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
-    else return __half_as_ushort(__float2half_rn(v));
-}
-__device__ __forceinline__ float warp_sum(float v) {
-    for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-    return v;
-}
+constexpr int MAX_TOKENS = 64, MAX_TOP = 16, MAX_EXPERTS = 512;
 
 struct MoeParams {
-    const uint16_t *x, *r, *g, *u, *dn;
-    uint16_t *y;
-    float *logits;   // (tokens, experts)
-    int32_t *ids;    // (tokens, top)
-    float *weights;  // (tokens, top)
-    uint16_t *h;     // (tokens, top, f)
-    int tokens, experts, top, d, f, renorm;
+    const uint16_t *x, *r;
+    uint16_t *y, *h;  // h: (chosen experts in ascending order, token_rows, f)
+    int32_t *ids;     // (tokens, top)
+    float *weights;   // (tokens, top)
+    int tokens, token_rows, experts, top, d, f, renorm;
+    int kc, bn, stages;
+    uint32_t stage_bytes, tmem_cols;
+    bool bf16;
+    uint32_t *status;
+    int debug;
 };
 
-template <bool BF16>
-__global__ void logits_simple(const MoeParams p) {
-    const int e = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
-    float acc = 0.0f;
-    for (int l = lane; l < p.d; l += 32) acc = fmaf(to_f32<BF16>(p.x[int64_t(t) * p.d + l]), to_f32<BF16>(p.r[int64_t(e) * p.d + l]), acc);
-    acc = warp_sum(acc);
-    if (lane == 0) p.logits[t * p.experts + e] = acc;
-}
+// ---- router -----------------------------------------------------------------
+// 64 warps share the experts' rows of four tokens; with fewer than 64 experts each row is cut into `parts` ranges of
+// d.  The sums go to the CTA that owns the token (the cluster's CTAs 0-3), which adds the parts in order and chooses.
+constexpr int ROUTER_THREADS = 256, ROUTER_CLUSTER = 8, ROUTER_TOKENS = 4;
 
-// One warp per token.
-__global__ void top_simple(const MoeParams p) {
-    const int t = blockIdx.x, lane = threadIdx.x;
-    float v[16];
-    float best = -INFINITY;
-    for (int j = 0; j < 16; j++) {
-        const int e = j * 32 + lane;
-        v[j] = e < p.experts ? p.logits[t * p.experts + e] : 0.0f;
-        if (e < p.experts) best = fmaxf(best, v[j]);
+template <bool BF16>
+__global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoeParams p) {
+    __shared__ float part[MAX_EXPERTS];
+    ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = int(ptx::cluster_ctarank()), t0 = int(blockIdx.x) / ROUTER_CLUSTER * ROUTER_TOKENS;
+    const int warps = ROUTER_CLUSTER * ROUTER_THREADS / 32, count = min(ROUTER_TOKENS, p.tokens - t0);
+    int parts = 1;
+    while (parts * 2 * p.experts <= warps && parts * 2 <= 8) parts *= 2;  // experts * parts <= MAX_EXPERTS
+    const int vecs = p.d / 8;
+    ptx::cluster_arrive();
+    ptx::cluster_wait();  // every CTA of the cluster runs: its shared memory may be written
+    for (int item = rank * (ROUTER_THREADS / 32) + warp; item < p.experts * parts; item += warps) {
+        const int e = item / parts, q = item - e * parts;
+        const uint16_t *r = p.r + int64_t(e) * p.d, *x = p.x + int64_t(t0) * p.d;
+        float acc[ROUTER_TOKENS] = {};
+        const int end = int(int64_t(vecs) * (q + 1) / parts);
+#pragma unroll 2
+        for (int c = int(int64_t(vecs) * q / parts) + lane; c < end; c += 32) {
+            const uint4 rv = *reinterpret_cast<const uint4 *>(r + 8 * c);
+            const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+#pragma unroll
+            for (int t = 0; t < ROUTER_TOKENS; t++) {
+                if (t >= count) break;
+                const uint4 xv = *reinterpret_cast<const uint4 *>(x + int64_t(t) * p.d + 8 * c);
+                const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 a = pair_f32<BF16>(rw[i]), b = pair_f32<BF16>(xw[i]);
+                    acc[t] = fmaf(a.y, b.y, fmaf(a.x, b.x, acc[t]));
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < ROUTER_TOKENS; t++) {
+            const float sum = warp_sum(acc[t]);
+            if (lane == 0 && t < count) ptx::st_shared_cluster(ptx::mapa(ptx::smem_u32(&part[item]), uint32_t(t)), sum);
+        }
     }
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    if (rank >= count || warp != 0) return;  // nothing reads another CTA's shared memory from here on
+    // One warp chooses for the token: lane l holds experts l, l + 32, ..
+    const int t = t0 + rank;
+    float v[MAX_EXPERTS / 32];
+    float best = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < MAX_EXPERTS / 32; j++) {
+        const int e = j * 32 + lane;
+        v[j] = -INFINITY;
+        if (e < p.experts) {
+            float sum = part[e * parts];
+            for (int q = 1; q < parts; q++) sum += part[e * parts + q];
+            v[j] = sum;
+            best = fmaxf(best, sum);
+        }
+    }
+#pragma unroll
     for (int s = 16; s > 0; s >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, s));
     float total = 0.0f;
-    for (int j = 0; j < 16; j++)
-        if (j * 32 + lane < p.experts) total += expf(v[j] - best);
-    total = warp_sum(total);
     uint32_t open = 0;
-    for (int j = 0; j < 16; j++) open |= (j * 32 + lane < p.experts ? 1u : 0u) << j;
-    float chosen_sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < MAX_EXPERTS / 32; j++)
+        if (j * 32 + lane < p.experts) {
+            total += expf(v[j] - best);
+            open |= 1u << j;
+        }
+    total = warp_sum(total);
+    float chosen_sum = 0.0f, my_w = 0.0f;
+    int my_id = 0;
     for (int i = 0; i < p.top; i++) {
-        float key = 0.0f;
+        // The largest open logit, the lowest index among equals; a NaN counts as the smallest (its weight is a NaN).
+        float key = -INFINITY;
         int at = 0x7fffffff;
-        for (int j = 0; j < 16; j++)
+#pragma unroll
+        for (int j = 0; j < MAX_EXPERTS / 32; j++)
             if ((open >> j) & 1u) {
                 const float c = v[j] == v[j] ? v[j] : -INFINITY;
                 if (at == 0x7fffffff || c > key) key = c, at = j * 32 + lane;
             }
+#pragma unroll
         for (int s = 16; s > 0; s >>= 1) {
             const float k2 = __shfl_xor_sync(0xffffffffu, key, s);
             const int a2 = __shfl_xor_sync(0xffffffffu, at, s);
@@ -77,41 +121,412 @@ __global__ void top_simple(const MoeParams p) {
         if ((at & 31) == lane) open &= ~(1u << (at >> 5));
         const float w = expf(key - best) / total;
         chosen_sum += w;
-        if (lane == 0) p.ids[t * p.top + i] = at, p.weights[t * p.top + i] = w;
+        if (lane == i) my_w = w, my_id = at;
     }
-    __syncwarp();
-    if (p.renorm && lane < p.top) p.weights[t * p.top + lane] /= chosen_sum;
+    if (lane < p.top) {
+        p.ids[t * p.top + lane] = my_id;
+        p.weights[t * p.top + lane] = p.renorm ? my_w / chosen_sum : my_w;
+    }
 }
 
-template <bool BF16>
-__global__ void up_simple(const MoeParams p) {
-    const int slot = blockIdx.y, t = slot / p.top, lane = threadIdx.x & 31;
-    const int j = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (j >= p.f) return;
-    const int64_t row = (int64_t(p.ids[slot]) * p.f + j) * p.d;
-    float g = 0.0f, u = 0.0f;
-    for (int l = lane; l < p.d; l += 32) {
-        const float x = to_f32<BF16>(p.x[int64_t(t) * p.d + l]);
-        g = fmaf(to_f32<BF16>(p.g[row + l]), x, g);
-        u = fmaf(to_f32<BF16>(p.u[row + l]), x, u);
+// ---- which experts are chosen, and by whom ----------------------------------------
+struct MoeHead {
+    uint64_t full[16], empty[16], tfull[2], tempty[2], plan, zeroed, done, drain;
+    uint32_t tmem, abort;
+    int32_t active, before[4];
+    int32_t expert[MAX_EXPERTS];                     // the chosen experts, ascending
+    unsigned long long who[MAX_EXPERTS];             // by expert: which tokens chose it
+    int32_t ids[MAX_TOKENS * MAX_TOP];
+    float weights[MAX_TOKENS * MAX_TOP];
+};
+constexpr uint32_t MOE_HEAD = 16 * 1024;
+static_assert(sizeof(MoeHead) <= MOE_HEAD, "head");
+
+// By 128 threads (t = 0..127).  The router's output is read from L2: the down kernel reads it ahead of its griddepcontrol.wait.
+__device__ __forceinline__ void find_active(MoeHead &h, const MoeParams &p, int t) {
+    const int lane = t & 31, w = t >> 5;
+    for (int e = t; e < MAX_EXPERTS; e += 128) h.who[e] = 0ull;
+    for (int i = t; i < p.tokens * p.top; i += 128) h.ids[i] = __ldcg(p.ids + i), h.weights[i] = __ldcg(p.weights + i);
+    ptx::named_barrier(1, 128);
+    for (int i = t; i < p.tokens * p.top; i += 128) atomicOr(&h.who[h.ids[i]], 1ull << (i / p.top));
+    ptx::named_barrier(1, 128);
+    int mine = 0;
+    for (int j = 0; j < 4; j++) mine += h.who[4 * t + j] != 0ull;
+    int upto = mine;
+    for (int s = 1; s < 32; s <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, upto, s);
+        if (lane >= s) upto += o;
     }
-    g = warp_sum(g), u = warp_sum(u);
-    if (lane == 0) p.h[int64_t(slot) * p.f + j] = from_f32<BF16>(p.weights[slot] * (g / (1.0f + expf(-g))) * u);
+    if (lane == 31) h.before[w] = upto;
+    ptx::named_barrier(1, 128);
+    int at = upto - mine, total = 0;
+    for (int i = 0; i < 4; i++) {
+        if (i < w) at += h.before[i];
+        total += h.before[i];
+    }
+    for (int j = 0; j < 4; j++)
+        if (h.who[4 * t + j] != 0ull) h.expert[at++] = 4 * t + j;
+    if (t == 0) h.active = total;
+    ptx::named_barrier(1, 128);
 }
 
-template <bool BF16>
-__global__ void down_simple(const MoeParams p) {
-    const int t = blockIdx.y, lane = threadIdx.x & 31;
-    const int j = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (j >= p.d) return;
-    float acc = 0.0f;
-    for (int s = t * p.top; s < (t + 1) * p.top; s++) {
-        const int64_t row = (int64_t(p.ids[s]) * p.d + j) * p.f;
-        for (int l = lane; l < p.f; l += 32) acc = fmaf(to_f32<BF16>(p.dn[row + l]), to_f32<BF16>(p.h[int64_t(s) * p.f + l]), acc);
+constexpr int MOE_THREADS = 192, MOE_MAX_STAGES = 16;
+constexpr uint32_t MOE_SMEM = 227 * 1024;
+
+// ---- up ---------------------------------------------------------------------------
+// The rows of the chosen experts' gate and up weights, eight of each to a group, are dealt out evenly over the CTAs;
+// a CTA takes its range in chunks of up to sixteen groups of one expert.  A chunk's MMA has N = 16 columns per group:
+// eight gate, eight up, so that a thread of the epilogue (a token) finds both of each pair in its registers.
+//   warp 0  TMA: per stage a block of X (64 of k) and 2 x 8 rows of the weights per group.
+//   warp 1  MMA, two accumulators in turn.   warps 2-5  epilogue: silu, product, routing weight, rounding.
+constexpr int UP_GROUPS = 16;
+
+// Calls f(expert's place in the list, first group, groups) for every chunk of this CTA; f returns false to stop.
+template <typename F>
+__device__ __forceinline__ void up_chunks(const MoeHead &h, const MoeParams &p, F f) {
+    const int per = p.f / 8;
+    const int64_t all = int64_t(h.active) * per;
+    int64_t g = all * blockIdx.x / gridDim.x;
+    const int64_t end = all * (blockIdx.x + 1) / gridDim.x;
+    while (g < end) {
+        const int a = int(g / per), g0 = int(g - int64_t(a) * per);
+        const int piece = int(min(end - g, int64_t(per - g0))), chunks = (piece + UP_GROUPS - 1) / UP_GROUPS;
+        for (int c = 0; c < chunks; c++) {
+            const int lo = piece * c / chunks, hi = piece * (c + 1) / chunks;
+            if (!f(a, g0 + lo, hi - lo)) return;
+        }
+        g += piece;
     }
-    acc = warp_sum(acc);
-    if (lane == 0) p.y[int64_t(t) * p.d + j] = from_f32<BF16>(acc);
 }
+
+__global__ void __launch_bounds__(MOE_THREADS, 1)
+    moe_up_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmU,
+                  const MoeParams p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    MoeHead &h = *reinterpret_cast<MoeHead *>(smem_raw + (base - raw));
+    const uint32_t ring = base + MOE_HEAD, x_bytes = uint32_t(p.token_rows) * 128u;
+    auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
+    volatile uint32_t *abort_flag = &h.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k_blocks = (p.d + 63) / 64;
+    const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            ptx::mbar_init(bar(h.full[s]), 1);
+            ptx::mbar_init(bar(h.empty[s]), 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            ptx::mbar_init(bar(h.tfull[b]), 1);
+            ptx::mbar_init(bar(h.tempty[b]), 4);
+        }
+        ptx::mbar_init(bar(h.plan), 1);
+        ptx::mbar_init(bar(h.drain), 1);
+        h.abort = 0u;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), 512);
+        ptx::tmem_relinquish<1>();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&h.tmem);
+    ptx::griddep_wait();
+    if (threadIdx.x == 0) ptx::griddep_launch_dependents();
+
+    if (warp == 0) {
+        int s = 0;
+        uint32_t ph = 0, filled = 0, filled_parity = 0;
+        bool ok = !(p.debug & 4) && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok)
+            up_chunks(h, p, [&](int a, int g0, int groups) {
+                const int row = h.expert[a] * p.f + 8 * g0;
+                for (int kb = 0; kb < k_blocks; kb++) {
+                    ok = wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) return false;
+                    const uint32_t dst = ring + uint32_t(s) * p.stage_bytes, full = bar(h.full[s]);
+                    if (lane == 0) {
+                        ptx::mbar_arrive_expect_tx(full, x_bytes + uint32_t(groups) * 2048u);
+                        ptx::tma_load_2d(dst, &tmX, full, kb * 64, 0);
+                    }
+                    __syncwarp();
+                    // A lane per box of eight rows: gate rows of group l to lane l, up rows to lane 16 + l.
+                    const int l = lane & 15;
+                    if (l < groups) ptx::tma_load_2d(dst + x_bytes + uint32_t(l) * 2048u + (lane >> 4) * 1024u, lane >> 4 ? &tmU : &tmG, full, kb * 64, row + 8 * l);
+                    __syncwarp();
+                    filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
+                    if (++s == p.stages) s = 0, ph ^= 1u;
+                }
+                return true;
+            });
+        if (!ok && lane == 0) {  // giving up: let the copies in flight land (bounded)
+            const uint64_t t0 = ptx::globaltimer_ns();
+            for (int i = 0; i < p.stages; i++)
+                while ((filled >> i & 1u) && !ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int s = 0, it = 0;
+            uint32_t ph = 0;
+            bool ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit), issued = false;
+            if (ok)
+                up_chunks(h, p, [&](int, int, int groups) {
+                    const int buf = it & 1;
+                    const uint32_t idesc = make_idesc(p.bf16, 128, 16 * groups), d = tmem + uint32_t(buf) * 256u;
+                    if (!(ok = wait_bar(bar(h.tempty[buf]), (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf), limit))) return false;
+                    ptx::tc_fence_after();
+                    for (int kb = 0; kb < k_blocks; kb++) {
+                        if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) return false;
+                        ptx::tc_fence_after();
+                        const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+                        const uint64_t a = sw128_desc(src), b = sw128_desc(src + x_bytes);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) ptx::umma_f16<1>(d, a + 2u * j, b + 2u * j, idesc, (kb > 0 || j > 0) ? 1u : 0u);
+                        issued = true;
+                        ptx::umma_commit<1>(bar(h.empty[s]));
+                        if (++s == p.stages) s = 0, ph ^= 1u;
+                    }
+                    ptx::umma_commit<1>(bar(h.tfull[buf]));
+                    it++;
+                    return true;
+                });
+            if (!ok && issued) {
+                ptx::umma_commit<1>(bar(h.drain));
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while (!ptx::mbar_try_wait(bar(h.drain), 0u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        find_active(h, p, threadIdx.x - 64);
+        if (threadIdx.x == 64) ptx::mbar_arrive(bar(h.plan));
+        const int q = warp & 3, token = 32 * q + lane;
+        int it = 0;
+        up_chunks(h, p, [&](int a, int g0, int groups) {
+            const int buf = it & 1;
+            const bool ok = wait_bar(bar(h.tfull[buf]), uint32_t(it >> 1) & 1u, abort_flag, p.status, WHERE_EPILOGUE, uint32_t(buf), limit);
+            if (!__all_sync(0xffffffffu, ok)) return false;
+            ptx::tc_fence_after();
+            const int e = h.expert[a];
+            const unsigned long long who = h.who[e];
+            if (q < 2 && uint32_t(who >> (32 * q)) != 0u) {
+                const bool mine = (who >> token) & 1ull;
+                float weight = 0.0f;
+                if (mine)
+                    for (int i = 0; i < p.top; i++)
+                        if (h.ids[token * p.top + i] == e) weight = h.weights[token * p.top + i];
+                uint16_t *out = p.h + (int64_t(a) * p.token_rows + token) * p.f + 8 * g0;
+                for (int g = 0; g < groups; g++) {
+                    uint32_t v[16];
+                    ptx::tmem_ld_32x16(tmem + (uint32_t(32 * q) << 16) + uint32_t(256 * buf + 16 * g), v);
+                    ptx::tmem_ld_wait_all();
+                    ptx::pin16(v);
+                    float o[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float gate = __uint_as_float(v[j]), up = __uint_as_float(v[8 + j]);
+                        o[j] = weight * (gate / (1.0f + expf(-gate))) * up;
+                    }
+                    // Rounded once, to the operands' type: the last product runs on 16-bit tensor-core operands.
+                    if (mine)
+                        *reinterpret_cast<uint4 *>(out + 8 * g) = make_uint4(pack_16(o[0], o[1], p.bf16), pack_16(o[2], o[3], p.bf16),
+                                                                            pack_16(o[4], o[5], p.bf16), pack_16(o[6], o[7], p.bf16));
+                }
+            }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(h.tempty[buf]));
+            it++;
+            return true;
+        });
+        __syncwarp();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, 512);
+}
+
+// ---- down -------------------------------------------------------------------------
+// A tile of bn columns of Y; the k of its product runs over all the chosen experts, f each, shared by a cluster of kc
+// CTAs.  An expert's MMAs are masked to the lanes of the tokens that chose it, so the accumulator, which starts
+// from zeros, is the sum over the experts.  The weights do not depend on the kernel before (which has waited for the
+// router): the first ring-full is loaded before griddepcontrol.wait, the h it is multiplied by after.
+__global__ void __launch_bounds__(MOE_THREADS, 1)
+    moe_down_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmD, const MoeParams p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    MoeHead &h = *reinterpret_cast<MoeHead *>(smem_raw + (base - raw));
+    const uint32_t ring = base + MOE_HEAD, h_bytes = uint32_t(p.token_rows) * 128u;
+    auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
+    volatile uint32_t *abort_flag = &h.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, f_blocks = (p.f + 63) / 64;
+    const uint32_t rank = p.kc > 1 ? ptx::cluster_ctarank() : 0u;
+    const int n0 = int(blockIdx.x) / p.kc * p.bn;
+    const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            ptx::mbar_init(bar(h.full[s]), 1);
+            ptx::mbar_init(bar(h.empty[s]), 1);
+        }
+        ptx::mbar_init(bar(h.plan), 1);
+        ptx::mbar_init(bar(h.done), 1);
+        ptx::mbar_init(bar(h.drain), 1);
+        h.abort = 0u;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), p.tmem_cols);
+        ptx::tmem_relinquish<1>();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&h.tmem);
+    if (threadIdx.x == 0) ptx::griddep_launch_dependents();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            ptx::prefetch_tensormap(&tmH);
+            ptx::prefetch_tensormap(&tmD);
+            bool ok = !(p.debug & 4) && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit);
+            uint32_t filled = 0, filled_parity = 0;
+            if (ok) {
+                const int64_t all = int64_t(h.active) * f_blocks;
+                const int i0 = int(all * rank / p.kc), i1 = int(all * (rank + 1) / p.kc), ahead = min(i1 - i0, p.stages);
+                const uint32_t bytes = h_bytes + uint32_t(p.bn) * 128u;
+                auto weights = [&](int i, int s) {
+                    const int a = i / f_blocks, kb = i - a * f_blocks;
+                    ptx::mbar_arrive_expect_tx(bar(h.full[s]), bytes);
+                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes + h_bytes, &tmD, bar(h.full[s]), kb * 64, h.expert[a] * p.d + n0);
+                };
+                auto rows = [&](int i, int s) {
+                    const int a = i / f_blocks, kb = i - a * f_blocks;
+                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes, &tmH, bar(h.full[s]), kb * 64, a * p.token_rows);
+                };
+                for (int i = 0; i < ahead; i++) weights(i0 + i, i);
+                ptx::griddep_wait();
+                for (int i = 0; i < ahead; i++) rows(i0 + i, i);
+                filled = ahead >= 32 ? 0xffffffffu : (1u << ahead) - 1u;
+                int s = ahead == p.stages ? 0 : ahead;
+                uint32_t ph = ahead == p.stages ? 1u : 0u;
+                for (int i = i0 + ahead; i < i1; i++) {
+                    if (!(ok = wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit))) break;
+                    weights(i, s);
+                    rows(i, s);
+                    filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
+                    if (++s == p.stages) s = 0, ph ^= 1u;
+                }
+            } else {
+                ptx::griddep_wait();
+            }
+            if (!ok) {
+                const uint64_t t0 = ptx::globaltimer_ns();
+                for (int i = 0; i < p.stages; i++)
+                    while ((filled >> i & 1u) && !ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
+                        if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            bool ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit), issued = false;
+            ptx::tc_fence_after();  // the zeros in the accumulator
+            const int64_t all = ok ? int64_t(h.active) * f_blocks : 0;
+            const int i0 = int(all * rank / p.kc), i1 = int(all * (rank + 1) / p.kc);
+            const uint32_t idesc = make_idesc(p.bf16, 128, p.bn);
+            int s = 0;
+            uint32_t ph = 0;
+            for (int i = i0; i < i1; i++) {
+                const unsigned long long who = h.who[h.expert[i / f_blocks]];
+                if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) break;
+                ptx::tc_fence_after();
+                const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+                const uint64_t a = sw128_desc(src), b = sw128_desc(src + h_bytes);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * j, idesc, 1u, ~uint32_t(who), ~uint32_t(who >> 32), 0xffffffffu, 0xffffffffu);
+                issued = true;
+                ptx::umma_commit<1>(bar(h.empty[s]));
+                if (++s == p.stages) s = 0, ph ^= 1u;
+            }
+            if (ok) {
+                ptx::umma_commit<1>(bar(h.done));
+            } else if (issued) {
+                ptx::umma_commit<1>(bar(h.drain));
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while (!ptx::mbar_try_wait(bar(h.drain), 0u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3;
+        const uint32_t lanes = tmem + (uint32_t(32 * q) << 16);
+        if (q < 2) {
+            for (int c = 0; c < p.bn; c += 32) ptx::tmem_zero_32x32(lanes + uint32_t(c));
+            ptx::tc_fence_before();
+        }
+        find_active(h, p, threadIdx.x - 64);  // ends with a barrier of these warps: the zeros are in place
+        if (threadIdx.x == 64) ptx::mbar_arrive(bar(h.plan));
+        const bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.done), 0, abort_flag, p.status, WHERE_EPILOGUE, 0u, limit));
+        const uint32_t pitch = uint32_t(p.bn + 4) * 4u;
+        if (ok && 32 * q < p.tokens) {
+            ptx::tc_fence_after();
+            ptx::fence_proxy_async_shared();
+            for (int c = 0; c < p.bn; c += 32) {
+                uint32_t v[32];
+                ptx::tmem_ld_32x32(lanes + uint32_t(c), v);
+                ptx::tmem_ld_wait(v);
+                if (32 * q + lane < p.tokens) {
+                    const uint32_t dst = ring + uint32_t(32 * q + lane) * pitch + uint32_t(c) * 4u;
+#pragma unroll
+                    for (int g = 0; g < 8; g++)
+                        if (c + 4 * g < p.bn) ptx::st_shared_v4(dst + 16u * g, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+                }
+            }
+        }
+        ptx::griddep_wait();  // Y is written below: nothing of an earlier kernel may still read it
+        __syncwarp();
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (p.kc > 1) {
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    if (!*abort_flag) {
+        const int quads = p.bn / 4, items = p.tokens * quads;
+        const uint32_t pitch = uint32_t(p.bn + 4) * 4u;
+        for (int i = int(rank) * MOE_THREADS + int(threadIdx.x); i < items; i += p.kc * MOE_THREADS) {
+            const int row = i / quads, col = (i - row * quads) * 4;
+            const uint32_t at = ring + uint32_t(row) * pitch + uint32_t(col) * 4u;
+            float4 v = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(at, 0) : at);
+            for (int c = 1; c < p.kc; c++) {
+                const float4 o = ptx::ld_shared_cluster_v4(ptx::mapa(at, uint32_t(c)));
+                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+            }
+            if (n0 + col < p.d)  // d is a multiple of 8: four columns are in or out together
+                *reinterpret_cast<uint2 *>(p.y + int64_t(row) * p.d + n0 + col) = make_uint2(pack_16(v.x, v.y, p.bf16), pack_16(v.z, v.w, p.bf16));
+        }
+    }
+    __syncthreads();
+    if (p.kc > 1) {
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, p.tmem_cols);
+}
+
+int g_down_clusters[64][4];
 
 constexpr uint64_t kAlign = 256;
 uint64_t round_up(uint64_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
@@ -133,28 +548,26 @@ cute_b200_status check_desc(const cute_b200_moe_desc &d, const char *who) {
     return CUTE_B200_OK;
 }
 
+int token_rows(const cute_b200_moe_desc &d) { return (d.tokens + 7) / 8 * 8; }
+int most_active(const cute_b200_moe_desc &d) { return d.experts < d.tokens * d.top ? d.experts : d.tokens * d.top; }
+
 struct Layout {
-    uint64_t logits, ids, weights, h, total;
+    uint64_t ids, weights, h, total;
 };
 Layout layout(const cute_b200_moe_desc &d) {
     Layout l;
-    l.logits = 0;
-    l.ids = l.logits + round_up(uint64_t(d.tokens) * d.experts * 4);
+    l.ids = 0;
     l.weights = l.ids + round_up(uint64_t(d.tokens) * d.top * 4);
     l.h = l.weights + round_up(uint64_t(d.tokens) * d.top * 4);
-    l.total = l.h + round_up(uint64_t(d.tokens) * d.top * d.f * 2) + kAlign;
+    l.total = l.h + round_up(uint64_t(most_active(d)) * token_rows(d) * d.f * 2) + kAlign;
     return l;
 }
 
-template <bool BF16>
-cute_b200_status run(const MoeParams &p, cudaStream_t stream) {
-    logits_simple<BF16><<<dim3(unsigned(p.experts), unsigned(p.tokens)), 32, 0, stream>>>(p);
-    top_simple<<<p.tokens, 32, 0, stream>>>(p);
-    up_simple<BF16><<<dim3(unsigned((p.f + 7) / 8), unsigned(p.tokens * p.top)), 256, 0, stream>>>(p);
-    down_simple<BF16><<<dim3(unsigned((p.d + 7) / 8), unsigned(p.tokens)), 256, 0, stream>>>(p);
-    CB_CUDA(cudaGetLastError());
-    count_launch(4);
-    return CUTE_B200_OK;
+// Stages of `bytes` behind the head; an MMA reads 128 rows of 128 bytes from a stage's start.
+int ring_stages(uint32_t bytes) {
+    const uint32_t ring = MOE_SMEM - MOE_HEAD - 1024, over = bytes < 16384 ? 16384 - bytes : 0;
+    const int stages = int((ring - over) / bytes);
+    return stages < MOE_MAX_STAGES ? stages : MOE_MAX_STAGES;
 }
 
 }  // namespace
@@ -178,24 +591,54 @@ cute_b200_status moe_tn_check(const cute_b200_moe_desc &d, const uint64_t ptr[7]
     return CUTE_B200_OK;
 }
 
-cute_b200_status moe_tn(const cute_b200_moe_desc &d, const uint64_t ptr[7], cudaStream_t stream, const DeviceState &) {
+cute_b200_status moe_tn(const cute_b200_moe_desc &d, const uint64_t ptr[7], cudaStream_t stream, const DeviceState &dev) {
     if (d.tokens == 0) return CUTE_B200_OK;
     const Layout l = layout(d);
+    int device = 0;
+    CB_CUDA(cudaGetDevice(&device));
     MoeParams p = {};
     p.x = reinterpret_cast<const uint16_t *>(ptr[0]);
     p.r = reinterpret_cast<const uint16_t *>(ptr[1]);
-    p.g = reinterpret_cast<const uint16_t *>(ptr[2]);
-    p.u = reinterpret_cast<const uint16_t *>(ptr[3]);
-    p.dn = reinterpret_cast<const uint16_t *>(ptr[4]);
     p.y = reinterpret_cast<uint16_t *>(ptr[5]);
-    p.logits = reinterpret_cast<float *>(ptr[6] + l.logits);
     p.ids = reinterpret_cast<int32_t *>(ptr[6] + l.ids);
     p.weights = reinterpret_cast<float *>(ptr[6] + l.weights);
     p.h = reinterpret_cast<uint16_t *>(ptr[6] + l.h);
-    p.tokens = d.tokens, p.experts = d.experts, p.top = d.top, p.d = d.d, p.f = d.f, p.renorm = d.renormalise;
-    return d.dtype == CUTE_B200_BF16 ? run<true>(p, stream) : run<false>(p, stream);
+    p.tokens = d.tokens, p.token_rows = token_rows(d), p.experts = d.experts, p.top = d.top, p.d = d.d, p.f = d.f, p.renorm = d.renormalise;
+    p.bf16 = d.dtype == CUTE_B200_BF16;
+    p.status = dev.status_word;
+    p.debug = d.tuning[1];
+
+    const dim3 groups(unsigned((d.tokens + ROUTER_TOKENS - 1) / ROUTER_TOKENS * ROUTER_CLUSTER));
+    CB_TRY(launch_dependent(p.bf16 ? moe_router_kernel<true> : moe_router_kernel<false>, groups, ROUTER_THREADS, 0, ROUTER_CLUSTER, stream, p));
+
+    CUtensorMap tmX, tmG, tmU, tmH, tmD;
+    CB_TRY(rows_tensor_map(&tmX, ptr[0], p.bf16, d.tokens, d.d, d.d, p.token_rows));
+    CB_TRY(rows_tensor_map(&tmG, ptr[2], p.bf16, uint64_t(d.experts) * d.f, d.d, d.d, 8));
+    CB_TRY(rows_tensor_map(&tmU, ptr[3], p.bf16, uint64_t(d.experts) * d.f, d.d, d.d, 8));
+    p.stage_bytes = uint32_t(p.token_rows + 16 * UP_GROUPS) * 128u;
+    p.stages = ring_stages(p.stage_bytes);
+    CB_TRY(launch_dependent(moe_up_kernel, dim3(unsigned(dev.sm_count)), MOE_THREADS, MOE_SMEM, 1, stream, tmX, tmG, tmU, p));
+
+    p.bn = 16, p.kc = 1;
+    const int f_blocks = (d.f + 63) / 64, expected = most_active(d);
+    int fits[4];
+    for (int c = 0; c < 4; c++) fits[c] = (1 << c) <= f_blocks ? g_down_clusters[device][c] : 0;  // every CTA has a block of one expert at least
+    stream_cut(d.d, f_blocks * expected, fits, &p.bn, &p.kc);
+    p.stage_bytes = uint32_t(p.token_rows + p.bn) * 128u;
+    p.stages = ring_stages(p.stage_bytes);
+    p.tmem_cols = p.bn <= 32 ? 32 : (p.bn <= 64 ? 64 : (p.bn <= 128 ? 128 : 256));
+    CB_TRY(rows_tensor_map(&tmH, ptr[6] + l.h, p.bf16, uint64_t(expected) * p.token_rows, d.f, d.f, p.token_rows));
+    CB_TRY(rows_tensor_map(&tmD, ptr[4], p.bf16, uint64_t(d.experts) * d.d, d.f, d.f, p.bn));
+    return launch_dependent(moe_down_kernel, dim3(unsigned((d.d + p.bn - 1) / p.bn * p.kc)), MOE_THREADS, MOE_SMEM, p.kc, stream, tmH, tmD, p);
 }
 
-cute_b200_status moe_init(const DeviceState &) { return CUTE_B200_OK; }
+cute_b200_status moe_init(const DeviceState &) {
+    int device = 0;
+    CB_CUDA(cudaGetDevice(&device));
+    CB_CUDA(cudaFuncSetAttribute(moe_up_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOE_SMEM));
+    CB_CUDA(cudaFuncSetAttribute(moe_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOE_SMEM));
+    for (int c = 0; c < 4; c++) CB_TRY(max_clusters(moe_down_kernel, MOE_THREADS, MOE_SMEM, 1 << c, &g_down_clusters[device][c]));
+    return CUTE_B200_OK;
+}
 
 }  // namespace cb

@@ -101,5 +101,25 @@ cute_b200_status max_clusters(void (*kernel)(P...), int threads, size_t smem, in
     return CUTE_B200_OK;
 }
 
+// How a product that streams an (n, k) weight past a few rows is cut: bn rows of the weight per tile, a cluster of kc CTAs per tile.  The launch is one wave
+// where it can be; the cut with the least time for the slowest CTA wins.  A CTA streams at most what an even share of
+// HBM gives it, and no faster than its MMAs take (four per k block, a fixed ~60 clocks or bn / 2 each).
+inline void stream_cut(int n, int k_blocks, const int (&max_clusters)[4], int *bn, int *kc) {
+    double best = 1e300;
+    for (int c = 0; c < 4; c++) {
+        const int parts = 1 << c, ctas_at_once = max_clusters[c] * parts;
+        if (parts > k_blocks || max_clusters[c] < 1) continue;
+        for (int b = 16; b <= 256; b += 16) {
+            const int64_t ctas = int64_t((n + b - 1) / b) * parts;
+            const int64_t waves = (ctas + ctas_at_once - 1) / ctas_at_once;
+            const double share = 6.5e12 / double(ctas < ctas_at_once ? ctas : ctas_at_once);
+            const double rate = share < 7.0e10 ? share : 7.0e10;
+            const double load = b * 128.0 / rate, math = 4.0 * (b / 2 > 60 ? b / 2 : 60) / 1.7e9;
+            const double t = double(waves) * (((k_blocks + parts - 1) / parts) * (load > math ? load : math) + 2.0e-6) + (parts > 1 ? 1.0e-6 : 0.0);
+            if (t < best * 0.999) best = t, *bn = b, *kc = parts;
+        }
+    }
+}
+
 }  // namespace
 }  // namespace cb
