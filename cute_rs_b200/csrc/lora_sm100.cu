@@ -69,11 +69,14 @@ __global__ void __launch_bounds__(SHRINK_THREADS) shrink_rows_kernel(const LoraP
 // shares a tile's k blocks and, after them, the adapters its rows name, and adds
 // its partial sums through shared memory.  Bound by HBM: every byte of W is
 // read once, the ring keeps ~190 KB of it in flight per SM.
-//   warp 0  TMA: per stage a (xr x 64) block of X and a (bn x 64) block of W;
-//           then, per adapter, blocks of T and of B[a].
+//   warp 0  TMA: per stage `kps` k blocks, each (xr x 64) of X and (bn x 64) of W;
+//           then T, once, and per adapter blocks of B[a].  A stage costs the
+//           issuing warp about 0.3 us whatever it holds (measured: 32 x 64 blocks, one per
+//           stage, stream at 1.9 TB/s, four per stage at 4.4 when lanes issue side by side),
+//           so a stage is made to hold about 28 KB and every block is another lane's.
 //   warp 1  MMA: M 128, N bn.  The MMA always reads 128 rows of X; those past
-//           the loaded xr rows are whatever lies behind them in the ring (in
-//           bounds, see few_smem), and end up in lanes that nothing reads.  An
+//           the loaded xr rows are whatever lies behind them in shared memory (in
+//           bounds, see forward_few), and end up in lanes that nothing reads.  An
 //           adapter's product is masked to the lanes of the rows that name it,
 //           so that nothing of it reaches another row.
 //   warps 2-5  which adapters the rows name, while the weights stream; then
@@ -89,14 +92,14 @@ struct FewParams {
     void *y;
     int64_t ldy;
     int m, n, rank, rp, adapters, c_dtype, vec;
-    int k_blocks, bn, kc, xr, stages;
-    uint32_t stage_bytes, w_offset, idesc, tmem_cols;
+    int k_blocks, bn, kc, xr, stages, kps;
+    uint32_t stage_bytes, x_bytes, w_bytes, idesc, tmem_cols;
     uint32_t *status;
     int debug;
 };
 
 struct FewHead {
-    uint64_t full[FEW_MAX_STAGES], empty[FEW_MAX_STAGES], plan, done, drain;
+    uint64_t full[FEW_MAX_STAGES], empty[FEW_MAX_STAGES], low, plan, done, drain;
     uint32_t tmem, abort;
     int32_t entries, entry_id[FEW_ROWS];
     uint32_t off[FEW_ROWS][4];  // lanes of entry e that keep their sums: bit set = not a row of this adapter
@@ -110,7 +113,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     FewHead &h = *reinterpret_cast<FewHead *>(smem_raw + (base - raw));
-    const uint32_t ring = base + FEW_HEAD;
+    const int q_blocks = ext_blocks(p.rp);
+    const uint32_t low = base + FEW_HEAD, ring = low + uint32_t(q_blocks) * p.x_bytes;  // T's blocks, then the ring
     auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
     volatile uint32_t *abort_flag = &h.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -124,6 +128,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             ptx::mbar_init(bar(h.full[s]), 1);
             ptx::mbar_init(bar(h.empty[s]), 1);
         }
+        ptx::mbar_init(bar(h.low), 1);
         ptx::mbar_init(bar(h.plan), 1);
         ptx::mbar_init(bar(h.done), 1);
         ptx::mbar_init(bar(h.drain), 1);
@@ -138,47 +143,62 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&h.tmem);
-    const int q_blocks = ext_blocks(p.rp);
     if (threadIdx.x == 0) ptx::griddep_launch_dependents();
 
     if (warp == 0) {
-        if (lane == 0) {
-            ptx::prefetch_tensormap(&tmX);
-            ptx::prefetch_tensormap(&tmW);
-            ptx::prefetch_tensormap(&tmT);
-            ptx::prefetch_tensormap(&tmB);
-            int s = 0;
-            uint32_t ph = 0, filled = 0, filled_parity = 0;
-            const uint32_t bytes = uint32_t(p.xr + p.bn) * 128u;
-            bool ok = !(p.debug & 4);
-            auto load = [&](const CUtensorMap *rows, int rx, const CUtensorMap *weights, int wx, int wy) {
-                if (!wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit)) return false;
-                const uint32_t dst = ring + uint32_t(s) * p.stage_bytes;
-                ptx::mbar_arrive_expect_tx(bar(h.full[s]), bytes);
-                ptx::tma_load_2d(dst + p.w_offset, weights, bar(h.full[s]), wx, wy);
-                ptx::tma_load_2d(dst, rows, bar(h.full[s]), rx, 0);
-                filled |= 1u << s;
-                filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
-                if (++s == p.stages) s = 0, ph ^= 1u;
-                return true;
-            };
-            for (int kb = kb0; kb < kb1 && ok; kb++) ok = load(&tmX, kb * 64, &tmW, kb * 64, n0);
-            if (ok) {
-                ptx::griddep_wait();
-                ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit);
+        int s = 0;
+        uint32_t ph = 0, filled = 0, filled_parity = 0;
+        bool ok = !(p.debug & 4);
+        // Waits for the next stage and announces `bytes`: its address, 0 when giving up.
+        auto next = [&](uint32_t bytes) -> uint32_t {
+            ok = __all_sync(0xffffffffu, wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit));
+            if (!ok) return 0u;
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.full[s]), bytes);
+            __syncwarp();
+            return ring + uint32_t(s) * p.stage_bytes;
+        };
+        auto issued = [&] {
+            __syncwarp();
+            filled |= 1u << s;
+            filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
+            if (++s == p.stages) s = 0, ph ^= 1u;
+        };
+        const uint32_t w0 = uint32_t(p.kps) * p.x_bytes;
+        const int kk = lane & 7;  // lanes 0-7 issue blocks of W, lanes 8-15 of X
+        for (int kb = kb0; kb < kb1 && ok; kb += p.kps) {
+            const int nk = min(p.kps, kb1 - kb);
+            const uint32_t dst = next(uint32_t(nk) * (p.x_bytes + p.w_bytes));
+            if (!ok) break;
+            if (kk < nk && lane < 8) ptx::tma_load_2d(dst + w0 + uint32_t(kk) * p.w_bytes, &tmW, bar(h.full[s]), (kb + kk) * 64, n0);
+            if (kk < nk && lane >= 8 && lane < 16) ptx::tma_load_2d(dst + uint32_t(kk) * p.x_bytes, &tmX, bar(h.full[s]), (kb + kk) * 64, 0);
+            issued();
+        }
+        ptx::griddep_wait();
+        ok = __all_sync(0xffffffffu, ok && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit));
+        const int mine = ok && h.entries > int(rank) ? (h.entries - int(rank) + p.kc - 1) / p.kc * q_blocks : 0;  // blocks of B
+        const bool has_low = mine > 0;
+        if (has_low) {
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.low), uint32_t(q_blocks) * p.x_bytes);
+            __syncwarp();
+            if (lane < q_blocks) ptx::tma_load_2d(low + uint32_t(lane) * p.x_bytes, &tmT, bar(h.low), ext_block(lane, p.rp, p.rank).t_col, 0);
+        }
+        for (int i = 0; i < mine && ok; i += p.kps) {
+            const int nk = min(p.kps, mine - i);
+            const uint32_t dst = next(uint32_t(nk) * p.w_bytes);
+            if (!ok) break;
+            if (lane < nk) {
+                const int e = int(rank) + (i + lane) / q_blocks * p.kc, q = (i + lane) % q_blocks;
+                ptx::tma_load_2d(dst + w0 + uint32_t(lane) * p.w_bytes, &tmB, bar(h.full[s]), ext_block(q, p.rp, p.rank).b_col, h.entry_id[e] * p.n + n0);
             }
-            for (int e = int(rank); ok && e < h.entries; e += p.kc)
-                for (int q = 0; q < q_blocks && ok; q++) {
-                    const ExtBlock b = ext_block(q, p.rp, p.rank);
-                    if (b.steps > 0) ok = load(&tmT, b.t_col, &tmB, b.b_col, h.entry_id[e] * p.n + n0);
-                }
-            if (!ok)  // giving up: let the copies in flight land (bounded) before the shared memory is handed back
-                for (int i = 0; i < p.stages; i++)
-                    if (filled & (1u << i)) {
-                        const uint64_t t0 = ptx::globaltimer_ns();
-                        while (!ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
-                            if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
-                    }
+            issued();
+        }
+        if (!ok && lane == 0) {  // giving up: let the copies in flight land (bounded) before the shared memory is handed back
+            const uint64_t t0 = ptx::globaltimer_ns();
+            for (int i = 0; i < p.stages; i++)
+                while ((filled >> i & 1u) && !ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+            while (has_low && !ptx::mbar_try_wait(bar(h.low), 0u))
+                if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -186,6 +206,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             int s = 0;
             uint32_t ph = 0;
             bool ok = true, issued = false;
+            const uint32_t w0 = uint32_t(p.kps) * p.x_bytes;
             auto ready = [&] {
                 if (!wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit)) return false;
                 ptx::tc_fence_after();
@@ -196,27 +217,33 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
                 ptx::umma_commit<1>(bar(h.empty[s]));
                 if (++s == p.stages) s = 0, ph ^= 1u;
             };
-            for (int kb = kb0; kb < kb1; kb++) {
+            for (int kb = kb0; kb < kb1; kb += p.kps) {
                 if (!(ok = ready())) break;
                 const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                const uint64_t a = sw128_desc(src), b = sw128_desc(src + p.w_offset);
+                const int nk = min(p.kps, kb1 - kb);
+                for (int kk = 0; kk < nk; kk++) {
+                    const uint64_t a = sw128_desc(src + uint32_t(kk) * p.x_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
 #pragma unroll
-                for (int j = 0; j < 4; j++) ptx::umma_f16<1>(tmem, a + 2u * j, b + 2u * j, p.idesc, (kb > kb0 || j > 0) ? 1u : 0u);
+                    for (int j = 0; j < 4; j++) ptx::umma_f16<1>(tmem, a + 2u * j, b + 2u * j, p.idesc, (kb > kb0 || kk > 0 || j > 0) ? 1u : 0u);
+                }
                 free_stage();
             }
             if (ok) ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit);
-            for (int e = int(rank); ok && e < h.entries; e += p.kc) {
-                const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
-                for (int q = 0; q < q_blocks; q++) {
+            const int mine = ok && h.entries > int(rank) ? (h.entries - int(rank) + p.kc - 1) / p.kc * q_blocks : 0;
+            if (mine > 0) ok = wait_bar(bar(h.low), 0, abort_flag, p.status, WHERE_MMA_FULL, 101u, limit);
+            for (int i = 0; i < mine && ok; i += p.kps) {
+                if (!(ok = ready())) break;
+                const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+                const int nk = min(p.kps, mine - i);
+                for (int kk = 0; kk < nk; kk++) {
+                    const int e = int(rank) + (i + kk) / q_blocks * p.kc, q = (i + kk) % q_blocks;
                     const ExtBlock x = ext_block(q, p.rp, p.rank);
-                    if (x.steps <= 0) continue;
-                    if (!(ok = ready())) break;
-                    const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                    const uint64_t a = sw128_desc(src), b = sw128_desc(src + p.w_offset);
+                    const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
+                    const uint64_t a = sw128_desc(low + uint32_t(q) * p.x_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
                     for (int j = 0; j < x.steps; j++)
                         ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * (j & x.b_mask), p.idesc, 1u, o0, o1, o2, o3);
-                    free_stage();
                 }
+                free_stage();
             }
             if (ok) {
                 ptx::umma_commit<1>(bar(h.done));
@@ -343,11 +370,13 @@ cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int de
     CB_CUDA(cudaGetDevice(&device));
     stream_cut(p.n, (p.k + 63) / 64, g_few_clusters[device], &f.bn, &f.kc);
     f.xr = (p.m + 7) / 8 * 8;
-    f.w_offset = uint32_t(f.xr) * 128u;
-    f.stage_bytes = uint32_t(f.xr + f.bn) * 128u;
-    // The head, the ring, and behind the last stage as much as an MMA reads past its rows of X.
-    const uint32_t ring = FEW_SMEM - FEW_HEAD - 1024;
-    const uint32_t over = f.stage_bytes < 16384 ? 16384 - f.stage_bytes : 0;
+    f.x_bytes = uint32_t(f.xr) * 128u;
+    f.w_bytes = uint32_t(f.bn) * 128u;
+    // The head, T, the ring, and behind the last stage as much as an MMA reads past its rows of X.
+    const uint32_t ring = FEW_SMEM - FEW_HEAD - 1024 - uint32_t(ext_blocks(p.rp)) * f.x_bytes;
+    f.kps = stream_blocks(f.bn, f.xr, ring);
+    f.stage_bytes = uint32_t(f.kps) * (f.x_bytes + f.w_bytes);
+    const uint32_t reach = uint32_t(f.kps - 1) * f.x_bytes + 16384, over = f.stage_bytes < reach ? reach - f.stage_bytes : 0;
     f.stages = int((ring - over) / f.stage_bytes);
     if (f.stages > FEW_MAX_STAGES) f.stages = FEW_MAX_STAGES;
     f.idesc = make_idesc(BF16, 128, f.bn);

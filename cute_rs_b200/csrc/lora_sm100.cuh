@@ -53,7 +53,7 @@ __host__ __device__ constexpr int padded_rank(int rank) { return rank <= 16 ? 16
 struct ExtBlock {
     int t_col, b_col, steps, b_mask;
 };
-__device__ __forceinline__ int ext_blocks(int rp) { return rp <= 32 ? 1 : rp / 32; }
+__host__ __device__ __forceinline__ int ext_blocks(int rp) { return rp <= 32 ? 1 : rp / 32; }
 __device__ __forceinline__ ExtBlock ext_block(int q, int rp, int rank) {
     if (rp <= 32) return {0, 0, rp / 8, rp / 16 - 1};
     const int half = q >> 1, left = (rank - 64 * half + 15) / 16;  // at least 1: rank > rp / 2

@@ -19,7 +19,7 @@ struct MoeParams {
     int32_t *ids;     // (tokens, top)
     float *weights;   // (tokens, top)
     int tokens, token_rows, experts, top, d, f, renorm;
-    int kc, bn, stages;
+    int kc, bn, stages, kps;
     uint32_t stage_bytes, tmem_cols;
     bool bf16;
     uint32_t *status;
@@ -176,10 +176,15 @@ constexpr uint32_t MOE_SMEM = 227 * 1024;
 // ---- up ---------------------------------------------------------------------------
 // The rows of the chosen experts' gate and up weights, eight of each to a group, are dealt out evenly over the CTAs;
 // a CTA takes its range in chunks of up to sixteen groups of one expert.  A chunk's MMA has N = 16 columns per group:
-// eight gate, eight up, so that a thread of the epilogue (a token) finds both of each pair in its registers.
-//   warp 0  TMA: per stage a block of X (64 of k) and 2 x 8 rows of the weights per group.
+// first the chunk's gate rows, then its up rows; a thread of the epilogue (a token) reads both of each pair.
+//   warp 0  TMA: per stage one or two k blocks of X and of the weights, 8 g rows of each matrix as boxes of 64, 32, 16
+//           and 8 rows, a lane per box (boxes of 8 rows alone would cap the stream at 4 TB/s, those of 16 at 6.5: measured).
 //   warp 1  MMA, two accumulators in turn.   warps 2-5  epilogue: silu, product, routing weight, rounding.
 constexpr int UP_GROUPS = 16;
+struct UpMaps {
+    CUtensorMap gate[4], up[4];  // boxes of 64, 32, 16 and 8 rows
+};
+__device__ __forceinline__ int up_blocks(int groups) { return groups <= 8 ? 2 : 1; }  // k blocks per stage
 
 // Calls f(expert's place in the list, first group, groups) for every chunk of this CTA; f returns false to stop.
 template <typename F>
@@ -200,8 +205,7 @@ __device__ __forceinline__ void up_chunks(const MoeHead &h, const MoeParams &p, 
 }
 
 __global__ void __launch_bounds__(MOE_THREADS, 1)
-    moe_up_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmU,
-                  const MoeParams p) {
+    moe_up_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ UpMaps maps, const MoeParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     MoeHead &h = *reinterpret_cast<MoeHead *>(smem_raw + (base - raw));
@@ -243,20 +247,26 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (ok)
             up_chunks(h, p, [&](int a, int g0, int groups) {
-                const int row = h.expert[a] * p.f + 8 * g0;
-                for (int kb = 0; kb < k_blocks; kb++) {
+                const int kps = up_blocks(groups), w_bytes = groups * 2048;
+                // Lanes 0-9 and 10-19 issue the boxes of a stage's two k blocks, five per matrix: two of 64 rows, then 32, 16, 8;
+                // lanes 30 and 31 the blocks of X.
+                const int kk = lane < 20 ? lane / 10 : lane & 1, up = lane % 10 / 5, box = lane % 5;
+                const int size = box < 2 ? 64 : 128 >> box;
+                const int off = box < 2 ? 64 * box : (8 * groups) & ~(2 * size - 1);  // the larger boxes lie before it
+                const bool mine = lane < 20 && (box < 2 ? groups >= 8 * (box + 1) : (8 * groups & size) != 0);
+                const CUtensorMap *map = (up ? maps.up : maps.gate) + (box < 2 ? 0 : box - 1);
+                const uint32_t to = uint32_t(kps) * x_bytes + uint32_t(kk * w_bytes + up * groups * 1024 + off * 128);
+                const int row = h.expert[a] * p.f + 8 * g0 + off;
+                for (int kb = 0; kb < k_blocks; kb += kps) {
+                    const int nk = min(kps, k_blocks - kb);
                     ok = wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) return false;
                     const uint32_t dst = ring + uint32_t(s) * p.stage_bytes, full = bar(h.full[s]);
-                    if (lane == 0) {
-                        ptx::mbar_arrive_expect_tx(full, x_bytes + uint32_t(groups) * 2048u);
-                        ptx::tma_load_2d(dst, &tmX, full, kb * 64, 0);
-                    }
+                    if (lane == 0) ptx::mbar_arrive_expect_tx(full, uint32_t(nk) * (x_bytes + uint32_t(w_bytes)));
                     __syncwarp();
-                    // A lane per box of eight rows: gate rows of group l to lane l, up rows to lane 16 + l.
-                    const int l = lane & 15;
-                    if (l < groups) ptx::tma_load_2d(dst + x_bytes + uint32_t(l) * 2048u + (lane >> 4) * 1024u, lane >> 4 ? &tmU : &tmG, full, kb * 64, row + 8 * l);
+                    if (mine && kk < nk) ptx::tma_load_2d(dst + to, map, full, (kb + kk) * 64, row);
+                    if (lane >= 30 && kk < nk) ptx::tma_load_2d(dst + uint32_t(kk) * x_bytes, &tmX, full, (kb + kk) * 64, 0);
                     __syncwarp();
                     filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
                     if (++s == p.stages) s = 0, ph ^= 1u;
@@ -281,13 +291,17 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
                     const uint32_t idesc = make_idesc(p.bf16, 128, 16 * groups), d = tmem + uint32_t(buf) * 256u;
                     if (!(ok = wait_bar(bar(h.tempty[buf]), (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf), limit))) return false;
                     ptx::tc_fence_after();
-                    for (int kb = 0; kb < k_blocks; kb++) {
+                    const int kps = up_blocks(groups);
+                    for (int kb = 0; kb < k_blocks; kb += kps) {
                         if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) return false;
                         ptx::tc_fence_after();
                         const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                        const uint64_t a = sw128_desc(src), b = sw128_desc(src + x_bytes);
+                        const int nk = min(kps, k_blocks - kb);
+                        for (int kk = 0; kk < nk; kk++) {
+                            const uint64_t a = sw128_desc(src + uint32_t(kk) * x_bytes), b = sw128_desc(src + uint32_t(kps) * x_bytes + uint32_t(kk * groups) * 2048u);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) ptx::umma_f16<1>(d, a + 2u * j, b + 2u * j, idesc, (kb > 0 || j > 0) ? 1u : 0u);
+                            for (int j = 0; j < 4; j++) ptx::umma_f16<1>(d, a + 2u * j, b + 2u * j, idesc, (kb > 0 || kk > 0 || j > 0) ? 1u : 0u);
+                        }
                         issued = true;
                         ptx::umma_commit<1>(bar(h.empty[s]));
                         if (++s == p.stages) s = 0, ph ^= 1u;
@@ -324,14 +338,17 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
                         if (h.ids[token * p.top + i] == e) weight = h.weights[token * p.top + i];
                 uint16_t *out = p.h + (int64_t(a) * p.token_rows + token) * p.f + 8 * g0;
                 for (int g = 0; g < groups; g++) {
-                    uint32_t v[16];
-                    ptx::tmem_ld_32x16(tmem + (uint32_t(32 * q) << 16) + uint32_t(256 * buf + 16 * g), v);
+                    uint32_t vg[8], vu[8];
+                    const uint32_t at = tmem + (uint32_t(32 * q) << 16) + uint32_t(256 * buf + 8 * g);
+                    ptx::tmem_ld_32x8(at, vg);
+                    ptx::tmem_ld_32x8(at + uint32_t(8 * groups), vu);
                     ptx::tmem_ld_wait_all();
-                    ptx::pin16(v);
+                    ptx::pin8(vg);
+                    ptx::pin8(vu);
                     float o[8];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const float gate = __uint_as_float(v[j]), up = __uint_as_float(v[8 + j]);
+                        const float gate = __uint_as_float(vg[j]), up = __uint_as_float(vu[j]);
                         o[j] = weight * (gate / (1.0f + expf(-gate))) * up;
                     }
                     // Rounded once, to the operands' type: the last product runs on 16-bit tensor-core operands.
@@ -392,47 +409,55 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&h.tmem);
     if (threadIdx.x == 0) ptx::griddep_launch_dependents();
 
+    const uint32_t w_bytes = uint32_t(p.bn) * 128u, w0 = uint32_t(p.kps) * h_bytes;
     if (warp == 0) {
-        if (lane == 0) {
-            ptx::prefetch_tensormap(&tmH);
-            ptx::prefetch_tensormap(&tmD);
-            bool ok = !(p.debug & 4) && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit);
-            uint32_t filled = 0, filled_parity = 0;
-            if (ok) {
-                const int64_t all = int64_t(h.active) * f_blocks;
-                const int i0 = int(all * rank / p.kc), i1 = int(all * (rank + 1) / p.kc), ahead = min(i1 - i0, p.stages);
-                const uint32_t bytes = h_bytes + uint32_t(p.bn) * 128u;
-                auto weights = [&](int i, int s) {
-                    const int a = i / f_blocks, kb = i - a * f_blocks;
-                    ptx::mbar_arrive_expect_tx(bar(h.full[s]), bytes);
-                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes + h_bytes, &tmD, bar(h.full[s]), kb * 64, h.expert[a] * p.d + n0);
-                };
-                auto rows = [&](int i, int s) {
-                    const int a = i / f_blocks, kb = i - a * f_blocks;
-                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes, &tmH, bar(h.full[s]), kb * 64, a * p.token_rows);
-                };
-                for (int i = 0; i < ahead; i++) weights(i0 + i, i);
-                ptx::griddep_wait();
-                for (int i = 0; i < ahead; i++) rows(i0 + i, i);
-                filled = ahead >= 32 ? 0xffffffffu : (1u << ahead) - 1u;
-                int s = ahead == p.stages ? 0 : ahead;
-                uint32_t ph = ahead == p.stages ? 1u : 0u;
-                for (int i = i0 + ahead; i < i1; i++) {
-                    if (!(ok = wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit))) break;
-                    weights(i, s);
-                    rows(i, s);
-                    filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
-                    if (++s == p.stages) s = 0, ph ^= 1u;
+        bool ok = !(p.debug & 4) && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit);
+        ok = __all_sync(0xffffffffu, ok);
+        uint32_t filled = 0, filled_parity = 0;
+        if (ok) {
+            const int64_t all = int64_t(h.active) * f_blocks;
+            const int i0 = int(all * rank / p.kc), i1 = int(all * (rank + 1) / p.kc);
+            const int ahead = min((i1 - i0 + p.kps - 1) / p.kps, p.stages);  // stages filled at once
+            const int kk = lane & 7;                                         // lanes 0-7 issue weights, lanes 8-15 rows of h
+            auto weights = [&](int i, int s) {
+                const int nk = min(p.kps, i1 - i);
+                if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.full[s]), uint32_t(nk) * (h_bytes + w_bytes));
+                __syncwarp();
+                if (kk < nk && lane < 8) {
+                    const int a = (i + kk) / f_blocks, kb = i + kk - a * f_blocks;
+                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes + w0 + uint32_t(kk) * w_bytes, &tmD, bar(h.full[s]), kb * 64, h.expert[a] * p.d + n0);
                 }
-            } else {
-                ptx::griddep_wait();
+            };
+            auto rows = [&](int i, int s) {
+                const int nk = min(p.kps, i1 - i);
+                if (kk < nk && lane >= 8 && lane < 16) {
+                    const int a = (i + kk) / f_blocks, kb = i + kk - a * f_blocks;
+                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes + uint32_t(kk) * h_bytes, &tmH, bar(h.full[s]), kb * 64, a * p.token_rows);
+                }
+                __syncwarp();
+            };
+            for (int i = 0; i < ahead; i++) weights(i0 + i * p.kps, i);
+            ptx::griddep_wait();
+            for (int i = 0; i < ahead; i++) rows(i0 + i * p.kps, i);
+            filled = (1u << ahead) - 1u;
+            int s = ahead == p.stages ? 0 : ahead;
+            uint32_t ph = ahead == p.stages ? 1u : 0u;
+            for (int i = i0 + ahead * p.kps; i < i1; i += p.kps) {
+                ok = __all_sync(0xffffffffu, wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit));
+                if (!ok) break;
+                weights(i, s);
+                rows(i, s);
+                filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
+                if (++s == p.stages) s = 0, ph ^= 1u;
             }
-            if (!ok) {
-                const uint64_t t0 = ptx::globaltimer_ns();
-                for (int i = 0; i < p.stages; i++)
-                    while ((filled >> i & 1u) && !ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
-                        if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
-            }
+        } else {
+            ptx::griddep_wait();
+        }
+        if (!ok && lane == 0) {
+            const uint64_t t0 = ptx::globaltimer_ns();
+            for (int i = 0; i < p.stages; i++)
+                while ((filled >> i & 1u) && !ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -444,15 +469,18 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
             const uint32_t idesc = make_idesc(p.bf16, 128, p.bn);
             int s = 0;
             uint32_t ph = 0;
-            for (int i = i0; i < i1; i++) {
-                const unsigned long long who = h.who[h.expert[i / f_blocks]];
+            for (int i = i0; i < i1; i += p.kps) {
                 if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) break;
                 ptx::tc_fence_after();
                 const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                const uint64_t a = sw128_desc(src), b = sw128_desc(src + h_bytes);
+                const int nk = min(p.kps, i1 - i);
+                for (int kk = 0; kk < nk; kk++) {
+                    const unsigned long long who = h.who[h.expert[(i + kk) / f_blocks]];
+                    const uint64_t a = sw128_desc(src + uint32_t(kk) * h_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * w_bytes);
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * j, idesc, 1u, ~uint32_t(who), ~uint32_t(who >> 32), 0xffffffffu, 0xffffffffu);
+                    for (int j = 0; j < 4; j++)
+                        ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * j, idesc, 1u, ~uint32_t(who), ~uint32_t(who >> 32), 0xffffffffu, 0xffffffffu);
+                }
                 issued = true;
                 ptx::umma_commit<1>(bar(h.empty[s]));
                 if (++s == p.stages) s = 0, ph ^= 1u;
@@ -563,9 +591,9 @@ Layout layout(const cute_b200_moe_desc &d) {
     return l;
 }
 
-// Stages of `bytes` behind the head; an MMA reads 128 rows of 128 bytes from a stage's start.
-int ring_stages(uint32_t bytes) {
-    const uint32_t ring = MOE_SMEM - MOE_HEAD - 1024, over = bytes < 16384 ? 16384 - bytes : 0;
+// Stages of `bytes` behind the head; an MMA reads 128 rows of 128 bytes from up to `last` bytes behind a stage's start.
+int ring_stages(uint32_t bytes, uint32_t last) {
+    const uint32_t ring = MOE_SMEM - MOE_HEAD - 1024, reach = last + 16384, over = bytes < reach ? reach - bytes : 0;
     const int stages = int((ring - over) / bytes);
     return stages < MOE_MAX_STAGES ? stages : MOE_MAX_STAGES;
 }
@@ -611,21 +639,25 @@ cute_b200_status moe_tn(const cute_b200_moe_desc &d, const uint64_t ptr[7], cuda
     const dim3 groups(unsigned((d.tokens + ROUTER_TOKENS - 1) / ROUTER_TOKENS * ROUTER_CLUSTER));
     CB_TRY(launch_dependent(p.bf16 ? moe_router_kernel<true> : moe_router_kernel<false>, groups, ROUTER_THREADS, 0, ROUTER_CLUSTER, stream, p));
 
-    CUtensorMap tmX, tmG, tmU, tmH, tmD;
+    CUtensorMap tmX, tmH, tmD;
+    UpMaps maps;
     CB_TRY(rows_tensor_map(&tmX, ptr[0], p.bf16, d.tokens, d.d, d.d, p.token_rows));
-    CB_TRY(rows_tensor_map(&tmG, ptr[2], p.bf16, uint64_t(d.experts) * d.f, d.d, d.d, 8));
-    CB_TRY(rows_tensor_map(&tmU, ptr[3], p.bf16, uint64_t(d.experts) * d.f, d.d, d.d, 8));
-    p.stage_bytes = uint32_t(p.token_rows + 16 * UP_GROUPS) * 128u;
-    p.stages = ring_stages(p.stage_bytes);
-    CB_TRY(launch_dependent(moe_up_kernel, dim3(unsigned(dev.sm_count)), MOE_THREADS, MOE_SMEM, 1, stream, tmX, tmG, tmU, p));
+    for (int i = 0; i < 4; i++) {
+        CB_TRY(rows_tensor_map(&maps.gate[i], ptr[2], p.bf16, uint64_t(d.experts) * d.f, d.d, d.d, 64 >> i));
+        CB_TRY(rows_tensor_map(&maps.up[i], ptr[3], p.bf16, uint64_t(d.experts) * d.f, d.d, d.d, 64 >> i));
+    }
+    p.stage_bytes = uint32_t(2 * p.token_rows + 16 * UP_GROUPS) * 128u;
+    p.stages = ring_stages(p.stage_bytes, 0);
+    CB_TRY(launch_dependent(moe_up_kernel, dim3(unsigned(dev.sm_count)), MOE_THREADS, MOE_SMEM, 1, stream, tmX, maps, p));
 
     p.bn = 16, p.kc = 1;
     const int f_blocks = (d.f + 63) / 64, expected = most_active(d);
     int fits[4];
     for (int c = 0; c < 4; c++) fits[c] = (1 << c) <= f_blocks ? g_down_clusters[device][c] : 0;  // every CTA has a block of one expert at least
     stream_cut(d.d, f_blocks * expected, fits, &p.bn, &p.kc);
-    p.stage_bytes = uint32_t(p.token_rows + p.bn) * 128u;
-    p.stages = ring_stages(p.stage_bytes);
+    p.kps = stream_blocks(p.bn, p.token_rows, MOE_SMEM - MOE_HEAD - 1024);
+    p.stage_bytes = uint32_t(p.kps * (p.token_rows + p.bn)) * 128u;
+    p.stages = ring_stages(p.stage_bytes, uint32_t((p.kps - 1) * p.token_rows) * 128u);
     p.tmem_cols = p.bn <= 32 ? 32 : (p.bn <= 64 ? 64 : (p.bn <= 128 ? 128 : 256));
     CB_TRY(rows_tensor_map(&tmH, ptr[6] + l.h, p.bf16, uint64_t(expected) * p.token_rows, d.f, d.f, p.token_rows));
     CB_TRY(rows_tensor_map(&tmD, ptr[4], p.bf16, uint64_t(d.experts) * d.d, d.f, d.f, p.bn));

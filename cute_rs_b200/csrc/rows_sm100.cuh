@@ -101,6 +101,14 @@ cute_b200_status max_clusters(void (*kernel)(P...), int threads, size_t smem, in
     return CUTE_B200_OK;
 }
 
+// k blocks per ring stage of a product that streams `bn` rows of a weight past `rows` rows: about 28 KB of the weight, but at
+// least four stages in a ring of `ring` bytes.
+inline int stream_blocks(int bn, int rows, uint32_t ring) {
+    int blocks = bn >= 160 ? 1 : (bn >= 80 ? 2 : 4);
+    while (blocks > 1 && ring / (uint32_t(blocks * (rows + bn)) * 128u) < 4) blocks /= 2;
+    return blocks;
+}
+
 // How a product that streams an (n, k) weight past a few rows is cut: bn rows of the weight per tile, a cluster of kc CTAs per tile.  The launch is one wave
 // where it can be; the cut with the least time for the slowest CTA wins.  A CTA streams at most what an even share of
 // HBM gives it, and no faster than its MMAs take (four per k block, a fixed ~60 clocks or bn / 2 each).
