@@ -92,8 +92,10 @@ struct FewParams {
     void *y;
     int64_t ldy;
     int m, n, rank, rp, adapters, c_dtype, vec;
-    int k_blocks, bn, kc, xr, stages, kps;
-    uint32_t stage_bytes, x_bytes, w_bytes, idesc, tmem_cols;
+    int k_blocks, bn, kc, xr, stages, kps, b_blocks;
+    uint32_t stage_bytes, x_bytes, w_bytes, low_bytes, idesc, tmem_cols;
+    const uint16_t *t, *b;
+    bool bf16;
     uint32_t *status;
     int debug;
 };
@@ -107,14 +109,69 @@ struct FewHead {
 };
 static_assert(sizeof(FewHead) <= FEW_HEAD, "head");
 
+// Where the adapters' products are taken.  On the tensor core, through the ring, in blocks of 64 columns of B[a]
+// (b_blocks > 0); or, b_blocks == 0, as dot products by the epilogue's 128 threads, idle while W streams, a thread per column
+// of Y, into `low` in f32, which the final sum adds.  The second way serves ranks up to 32, whose rows of B[a] are 16 to
+// 64 bytes: TMA fetches those no faster than full rows of 128 (0.5 us for a box of 128 rows, measured; 48 rows with an
+// adapter each, rank 16, n = 8192: 35 us by the tensor core).  Its results must leave the ring most of shared memory.
+constexpr uint32_t FEW_DOTS = 40 * 1024;
+// Blocks of B that this CTA of the cluster takes: every kc-th adapter.
+__device__ __forceinline__ int low_blocks(int entries, int rank, int kc, int b_blocks) {
+    return b_blocks > 0 && entries > rank ? (entries - rank + kc - 1) / kc * b_blocks : 0;
+}
+
+// The adapters' part of columns n0.. of Y for rows rank, rank + kc, .. (row r of `t` and `out` is row rank + r kc of Y), by
+// 128 threads; id[row] < 0 = no adapter.
+template <bool BF16>
+__device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, float *t, float *out, int rank, int n0, int thread) {
+    const int rows = (p.m - rank + p.kc - 1) / p.kc;
+    for (int i = thread; i < rows * p.rp; i += 128) {
+        const int r = i / p.rp, j = i - r * p.rp;
+        const uint16_t *src = p.t + int64_t(rank + r * p.kc) * 2 * p.rp + j;
+        t[i] = to_f32<BF16>(src[0]) + to_f32<BF16>(src[p.rp]);
+    }
+    ptx::named_barrier(1, 128);
+    const int vecs = p.rank / 8;  // 16-byte pieces of a row of B, at most four
+    for (int c = thread; c < p.bn && n0 + c < p.n; c += 128) {
+        int held = -1;
+        uint4 b[4];
+        for (int r = 0; r < rows; r++) {
+            const int a = id[rank + r * p.kc];
+            float sum = 0.0f;
+            if (a >= 0) {
+                if (a != held) {
+                    const uint4 *src = reinterpret_cast<const uint4 *>(p.b + (int64_t(a) * p.n + n0 + c) * p.rank);
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+                        if (v < vecs) b[v] = __ldg(src + v);
+                    held = a;
+                }
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    if (v < vecs) {
+                        const float *tv = t + r * p.rp + 8 * v;
+                        const uint32_t w[4] = {b[v].x, b[v].y, b[v].z, b[v].w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float2 f = pair_f32<BF16>(w[i]);
+                            sum = fmaf(f.y, tv[2 * i + 1], fmaf(f.x, tv[2 * i], sum));
+                        }
+                    }
+            }
+            out[r * p.bn + c] = sum;
+        }
+    }
+}
+
 __global__ void __launch_bounds__(FEW_THREADS, 1)
     lora_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT,
                     const __grid_constant__ CUtensorMap tmB, const FewParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     FewHead &h = *reinterpret_cast<FewHead *>(smem_raw + (base - raw));
-    const int q_blocks = ext_blocks(p.rp);
-    const uint32_t low = base + FEW_HEAD, ring = low + uint32_t(q_blocks) * p.x_bytes;  // T's blocks, then the ring
+    const int b_blocks = p.b_blocks, t_blocks = ext_blocks(p.rp);
+    // T's blocks for the tensor core, or T and the dot products, then the ring.
+    const uint32_t low = base + FEW_HEAD, ring = low + p.low_bytes;
     auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
     volatile uint32_t *abort_flag = &h.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -163,6 +220,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
             if (++s == p.stages) s = 0, ph ^= 1u;
         };
+        if (lane == 0) {
+            ptx::prefetch_tensormap(&tmX);
+            ptx::prefetch_tensormap(&tmW);
+            if (b_blocks > 0) {
+                ptx::prefetch_tensormap(&tmT);
+                ptx::prefetch_tensormap(&tmB);
+            }
+        }
         const uint32_t w0 = uint32_t(p.kps) * p.x_bytes;
         const int kk = lane & 7;  // lanes 0-7 issue blocks of W, lanes 8-15 of X
         for (int kb = kb0; kb < kb1 && ok; kb += p.kps) {
@@ -175,20 +240,20 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
         ptx::griddep_wait();
         ok = __all_sync(0xffffffffu, ok && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit));
-        const int mine = ok && h.entries > int(rank) ? (h.entries - int(rank) + p.kc - 1) / p.kc * q_blocks : 0;  // blocks of B
+        const int mine = ok ? low_blocks(h.entries, int(rank), p.kc, b_blocks) : 0;
         const bool has_low = mine > 0;
         if (has_low) {
-            if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.low), uint32_t(q_blocks) * p.x_bytes);
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.low), uint32_t(t_blocks) * p.x_bytes);
             __syncwarp();
-            if (lane < q_blocks) ptx::tma_load_2d(low + uint32_t(lane) * p.x_bytes, &tmT, bar(h.low), ext_block(lane, p.rp, p.rank).t_col, 0);
+            if (lane < t_blocks) ptx::tma_load_2d(low + uint32_t(lane) * p.x_bytes, &tmT, bar(h.low), ext_block(lane, p.rp, p.rank).t_col, 0);
         }
         for (int i = 0; i < mine && ok; i += p.kps) {
             const int nk = min(p.kps, mine - i);
             const uint32_t dst = next(uint32_t(nk) * p.w_bytes);
             if (!ok) break;
             if (lane < nk) {
-                const int e = int(rank) + (i + lane) / q_blocks * p.kc, q = (i + lane) % q_blocks;
-                ptx::tma_load_2d(dst + w0 + uint32_t(lane) * p.w_bytes, &tmB, bar(h.full[s]), ext_block(q, p.rp, p.rank).b_col, h.entry_id[e] * p.n + n0);
+                const int e = int(rank) + (i + lane) / b_blocks * p.kc, q = (i + lane) % b_blocks;
+                ptx::tma_load_2d(dst + w0 + uint32_t(lane) * p.w_bytes, &tmB, bar(h.full[s]), 64 * q, h.entry_id[e] * p.n + n0);
             }
             issued();
         }
@@ -202,49 +267,62 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true, issued = false;
-            const uint32_t w0 = uint32_t(p.kps) * p.x_bytes;
-            auto ready = [&] {
-                if (!wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit)) return false;
-                ptx::tc_fence_after();
-                return true;
-            };
-            auto free_stage = [&] {
-                issued = true;
-                ptx::umma_commit<1>(bar(h.empty[s]));
-                if (++s == p.stages) s = 0, ph ^= 1u;
-            };
-            for (int kb = kb0; kb < kb1; kb += p.kps) {
-                if (!(ok = ready())) break;
-                const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                const int nk = min(p.kps, kb1 - kb);
-                for (int kk = 0; kk < nk; kk++) {
-                    const uint64_t a = sw128_desc(src + uint32_t(kk) * p.x_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
+        // The whole warp runs the loop and one thread issues: the descriptors are then the same in every lane for the
+        // compiler too, and an MMA of N <= 128 goes out every 65 clocks (from a loop of one lane: 115 and more, measured).
+        const bool leader = ptx::elect_one();
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true, issued = false;
+        const uint32_t w0 = uint32_t(p.kps) * p.x_bytes;
+        auto ready = [&] {
+            ok = __all_sync(0xffffffffu, wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
+            ptx::tc_fence_after();
+            return ok;
+        };
+        auto free_stage = [&] {
+            issued = true;
+            if (leader) ptx::umma_commit<1>(bar(h.empty[s]));
+            __syncwarp();
+            if (++s == p.stages) s = 0, ph ^= 1u;
+        };
+        for (int kb = kb0; kb < kb1; kb += p.kps) {
+            if (!ready()) break;
+            const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+            const int nk = min(p.kps, kb1 - kb);
+            for (int kk = 0; kk < nk; kk++) {
+                const uint64_t a = sw128_desc(src + uint32_t(kk) * p.x_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
+                const uint32_t more = kb > kb0 || kk > 0 ? 1u : 0u;
+                if (leader) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) ptx::umma_f16<1>(tmem, a + 2u * j, b + 2u * j, p.idesc, (kb > kb0 || kk > 0 || j > 0) ? 1u : 0u);
+                    for (int j = 0; j < 4; j++) ptx::umma_f16<1>(tmem, a + 2u * j, b + 2u * j, p.idesc, j > 0 ? 1u : more);
                 }
-                free_stage();
+                __syncwarp();
             }
-            if (ok) ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit);
-            const int mine = ok && h.entries > int(rank) ? (h.entries - int(rank) + p.kc - 1) / p.kc * q_blocks : 0;
-            if (mine > 0) ok = wait_bar(bar(h.low), 0, abort_flag, p.status, WHERE_MMA_FULL, 101u, limit);
-            for (int i = 0; i < mine && ok; i += p.kps) {
-                if (!(ok = ready())) break;
-                const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                const int nk = min(p.kps, mine - i);
-                for (int kk = 0; kk < nk; kk++) {
-                    const int e = int(rank) + (i + kk) / q_blocks * p.kc, q = (i + kk) % q_blocks;
-                    const ExtBlock x = ext_block(q, p.rp, p.rank);
-                    const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
-                    const uint64_t a = sw128_desc(low + uint32_t(q) * p.x_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
-                    for (int j = 0; j < x.steps; j++)
-                        ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * (j & x.b_mask), p.idesc, 1u, o0, o1, o2, o3);
+            free_stage();
+        }
+        if (ok) ok = __all_sync(0xffffffffu, wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit));
+        const int mine = ok ? low_blocks(h.entries, int(rank), p.kc, b_blocks) : 0;
+        if (mine > 0) ok = __all_sync(0xffffffffu, wait_bar(bar(h.low), 0, abort_flag, p.status, WHERE_MMA_FULL, 101u, limit));
+        for (int i = 0; i < mine && ok; i += p.kps) {
+            if (!ready()) break;
+            const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+            const int nk = min(p.kps, mine - i);
+            for (int kk = 0; kk < nk; kk++) {
+                const int e = int(rank) + (i + kk) / b_blocks * p.kc, q = (i + kk) % b_blocks;
+                const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
+                const uint64_t b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
+                // The numbers' block of T, then their remainders' (with rp <= 32 one block holds both), against one block of B.
+                for (int part = 0; part < t_blocks / b_blocks; part++) {
+                    const ExtBlock x = ext_block(2 * q + part, p.rp, p.rank);
+                    const uint64_t a = sw128_desc(low + uint32_t(2 * q + part) * p.x_bytes);
+                    if (leader)
+                        for (int j = 0; j < x.steps; j++) ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * (j & x.b_mask), p.idesc, 1u, o0, o1, o2, o3);
+                    __syncwarp();
                 }
-                free_stage();
             }
+            free_stage();
+        }
+        if (leader) {
             if (ok) {
                 ptx::umma_commit<1>(bar(h.done));
             } else if (issued) {  // giving up: wait (bounded) until the tensor core is done with shared memory and TMEM
@@ -283,12 +361,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         if (first) h.entry_id[at] = id;
         if (threadIdx.x == 64) h.entries = total;
         ptx::named_barrier(1, 128);
-        for (int e = 0; e < total; e++) {
+        for (int e = 0; e < (b_blocks > 0 ? total : 0); e++) {
             const uint32_t mine = __ballot_sync(0xffffffffu, id == h.entry_id[e]);
             if (lane == 0) h.off[e][w] = ~mine;
         }
         ptx::named_barrier(1, 128);
         if (threadIdx.x == 64) ptx::mbar_arrive(bar(h.plan));
+        if (b_blocks == 0) {
+            float *t = reinterpret_cast<float *>(smem_raw + (low - raw)), *dots = t + (p.m + p.kc - 1) / p.kc * p.rp;
+            if (p.bf16) few_dots<true>(p, h.id, t, dots, int(rank), n0, row);
+            else few_dots<false>(p, h.id, t, dots, int(rank), n0, row);
+        }
 
         // The accumulator's rows to shared memory (the ring is idle: every load has been consumed).
         const bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.done), 0, abort_flag, p.status, WHERE_EPILOGUE, 0u, limit));
@@ -327,6 +410,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             float4 v = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(at, 0) : at);
             for (int c = 1; c < p.kc; c++) {  // in ascending order of the k ranges
                 const float4 o = ptx::ld_shared_cluster_v4(ptx::mapa(at, uint32_t(c)));
+                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+            }
+            if (b_blocks == 0) {  // the dot products of this row were taken by CTA row % kc
+                const uint32_t dots = low + uint32_t((p.m + p.kc - 1) / p.kc * p.rp + row / p.kc * p.bn + col) * 4u;
+                const float4 o = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(dots, uint32_t(row % p.kc)) : dots);
                 v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
             }
             const int64_t gcol = n0 + col, out = int64_t(row) * p.ldy + gcol;
@@ -373,7 +461,11 @@ cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int de
     f.x_bytes = uint32_t(f.xr) * 128u;
     f.w_bytes = uint32_t(f.bn) * 128u;
     // The head, T, the ring, and behind the last stage as much as an MMA reads past its rows of X.
-    const uint32_t ring = FEW_SMEM - FEW_HEAD - 1024 - uint32_t(ext_blocks(p.rp)) * f.x_bytes;
+    const uint64_t dots = uint64_t((p.m + f.kc - 1) / f.kc) * uint64_t(p.rp + f.bn) * 4;
+    f.b_blocks = p.rp <= 32 && dots <= FEW_DOTS ? 0 : (p.rp <= 64 ? 1 : 2);
+    f.low_bytes = f.b_blocks == 0 ? uint32_t((dots + 1023) / 1024 * 1024) : uint32_t(ext_blocks(p.rp)) * f.x_bytes;
+    f.t = p.t, f.b = p.b, f.bf16 = BF16;
+    const uint32_t ring = FEW_SMEM - FEW_HEAD - 1024 - f.low_bytes;
     f.kps = stream_blocks(f.bn, f.xr, ring);
     f.stage_bytes = uint32_t(f.kps) * (f.x_bytes + f.w_bytes);
     const uint32_t reach = uint32_t(f.kps - 1) * f.x_bytes + 16384, over = f.stage_bytes < reach ? reach - f.stage_bytes : 0;

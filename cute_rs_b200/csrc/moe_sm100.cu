@@ -281,41 +281,48 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int s = 0, it = 0;
-            uint32_t ph = 0;
-            bool ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit), issued = false;
-            if (ok)
-                up_chunks(h, p, [&](int, int, int groups) {
-                    const int buf = it & 1;
-                    const uint32_t idesc = make_idesc(p.bf16, 128, 16 * groups), d = tmem + uint32_t(buf) * 256u;
-                    if (!(ok = wait_bar(bar(h.tempty[buf]), (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf), limit))) return false;
+        // The whole warp runs the loop and one thread issues: see lora_few_kernel.
+        const bool leader = ptx::elect_one();
+        int s = 0, it = 0;
+        uint32_t ph = 0;
+        bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit)), issued = false;
+        if (ok)
+            up_chunks(h, p, [&](int, int, int groups) {
+                const int buf = it & 1, kps = up_blocks(groups);
+                const uint32_t idesc = make_idesc(p.bf16, 128, 16 * groups), d = tmem + uint32_t(buf) * 256u;
+                ok = __all_sync(0xffffffffu, wait_bar(bar(h.tempty[buf]), (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf), limit));
+                if (!ok) return false;
+                ptx::tc_fence_after();
+                for (int kb = 0; kb < k_blocks; kb += kps) {
+                    ok = __all_sync(0xffffffffu, wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
+                    if (!ok) return false;
                     ptx::tc_fence_after();
-                    const int kps = up_blocks(groups);
-                    for (int kb = 0; kb < k_blocks; kb += kps) {
-                        if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) return false;
-                        ptx::tc_fence_after();
-                        const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                        const int nk = min(kps, k_blocks - kb);
-                        for (int kk = 0; kk < nk; kk++) {
-                            const uint64_t a = sw128_desc(src + uint32_t(kk) * x_bytes), b = sw128_desc(src + uint32_t(kps) * x_bytes + uint32_t(kk * groups) * 2048u);
+                    const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+                    const int nk = min(kps, k_blocks - kb);
+                    for (int kk = 0; kk < nk; kk++) {
+                        const uint64_t a = sw128_desc(src + uint32_t(kk) * x_bytes), b = sw128_desc(src + uint32_t(kps) * x_bytes + uint32_t(kk * groups) * 2048u);
+                        const uint32_t more = kb > 0 || kk > 0 ? 1u : 0u;
+                        if (leader) {
 #pragma unroll
-                            for (int j = 0; j < 4; j++) ptx::umma_f16<1>(d, a + 2u * j, b + 2u * j, idesc, (kb > 0 || kk > 0 || j > 0) ? 1u : 0u);
+                            for (int j = 0; j < 4; j++) ptx::umma_f16<1>(d, a + 2u * j, b + 2u * j, idesc, j > 0 ? 1u : more);
                         }
-                        issued = true;
-                        ptx::umma_commit<1>(bar(h.empty[s]));
-                        if (++s == p.stages) s = 0, ph ^= 1u;
+                        __syncwarp();
                     }
-                    ptx::umma_commit<1>(bar(h.tfull[buf]));
-                    it++;
-                    return true;
-                });
-            if (!ok && issued) {
-                ptx::umma_commit<1>(bar(h.drain));
-                const uint64_t t0 = ptx::globaltimer_ns();
-                while (!ptx::mbar_try_wait(bar(h.drain), 0u))
-                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
-            }
+                    issued = true;
+                    if (leader) ptx::umma_commit<1>(bar(h.empty[s]));
+                    __syncwarp();
+                    if (++s == p.stages) s = 0, ph ^= 1u;
+                }
+                if (leader) ptx::umma_commit<1>(bar(h.tfull[buf]));
+                __syncwarp();
+                it++;
+                return true;
+            });
+        if (!ok && issued && leader) {
+            ptx::umma_commit<1>(bar(h.drain));
+            const uint64_t t0 = ptx::globaltimer_ns();
+            while (!ptx::mbar_try_wait(bar(h.drain), 0u))
+                if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
         }
         __syncwarp();
     } else {
@@ -411,6 +418,10 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
 
     const uint32_t w_bytes = uint32_t(p.bn) * 128u, w0 = uint32_t(p.kps) * h_bytes;
     if (warp == 0) {
+        if (lane == 0) {
+            ptx::prefetch_tensormap(&tmH);
+            ptx::prefetch_tensormap(&tmD);
+        }
         bool ok = !(p.debug & 4) && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit);
         ok = __all_sync(0xffffffffu, ok);
         uint32_t filled = 0, filled_parity = 0;
@@ -419,21 +430,29 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
             const int i0 = int(all * rank / p.kc), i1 = int(all * (rank + 1) / p.kc);
             const int ahead = min((i1 - i0 + p.kps - 1) / p.kps, p.stages);  // stages filled at once
             const int kk = lane & 7;                                         // lanes 0-7 issue weights, lanes 8-15 rows of h
+            // Lane kk follows block i0 + kk, i0 + kps + kk, ..: expert a, block kb of its f.
+            struct At {
+                int a, kb;
+            };
+            auto start = [&] { return At{(i0 + kk) / f_blocks, (i0 + kk) % f_blocks}; };
+            auto step = [&](At &at) {
+                at.kb += p.kps;
+                while (at.kb >= f_blocks) at.kb -= f_blocks, at.a++;
+            };
+            At w = start(), r = start();
             auto weights = [&](int i, int s) {
                 const int nk = min(p.kps, i1 - i);
                 if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.full[s]), uint32_t(nk) * (h_bytes + w_bytes));
                 __syncwarp();
-                if (kk < nk && lane < 8) {
-                    const int a = (i + kk) / f_blocks, kb = i + kk - a * f_blocks;
-                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes + w0 + uint32_t(kk) * w_bytes, &tmD, bar(h.full[s]), kb * 64, h.expert[a] * p.d + n0);
-                }
+                if (kk < nk && lane < 8)
+                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes + w0 + uint32_t(kk) * w_bytes, &tmD, bar(h.full[s]), w.kb * 64, h.expert[w.a] * p.d + n0);
+                step(w);
             };
             auto rows = [&](int i, int s) {
                 const int nk = min(p.kps, i1 - i);
-                if (kk < nk && lane >= 8 && lane < 16) {
-                    const int a = (i + kk) / f_blocks, kb = i + kk - a * f_blocks;
-                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes + uint32_t(kk) * h_bytes, &tmH, bar(h.full[s]), kb * 64, a * p.token_rows);
-                }
+                if (kk < nk && lane >= 8 && lane < 16)
+                    ptx::tma_load_2d(ring + uint32_t(s) * p.stage_bytes + uint32_t(kk) * h_bytes, &tmH, bar(h.full[s]), r.kb * 64, r.a * p.token_rows);
+                step(r);
                 __syncwarp();
             };
             for (int i = 0; i < ahead; i++) weights(i0 + i * p.kps, i);
@@ -461,30 +480,41 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            bool ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit), issued = false;
-            ptx::tc_fence_after();  // the zeros in the accumulator
-            const int64_t all = ok ? int64_t(h.active) * f_blocks : 0;
-            const int i0 = int(all * rank / p.kc), i1 = int(all * (rank + 1) / p.kc);
-            const uint32_t idesc = make_idesc(p.bf16, 128, p.bn);
-            int s = 0;
-            uint32_t ph = 0;
-            for (int i = i0; i < i1; i += p.kps) {
-                if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) break;
-                ptx::tc_fence_after();
-                const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                const int nk = min(p.kps, i1 - i);
-                for (int kk = 0; kk < nk; kk++) {
-                    const unsigned long long who = h.who[h.expert[(i + kk) / f_blocks]];
-                    const uint64_t a = sw128_desc(src + uint32_t(kk) * h_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * w_bytes);
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * j, idesc, 1u, ~uint32_t(who), ~uint32_t(who >> 32), 0xffffffffu, 0xffffffffu);
+        // The whole warp runs the loop and one thread issues: see lora_few_kernel.
+        const bool leader = ptx::elect_one();
+        bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit)), issued = false;
+        ptx::tc_fence_after();  // the zeros in the accumulator
+        const int64_t all = ok ? int64_t(h.active) * f_blocks : 0;
+        const int i0 = int(all * rank / p.kc), i1 = int(all * (rank + 1) / p.kc);
+        const uint32_t idesc = make_idesc(p.bf16, 128, p.bn);
+        int s = 0, kk = 0, a_at = i0 / f_blocks, left = f_blocks - i0 % f_blocks;  // blocks left of this expert
+        uint32_t ph = 0, src = 0;
+        for (int i = i0; i < i1 && ok; a_at++, left = f_blocks) {
+            const unsigned long long who = h.who[h.expert[a_at]];
+            const uint32_t off0 = __shfl_sync(0xffffffffu, ~uint32_t(who), 0), off1 = __shfl_sync(0xffffffffu, ~uint32_t(who >> 32), 0);
+            for (const int end = min(i1, i + left); i < end; i++) {
+                if (kk == 0) {
+                    ok = __all_sync(0xffffffffu, wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    src = ring + uint32_t(s) * p.stage_bytes;
                 }
+                const uint64_t a = sw128_desc(src + uint32_t(kk) * h_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * w_bytes);
+                if (leader) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * j, idesc, 1u, off0, off1, 0xffffffffu, 0xffffffffu);
+                }
+                __syncwarp();
                 issued = true;
-                ptx::umma_commit<1>(bar(h.empty[s]));
-                if (++s == p.stages) s = 0, ph ^= 1u;
+                if (++kk == p.kps || i + 1 == i1) {
+                    if (leader) ptx::umma_commit<1>(bar(h.empty[s]));
+                    __syncwarp();
+                    kk = 0;
+                    if (++s == p.stages) s = 0, ph ^= 1u;
+                }
             }
+        }
+        if (leader) {
             if (ok) {
                 ptx::umma_commit<1>(bar(h.done));
             } else if (issued) {

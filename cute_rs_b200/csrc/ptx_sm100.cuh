@@ -217,6 +217,16 @@ __device__ __forceinline__ void umma_f16_lanes_pair(uint32_t d_tmem, uint64_t a_
         "r"(off[5]), "r"(off[6]), "r"(off[7])
         : "memory");
 }
+// One thread of a converged warp, always the same: true for it alone.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
 // Make `cluster_bar` (shared::cluster address, own or peer CTA) receive one
 // arrival when every tcgen05.mma issued so far by this thread has finished.
 template <int CTA_GROUP>

@@ -111,7 +111,7 @@ inline int stream_blocks(int bn, int rows, uint32_t ring) {
 
 // How a product that streams an (n, k) weight past a few rows is cut: bn rows of the weight per tile, a cluster of kc CTAs per tile.  The launch is one wave
 // where it can be; the cut with the least time for the slowest CTA wins.  A CTA streams at most what an even share of
-// HBM gives it, and no faster than its MMAs take (four per k block, a fixed ~60 clocks or bn / 2 each).
+// HBM gives it, and no faster than its MMAs are issued (per k block four of 65 clocks or bn / 2 each, and some 80 of loop).
 inline void stream_cut(int n, int k_blocks, const int (&max_clusters)[4], int *bn, int *kc) {
     double best = 1e300;
     for (int c = 0; c < 4; c++) {
@@ -122,7 +122,7 @@ inline void stream_cut(int n, int k_blocks, const int (&max_clusters)[4], int *b
             const int64_t waves = (ctas + ctas_at_once - 1) / ctas_at_once;
             const double share = 6.5e12 / double(ctas < ctas_at_once ? ctas : ctas_at_once);
             const double rate = share < 7.0e10 ? share : 7.0e10;
-            const double load = b * 128.0 / rate, math = 4.0 * (b / 2 > 60 ? b / 2 : 60) / 1.7e9;
+            const double load = b * 128.0 / rate, math = (4.0 * (b / 2 > 65 ? b / 2 : 65) + 80.0) / 1.8e9;
             const double t = double(waves) * (((k_blocks + parts - 1) / parts) * (load > math ? load : math) + 2.0e-6) + (parts > 1 ? 1.0e-6 : 0.0);
             if (t < best * 0.999) best = t, *bn = b, *kc = parts;
         }
