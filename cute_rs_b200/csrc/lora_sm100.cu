@@ -121,7 +121,39 @@ __device__ __forceinline__ int low_blocks(int entries, int rank, int kc, int b_b
 }
 
 // The adapters' part of columns n0.. of Y for rows rank, rank + kc, .. (row r of `t` and `out` is row rank + r kc of Y), by
-// 128 threads; id[row] < 0 = no adapter.
+// 128 threads; id[row] < 0 = no adapter.  V: 16-byte pieces of a row of B; R: rows whose B is fetched at once, so that
+// eight or more loads are on their way (one row at a time took 0.7 us each, the latency of its loads).
+template <bool BF16, int V, int R>
+__device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, const float *t, float *out, int rank, int rows, int n0, int thread) {
+    for (int c = thread; c < p.bn && n0 + c < p.n; c += 128)
+        for (int r0 = 0; r0 < rows; r0 += R) {
+            uint4 b[R][V];
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const int a = r0 + r < rows ? id[rank + (r0 + r) * p.kc] : -1;
+                const uint4 *src = reinterpret_cast<const uint4 *>(p.b + (int64_t(a) * p.n + n0 + c) * p.rank);
+#pragma unroll
+                for (int v = 0; v < V; v++) b[r][v] = a >= 0 ? __ldg(src + v) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                if (r0 + r >= rows) break;
+                const float *tv = t + (r0 + r) * p.rp;  // zeros where the row has no adapter
+                float sum = 0.0f;
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const uint32_t w[4] = {b[r][v].x, b[r][v].y, b[r][v].z, b[r][v].w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float2 f = pair_f32<BF16>(w[i]);
+                        sum = fmaf(f.y, tv[8 * v + 2 * i + 1], fmaf(f.x, tv[8 * v + 2 * i], sum));
+                    }
+                }
+                out[(r0 + r) * p.bn + c] = sum;
+            }
+        }
+}
+
 template <bool BF16>
 __device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, float *t, float *out, int rank, int n0, int thread) {
     const int rows = (p.m - rank + p.kc - 1) / p.kc;
@@ -131,36 +163,10 @@ __device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, 
         t[i] = to_f32<BF16>(src[0]) + to_f32<BF16>(src[p.rp]);
     }
     ptx::named_barrier(1, 128);
-    const int vecs = p.rank / 8;  // 16-byte pieces of a row of B, at most four
-    for (int c = thread; c < p.bn && n0 + c < p.n; c += 128) {
-        int held = -1;
-        uint4 b[4];
-        for (int r = 0; r < rows; r++) {
-            const int a = id[rank + r * p.kc];
-            float sum = 0.0f;
-            if (a >= 0) {
-                if (a != held) {
-                    const uint4 *src = reinterpret_cast<const uint4 *>(p.b + (int64_t(a) * p.n + n0 + c) * p.rank);
-#pragma unroll
-                    for (int v = 0; v < 4; v++)
-                        if (v < vecs) b[v] = __ldg(src + v);
-                    held = a;
-                }
-#pragma unroll
-                for (int v = 0; v < 4; v++)
-                    if (v < vecs) {
-                        const float *tv = t + r * p.rp + 8 * v;
-                        const uint32_t w[4] = {b[v].x, b[v].y, b[v].z, b[v].w};
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float2 f = pair_f32<BF16>(w[i]);
-                            sum = fmaf(f.y, tv[2 * i + 1], fmaf(f.x, tv[2 * i], sum));
-                        }
-                    }
-            }
-            out[r * p.bn + c] = sum;
-        }
-    }
+    if (p.rank == 8) few_dots<BF16, 1, 8>(p, id, t, out, rank, rows, n0, thread);
+    else if (p.rank == 16) few_dots<BF16, 2, 8>(p, id, t, out, rank, rows, n0, thread);
+    else if (p.rank == 24) few_dots<BF16, 3, 4>(p, id, t, out, rank, rows, n0, thread);
+    else few_dots<BF16, 4, 4>(p, id, t, out, rank, rows, n0, thread);
 }
 
 __global__ void __launch_bounds__(FEW_THREADS, 1)
@@ -407,11 +413,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         for (int i = int(rank) * FEW_THREADS + int(threadIdx.x); i < items; i += p.kc * FEW_THREADS) {
             const int row = i / quads, col = (i - row * quads) * 4;
             const uint32_t at = ring + uint32_t(row) * pitch + uint32_t(col) * 4u;
-            float4 v = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(at, 0) : at);
-            for (int c = 1; c < p.kc; c++) {  // in ascending order of the k ranges
-                const float4 o = ptx::ld_shared_cluster_v4(ptx::mapa(at, uint32_t(c)));
-                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-            }
+            float4 v = cluster_sum(at, p.kc);
             if (b_blocks == 0) {  // the dot products of this row were taken by CTA row % kc
                 const uint32_t dots = low + uint32_t((p.m + p.kc - 1) / p.kc * p.rp + row / p.kc * p.bn + col) * 4u;
                 const float4 o = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(dots, uint32_t(row % p.kc)) : dots);
@@ -439,7 +441,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     if (warp == 1) ptx::tmem_dealloc<1>(tmem, p.tmem_cols);
 }
 
-constexpr uint32_t FEW_SMEM = 227 * 1024;
+// Less than all of it: the CTAs of the kernel that computes T (1.2 KB each) have to fit beside, or W would not stream until
+// they are gone.
+constexpr uint32_t FEW_SMEM = 216 * 1024;
 
 int g_few_clusters[64][4];  // clusters of 1, 2, 4, 8 CTAs of the few-row kernel that fit each device at once
 

@@ -260,11 +260,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (id >= 0 && col < p.rank) {  // lanes of rows without an adapter hold nothing; past the rank lie the next adapter's sums
                 const uint32_t at = xring + uint32_t(row) * pitch + uint32_t(col) * 4u;
-                v = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(at, 0) : at);
-                for (int c = 1; c < p.kc; c++) {
-                    const float4 o = ptx::ld_shared_cluster_v4(ptx::mapa(at, uint32_t(c)));
-                    v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-                }
+                v = cluster_sum(at, p.kc);
                 const float s = p.scale[id];
                 v.x *= s, v.y *= s, v.z *= s, v.w *= s;
             }

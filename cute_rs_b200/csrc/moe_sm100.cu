@@ -76,10 +76,12 @@ __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoePar
     if (rank >= count || warp != 0) return;  // nothing reads another CTA's shared memory from here on
     // One warp chooses for the token: lane l holds experts l, l + 32, ..
     const int t = t0 + rank;
+    const int per_lane = (p.experts + 31) / 32;
     float v[MAX_EXPERTS / 32];
     float best = -INFINITY;
 #pragma unroll
     for (int j = 0; j < MAX_EXPERTS / 32; j++) {
+        if (j >= per_lane) break;
         const int e = j * 32 + lane;
         v[j] = -INFINITY;
         if (e < p.experts) {
@@ -94,11 +96,13 @@ __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoePar
     float total = 0.0f;
     uint32_t open = 0;
 #pragma unroll
-    for (int j = 0; j < MAX_EXPERTS / 32; j++)
+    for (int j = 0; j < MAX_EXPERTS / 32; j++) {
+        if (j >= per_lane) break;
         if (j * 32 + lane < p.experts) {
             total += expf(v[j] - best);
             open |= 1u << j;
         }
+    }
     total = warp_sum(total);
     float chosen_sum = 0.0f, my_w = 0.0f;
     int my_id = 0;
@@ -107,11 +111,13 @@ __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoePar
         float key = -INFINITY;
         int at = 0x7fffffff;
 #pragma unroll
-        for (int j = 0; j < MAX_EXPERTS / 32; j++)
+        for (int j = 0; j < MAX_EXPERTS / 32; j++) {
+            if (j >= per_lane) break;
             if ((open >> j) & 1u) {
                 const float c = v[j] == v[j] ? v[j] : -INFINITY;
                 if (at == 0x7fffffff || c > key) key = c, at = j * 32 + lane;
             }
+        }
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) {
             const float k2 = __shfl_xor_sync(0xffffffffu, key, s);
@@ -171,7 +177,7 @@ __device__ __forceinline__ void find_active(MoeHead &h, const MoeParams &p, int 
 }
 
 constexpr int MOE_THREADS = 192, MOE_MAX_STAGES = 16;
-constexpr uint32_t MOE_SMEM = 227 * 1024;
+constexpr uint32_t MOE_SMEM = 216 * 1024;  // leaves room for the next kernels' first CTAs, the router's among them
 
 // ---- up ---------------------------------------------------------------------------
 // The rows of the chosen experts' gate and up weights, eight of each to a group, are dealt out evenly over the CTAs;
@@ -567,11 +573,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         for (int i = int(rank) * MOE_THREADS + int(threadIdx.x); i < items; i += p.kc * MOE_THREADS) {
             const int row = i / quads, col = (i - row * quads) * 4;
             const uint32_t at = ring + uint32_t(row) * pitch + uint32_t(col) * 4u;
-            float4 v = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(at, 0) : at);
-            for (int c = 1; c < p.kc; c++) {
-                const float4 o = ptx::ld_shared_cluster_v4(ptx::mapa(at, uint32_t(c)));
-                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-            }
+            const float4 v = cluster_sum(at, p.kc);
             if (n0 + col < p.d)  // d is a multiple of 8: four columns are in or out together
                 *reinterpret_cast<uint2 *>(p.y + int64_t(row) * p.d + n0 + col) = make_uint2(pack_16(v.x, v.y, p.bf16), pack_16(v.z, v.w, p.bf16));
         }

@@ -41,6 +41,21 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// The sum of four floats at the same place of the shared memory of a cluster's `kc` <= 8 CTAs, in ascending order; the loads
+// are all on their way before the first is used.
+__device__ __forceinline__ float4 cluster_sum(uint32_t at, int kc) {
+    if (kc == 1) return ptx::ld_shared_cluster_v4(at);
+    float4 part[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+        if (c < kc) part[c] = ptx::ld_shared_cluster_v4(ptx::mapa(at, uint32_t(c)));
+    float4 v = part[0];
+#pragma unroll
+    for (int c = 1; c < 8; c++)
+        if (c < kc) v.x += part[c].x, v.y += part[c].y, v.z += part[c].z, v.w += part[c].w;
+    return v;
+}
+
 // Tensor map of a row-major 16-bit matrix of `rows` x `cols`, `pitch` elements between rows, in boxes of 64 columns
 // (one 128-byte swizzled row) by box_rows; what lies outside reads as zero.  Encoded anew for every call: it takes
 // a fraction of a microsecond on the host, and nothing is kept by an operand's address.
@@ -69,15 +84,17 @@ cute_b200_status launch_dependent(void (*kernel)(P...), dim3 grid, int threads, 
     cfg.blockDim = dim3(unsigned(threads));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[3];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[2].id = cudaLaunchAttributeClusterSchedulingPolicyPreference;
+    attr[2].val.clusterSchedulingPolicyPreference = cudaClusterSchedulingPolicySpread;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = unsigned(cluster);
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    cfg.numAttrs = cluster > 1 ? 3 : 1;
     CB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     count_launch();
     return CUTE_B200_OK;
