@@ -62,28 +62,6 @@ __global__ void __launch_bounds__(LIST_THREADS) row_list_kernel(const int32_t *i
     }
 }
 
-// (rows, cols) -> (cols, rows) of each adapter's 16-bit matrix, 64 x 64 values per CTA; adapters without a row are left out.
-__global__ void __launch_bounds__(256) transpose_kernel(const uint16_t *in, uint16_t *out, int rows, int cols, const int32_t *first) {
-    __shared__ uint16_t tile[64][66];
-    ptx::griddep_wait();
-    ptx::griddep_launch_dependents();
-    const int per_col = (cols + 63) / 64, per_row = (rows + 63) / 64;
-    const int64_t block = blockIdx.x;
-    const int a = int(block / (per_col * per_row)), left = int(block % (per_col * per_row));
-    if (first[a] == first[a + 1]) return;
-    const int r0 = left / per_col * 64, c0 = left % per_col * 64;
-    const int64_t base = int64_t(a) * rows * cols;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        if (r0 + r < rows && c0 + c < cols) tile[r][c] = in[base + int64_t(r0 + r) * cols + c0 + c];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int c = i >> 6, r = i & 63;
-        if (r0 + r < rows && c0 + c < cols) out[base + int64_t(c0 + c) * rows + r0 + r] = tile[r][c];
-    }
-}
-
 constexpr int GRAD_THREADS = 192, GRAD_M = 128, GRAD_ROWS = 64, GRAD_STAGES = 4;
 constexpr uint32_t GRAD_BOX = GRAD_ROWS * 128, GRAD_RING = 96 * 1024, GRAD_HEAD = 1024;
 constexpr uint32_t GRAD_SMEM = 1024 + GRAD_HEAD + GRAD_RING;
@@ -105,14 +83,6 @@ struct GradHead {
     uint64_t full[GRAD_STAGES], empty[GRAD_STAGES], done, drain;
     uint32_t tmem, abort;
 };
-
-// Shared-memory matrix descriptor of an MN-major tile in 128-byte rows with the 128B swizzle: 64 values of M or N per
-// row, the rows are k.  Leading byte offset: from 64 values to the next 64 (one box); stride byte offset: from eight k
-// to the next eight.
-__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
-    return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(GRAD_BOX >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
-           (uint64_t(2) << 61);
-}
 
 __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -209,10 +179,10 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
                 if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) break;
                 ptx::tc_fence_after();
                 const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                const uint64_t wide = mn_desc(src), low = mn_desc(src + 2 * GRAD_BOX);
+                const uint64_t wide = mn_desc(src, GRAD_BOX), low = mn_desc(src + 2 * GRAD_BOX, GRAD_BOX);
 #pragma unroll
-                for (int j = 0; j < 4; j++)  // 16 rows of 128 bytes further
-                    ptx::umma_f16<1>(tmem, wide + 128u * j, low + 128u * j, p.idesc, (b > b0 || j > 0) ? 1u : 0u);
+                for (int j = 0; j < 4; j++)
+                    ptx::umma_f16<1>(tmem, wide + MN_K_STEP * j, low + MN_K_STEP * j, p.idesc, (b > b0 || j > 0) ? 1u : 0u);
                 issued = true;
                 ptx::umma_commit<1>(bar(h.empty[s]));
                 if (++s == p.stages) s = 0, ph ^= 1u;
@@ -293,13 +263,6 @@ cute_b200_status lora_row_lists(const int32_t *ids, int m, int adapters, int32_t
     return launch_dependent(row_list_kernel, dim3(unsigned(adapters)), LIST_THREADS, 0, 1, stream, ids, m, adapters, first, list);
 }
 
-cute_b200_status lora_transpose(const uint16_t *in, uint16_t *out, int adapters, int rows, int cols, const int32_t *first,
-                                cudaStream_t stream) {
-    const int64_t blocks = int64_t(adapters) * ((rows + 63) / 64) * ((cols + 63) / 64);
-    if (blocks > 0x7fffffff) return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "lora_tn_backward: the adapters are too large");
-    return launch_dependent(transpose_kernel, dim3(unsigned(blocks)), 256, 0, 1, stream, in, out, rows, cols, first);
-}
-
 cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream) {
     GradParams p = {};
     GradMaps maps;
@@ -318,7 +281,7 @@ cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const Devi
     p.stage_bytes = uint32_t(2 + (2 * g.rp + 63) / 64) * GRAD_BOX;
     p.stages = int(GRAD_RING / p.stage_bytes);
     if (p.stages > GRAD_STAGES) p.stages = GRAD_STAGES;
-    p.idesc = make_idesc(bf16, GRAD_M, 2 * g.rp) | (1u << 15) | (1u << 16);  // both operands MN-major
+    p.idesc = make_idesc(bf16, GRAD_M, 2 * g.rp) | IDESC_A_MN | IDESC_B_MN;
     p.tmem_cols = uint32_t(2 * g.rp);
     p.status = dev.status_word;
     p.debug = debug;

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS) shrink_rows_kernel(const LoraP
 // W and X do not depend on the kernel that computes T, which has waited for all
 // before it: they are loaded before griddepcontrol.wait, T and the ids after.
 constexpr int FEW_THREADS = 192, FEW_MAX_STAGES = 16, FEW_ROWS = 128;
-constexpr uint32_t FEW_HEAD = 4096;  // barriers, masks and ids, ahead of the ring
+constexpr uint32_t FEW_HEAD = 8192;  // barriers, masks and ids, ahead of the ring
 
 struct FewParams {
     const int32_t *ids;
@@ -105,7 +105,8 @@ struct FewHead {
     uint32_t tmem, abort;
     int32_t entries, entry_id[FEW_ROWS];
     uint32_t off[FEW_ROWS][4];  // lanes of entry e that keep their sums: bit set = not a row of this adapter
-    int32_t id[FEW_ROWS], before[4];
+    int32_t id[FEW_ROWS];
+    IdTable<FEW_ROWS> table;
 };
 static_assert(sizeof(FewHead) <= FEW_HEAD, "head");
 
@@ -341,38 +342,21 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         __syncwarp();
     } else {
         // The adapters the rows name, in the order of their first row.
-        const int row = threadIdx.x - 64, w = warp - 2;
+        const int row = threadIdx.x - 64;
         ptx::griddep_wait();
         int id = row < p.m ? p.ids[row] : -1;
         if (id < 0 || id >= p.adapters) id = -1;
         h.id[row] = id;
-        ptx::named_barrier(1, 128);
-        const uint32_t same = __match_any_sync(0xffffffffu, id);  // every lane takes part, those without an adapter too
-        bool first = id >= 0 && __ffs(same) - 1 == lane;
-        if (first)
-            for (int i = 0; i < 32 * w; i++)
-                if (h.id[i] == id) {
-                    first = false;
-                    break;
-                }
-        __syncwarp();
-        const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-        if (lane == 0) h.before[w] = __popc(firsts);
-        ptx::named_barrier(1, 128);
-        int at = __popc(firsts & ((1u << lane) - 1u)), total = 0;
-        for (int i = 0; i < 4; i++) {
-            if (i < w) at += h.before[i];
-            total += h.before[i];
-        }
-        if (first) h.entry_id[at] = id;
-        if (threadIdx.x == 64) h.entries = total;
-        ptx::named_barrier(1, 128);
-        for (int e = 0; e < (b_blocks > 0 ? total : 0); e++) {
-            const uint32_t mine = __ballot_sync(0xffffffffu, id == h.entry_id[e]);
-            if (lane == 0) h.off[e][w] = ~mine;
+        if (b_blocks > 0) {
+            for (int i = row; i < FEW_ROWS * 4; i += 128) h.off[i / 4][i % 4] = 0xffffffffu;
+            const int32_t ids[1] = {id};
+            int32_t mine[1];
+            const int total = distinct_ids<FEW_ROWS>(ids, h.table, row, mine, [&](int e, int which) { h.entry_id[e] = which; });
+            if (mine[0] >= 0) atomicAnd(&h.off[mine[0]][row / 32], ~(1u << (row % 32)));
+            if (row == 0) h.entries = total;
         }
         ptx::named_barrier(1, 128);
-        if (threadIdx.x == 64) ptx::mbar_arrive(bar(h.plan));
+        if (row == 0) ptx::mbar_arrive(bar(h.plan));
         if (b_blocks == 0) {
             float *t = reinterpret_cast<float *>(smem_raw + (low - raw)), *dots = t + (p.m + p.kc - 1) / p.kc * p.rp;
             if (p.bf16) few_dots<true>(p, h.id, t, dots, int(rank), n0, row);
@@ -494,15 +478,13 @@ uint64_t t_bytes(const cute_b200_lora_desc &d) { return round_up(uint64_t(d.m) *
 
 uint64_t plan_bytes(const cute_b200_lora_desc &d) { return round_up(lora_plan_bytes(d.m, d.adapters)) + kAlign; }
 
-// The backward call's workspace: U and the plan of its product, the adapters transposed, the row lists.
+// The backward call's workspace: U and the plan of its product, the row lists.
 struct BackLayout {
-    uint64_t at, bt, first, list, total;
+    uint64_t first, list, total;
 };
 BackLayout back_layout(const cute_b200_lora_desc &d) {
     BackLayout l;
-    l.at = t_bytes(d) + plan_bytes(d);
-    l.bt = l.at + round_up(uint64_t(d.adapters) * d.rank * d.k * 2);
-    l.first = l.bt + round_up(uint64_t(d.adapters) * d.rank * d.n * 2);
+    l.first = t_bytes(d) + plan_bytes(d);
     l.list = l.first + round_up((uint64_t(d.adapters) + 1) * 4);
     l.total = l.list + round_up(uint64_t(d.m) * 4) + kAlign;
     return l;
@@ -529,8 +511,8 @@ cute_b200_status check_desc(const cute_b200_lora_desc &d, const char *who) {
         return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: ldx must be 0 or a multiple of 8 of at least k = %d, got %d", who, d.k, d.ldx);
     if (d.ldy != 0 && d.ldy < d.n)
         return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: ldy must be 0 or at least n = %d, got %d", who, d.n, d.ldy);
-    if (d.tuning[0] < 0 || d.tuning[0] > 5 || (d.tuning[0] == 1 && d.m > 128))
-        return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: tuning[0] must be 0, 1 (with m <= 128) or 2 to 5, got %d", who, d.tuning[0]);
+    if (d.tuning[0] < 0 || d.tuning[0] > 6 || (d.tuning[0] == 1 && d.m > 128))
+        return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "%s: tuning[0] must be 0, 1 (with m <= 128) or 2 to 6, got %d", who, d.tuning[0]);
     return CUTE_B200_OK;
 }
 
@@ -624,16 +606,14 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
     }
     uint16_t *u = reinterpret_cast<uint16_t *>(ptr[11]);
     const BackLayout l = back_layout(d);
-    uint16_t *at = reinterpret_cast<uint16_t *>(ptr[11] + l.at), *bt = reinterpret_cast<uint16_t *>(ptr[11] + l.bt);
     int32_t *first = reinterpret_cast<int32_t *>(ptr[11] + l.first), *list = reinterpret_cast<int32_t *>(ptr[11] + l.list);
     CB_TRY(lora_row_lists(reinterpret_cast<const int32_t *>(ptr[4]), d.m, d.adapters, first, list, stream));
-    if (ptr[8]) CB_TRY(lora_transpose(reinterpret_cast<const uint16_t *>(ptr[2]), at, d.adapters, d.rank, d.k, first, stream));
-    CB_TRY(lora_transpose(reinterpret_cast<const uint16_t *>(ptr[3]), bt, d.adapters, d.n, d.rank, first, stream));
     LoraParams p = {};
     p.x = reinterpret_cast<const uint16_t *>(ptr[6]);
     p.w = reinterpret_cast<const uint16_t *>(ptr[1]);
-    p.a = bt;
-    p.b = at;
+    p.a = reinterpret_cast<const uint16_t *>(ptr[3]);
+    p.b = reinterpret_cast<const uint16_t *>(ptr[2]);
+    p.low_mn = true;
     p.ids = reinterpret_cast<const int32_t *>(ptr[4]);
     p.scale = reinterpret_cast<const float *>(ptr[5]);
     p.y = reinterpret_cast<void *>(ptr[8]);
@@ -642,7 +622,7 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
     p.m = d.m, p.n = d.k, p.k = d.n, p.rank = d.rank, p.rp = padded_rank(d.rank), p.adapters = d.adapters, p.c_dtype = d.c_dtype;
     p.ldx = ldy;
     p.ldy = ldx;
-    CB_TRY(forward(p, bf16, d.tuning, dev, stream));
+    CB_TRY(lora_tiled(p, bf16, d.tuning[0] - 3, d.tuning[1], dev, stream));
     if (da) {
         LoraGrads g = {};
         g.out[0] = da, g.out[1] = db;

@@ -14,9 +14,12 @@ struct LoraParams {
     uint32_t *plan; // which adapters each tile of rows names (tiled kernels)
     int m, n, k, rank, rp, adapters, c_dtype;
     int64_t ldx, ldy;
+    // The backward product: `a` is (adapters, k, rank) and `b` (adapters, rank, n), the forward's matrices as they lie, read
+    // as MN-major operands; and the kernel before T's is one that T's need not wait for (the row lists).
+    bool low_mn;
 };
 
-// The tiled forward product (any m; cut 0..2 names a tile, a negative one chooses) and the bytes of its plan.
+// The tiled forward product (any m; cut 0..3 names a tile, a negative one chooses) and the bytes of its plan.
 cute_b200_status lora_tiled(const LoraParams &p, bool bf16, int cut, int debug, const DeviceState &dev, cudaStream_t stream);
 uint64_t lora_plan_bytes(int m, int adapters);
 cute_b200_status lora_tiled_init();
@@ -30,8 +33,6 @@ struct LoraGrads {
     const int32_t *first, *list;
 };
 cute_b200_status lora_row_lists(const int32_t *ids, int m, int adapters, int32_t *first, int32_t *list, cudaStream_t stream);
-cute_b200_status lora_transpose(const uint16_t *in, uint16_t *out, int adapters, int rows, int cols, const int32_t *first,
-                                cudaStream_t stream);
 cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream);
 cute_b200_status lora_grad_init();
 
@@ -45,6 +46,60 @@ __device__ __forceinline__ void store_c(void *c, int dtype, size_t i, float v) {
 
 // Width of the rank in T: 16, 32, 64 or 128.
 __host__ __device__ constexpr int padded_rank(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
+
+// First occurrences of ids by a hash table in shared memory.
+template <int ROWS>
+struct IdTable {
+    static constexpr int SIZE = 2 * ROWS;  // a power of two: at most half full, so a probe ends
+    int32_t key[SIZE], first[SIZE], entry[SIZE], before[4];
+};
+
+// The distinct ids of ROWS rows (128, 256 or 512; negative = none) in the order of their first row, by 128 threads that all
+// call this: thread t holds rows t, t + 128, ..  emit(e, id) receives the list; mine[i] becomes the place in it of row
+// t + 128 i (-1 = none).  Returns the length.  The order does not depend on timing: `first` is a minimum over rows.
+template <int ROWS, typename Emit>
+__device__ __forceinline__ int distinct_ids(const int32_t (&id)[ROWS / 128], IdTable<ROWS> &h, int t, int32_t (&mine)[ROWS / 128], Emit emit) {
+    constexpr int N = ROWS / 128;
+    const int lane = t & 31, w = t >> 5;
+    for (int i = t; i < h.SIZE; i += 128) h.key[i] = -1, h.first[i] = 0x7fffffff;
+    ptx::named_barrier(1, 128);
+    uint32_t slot[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        slot[i] = (uint32_t(id[i]) * 2654435761u) & uint32_t(h.SIZE - 1);
+        if (id[i] >= 0) {
+            for (;;) {
+                const int old = atomicCAS(&h.key[slot[i]], -1, id[i]);
+                if (old == -1 || old == id[i]) break;
+                slot[i] = (slot[i] + 1u) & uint32_t(h.SIZE - 1);
+            }
+            atomicMin(&h.first[slot[i]], t + 128 * i);
+        }
+    }
+    ptx::named_barrier(1, 128);
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const bool first = id[i] >= 0 && h.first[slot[i]] == t + 128 * i;
+        __syncwarp();
+        const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+        if (lane == 0) h.before[w] = __popc(firsts);
+        ptx::named_barrier(1, 128);
+        int at = total + __popc(firsts & ((1u << lane) - 1u));
+        for (int j = 0; j < 4; j++) {
+            if (j < w) at += h.before[j];
+            total += h.before[j];
+        }
+        if (first) {
+            h.entry[slot[i]] = at;
+            emit(at, id[i]);
+        }
+        ptx::named_barrier(1, 128);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) mine[i] = id[i] >= 0 ? h.entry[slot[i]] : -1;
+    return total;
+}
 
 // An adapter's part of the product runs over the 2 rp columns of T in blocks of
 // 64: block q pairs columns t_col.. of T with columns b_col.. of B; `steps` MMAs

@@ -20,79 +20,56 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 // a cluster.  M = the rows, N = the padded rank: every adapter's MMAs are masked to
 // the lanes of its rows, so one accumulator serves all of them.  Bound by reading X
 // (and, where nearly every row has an adapter of its own, A).
-//   warp 0  TMA: per k block a (128 x 64) block of X into one ring, then for every
-//           adapter of the tile a (rp x 64) block of A into another.
-//   warp 1  MMA.   warps 2-5  plan (own rows for the masks; the cluster's first CTA also
+//   warp 0  TMA: per k block a (128 x 64) block of X into one ring, then the blocks
+//           of A of the tile's adapters into another, 16 KB of them per stage, a lane each.
+//   warp 1  MMA.   warps 2-5  the adapters the rows name (and, by the cluster's first CTA,
 //           the plan of the GEMM's tile that starts at its rows), then the sum over the
 //           cluster, scale, split into two 16-bit numbers.
-constexpr int SHRINK_THREADS = 192, X_STAGES = 7, A_STAGES = 16;
-constexpr uint32_t X_BYTES = BM * BK * 2, A_RING = 64 * 1024, SHRINK_HEAD = 8192;
-constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + X_STAGES * X_BYTES + A_RING;
+// On the way back A is B[a] as it lies, (n, rank): rank is the fast index, so it is an MN-major operand.
+constexpr int SHRINK_THREADS = 192, X_STAGES = 7, A_STAGES = 5;
+constexpr uint32_t X_BYTES = BM * BK * 2, A_BYTES = 16 * 1024, SHRINK_HEAD = 20 * 1024;
+constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + X_STAGES * X_BYTES + A_STAGES * A_BYTES;
 
 struct ShrinkParams {
     const int32_t *ids;
     const float *scale;
     uint16_t *t;
     uint32_t *plan;
-    int m, rank, rp, adapters, k_blocks, kc, plan_rows, a_stages;
+    int m, rank, rp, adapters, k_blocks, kc;
+    int boxes;       // of A per adapter and k block
+    uint32_t box_bytes;
     uint32_t idesc, tmem_cols;
+    bool bf16, mn, early;
     uint32_t *status;
     int debug;
 };
 
+template <int P>
 struct ShrinkHead {
     uint64_t xfull[X_STAGES], xempty[X_STAGES], afull[A_STAGES], aempty[A_STAGES], plan, done, drain;
     uint32_t tmem, abort;
-    int32_t entries, entry_id[BM], before[4];
+    int32_t entries, entry_id[BM], id[BM];
     uint32_t off[BM][4];
-    int32_t id[BM], wide[512];  // this CTA's rows; the rows of the GEMM's tile
+    IdTable<128> rows;  // of this CTA's rows
+    IdTable<P> tile;    // of the GEMM's tile
 };
-static_assert(sizeof(ShrinkHead) <= SHRINK_HEAD, "head");
 
-// Which of `rows` (a multiple of 128, at most 512) ids are the first of their kind, and the list of those, by 128 threads:
-// thread `t` holds rows t, t + 128, ..  `id` is in shared memory, negative = none.  `emit(e, id)` receives the list,
-// the count is returned to every thread.
-template <typename Emit>
-__device__ __forceinline__ int distinct_ids(const int32_t *id, int rows, int t, int32_t (&before)[4], Emit emit) {
-    const int lane = t & 31, w = t >> 5;
-    int total = 0;
-    for (int r0 = 0; r0 < rows; r0 += 128) {
-        const int r = r0 + t, mine = id[r];
-        bool first = mine >= 0 && (r == 0 || id[r - 1] != mine);
-        if (first)
-            for (int i = 0; i + 1 < r; i++)
-                if (id[i] == mine) {
-                    first = false;
-                    break;
-                }
-        __syncwarp();
-        const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-        if (lane == 0) before[w] = __popc(firsts);
-        ptx::named_barrier(1, 128);
-        int at = total + __popc(firsts & ((1u << lane) - 1u));
-        for (int i = 0; i < 4; i++) {
-            if (i < w) at += before[i];
-            total += before[i];
-        }
-        if (first) emit(at, mine);
-        ptx::named_barrier(1, 128);
-    }
-    return total;
-}
-
-template <bool BF16>
+template <int P>
 __global__ void __launch_bounds__(SHRINK_THREADS, 1)
     shrink_tile_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA, const ShrinkParams p) {
+    static_assert(sizeof(ShrinkHead<P>) <= SHRINK_HEAD, "head");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    ShrinkHead &h = *reinterpret_cast<ShrinkHead *>(smem_raw + (base - raw));
-    const uint32_t xring = base + SHRINK_HEAD, aring = xring + X_STAGES * X_BYTES, a_bytes = uint32_t(p.rp) * 128u;
+    ShrinkHead<P> &h = *reinterpret_cast<ShrinkHead<P> *>(smem_raw + (base - raw));
+    const uint32_t xring = base + SHRINK_HEAD, aring = xring + X_STAGES * X_BYTES;
     auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
     volatile uint32_t *abort_flag = &h.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = p.kc > 1 ? ptx::cluster_ctarank() : 0u;
-    const int tile = int(blockIdx.x) / p.kc, row0 = tile * BM;
+    const int row0 = int(blockIdx.x) / p.kc * BM;
     const int kb0 = int(int64_t(p.k_blocks) * rank / p.kc), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / p.kc);
+    const uint32_t entry_bytes = uint32_t(p.boxes) * p.box_bytes;
+    const int group = int(A_BYTES / entry_bytes);  // adapters per stage of A: 1 to 8
     const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
 
     if (threadIdx.x == 0) {
@@ -118,67 +95,97 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&h.tmem);
-    ptx::griddep_wait();
+    // early: nothing here depends on the kernel before, which has waited for all before it; it is waited for at the end.
+    if (!p.early) ptx::griddep_wait();
     if (threadIdx.x == 0) ptx::griddep_launch_dependents();
 
     if (warp == 0) {
         if (lane == 0) {
             ptx::prefetch_tensormap(&tmX);
             ptx::prefetch_tensormap(&tmA);
-            bool ok = !(p.debug & 4) && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit);
-            const int entries = ok ? h.entries : 0;
-            int sx = 0, sa = 0;
-            uint32_t px = 0, pa = 0, xfilled = 0, xparity = 0, afilled = 0, aparity = 0;
-            for (int kb = kb0; kb < kb1 && ok && entries > 0; kb++) {
-                if (!(ok = wait_bar(bar(h.xempty[sx]), px ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(sx), limit))) break;
+        }
+        bool ok = !(p.debug & 4);
+        ok = __all_sync(0xffffffffu, ok && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit));
+        const int entries = ok ? h.entries : 0, my_e = lane / p.boxes, my_box = lane % p.boxes;
+        int sx = 0, sa = 0;
+        uint32_t px = 0, pa = 0, xfilled = 0, xparity = 0, afilled = 0, aparity = 0;
+        for (int kb = kb0; kb < kb1 && ok && entries > 0; kb++) {
+            ok = __all_sync(0xffffffffu, wait_bar(bar(h.xempty[sx]), px ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(sx), limit));
+            if (!ok) break;
+            if (lane == 0) {
                 ptx::mbar_arrive_expect_tx(bar(h.xfull[sx]), X_BYTES);
                 ptx::tma_load_2d(xring + uint32_t(sx) * X_BYTES, &tmX, bar(h.xfull[sx]), kb * BK, row0);
-                xfilled |= 1u << sx, xparity = (xparity & ~(1u << sx)) | (px << sx);
-                if (++sx == X_STAGES) sx = 0, px ^= 1u;
-                for (int e = 0; e < entries; e++) {
-                    if (!(ok = wait_bar(bar(h.aempty[sa]), pa ^ 1u, abort_flag, p.status, WHERE_PRODUCER, 32u + uint32_t(sa), limit))) break;
-                    ptx::mbar_arrive_expect_tx(bar(h.afull[sa]), a_bytes);
-                    ptx::tma_load_2d(aring + uint32_t(sa) * a_bytes, &tmA, bar(h.afull[sa]), kb * BK, h.entry_id[e] * p.rank);
-                    afilled |= 1u << sa, aparity = (aparity & ~(1u << sa)) | (pa << sa);
-                    if (++sa == p.a_stages) sa = 0, pa ^= 1u;
+            }
+            __syncwarp();
+            xfilled |= 1u << sx, xparity = (xparity & ~(1u << sx)) | (px << sx);
+            if (++sx == X_STAGES) sx = 0, px ^= 1u;
+            for (int e0 = 0; e0 < entries; e0 += group) {
+                ok = __all_sync(0xffffffffu, wait_bar(bar(h.aempty[sa]), pa ^ 1u, abort_flag, p.status, WHERE_PRODUCER, 32u + uint32_t(sa), limit));
+                if (!ok) break;
+                const int count = min(group, entries - e0);
+                if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.afull[sa]), uint32_t(count) * entry_bytes);
+                __syncwarp();
+                if (my_e < count) {
+                    const int id = h.entry_id[e0 + my_e];
+                    const uint32_t dst = aring + uint32_t(sa) * A_BYTES + uint32_t(lane) * p.box_bytes;
+                    if (p.mn) ptx::tma_load_3d(dst, &tmA, bar(h.afull[sa]), 64 * my_box, kb * BK, id);
+                    else ptx::tma_load_2d(dst, &tmA, bar(h.afull[sa]), kb * BK, id * p.rank);
                 }
+                __syncwarp();
+                afilled |= 1u << sa, aparity = (aparity & ~(1u << sa)) | (pa << sa);
+                if (++sa == A_STAGES) sa = 0, pa ^= 1u;
             }
-            if (!ok) {  // giving up: let the copies in flight land (bounded)
-                const uint64_t t0 = ptx::globaltimer_ns();
-                for (int i = 0; i < X_STAGES; i++)
-                    while ((xfilled >> i & 1u) && !ptx::mbar_try_wait(bar(h.xfull[i]), (xparity >> i) & 1u))
-                        if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
-                for (int i = 0; i < A_STAGES; i++)
-                    while ((afilled >> i & 1u) && !ptx::mbar_try_wait(bar(h.afull[i]), (aparity >> i) & 1u))
-                        if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
-            }
+        }
+        if (!ok && lane == 0) {  // giving up: let the copies in flight land (bounded)
+            const uint64_t t0 = ptx::globaltimer_ns();
+            for (int i = 0; i < X_STAGES; i++)
+                while ((xfilled >> i & 1u) && !ptx::mbar_try_wait(bar(h.xfull[i]), (xparity >> i) & 1u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+            for (int i = 0; i < A_STAGES; i++)
+                while ((afilled >> i & 1u) && !ptx::mbar_try_wait(bar(h.afull[i]), (aparity >> i) & 1u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            bool ok = wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit), issued = false;
-            const int entries = ok ? h.entries : 0;
-            int sx = 0, sa = 0;
-            uint32_t px = 0, pa = 0;
-            for (int kb = kb0; kb < kb1 && ok && entries > 0; kb++) {
-                if (!(ok = wait_bar(bar(h.xfull[sx]), px, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(sx), limit))) break;
-                const uint64_t a = sw128_desc(xring + uint32_t(sx) * X_BYTES);
-                for (int e = 0; e < entries; e++) {
-                    if (!(ok = wait_bar(bar(h.afull[sa]), pa, abort_flag, p.status, WHERE_MMA_FULL, 32u + uint32_t(sa), limit))) break;
-                    ptx::tc_fence_after();
-                    const uint64_t b = sw128_desc(aring + uint32_t(sa) * a_bytes);
-                    const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * j, p.idesc, (kb > kb0 || j > 0) ? 1u : 0u, o0, o1, o2, o3);
-                    issued = true;
-                    ptx::umma_commit<1>(bar(h.aempty[sa]));
-                    if (++sa == p.a_stages) sa = 0, pa ^= 1u;
-                }
+        // The whole warp runs the loop and one thread issues: see lora_few_kernel.
+        const bool leader = ptx::elect_one();
+        bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit)), issued = false;
+        const int entries = ok ? h.entries : 0;
+        int sx = 0, sa = 0;
+        uint32_t px = 0, pa = 0;
+        for (int kb = kb0; kb < kb1 && ok && entries > 0; kb++) {
+            ok = __all_sync(0xffffffffu, wait_bar(bar(h.xfull[sx]), px, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(sx), limit));
+            if (!ok) break;
+            const uint64_t a = sw128_desc(xring + uint32_t(sx) * X_BYTES);
+            const uint32_t more = kb > kb0 ? 1u : 0u;
+            for (int e0 = 0; e0 < entries; e0 += group) {
+                ok = __all_sync(0xffffffffu, wait_bar(bar(h.afull[sa]), pa, abort_flag, p.status, WHERE_MMA_FULL, 32u + uint32_t(sa), limit));
                 if (!ok) break;
-                ptx::umma_commit<1>(bar(h.xempty[sx]));
-                if (++sx == X_STAGES) sx = 0, px ^= 1u;
+                ptx::tc_fence_after();
+                const int count = min(group, entries - e0);
+                for (int e = 0; e < count; e++) {
+                    const uint32_t src = aring + uint32_t(sa) * A_BYTES + uint32_t(e) * entry_bytes;
+                    const uint64_t b = p.mn ? mn_desc(src, p.box_bytes) : sw128_desc(src);
+                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u;
+                    const uint32_t o0 = h.off[e0 + e][0], o1 = h.off[e0 + e][1], o2 = h.off[e0 + e][2], o3 = h.off[e0 + e][3];
+                    if (leader) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            ptx::umma_f16_lanes(tmem, a + 2u * j, b + k_step * j, p.idesc, j > 0 ? 1u : more, o0, o1, o2, o3);
+                    }
+                    __syncwarp();
+                }
+                issued = true;
+                if (leader) ptx::umma_commit<1>(bar(h.aempty[sa]));
+                __syncwarp();
+                if (++sa == A_STAGES) sa = 0, pa ^= 1u;
             }
+            if (!ok) break;
+            if (leader) ptx::umma_commit<1>(bar(h.xempty[sx]));
+            __syncwarp();
+            if (++sx == X_STAGES) sx = 0, px ^= 1u;
+        }
+        if (leader) {
             if (ok) {
                 ptx::umma_commit<1>(bar(h.done));
             } else if (issued) {
@@ -190,39 +197,36 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         }
         __syncwarp();
     } else {
-        const int t = threadIdx.x - 64, w = t >> 5;
+        const int t = threadIdx.x - 64;
         auto read_id = [&](int row) {
-            const int id = row < p.m ? p.ids[row] : -1;
+            const int id = row < p.m ? __ldcg(p.ids + row) : -1;
             return id < 0 || id >= p.adapters ? -1 : id;
         };
-        h.id[t] = read_id(row0 + t);
-        ptx::named_barrier(1, 128);
-        const int total = distinct_ids(h.id, 128, t, h.before, [&](int e, int id) { h.entry_id[e] = id; });
-        if (t == 0) h.entries = total;
-        for (int e = 0; e < total; e++) {
-            const uint32_t mine = __ballot_sync(0xffffffffu, h.id[t] == h.entry_id[e]);
-            if (lane == 0) h.off[e][w] = ~mine;
-        }
-        ptx::named_barrier(1, 128);
-        if (t == 0) ptx::mbar_arrive(bar(h.plan));
-        // The GEMM's plan, by the first CTA of the cluster at the tile's first 128 rows.
-        if (rank == 0 && row0 % p.plan_rows == 0) {
-            const int P = p.plan_rows, words = P / 32;
-            uint32_t *plan = p.plan + uint64_t(row0 / P) * plan_stride(P, p.adapters);
-            for (int i = t; i < P; i += 128) h.wide[i] = read_id(row0 + i);
+        {
+            const int32_t ids[1] = {read_id(row0 + t)};
+            int32_t mine[1];
+            h.id[t] = ids[0];
+            for (int i = t; i < BM * 4; i += 128) h.off[i / 4][i % 4] = 0xffffffffu;
+            const int total = distinct_ids<128>(ids, h.rows, t, mine, [&](int e, int id) { h.entry_id[e] = id; });
+            if (mine[0] >= 0) atomicAnd(&h.off[mine[0]][t / 32], ~(1u << (t % 32)));
+            if (t == 0) h.entries = total;
             ptx::named_barrier(1, 128);
-            const int count = distinct_ids(h.wide, P, t, h.before, [&](int e, int id) { plan[4 + e * (4 + words)] = uint32_t(id); });
+            if (t == 0) ptx::mbar_arrive(bar(h.plan));
+        }
+        if (rank == 0 && row0 % P == 0 && p.plan) {
+            constexpr int WORDS = P / 32, ENTRY = 4 + WORDS;
+            uint32_t *plan = p.plan + uint64_t(row0 / P) * plan_stride(P, p.adapters);
+            int32_t ids[P / 128], mine[P / 128];
+#pragma unroll
+            for (int i = 0; i < P / 128; i++) ids[i] = read_id(row0 + t + 128 * i);
+            const int count = distinct_ids<P>(ids, h.tile, t, mine, [&](int e, int id) { plan[4 + e * ENTRY] = uint32_t(id); });
             if (t == 0) plan[0] = uint32_t(count);
-            __threadfence_block();
-            ptx::named_barrier(1, 128);  // the ids above are read below by the other threads
-            for (int e = 0; e < count; e++) {
-                uint32_t *entry = plan + 4 + e * (4 + words);
-                const int id = int(*reinterpret_cast<volatile uint32_t *>(entry));
-                for (int r0 = 0; r0 < P; r0 += 128) {
-                    const uint32_t mine = __ballot_sync(0xffffffffu, h.wide[r0 + t] == id);
-                    if (lane == 0) entry[4 + r0 / 32 + w] = ~mine;
-                }
-            }
+            for (int i = t; i < count * WORDS; i += 128) plan[4 + i / WORDS * ENTRY + 4 + i % WORDS] = 0xffffffffu;
+            __threadfence();  // the words above are in place before another thread clears bits of them
+            ptx::named_barrier(1, 128);
+#pragma unroll
+            for (int i = 0; i < P / 128; i++)
+                if (mine[i] >= 0) atomicAnd(plan + 4 + mine[i] * ENTRY + 4 + (t + 128 * i) / 32, ~(1u << (t % 32)));
         }
         // Partial sums to shared memory: the rings are idle.
         const bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.done), 0, abort_flag, p.status, WHERE_EPILOGUE, 0u, limit));
@@ -258,19 +262,19 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             if (row0 + row >= p.m) break;
             const int id = h.id[row];
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (id >= 0 && col < p.rank) {  // lanes of rows without an adapter hold nothing; past the rank lie the next adapter's sums
-                const uint32_t at = xring + uint32_t(row) * pitch + uint32_t(col) * 4u;
-                v = cluster_sum(at, p.kc);
-                const float s = p.scale[id];
+            if (id >= 0 && col < p.rank) {  // lanes of rows without an adapter hold nothing; past the rank may lie another adapter's sums
+                v = cluster_sum(xring + uint32_t(row) * pitch + uint32_t(col) * 4u, p.kc);
+                const float s = __ldcg(p.scale + id);
                 v.x *= s, v.y *= s, v.z *= s, v.w *= s;
             }
-            const uint32_t h0 = pack_16(v.x, v.y, BF16), h1 = pack_16(v.z, v.w, BF16);
-            const float2 f0 = pair_f32<BF16>(h0), f1 = pair_f32<BF16>(h1);
+            const uint32_t h0 = pack_16(v.x, v.y, p.bf16), h1 = pack_16(v.z, v.w, p.bf16);
+            const float2 f0 = p.bf16 ? pair_f32<true>(h0) : pair_f32<false>(h0), f1 = p.bf16 ? pair_f32<true>(h1) : pair_f32<false>(h1);
             uint16_t *t = p.t + int64_t(row0 + row) * 2 * p.rp + col;
             *reinterpret_cast<uint2 *>(t) = make_uint2(h0, h1);
-            *reinterpret_cast<uint2 *>(t + p.rp) = make_uint2(pack_16(v.x - f0.x, v.y - f0.y, BF16), pack_16(v.z - f1.x, v.w - f1.y, BF16));
+            *reinterpret_cast<uint2 *>(t + p.rp) = make_uint2(pack_16(v.x - f0.x, v.y - f0.y, p.bf16), pack_16(v.z - f1.x, v.w - f1.y, p.bf16));
         }
     }
+    if (p.early) ptx::griddep_wait();
     __syncthreads();
     if (p.kc > 1) {
         ptx::cluster_arrive();
@@ -284,6 +288,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
 // ring of 192 KiB.  G: CTAs per MMA; BN: columns per tile; MH: 128-row accumulators per CTA.  Behind a tile's k blocks
 // of W come, for every adapter its rows name, the blocks of T (in place of X) and of B[a] (in place of W), their MMAs
 // masked to the lanes of the adapter's rows.  One adapter of rank 64 costs 2 blocks beside the 64 of k = 4096.
+// On the way back B is A[a] as it lies, (rank, k): an MN-major operand, in boxes of 64 columns by up to 64 ranks.
 constexpr uint32_t RING_BYTES = 192 * 1024;
 constexpr int TILE_THREADS = 64 + 256;
 
@@ -308,7 +313,7 @@ struct TileParams {
     int64_t ldy;
     int m, n, rank, rp, adapters, c_dtype, vec;
     int k_blocks, m_tiles, n_tiles, group_m;
-    uint32_t idesc;
+    uint32_t idesc, low_idesc, low_box;  // low_box: bytes of an MN-major box of B, 0 = B is K-major
     uint32_t *status;
     int debug;
 };
@@ -415,70 +420,87 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             ptx::prefetch_tensormap(&tmW);
             ptx::prefetch_tensormap(&tmT);
             ptx::prefetch_tensormap(&tmB);
-            int s = 0;
-            uint32_t ph = 0, filled = 0, filled_parity = 0;
-            bool ok = !(p.debug & 4), waited = false;
-            // One stage of `nk` k blocks from column ax of `rows` and bx of `weights`.
-            auto load = [&](int nk, const CUtensorMap *rows, int ax, int ay, const CUtensorMap *weights, int bx, int by) {
-                if (!wait_bar(empty_bar(s), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit)) return false;
-                const uint32_t dst = ring + uint32_t(s) * C::STAGE_BYTES;
-                if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(s), uint32_t(nk) * C::EXPECT);
-                const uint32_t bar = G == 1 ? full_bar(s) : ptx::mapa(full_bar(s), 0);
-#pragma unroll
-                for (int kk = 0; kk < C::KPS; kk++)
-                    if (kk < nk) {
-                        if constexpr (G == 1) {
-                            ptx::tma_load_2d(dst + kk * C::KB_BYTES, rows, bar, ax + kk * BK, ay);
-                            ptx::tma_load_2d(dst + kk * C::KB_BYTES + C::A_BYTES, weights, bar, bx + kk * BK, by);
-                        } else {
-                            ptx::tma_load_2d_pair(dst + kk * C::KB_BYTES, rows, bar, ax + kk * BK, ay);
-                            ptx::tma_load_2d_pair(dst + kk * C::KB_BYTES + C::A_BYTES, weights, bar, bx + kk * BK, by);
-                        }
+        }
+        int s = 0;
+        uint32_t ph = 0, filled = 0, filled_parity = 0;
+        bool ok = !(p.debug & 4), waited = false;
+        // Waits for the next stage and announces `bytes` per CTA.
+        auto next = [&](uint32_t bytes) {
+            ok = __all_sync(0xffffffffu, wait_bar(empty_bar(s), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit));
+            if (ok && lane == 0 && rank == 0) ptx::mbar_arrive_expect_tx(full_bar(s), uint32_t(G) * bytes);
+            __syncwarp();
+            return ok;
+        };
+        auto issued = [&] {
+            __syncwarp();
+            filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
+            if (++s == C::STAGES) s = 0, ph ^= 1u;
+        };
+        auto load = [&](uint32_t dst, const CUtensorMap *map, int x, int y) {
+            if constexpr (G == 1) ptx::tma_load_2d(dst, map, full_bar(s), x, y);
+            else ptx::tma_load_2d_pair(dst, map, ptx::mapa(full_bar(s), 0), x, y);
+        };
+        const uint32_t low_bytes = p.low_box ? uint32_t(C::B_ROWS / 64) * p.low_box : C::B_BYTES;
+        for (int t = first; t < tiles && ok; t += step) {
+            const TileAt at = tile_at(t, p);
+            const int row = at.tm * C::ROWS + int(rank) * C::CTA_ROWS, col = at.tn * BN + int(rank) * C::B_ROWS;
+            const int kk = lane >> 1;  // lane 2 kk issues k block kk of X, lane 2 kk + 1 that of W
+            for (int kb = 0; kb < p.k_blocks && ok; kb += C::KPS) {
+                const int nk = min(C::KPS, p.k_blocks - kb);
+                if (!next(uint32_t(nk) * C::KB_BYTES)) break;
+                const uint32_t dst = ring + uint32_t(s) * C::STAGE_BYTES + uint32_t(kk) * C::KB_BYTES;
+                if (kk < nk) load(dst + (lane & 1 ? C::A_BYTES : 0u), lane & 1 ? &tmW : &tmX, (kb + kk) * BK, lane & 1 ? col : row);
+                issued();
+            }
+            if (!ok) break;
+            if (!waited) ptx::griddep_wait(), waited = true;  // T and the plan; X and W are older than their kernel
+            const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
+            const int entries = int(plan[0]);
+            for (int e = 0; e < entries && ok; e++) {
+                const int id = int(plan[4 + e * ENTRY]);
+                for (int q = 0; q < q_blocks; q++) {
+                    const ExtBlock b = ext_block(q, p.rp, p.rank);
+                    if (!next(C::A_BYTES + low_bytes)) break;
+                    const uint32_t dst = ring + uint32_t(s) * C::STAGE_BYTES;
+                    if (lane == 0) load(dst, &tmT, b.t_col, row);
+                    if (p.low_box == 0) {
+                        if (lane == 1) load(dst + C::A_BYTES, &tmB, b.b_col, id * p.n + col);
+                    } else if (lane >= 1 && lane <= C::B_ROWS / 64) {
+                        const uint32_t to = dst + C::A_BYTES + uint32_t(lane - 1) * p.low_box;
+                        if constexpr (G == 1) ptx::tma_load_3d(to, &tmB, full_bar(s), col + 64 * (lane - 1), b.b_col, id);
+                        else ptx::tma_load_3d_pair(to, &tmB, ptx::mapa(full_bar(s), 0), col + 64 * (lane - 1), b.b_col, id);
                     }
-                filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
-                if (++s == C::STAGES) s = 0, ph ^= 1u;
-                return true;
-            };
-            for (int t = first; t < tiles && ok; t += step) {
-                const TileAt at = tile_at(t, p);
-                const int row = at.tm * C::ROWS + int(rank) * C::CTA_ROWS, col = at.tn * BN + int(rank) * C::B_ROWS;
-                for (int kb = 0; kb < p.k_blocks && ok; kb += C::KPS)
-                    ok = load(min(C::KPS, p.k_blocks - kb), &tmX, kb * BK, row, &tmW, kb * BK, col);
-                if (!ok) break;
-                if (!waited) ptx::griddep_wait(), waited = true;  // T and the plan; X and W are older than their kernel
-                const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
-                const int entries = int(plan[0]);
-                for (int e = 0; e < entries && ok; e++) {
-                    const int id = int(plan[4 + e * ENTRY]);
-                    for (int q = 0; q < q_blocks && ok; q++) {
-                        const ExtBlock b = ext_block(q, p.rp, p.rank);
-                        ok = load(1, &tmT, b.t_col, row, &tmB, b.b_col, id * p.n + col);
-                    }
+                    issued();
                 }
             }
-            if (!ok && rank == 0) {  // giving up: let the copies in flight land (bounded)
-                const uint64_t t0 = ptx::globaltimer_ns();
-                for (int i = 0; i < C::STAGES; i++)
-                    while ((filled >> i & 1u) && !ptx::mbar_try_wait(full_bar(i), (filled_parity >> i) & 1u))
-                        if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
-            }
-            if (!waited) ptx::griddep_wait();
         }
+        if (!ok && rank == 0 && lane == 0) {  // giving up: let the copies in flight land (bounded)
+            const uint64_t t0 = ptx::globaltimer_ns();
+            for (int i = 0; i < C::STAGES; i++)
+                while ((filled >> i & 1u) && !ptx::mbar_try_wait(full_bar(i), (filled_parity >> i) & 1u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+        }
+        if (!waited) ptx::griddep_wait();
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            // The whole warp runs the loop and one thread issues: see lora_few_kernel.
+            const bool leader = ptx::elect_one();
             int s = 0, it = 0;
             uint32_t ph = 0;
             bool ok = true, issued = false, waited = false;
             auto ready = [&] {
-                if (!wait_bar(full_bar(s), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit)) return false;
+                ok = __all_sync(0xffffffffu, wait_bar(full_bar(s), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
                 ptx::tc_fence_after();
-                return true;
+                return ok;
             };
             auto free_stage = [&] {
                 issued = true;
-                ptx::umma_commit<G>(empty_bar(s));
-                if constexpr (G == 2) ptx::umma_commit<G>(ptx::mapa(empty_bar(s), 1));
+                if (leader) {
+                    ptx::umma_commit<G>(empty_bar(s));
+                    if constexpr (G == 2) ptx::umma_commit<G>(ptx::mapa(empty_bar(s), 1));
+                }
+                __syncwarp();
                 if (++s == C::STAGES) s = 0, ph ^= 1u;
             };
             for (int t = first; t < tiles && ok; t += step, it++) {
@@ -486,7 +508,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 const int buf = it % C::ACC_BUFS;
                 const uint32_t aph = uint32_t(it / C::ACC_BUFS) & 1u, d = tmem + uint32_t(buf * C::ACC_COLS);
                 for (int k0 = 0; k0 < p.k_blocks; k0 += C::KPS) {
-                    if (!(ok = ready())) break;
+                    if (!ready()) break;
                     const uint32_t stage = ring + uint32_t(s) * C::STAGE_BYTES;
 #pragma unroll
                     for (int kk = 0; kk < C::KPS; kk++) {
@@ -497,12 +519,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll
                         for (int h = 0; h < MH; h++) {
                             if (fresh) {  // the epilogue must have drained this half of the buffer
-                                if (!(ok = wait_bar(tempty_bar(buf, h), aph ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf * 2 + h), limit))) break;
+                                ok = __all_sync(0xffffffffu, wait_bar(tempty_bar(buf, h), aph ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf * 2 + h), limit));
+                                if (!ok) break;
                                 ptx::tc_fence_after();
                             }
                             const uint64_t a = sw128_desc(src + uint32_t(h) * (BM * BK * 2));
+                            if (leader) {
 #pragma unroll
-                            for (int j = 0; j < 4; j++) ptx::umma_f16<G>(d + uint32_t(h * BN), a + 2u * j, b + 2u * j, p.idesc, (!fresh || j > 0) ? 1u : 0u);
+                                for (int j = 0; j < 4; j++) ptx::umma_f16<G>(d + uint32_t(h * BN), a + 2u * j, b + 2u * j, p.idesc, (!fresh || j > 0) ? 1u : 0u);
+                            }
+                            __syncwarp();
                             issued = true;
                         }
                         if (!ok) break;
@@ -514,6 +540,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 if (!waited) ptx::griddep_wait(), waited = true;
                 const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
                 const int entries = int(plan[0]);
+                const uint32_t k_step = p.low_box ? MN_K_STEP : 2u;
                 for (int e = 0; e < entries && ok; e++) {
                     uint32_t off[C::ROWS / 32];
 #pragma unroll
@@ -523,9 +550,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     }
                     for (int q = 0; q < q_blocks; q++) {
                         const ExtBlock x = ext_block(q, p.rp, p.rank);
-                        if (!(ok = ready())) break;
+                        if (!ready()) break;
                         const uint32_t src = ring + uint32_t(s) * C::STAGE_BYTES;
-                        const uint64_t b = sw128_desc(src + C::A_BYTES);
+                        const uint64_t b = p.low_box ? mn_desc(src + C::A_BYTES, p.low_box) : sw128_desc(src + C::A_BYTES);
 #pragma unroll
                         for (int h = 0; h < MH; h++) {
                             const uint64_t a = sw128_desc(src + uint32_t(h) * (BM * BK * 2));
@@ -535,22 +562,25 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                             uint32_t all = 0xffffffffu;
 #pragma unroll
                             for (int i = 0; i < 4 * G; i++) all &= m[i];
-                            if (all == 0xffffffffu) continue;  // no row of these accumulators
-                            for (int j = 0; j < x.steps; j++) {
-                                if constexpr (G == 1)
-                                    ptx::umma_f16_lanes(d + uint32_t(h * BN), a + 2u * j, b + 2u * (j & x.b_mask), p.idesc, 1u, m[0], m[1], m[2], m[3]);
-                                else
-                                    ptx::umma_f16_lanes_pair(d + uint32_t(h * BN), a + 2u * j, b + 2u * (j & x.b_mask), p.idesc, 1u, m);
-                            }
+                            if (leader && all != 0xffffffffu)  // else no row of these accumulators
+                                for (int j = 0; j < x.steps; j++) {
+                                    const uint64_t bj = b + uint64_t(k_step * uint32_t(j & x.b_mask));
+                                    if constexpr (G == 1) ptx::umma_f16_lanes(d + uint32_t(h * BN), a + 2u * j, bj, p.low_idesc, 1u, m[0], m[1], m[2], m[3]);
+                                    else ptx::umma_f16_lanes_pair(d + uint32_t(h * BN), a + 2u * j, bj, p.low_idesc, 1u, m);
+                                }
+                            __syncwarp();
                         }
                         free_stage();
                     }
                 }
                 if (!ok) break;
-                ptx::umma_commit<G>(tfull_bar(buf));
-                if constexpr (G == 2) ptx::umma_commit<G>(ptx::mapa(tfull_bar(buf), 1));
+                if (leader) {
+                    ptx::umma_commit<G>(tfull_bar(buf));
+                    if constexpr (G == 2) ptx::umma_commit<G>(ptx::mapa(tfull_bar(buf), 1));
+                }
+                __syncwarp();
             }
-            if (!ok && issued) {
+            if (!ok && issued && leader) {
                 ptx::umma_commit<G>(drain_bar);
                 const uint64_t t0 = ptx::globaltimer_ns();
                 while (!ptx::mbar_try_wait(drain_bar, 0u))
@@ -605,16 +635,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 // ---- host -------------------------------------------------------------------------
 int g_shrink_clusters[64][4];  // clusters of 1, 2, 4, 8 CTAs of the T kernel that fit each device at once
 
-template <bool BF16>
-cute_b200_status shrink(const LoraParams &p, int plan_rows, int debug, const DeviceState &dev, cudaStream_t stream) {
+template <int P>
+cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream) {
     ShrinkParams s = {};
-    s.ids = p.ids, s.scale = p.scale, s.t = p.t, s.plan = p.plan;
+    s.ids = p.ids, s.scale = p.scale, s.t = p.t, s.plan = p.y ? p.plan : nullptr;
     s.m = p.m, s.rank = p.rank, s.rp = p.rp, s.adapters = p.adapters;
     s.k_blocks = (p.k + BK - 1) / BK;
-    s.plan_rows = plan_rows;
-    s.a_stages = int(A_RING / (uint32_t(p.rp) * 128u));
-    if (s.a_stages > A_STAGES) s.a_stages = A_STAGES;
-    s.idesc = make_idesc(BF16, 128, p.rp);
+    s.mn = s.early = p.low_mn;
+    s.boxes = p.low_mn ? (p.rp + 63) / 64 : 1;
+    s.box_bytes = p.low_mn ? BK * 128 : uint32_t(p.rp) * 128u;
+    s.bf16 = bf16;
+    s.idesc = make_idesc(bf16, 128, p.rp) | (p.low_mn ? IDESC_B_MN : 0u);
     s.tmem_cols = p.rp <= 32 ? 32 : uint32_t(p.rp);
     s.status = dev.status_word;
     s.debug = debug;
@@ -626,9 +657,10 @@ cute_b200_status shrink(const LoraParams &p, int plan_rows, int debug, const Dev
     for (int c = 1; c < 4; c++)
         if (tiles <= g_shrink_clusters[device][c] && s.k_blocks >= (4 << c)) s.kc = 1 << c;
     CUtensorMap tmX, tmA;
-    CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), BF16, p.m, p.k, p.ldx, BM));
-    CB_TRY(rows_tensor_map(&tmA, reinterpret_cast<uint64_t>(p.a), BF16, uint64_t(p.adapters) * p.rank, p.k, p.k, p.rp));
-    return launch_dependent(shrink_tile_kernel<BF16>, dim3(unsigned(tiles * s.kc)), SHRINK_THREADS, SHRINK_SMEM, s.kc, stream, tmX, tmA, s);
+    CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), bf16, p.m, p.k, p.ldx, BM));
+    if (p.low_mn) CB_TRY(stack_tensor_map(&tmA, reinterpret_cast<uint64_t>(p.a), bf16, p.adapters, p.k, p.rank, BK));
+    else CB_TRY(rows_tensor_map(&tmA, reinterpret_cast<uint64_t>(p.a), bf16, uint64_t(p.adapters) * p.rank, p.k, p.k, p.rp));
+    return launch_dependent(shrink_tile_kernel<P>, dim3(unsigned(tiles * s.kc)), SHRINK_THREADS, SHRINK_SMEM, s.kc, stream, tmX, tmA, s);
 }
 
 template <int G, int BN, int MH>
@@ -650,13 +682,17 @@ cute_b200_status launch_tile(const LoraParams &p, bool bf16, int debug, const De
     while (gm * gm * 2 <= clusters) gm *= 2;
     t.group_m = gm < t.m_tiles ? gm : t.m_tiles;
     t.idesc = make_idesc(bf16, 128 * G, BN);
+    const int low_rows = p.rp < 64 ? p.rp : 64;  // ranks per box of an MN-major B
+    t.low_idesc = t.idesc | (p.low_mn ? IDESC_B_MN : 0u);
+    t.low_box = p.low_mn ? uint32_t(low_rows) * 128u : 0u;
     t.status = dev.status_word;
     t.debug = debug;
     CUtensorMap tmX, tmW, tmT, tmB;
     CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), bf16, p.m, p.k, p.ldx, C::CTA_ROWS));
     CB_TRY(rows_tensor_map(&tmW, reinterpret_cast<uint64_t>(p.w), bf16, p.n, p.k, p.k, C::B_ROWS));
     CB_TRY(rows_tensor_map(&tmT, reinterpret_cast<uint64_t>(p.t), bf16, p.m, 2 * p.rp, 2 * p.rp, C::CTA_ROWS));
-    CB_TRY(rows_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), bf16, uint64_t(p.adapters) * p.n, p.rank, p.rank, C::B_ROWS));
+    if (p.low_mn) CB_TRY(stack_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), bf16, p.adapters, p.rank, p.n, low_rows));
+    else CB_TRY(rows_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), bf16, uint64_t(p.adapters) * p.n, p.rank, p.rank, C::B_ROWS));
     return launch_dependent(lora_tile_kernel<G, BN, MH>, dim3(unsigned(clusters * G)), TILE_THREADS, C::SMEM_BYTES, G, stream, tmX, tmW, tmT, tmB, t);
 }
 
@@ -666,12 +702,13 @@ struct Cut {
     int rows, cols;
     double rate;
 };
-constexpr Cut CUTS[3] = {{512, 256, 1.0}, {128, 256, 0.86}, {128, 128, 0.7}};
+constexpr int NUM_CUTS = 4;
+constexpr Cut CUTS[NUM_CUTS] = {{512, 256, 1.0}, {256, 256, 0.92}, {128, 256, 0.86}, {128, 128, 0.7}};
 int choose_cut(int m, int n, int k, int sm_count) {
     int best = 0;
     double best_t = 1e300;
-    for (int i = 0; i < 3; i++) {
-        const int pair = CUTS[i].rows == 512 ? 2 : 1;
+    for (int i = 0; i < NUM_CUTS; i++) {
+        const int pair = CUTS[i].rows >= 256 ? 2 : 1;
         const int64_t tiles = int64_t((m + CUTS[i].rows - 1) / CUTS[i].rows) * ((n + CUTS[i].cols - 1) / CUTS[i].cols);
         const int64_t at_once = sm_count / pair, waves = (tiles + at_once - 1) / at_once;
         const double unit = 2.0 * CUTS[i].rows * CUTS[i].cols * k / (pair * 1.0e13 * CUTS[i].rate);
@@ -685,7 +722,7 @@ int choose_cut(int m, int n, int k, int sm_count) {
 
 uint64_t lora_plan_bytes(int m, int adapters) {
     uint64_t most = 0;
-    for (int rows : {128, 512}) {
+    for (int rows : {128, 256, 512}) {
         const uint64_t b = uint64_t((int64_t(m) + rows - 1) / rows) * plan_stride(rows, adapters) * 4;
         if (b > most) most = b;
     }
@@ -694,23 +731,28 @@ uint64_t lora_plan_bytes(int m, int adapters) {
 
 cute_b200_status lora_tiled(const LoraParams &p, bool bf16, int cut, int debug, const DeviceState &dev, cudaStream_t stream) {
     if (cut < 0) cut = choose_cut(p.m, p.n, p.k, dev.sm_count);
-    CB_TRY(bf16 ? shrink<true>(p, CUTS[cut].rows, debug, dev, stream) : shrink<false>(p, CUTS[cut].rows, debug, dev, stream));
+    if (CUTS[cut].rows == 512) CB_TRY(shrink<512>(p, bf16, debug, dev, stream));
+    else if (CUTS[cut].rows == 256) CB_TRY(shrink<256>(p, bf16, debug, dev, stream));
+    else CB_TRY(shrink<128>(p, bf16, debug, dev, stream));
     if (!p.y) return CUTE_B200_OK;
     if (cut == 0) return launch_tile<2, 256, 2>(p, bf16, debug, dev, stream);
-    if (cut == 1) return launch_tile<1, 256, 1>(p, bf16, debug, dev, stream);
+    if (cut == 1) return launch_tile<2, 256, 1>(p, bf16, debug, dev, stream);
+    if (cut == 2) return launch_tile<1, 256, 1>(p, bf16, debug, dev, stream);
     return launch_tile<1, 128, 1>(p, bf16, debug, dev, stream);
 }
 
 cute_b200_status lora_tiled_init() {
     int device = 0;
     CB_CUDA(cudaGetDevice(&device));
-    CB_CUDA(cudaFuncSetAttribute(shrink_tile_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHRINK_SMEM));
-    CB_CUDA(cudaFuncSetAttribute(shrink_tile_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHRINK_SMEM));
+    CB_CUDA(cudaFuncSetAttribute(shrink_tile_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHRINK_SMEM));
+    CB_CUDA(cudaFuncSetAttribute(shrink_tile_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHRINK_SMEM));
+    CB_CUDA(cudaFuncSetAttribute(shrink_tile_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHRINK_SMEM));
     CB_CUDA(cudaFuncSetAttribute(lora_tile_kernel<2, 256, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<2, 256, 2>::SMEM_BYTES));
+    CB_CUDA(cudaFuncSetAttribute(lora_tile_kernel<2, 256, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<2, 256, 1>::SMEM_BYTES));
     CB_CUDA(cudaFuncSetAttribute(lora_tile_kernel<1, 256, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<1, 256, 1>::SMEM_BYTES));
     CB_CUDA(cudaFuncSetAttribute(lora_tile_kernel<1, 128, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<1, 128, 1>::SMEM_BYTES));
     for (int c = 0; c < 4; c++)
-        CB_TRY(max_clusters(shrink_tile_kernel<true>, SHRINK_THREADS, SHRINK_SMEM, 1 << c, &g_shrink_clusters[device][c]));
+        CB_TRY(max_clusters(shrink_tile_kernel<128>, SHRINK_THREADS, SHRINK_SMEM, 1 << c, &g_shrink_clusters[device][c]));
     return CUTE_B200_OK;
 }
 

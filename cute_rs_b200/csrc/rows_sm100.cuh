@@ -75,6 +75,33 @@ inline cute_b200_status rows_tensor_map(CUtensorMap *tm, uint64_t base, bool bf1
     return CUTE_B200_OK;
 }
 
+// The same of `count` matrices one behind the other: a box lies within one of them, what lies outside reads as zero.
+inline cute_b200_status stack_tensor_map(CUtensorMap *tm, uint64_t base, bool bf16, uint64_t count, uint64_t rows, uint64_t cols, int box_rows) {
+    EncodeTiledFn encode;
+    CB_TRY(encode_fn(&encode));
+    const cuuint64_t dims[3] = {cols, rows, count};
+    const cuuint64_t strides[2] = {cols * 2, rows * cols * 2};
+    const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    const CUresult r = encode(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                              reinterpret_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(CUTE_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed: CUresult %d (%llu matrices of %llu x %llu, box %d)", int(r),
+                    (unsigned long long)count, (unsigned long long)rows, (unsigned long long)cols, box_rows);
+    return CUTE_B200_OK;
+}
+
+// Shared-memory matrix descriptor of an MN-major tile in 128-byte rows with the 128B swizzle: 64 values of M or N per
+// row, the rows are k.  Leading byte offset: from 64 values to the next 64, one box of `box_bytes`; stride byte offset:
+// from eight k to the next eight.  16 k further: MN_K_STEP in the address field.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t box_bytes) {
+    return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(box_bytes >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+           (uint64_t(2) << 61);
+}
+constexpr uint32_t MN_K_STEP = (16 * 128) >> 4;
+constexpr uint32_t IDESC_A_MN = 1u << 15, IDESC_B_MN = 1u << 16;  // instruction descriptor: that operand is MN-major
+
 // Launch as a programmatic dependent of the kernel before it in the stream, in clusters of `cluster` CTAs.
 template <typename... P, typename... A>
 cute_b200_status launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,

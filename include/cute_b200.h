@@ -219,7 +219,7 @@ typedef struct {
     int32_t c_dtype;   /* CUTE_B200_F32, CUTE_B200_F16 or CUTE_B200_BF16: Y, dX */
     int32_t ldx, ldy;  /* elements between rows of X (a multiple of 8) and of Y; 0 = dense (k, n) */
     int32_t tuning[2]; /* zero.  Measurement and test knobs: [0] 1 = the kernels for few rows (m <= 128), 2 = the tiled kernels,
-                          3, 4, 5 = those with a tile of 512 x 256, 128 x 256, 128 x 128;
+                          3 to 6 = those with a tile of 512 x 256, 256 x 256, 128 x 256, 128 x 128;
                           [1] bits 2 + 3 make every in-kernel wait run out after 20 ms, as in cute_b200_gemm_desc */
 } cute_b200_lora_desc;
 

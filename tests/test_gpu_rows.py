@@ -149,7 +149,7 @@ class Lora:
 
 
 def variants(m):
-    return [(0, 0), (2, 0), (3, 0), (4, 0), (5, 0)] + ([(1, 0)] if m <= 128 else [])
+    return [(0, 0), (2, 0), (3, 0), (4, 0), (5, 0), (6, 0)] + ([(1, 0)] if m <= 128 else [])
 
 
 SHAPES = [  # m, n, k, rank, adapters, ids
@@ -270,6 +270,8 @@ def test_lora_backward(lib, gpu, m, n, k, rank, adapters, ids, ab, c):
     p.check_back(*first)
     again = p.back()
     assert all(torch.equal(a, b) for a, b in zip(first, again)), "the same call gave other bits"
+    for tuning in variants(m)[2:]:
+        p.check_back(*p.back(tuning=tuning))
     dx, _, _ = p.back(with_dw=False)
     assert torch.equal(dx, first[0])
     _, da, db = p.back(with_dx=False)

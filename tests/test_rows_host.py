@@ -39,8 +39,8 @@ LORA_SIZES = [
     (dict(ldx=8), "lora_tn: ldx must be 0 or a multiple of 8 of at least k = 16, got 8"),
     (dict(ldy=15), "lora_tn: ldy must be 0 or at least n = 16, got 15"),
     (dict(m=(1 << 30) + 1), "lora_tn: m, n and k may be at most 2^30, got 1073741825x16x16"),
-    (dict(tuning=(6, 0)), "lora_tn: tuning[0] must be 0, 1 (with m <= 128) or 2 to 5, got 6"),
-    (dict(tuning=(1, 0), m=129), "lora_tn: tuning[0] must be 0, 1 (with m <= 128) or 2 to 5, got 1"),
+    (dict(tuning=(7, 0)), "lora_tn: tuning[0] must be 0, 1 (with m <= 128) or 2 to 6, got 7"),
+    (dict(tuning=(1, 0), m=129), "lora_tn: tuning[0] must be 0, 1 (with m <= 128) or 2 to 6, got 1"),
 ]
 
 
