@@ -148,11 +148,9 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
             const uint32_t dst = ring + uint32_t(s) * p.stage_bytes, full = bar(h.full[s]);
             if (lane == 0) ptx::mbar_arrive_expect_tx(full, bytes);
             __syncwarp();
-            if (run) {
-                if (lane == 0) {
-                    for (int x = 0; x < 2; x++) ptx::tma_load_2d(dst + x * GRAD_BOX, &maps.wide[job], full, c0 + 64 * x, first_row);
-                    for (int x = 0; x < low_boxes; x++) ptx::tma_load_2d(dst + (2 + x) * GRAD_BOX, &maps.low[job], full, 64 * x, first_row);
-                }
+            if (run) {  // a lane per box
+                if (lane < 2) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.wide[job], full, c0 + 64 * lane, first_row);
+                else if (lane < 2 + low_boxes) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.low[job], full, 64 * (lane - 2), first_row);
             } else if (lane < 16) {
                 for (int x = 0; x < 2; x++)
                     ptx::tma_gather4(dst + x * GRAD_BOX + 512u * lane, &maps.wide_rows[job], full, c0 + 64 * x, row[0], row[1], row[2], row[3]);
@@ -171,22 +169,28 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true, issued = false;
-            for (int b = b0; b < b1; b++) {
-                if (!(ok = wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit))) break;
-                ptx::tc_fence_after();
-                const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-                const uint64_t wide = mn_desc(src, GRAD_BOX), low = mn_desc(src + 2 * GRAD_BOX, GRAD_BOX);
+        // The whole warp runs the loop and one thread issues: see lora_few_kernel.
+        const bool leader = ptx::elect_one();
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true, issued = false;
+        for (int b = b0; b < b1; b++) {
+            ok = __all_sync(0xffffffffu, wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+            const uint64_t wide = mn_desc(src, GRAD_BOX), low = mn_desc(src + 2 * GRAD_BOX, GRAD_BOX);
+            const uint32_t more = b > b0 ? 1u : 0u;
+            if (leader) {
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    ptx::umma_f16<1>(tmem, wide + MN_K_STEP * j, low + MN_K_STEP * j, p.idesc, (b > b0 || j > 0) ? 1u : 0u);
-                issued = true;
+                for (int j = 0; j < 4; j++) ptx::umma_f16<1>(tmem, wide + MN_K_STEP * j, low + MN_K_STEP * j, p.idesc, j > 0 ? 1u : more);
                 ptx::umma_commit<1>(bar(h.empty[s]));
-                if (++s == p.stages) s = 0, ph ^= 1u;
             }
+            __syncwarp();
+            issued = true;
+            if (++s == p.stages) s = 0, ph ^= 1u;
+        }
+        if (leader) {
             if (ok) {
                 ptx::umma_commit<1>(bar(h.done));
             } else if (issued) {

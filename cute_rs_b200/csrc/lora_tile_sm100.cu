@@ -20,15 +20,16 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 // a cluster.  M = the rows, N = the padded rank: every adapter's MMAs are masked to
 // the lanes of its rows, so one accumulator serves all of them.  Bound by reading X
 // (and, where nearly every row has an adapter of its own, A).
-//   warp 0  TMA: per k block a (128 x 64) block of X into one ring, then the blocks
-//           of A of the tile's adapters into another, 16 KB of them per stage, a lane each.
+//   warp 0  TMA: two (128 x 64) blocks of X per stage of one ring, then the blocks of A
+//           of the tile's adapters for them through another, 32 KB per stage, a lane each
+//           (with 16 KB per stage of either the issuing warp was the bound: 0.3 us a stage).
 //   warp 1  MMA.   warps 2-5  the adapters the rows name (and, by the cluster's first CTA,
 //           the plan of the GEMM's tile that starts at its rows), then the sum over the
 //           cluster, scale, split into two 16-bit numbers.
 // On the way back A is B[a] as it lies, (n, rank): rank is the fast index, so it is an MN-major operand.
-constexpr int SHRINK_THREADS = 192, X_STAGES = 7, A_STAGES = 5;
-constexpr uint32_t X_BYTES = BM * BK * 2, A_BYTES = 16 * 1024, SHRINK_HEAD = 20 * 1024;
-constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + X_STAGES * X_BYTES + A_STAGES * A_BYTES;
+constexpr int SHRINK_THREADS = 192, X_STAGES = 3, A_STAGES = 3, X_BLOCKS = 2;
+constexpr uint32_t X_BYTES = BM * BK * 2, A_BYTES = 32 * 1024, SHRINK_HEAD = 20 * 1024;
+constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + X_STAGES * X_BLOCKS * X_BYTES + A_STAGES * A_BYTES;
 
 struct ShrinkParams {
     const int32_t *ids;
@@ -61,7 +62,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     ShrinkHead<P> &h = *reinterpret_cast<ShrinkHead<P> *>(smem_raw + (base - raw));
-    const uint32_t xring = base + SHRINK_HEAD, aring = xring + X_STAGES * X_BYTES;
+    const uint32_t xring = base + SHRINK_HEAD, aring = xring + X_STAGES * X_BLOCKS * X_BYTES;
     auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
     volatile uint32_t *abort_flag = &h.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
     const int row0 = int(blockIdx.x) / p.kc * BM;
     const int kb0 = int(int64_t(p.k_blocks) * rank / p.kc), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / p.kc);
     const uint32_t entry_bytes = uint32_t(p.boxes) * p.box_bytes;
-    const int group = int(A_BYTES / entry_bytes);  // adapters per stage of A: 1 to 8
+    const int group = min(int(A_BYTES / entry_bytes), 32 / p.boxes);  // (k block, adapter) pairs per stage of A: 2 to 16
     const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
 
     if (threadIdx.x == 0) {
@@ -106,30 +107,30 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         }
         bool ok = !(p.debug & 4);
         ok = __all_sync(0xffffffffu, ok && wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_PRODUCER, 100u, limit));
-        const int entries = ok ? h.entries : 0, my_e = lane / p.boxes, my_box = lane % p.boxes;
+        const int entries = ok ? h.entries : 0, my_item = lane / p.boxes, my_box = lane % p.boxes;
         int sx = 0, sa = 0;
         uint32_t px = 0, pa = 0, xfilled = 0, xparity = 0, afilled = 0, aparity = 0;
-        for (int kb = kb0; kb < kb1 && ok && entries > 0; kb++) {
+        for (int kb = kb0; kb < kb1 && ok && entries > 0; kb += X_BLOCKS) {
+            const int nk = min(X_BLOCKS, kb1 - kb), items = nk * entries;
             ok = __all_sync(0xffffffffu, wait_bar(bar(h.xempty[sx]), px ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(sx), limit));
             if (!ok) break;
-            if (lane == 0) {
-                ptx::mbar_arrive_expect_tx(bar(h.xfull[sx]), X_BYTES);
-                ptx::tma_load_2d(xring + uint32_t(sx) * X_BYTES, &tmX, bar(h.xfull[sx]), kb * BK, row0);
-            }
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.xfull[sx]), uint32_t(nk) * X_BYTES);
+            __syncwarp();
+            if (lane < nk) ptx::tma_load_2d(xring + uint32_t(sx * X_BLOCKS + lane) * X_BYTES, &tmX, bar(h.xfull[sx]), (kb + lane) * BK, row0);
             __syncwarp();
             xfilled |= 1u << sx, xparity = (xparity & ~(1u << sx)) | (px << sx);
             if (++sx == X_STAGES) sx = 0, px ^= 1u;
-            for (int e0 = 0; e0 < entries; e0 += group) {
+            for (int i0 = 0; i0 < items; i0 += group) {
                 ok = __all_sync(0xffffffffu, wait_bar(bar(h.aempty[sa]), pa ^ 1u, abort_flag, p.status, WHERE_PRODUCER, 32u + uint32_t(sa), limit));
                 if (!ok) break;
-                const int count = min(group, entries - e0);
+                const int count = min(group, items - i0);
                 if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.afull[sa]), uint32_t(count) * entry_bytes);
                 __syncwarp();
-                if (my_e < count) {
-                    const int id = h.entry_id[e0 + my_e];
+                if (my_item < count) {
+                    const int second = i0 + my_item >= entries ? 1 : 0, id = h.entry_id[i0 + my_item - second * entries];
                     const uint32_t dst = aring + uint32_t(sa) * A_BYTES + uint32_t(lane) * p.box_bytes;
-                    if (p.mn) ptx::tma_load_3d(dst, &tmA, bar(h.afull[sa]), 64 * my_box, kb * BK, id);
-                    else ptx::tma_load_2d(dst, &tmA, bar(h.afull[sa]), kb * BK, id * p.rank);
+                    if (p.mn) ptx::tma_load_3d(dst, &tmA, bar(h.afull[sa]), 64 * my_box, (kb + second) * BK, id);
+                    else ptx::tma_load_2d(dst, &tmA, bar(h.afull[sa]), (kb + second) * BK, id * p.rank);
                 }
                 __syncwarp();
                 afilled |= 1u << sa, aparity = (aparity & ~(1u << sa)) | (pa << sa);
@@ -153,21 +154,22 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         const int entries = ok ? h.entries : 0;
         int sx = 0, sa = 0;
         uint32_t px = 0, pa = 0;
-        for (int kb = kb0; kb < kb1 && ok && entries > 0; kb++) {
+        for (int kb = kb0; kb < kb1 && ok && entries > 0; kb += X_BLOCKS) {
+            const int items = min(X_BLOCKS, kb1 - kb) * entries;
             ok = __all_sync(0xffffffffu, wait_bar(bar(h.xfull[sx]), px, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(sx), limit));
             if (!ok) break;
-            const uint64_t a = sw128_desc(xring + uint32_t(sx) * X_BYTES);
-            const uint32_t more = kb > kb0 ? 1u : 0u;
-            for (int e0 = 0; e0 < entries; e0 += group) {
+            for (int i0 = 0; i0 < items; i0 += group) {
                 ok = __all_sync(0xffffffffu, wait_bar(bar(h.afull[sa]), pa, abort_flag, p.status, WHERE_MMA_FULL, 32u + uint32_t(sa), limit));
                 if (!ok) break;
                 ptx::tc_fence_after();
-                const int count = min(group, entries - e0);
-                for (int e = 0; e < count; e++) {
-                    const uint32_t src = aring + uint32_t(sa) * A_BYTES + uint32_t(e) * entry_bytes;
+                const int count = min(group, items - i0);
+                for (int i = 0; i < count; i++) {
+                    const int second = i0 + i >= entries ? 1 : 0, e = i0 + i - second * entries;
+                    const uint32_t src = aring + uint32_t(sa) * A_BYTES + uint32_t(i) * entry_bytes;
+                    const uint64_t a = sw128_desc(xring + uint32_t(sx * X_BLOCKS + second) * X_BYTES);
                     const uint64_t b = p.mn ? mn_desc(src, p.box_bytes) : sw128_desc(src);
-                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u;
-                    const uint32_t o0 = h.off[e0 + e][0], o1 = h.off[e0 + e][1], o2 = h.off[e0 + e][2], o3 = h.off[e0 + e][3];
+                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u, more = kb > kb0 || second ? 1u : 0u;
+                    const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
                     if (leader) {
 #pragma unroll
                         for (int j = 0; j < 4; j++)
@@ -445,6 +447,15 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             const TileAt at = tile_at(t, p);
             const int row = at.tm * C::ROWS + int(rank) * C::CTA_ROWS, col = at.tn * BN + int(rank) * C::B_ROWS;
             const int kk = lane >> 1;  // lane 2 kk issues k block kk of X, lane 2 kk + 1 that of W
+            const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
+            // Lane l holds the id of entry l, 32 of them at a time, on their way while the tile's blocks of W are issued.
+            int entries = 0, ids = 0;
+            auto read_ids = [&](int e0) { ids = e0 + lane < entries ? int(plan[4 + (e0 + lane) * ENTRY]) : 0; };
+            auto read_plan = [&] {
+                entries = int(plan[0]);
+                read_ids(0);
+            };
+            if (waited) read_plan();
             for (int kb = 0; kb < p.k_blocks && ok; kb += C::KPS) {
                 const int nk = min(C::KPS, p.k_blocks - kb);
                 if (!next(uint32_t(nk) * C::KB_BYTES)) break;
@@ -453,11 +464,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 issued();
             }
             if (!ok) break;
-            if (!waited) ptx::griddep_wait(), waited = true;  // T and the plan; X and W are older than their kernel
-            const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
-            const int entries = int(plan[0]);
+            if (!waited) {
+                ptx::griddep_wait();  // T and the plan; X and W are older than their kernel
+                waited = true;
+                read_plan();
+            }
             for (int e = 0; e < entries && ok; e++) {
-                const int id = int(plan[4 + e * ENTRY]);
+                if (e > 0 && e % 32 == 0) read_ids(e);
+                const int id = __shfl_sync(0xffffffffu, ids, e % 32);
                 for (int q = 0; q < q_blocks; q++) {
                     const ExtBlock b = ext_block(q, p.rp, p.rank);
                     if (!next(C::A_BYTES + low_bytes)) break;
@@ -507,6 +521,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 const TileAt at = tile_at(t, p);
                 const int buf = it % C::ACC_BUFS;
                 const uint32_t aph = uint32_t(it / C::ACC_BUFS) & 1u, d = tmem + uint32_t(buf * C::ACC_COLS);
+                const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
+                // Lane l holds word l of an entry's masks, read one entry ahead.
+                int entries = 0;
+                uint32_t ahead = 0;
+                auto read_off = [&](int e) { ahead = e < entries && lane < C::ROWS / 32 ? plan[4 + e * ENTRY + 4 + lane] : 0u; };
+                auto read_plan = [&] {
+                    entries = int(plan[0]);
+                    read_off(0);
+                };
+                if (waited) read_plan();
                 for (int k0 = 0; k0 < p.k_blocks; k0 += C::KPS) {
                     if (!ready()) break;
                     const uint32_t stage = ring + uint32_t(s) * C::STAGE_BYTES;
@@ -537,17 +561,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     free_stage();
                 }
                 if (!ok) break;
-                if (!waited) ptx::griddep_wait(), waited = true;
-                const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
-                const int entries = int(plan[0]);
+                if (!waited) {
+                    ptx::griddep_wait();
+                    waited = true;
+                    read_plan();
+                }
                 const uint32_t k_step = p.low_box ? MN_K_STEP : 2u;
                 for (int e = 0; e < entries && ok; e++) {
                     uint32_t off[C::ROWS / 32];
 #pragma unroll
-                    for (int i = 0; i < C::ROWS / 32; i += 4) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(plan + 4 + e * ENTRY + 4 + i);
-                        off[i] = v.x, off[i + 1] = v.y, off[i + 2] = v.z, off[i + 3] = v.w;
-                    }
+                    for (int i = 0; i < C::ROWS / 32; i++) off[i] = __shfl_sync(0xffffffffu, ahead, i);
+                    read_off(e + 1);
                     for (int q = 0; q < q_blocks; q++) {
                         const ExtBlock x = ext_block(q, p.rp, p.rank);
                         if (!ready()) break;
