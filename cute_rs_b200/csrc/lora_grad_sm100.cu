@@ -73,7 +73,7 @@ struct GradMaps {
 struct GradParams {
     float *out[2];
     const int32_t *first, *list;
-    int cols[2], tiles[2], m, rank, rp, kc, stages;
+    int cols[2], tiles[2], m, rank, rp, kc, stages, vec;
     uint32_t stage_bytes, idesc, tmem_cols;
     uint32_t *status;
     int debug;
@@ -241,16 +241,22 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
     }
     if (!*abort_flag) {
         const uint32_t pitch = uint32_t(p.rp + 4) * 4u;
-        const int cols = p.cols[job], wide = min(GRAD_M, cols - c0), items = GRAD_M * p.rank;
+        // Four ranks of one column of V per step.  Neighbouring threads write neighbouring addresses: of dA the columns, of dB
+        // the ranks, 16 bytes at once.
+        const int cols = p.cols[job], wide = min(GRAD_M, cols - c0), quads = p.rank / 4, items = GRAD_M * quads;
         float *out = p.out[job] + int64_t(a) * p.rank * cols;
         for (int i = int(rank) * GRAD_THREADS + int(threadIdx.x); i < items; i += p.kc * GRAD_THREADS) {
-            // Neighbouring threads write neighbouring addresses: columns of dA, ranks of dB.
-            const int c = job ? i / p.rank : i % GRAD_M, j = job ? i % p.rank : i / GRAD_M;
+            const int c = job ? i / quads : i % GRAD_M, j = 4 * (job ? i % quads : i / GRAD_M);
             if (c >= wide) continue;
-            const uint32_t at = ring + uint32_t(c) * pitch + uint32_t(j) * 4u;
-            float v = ptx::ld_shared_cluster(p.kc > 1 ? ptx::mapa(at, 0) : at);
-            for (int x = 1; x < p.kc; x++) v += ptx::ld_shared_cluster(ptx::mapa(at, uint32_t(x)));
-            out[job ? int64_t(c0 + c) * p.rank + j : int64_t(j) * cols + c0 + c] = v;
+            const float4 v = cluster_sum(ring + uint32_t(c) * pitch + uint32_t(j) * 4u, p.kc);
+            if (job) {
+                float *to = out + int64_t(c0 + c) * p.rank + j;
+                if (p.vec) *reinterpret_cast<float4 *>(to) = v;
+                else to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+            } else {
+                float *to = out + int64_t(j) * cols + c0 + c;
+                to[0] = v.x, to[cols] = v.y, to[2 * int64_t(cols)] = v.z, to[3 * int64_t(cols)] = v.w;
+            }
         }
     }
     __syncthreads();
@@ -281,6 +287,7 @@ cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const Devi
         CB_TRY(rows_tensor_map(&maps.low_rows[i], low, bf16, g.m, 2 * g.rp, 2 * g.rp, 1));
     }
     p.first = g.first, p.list = g.list;
+    p.vec = reinterpret_cast<uint64_t>(g.out[1]) % 16 == 0;
     p.m = g.m, p.rank = g.rank, p.rp = g.rp;
     p.stage_bytes = uint32_t(2 + (2 * g.rp + 63) / 64) * GRAD_BOX;
     p.stages = int(GRAD_RING / p.stage_bytes);

@@ -176,7 +176,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     FewHead &h = *reinterpret_cast<FewHead *>(smem_raw + (base - raw));
-    const int b_blocks = p.b_blocks, t_blocks = ext_blocks(p.rp);
+    const bool whole = whole_t(p.c_dtype);
+    const int b_blocks = p.b_blocks, t_blocks = ext_blocks(p.rp, whole);
     // T's blocks for the tensor core, or T and the dot products, then the ring.
     const uint32_t low = base + FEW_HEAD, ring = low + p.low_bytes;
     auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         if (has_low) {
             if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.low), uint32_t(t_blocks) * p.x_bytes);
             __syncwarp();
-            if (lane < t_blocks) ptx::tma_load_2d(low + uint32_t(lane) * p.x_bytes, &tmT, bar(h.low), ext_block(lane, p.rp, p.rank).t_col, 0);
+            if (lane < t_blocks) ptx::tma_load_2d(low + uint32_t(lane) * p.x_bytes, &tmT, bar(h.low), ext_block(lane, p.rp, p.rank, whole).t_col, 0);
         }
         for (int i = 0; i < mine && ok; i += p.kps) {
             const int nk = min(p.kps, mine - i);
@@ -318,10 +319,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
                 const int e = int(rank) + (i + kk) / b_blocks * p.kc, q = (i + kk) % b_blocks;
                 const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
                 const uint64_t b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
-                // The numbers' block of T, then their remainders' (with rp <= 32 one block holds both), against one block of B.
-                for (int part = 0; part < t_blocks / b_blocks; part++) {
-                    const ExtBlock x = ext_block(2 * q + part, p.rp, p.rank);
-                    const uint64_t a = sw128_desc(low + uint32_t(2 * q + part) * p.x_bytes);
+                // The blocks of T that go with this block of B.
+                const int parts = t_blocks / b_blocks;
+                for (int part = 0; part < parts; part++) {
+                    const ExtBlock x = ext_block(parts * q + part, p.rp, p.rank, whole);
+                    const uint64_t a = sw128_desc(low + uint32_t(parts * q + part) * p.x_bytes);
                     if (leader)
                         for (int j = 0; j < x.steps; j++) ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * (j & x.b_mask), p.idesc, 1u, o0, o1, o2, o3);
                     __syncwarp();
@@ -451,7 +453,7 @@ cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int de
     // The head, T, the ring, and behind the last stage as much as an MMA reads past its rows of X.
     const uint64_t dots = uint64_t((p.m + f.kc - 1) / f.kc) * uint64_t(p.rp + f.bn) * 4;
     f.b_blocks = p.rp <= 32 && dots <= FEW_DOTS ? 0 : (p.rp <= 64 ? 1 : 2);
-    f.low_bytes = f.b_blocks == 0 ? uint32_t((dots + 1023) / 1024 * 1024) : uint32_t(ext_blocks(p.rp)) * f.x_bytes;
+    f.low_bytes = f.b_blocks == 0 ? uint32_t((dots + 1023) / 1024 * 1024) : uint32_t(ext_blocks(p.rp, whole_t(p.c_dtype))) * f.x_bytes;
     f.t = p.t, f.b = p.b, f.bf16 = BF16;
     const uint32_t ring = FEW_SMEM - FEW_HEAD - 1024 - f.low_bytes;
     f.kps = stream_blocks(f.bn, f.xr, ring);

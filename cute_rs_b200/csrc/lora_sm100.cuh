@@ -101,18 +101,19 @@ __device__ __forceinline__ int distinct_ids(const int32_t (&id)[ROWS / 128], IdT
     return total;
 }
 
-// An adapter's part of the product runs over the 2 rp columns of T in blocks of
-// 64: block q pairs columns t_col.. of T with columns b_col.. of B; `steps` MMAs
-// of 16, whose step of B is s & b_mask (with rp <= 32 the numbers and their
-// remainders lie in one block and B's columns are used for both).
+// An adapter's part of the product runs over columns of T in blocks of 64: block q pairs columns t_col.. of T with columns
+// b_col.. of B; `steps` MMAs of 16, whose step of B is s & b_mask.  An f32 result takes both numbers of a value of T, the
+// rounded one and the remainder (with rp <= 32 they lie in one block and B's columns serve both).  A 16-bit result takes
+// the rounded one alone: its own rounding is as coarse, and the tensor core's share of an adapter halves.
 struct ExtBlock {
     int t_col, b_col, steps, b_mask;
 };
-__host__ __device__ __forceinline__ int ext_blocks(int rp) { return rp <= 32 ? 1 : rp / 32; }
-__device__ __forceinline__ ExtBlock ext_block(int q, int rp, int rank) {
-    if (rp <= 32) return {0, 0, rp / 8, rp / 16 - 1};
-    const int half = q >> 1, left = (rank - 64 * half + 15) / 16;  // at least 1: rank > rp / 2
-    return {(q & 1) * rp + 64 * half, 64 * half, left < 4 ? left : 4, 3};
+__host__ __device__ __forceinline__ bool whole_t(int c_dtype) { return c_dtype == CUTE_B200_F32; }
+__host__ __device__ __forceinline__ int ext_blocks(int rp, bool whole) { return rp <= 32 ? 1 : (whole ? rp / 32 : rp / 64); }
+__device__ __forceinline__ ExtBlock ext_block(int q, int rp, int rank, bool whole) {
+    if (rp <= 32) return {0, 0, whole ? rp / 8 : rp / 16, rp / 16 - 1};
+    const int half = whole ? q >> 1 : q, left = (rank - 64 * half + 15) / 16;  // at least 1: rank > rp / 2
+    return {(whole ? (q & 1) * rp : 0) + 64 * half, 64 * half, left < 4 ? left : 4, 3};
 }
 
 }  // namespace

@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
 // The structure of the library's GEMM: persistent CTAs or CTA pairs, a TMA warp, an MMA warp, eight epilogue warps, a
 // ring of 192 KiB.  G: CTAs per MMA; BN: columns per tile; MH: 128-row accumulators per CTA.  Behind a tile's k blocks
 // of W come, for every adapter its rows name, the blocks of T (in place of X) and of B[a] (in place of W), their MMAs
-// masked to the lanes of the adapter's rows.  One adapter of rank 64 costs 2 blocks beside the 64 of k = 4096.
+// masked to the lanes of the adapter's rows.  One adapter of rank 64 costs 1 block (2 for
+// an f32 result) beside the 64 of k = 4096.
 // On the way back B is A[a] as it lies, (rank, k): an MN-major operand, in boxes of 64 columns by up to 64 ranks.
 constexpr uint32_t RING_BYTES = 192 * 1024;
 constexpr int TILE_THREADS = 64 + 256;
@@ -387,7 +388,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
     const uint64_t stride = plan_stride(C::ROWS, p.adapters);
     constexpr int ENTRY = 4 + C::ROWS / 32;
-    const int q_blocks = ext_blocks(p.rp);
+    const bool whole = whole_t(p.c_dtype);
+    const int q_blocks = ext_blocks(p.rp, whole);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) {
@@ -473,7 +475,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 if (e > 0 && e % 32 == 0) read_ids(e);
                 const int id = __shfl_sync(0xffffffffu, ids, e % 32);
                 for (int q = 0; q < q_blocks; q++) {
-                    const ExtBlock b = ext_block(q, p.rp, p.rank);
+                    const ExtBlock b = ext_block(q, p.rp, p.rank, whole);
                     if (!next(C::A_BYTES + low_bytes)) break;
                     const uint32_t dst = ring + uint32_t(s) * C::STAGE_BYTES;
                     if (lane == 0) load(dst, &tmT, b.t_col, row);
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     for (int i = 0; i < C::ROWS / 32; i++) off[i] = __shfl_sync(0xffffffffu, ahead, i);
                     read_off(e + 1);
                     for (int q = 0; q < q_blocks; q++) {
-                        const ExtBlock x = ext_block(q, p.rp, p.rank);
+                        const ExtBlock x = ext_block(q, p.rp, p.rank, whole);
                         if (!ready()) break;
                         const uint32_t src = ring + uint32_t(s) * C::STAGE_BYTES;
                         const uint64_t b = p.low_box ? mn_desc(src + C::A_BYTES, p.low_box) : sw128_desc(src + C::A_BYTES);
@@ -674,12 +676,12 @@ cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceS
     s.status = dev.status_word;
     s.debug = debug;
     const int tiles = (p.m + BM - 1) / BM;
-    // k is cut while that puts more CTAs to work and leaves each at least four blocks.
+    // k is cut while that puts more CTAs to work and leaves each at least two blocks.
     int device = 0;
     CB_CUDA(cudaGetDevice(&device));
     s.kc = 1;
     for (int c = 1; c < 4; c++)
-        if (tiles <= g_shrink_clusters[device][c] && s.k_blocks >= (4 << c)) s.kc = 1 << c;
+        if (tiles <= g_shrink_clusters[device][c] && s.k_blocks >= (2 << c)) s.kc = 1 << c;
     CUtensorMap tmX, tmA;
     CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), bf16, p.m, p.k, p.ldx, BM));
     if (p.low_mn) CB_TRY(stack_tensor_map(&tmA, reinterpret_cast<uint64_t>(p.a), bf16, p.adapters, p.k, p.rank, BK));

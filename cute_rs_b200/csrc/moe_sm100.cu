@@ -27,9 +27,10 @@ struct MoeParams {
 };
 
 // ---- router -----------------------------------------------------------------
-// 64 warps share the experts' rows of four tokens; with fewer than 64 experts each row is cut into `parts` ranges of
-// d.  The sums go to the CTA that owns the token (the cluster's CTAs 0-3), which adds the parts in order and chooses.
-constexpr int ROUTER_THREADS = 256, ROUTER_CLUSTER = 8, ROUTER_TOKENS = 4;
+// 256 warps share the experts' rows of four tokens; with fewer experts each row is cut into `parts` ranges of d.  The
+// sums go to the CTA that owns the token (the cluster's CTAs 0-3), which adds the parts in order and chooses.  Bound by
+// the latency of its loads, hence the many warps (64 tokens, 128 experts of d = 2048: 28 us with 64 warps).
+constexpr int ROUTER_THREADS = 1024, ROUTER_CLUSTER = 8, ROUTER_TOKENS = 4;
 
 template <bool BF16>
 __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoeParams p) {
@@ -40,7 +41,7 @@ __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoePar
     const int rank = int(ptx::cluster_ctarank()), t0 = int(blockIdx.x) / ROUTER_CLUSTER * ROUTER_TOKENS;
     const int warps = ROUTER_CLUSTER * ROUTER_THREADS / 32, count = min(ROUTER_TOKENS, p.tokens - t0);
     int parts = 1;
-    while (parts * 2 * p.experts <= warps && parts * 2 <= 8) parts *= 2;  // experts * parts <= MAX_EXPERTS
+    while (parts * 2 * p.experts <= warps && parts * 2 <= 16) parts *= 2;  // experts * parts <= MAX_EXPERTS
     const int vecs = p.d / 8;
     ptx::cluster_arrive();
     ptx::cluster_wait();  // every CTA of the cluster runs: its shared memory may be written

@@ -194,9 +194,10 @@ cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint6
  *   m >= 0; n >= 1; k >= 8 and a multiple of 8; none above 2^30; rank a multiple of 8 in 8..128
  *   (an adapter of a smaller rank is padded with zeros); adapters >= 1 with
  *   adapters * n, adapters * k and adapters * rank below 2^31.
- *   A[a] x is rounded to the sum of two 16-bit numbers (16 significant bits for
- *   bf16, 22 for f16 where it lies inside f16's range; past +-65504 an f16
- *   product is infinite) before it is multiplied by B.
+ *   Before it is multiplied by B, scale[a] * A[a] x is rounded to the operands'
+ *   type for a 16-bit Y, and to the sum of two such numbers (16 significant bits
+ *   for bf16, 22 for f16) for an f32 Y and for the gradients; an f16 value past
+ *   +-65504 becomes infinite.
  *   The workspace begins with these numbers, which the backward pass reads.
  *
  * cute_b200_lora_tn_backward: the gradients for dY (m, n) in the operands' type

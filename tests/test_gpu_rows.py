@@ -2,8 +2,9 @@
 
 Tolerances, from the operators' arithmetic (every bound is per element):
 * a sum of K products of 16-bit numbers in f32: 2 K 2^-23 sum|a b|, the bound the tensor-core GEMM is held to;
-* the inner product T is carried as two 16-bit numbers: half a step of half a step, 2^-16 |T| (bf16) or 2^-22 |T| plus half
-  the smallest f16 step, 2^-25 (f16);
+* the inner product T is carried as two 16-bit numbers where the result is f32 and in the gradients: half a step of half a
+  step, 2^-16 |T| (bf16) or 2^-22 |T| plus half the smallest f16 step, 2^-25 (f16); towards a 16-bit result it is rounded
+  once, half a step: 2^-8 |T| (bf16) or 2^-11 |T| plus 2^-25 (f16);
 * one rounding to the result's type: half a step, eps / 2, and 2^-25 for f16 below its normal range.
 """
 import pytest
@@ -76,8 +77,8 @@ class Lora:
     def rows(self, i):
         return torch.nonzero(self.ids == i).flatten()
 
-    def inner(self, x, a):
-        """T and its bound for every row, 64 bits."""
+    def inner(self, x, a, whole=True):
+        """T and its bound for every row, 64 bits; whole: as two 16-bit numbers."""
         t = torch.zeros(self.m, self.rank, device="cuda", dtype=torch.float64)
         e = torch.zeros_like(t)
         x = x.double()
@@ -87,12 +88,12 @@ class Lora:
                 s = float(self.scale[i])
                 t[r] = s * (x[r] @ a[i].double().t())
                 e[r] = abs(s) * acc(x.shape[1]) * (x[r].abs() @ a[i].double().abs().t()) + t[r].abs() * 2.0 ** -23
-        split = 2.0 ** -16 if self.ab == BF16 else 2.0 ** -22
+        split = HALF[self.ab] ** 2 if whole else HALF[self.ab]
         return t, e + (t.abs() + e) * split + (2.0 ** -25 if self.ab == F16 else 0.0)
 
     def expect(self, x, w, a, b):
         """(result, bound) of the forward operator in 64 bits."""
-        t, et = self.inner(x, a)
+        t, et = self.inner(x, a, whole=self.c == F32)
         xd, wd = x.double(), w.double()
         y = xd @ wd.t()
         mag = xd.abs() @ wd.abs().t()
