@@ -27,14 +27,22 @@ struct MoeParams {
 };
 
 // ---- router -----------------------------------------------------------------
-// 256 warps share the experts' rows of four tokens; with fewer experts each row is cut into `parts` ranges of d.  The
+// 128 warps share the experts' rows of four tokens; with fewer experts each row is cut into `parts` ranges of d.  The
 // sums go to the CTA that owns the token (the cluster's CTAs 0-3), which adds the parts in order and chooses.  Bound by
-// the latency of its loads, hence the many warps (64 tokens, 128 experts of d = 2048: 28 us with 64 warps).
-constexpr int ROUTER_THREADS = 1024, ROUTER_CLUSTER = 8, ROUTER_TOKENS = 4;
+// latency: what it reads is asked into L2 while the kernel before still runs (which is safe whatever that kernel
+// writes), the loads of two steps are on their way at once, a round of the choice is two warp-wide reductions.
+constexpr int ROUTER_THREADS = 512, ROUTER_CLUSTER = 8, ROUTER_TOKENS = 4;
 
 template <bool BF16>
 __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoeParams p) {
     __shared__ float part[MAX_EXPERTS];
+    {
+        const int64_t cta = ptx::cluster_ctarank(), t0 = int64_t(blockIdx.x) / ROUTER_CLUSTER * ROUTER_TOKENS;
+        const int64_t r_bytes = int64_t(p.experts) * p.d * 2, x_bytes = int64_t(min(ROUTER_TOKENS, p.tokens - int(t0))) * p.d * 2;
+        const char *r = reinterpret_cast<const char *>(p.r), *x = reinterpret_cast<const char *>(p.x + t0 * p.d);
+        for (int64_t i = (cta * ROUTER_THREADS + threadIdx.x) * 128; i < r_bytes; i += ROUTER_CLUSTER * ROUTER_THREADS * 128) ptx::prefetch_l2(r + i);
+        for (int64_t i = int64_t(threadIdx.x) * 128; i < x_bytes; i += ROUTER_THREADS * 128) ptx::prefetch_l2(x + i);
+    }
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -54,11 +62,12 @@ __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoePar
         for (int c = int(int64_t(vecs) * q / parts) + lane; c < end; c += 32) {
             const uint4 rv = *reinterpret_cast<const uint4 *>(r + 8 * c);
             const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+            uint4 xv[ROUTER_TOKENS];  // a token past the last is the first once more: no branch between the loads
+#pragma unroll
+            for (int t = 0; t < ROUTER_TOKENS; t++) xv[t] = *reinterpret_cast<const uint4 *>(x + (t < count ? int64_t(t) * p.d : 0) + 8 * c);
 #pragma unroll
             for (int t = 0; t < ROUTER_TOKENS; t++) {
-                if (t >= count) break;
-                const uint4 xv = *reinterpret_cast<const uint4 *>(x + int64_t(t) * p.d + 8 * c);
-                const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+                const uint32_t xw[4] = {xv[t].x, xv[t].y, xv[t].z, xv[t].w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float2 a = pair_f32<BF16>(rw[i]), b = pair_f32<BF16>(xw[i]);
@@ -105,34 +114,37 @@ __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoePar
         }
     }
     total = warp_sum(total);
-    float chosen_sum = 0.0f, my_w = 0.0f;
+    // A logit as an unsigned number of the same order (-0 as +0); a NaN counts as the smallest, its weight is a NaN.
+    auto order = [](float f) -> uint32_t {
+        if (!(f == f)) return 0u;
+        const uint32_t u = __float_as_uint(f + 0.0f);
+        return (u >> 31) ? ~u : u | 0x80000000u;
+    };
+    float my_logit = 0.0f;
     int my_id = 0;
     for (int i = 0; i < p.top; i++) {
-        // The largest open logit, the lowest index among equals; a NaN counts as the smallest (its weight is a NaN).
-        float key = -INFINITY;
+        // The largest open logit, the lowest index among equals.  The lane's own first.
+        uint32_t key = 0u;
         int at = 0x7fffffff;
+        float logit = 0.0f;
 #pragma unroll
         for (int j = 0; j < MAX_EXPERTS / 32; j++) {
             if (j >= per_lane) break;
             if ((open >> j) & 1u) {
-                const float c = v[j] == v[j] ? v[j] : -INFINITY;
-                if (at == 0x7fffffff || c > key) key = c, at = j * 32 + lane;
+                const uint32_t k = order(v[j]);
+                if (at == 0x7fffffff || k > key) key = k, at = j * 32 + lane, logit = v[j];
             }
         }
-#pragma unroll
-        for (int s = 16; s > 0; s >>= 1) {
-            const float k2 = __shfl_xor_sync(0xffffffffu, key, s);
-            const int a2 = __shfl_xor_sync(0xffffffffu, at, s);
-            if (a2 != 0x7fffffff && (at == 0x7fffffff || k2 > key || (k2 == key && a2 < at))) key = k2, at = a2;
-        }
-        if ((at & 31) == lane) open &= ~(1u << (at >> 5));
-        const float w = expf(key - best) / total;
-        chosen_sum += w;
-        if (lane == i) my_w = w, my_id = at;
+        const uint32_t best_key = __reduce_max_sync(0xffffffffu, key);
+        const int winner = int(__reduce_min_sync(0xffffffffu, key == best_key ? uint32_t(at) : 0x7fffffffu));
+        const float w = __shfl_sync(0xffffffffu, logit, winner & 31);
+        if ((winner & 31) == lane) open &= ~(1u << (winner >> 5));
+        if (lane == i) my_logit = w, my_id = winner;
     }
+    const float w = lane < p.top ? expf(my_logit - best) / total : 0.0f, chosen_sum = warp_sum(w);
     if (lane < p.top) {
         p.ids[t * p.top + lane] = my_id;
-        p.weights[t * p.top + lane] = p.renorm ? my_w / chosen_sum : my_w;
+        p.weights[t * p.top + lane] = p.renorm ? w / chosen_sum : w;
     }
 }
 
