@@ -157,6 +157,8 @@ struct MoeHead {
     unsigned long long who[MAX_EXPERTS];             // by expert: which tokens chose it
     int32_t ids[MAX_TOKENS * MAX_TOP];
     float weights[MAX_TOKENS * MAX_TOP];
+    int32_t row[MAX_TOKENS];  // of the chunk at hand: the tokens that chose its expert
+    float row_weight[MAX_TOKENS];
 };
 constexpr uint32_t MOE_HEAD = 16 * 1024;
 static_assert(sizeof(MoeHead) <= MOE_HEAD, "head");
@@ -195,15 +197,24 @@ constexpr uint32_t MOE_SMEM = 216 * 1024;  // leaves room for the next kernels' 
 // ---- up ---------------------------------------------------------------------------
 // The rows of the chosen experts' gate and up weights, eight of each to a group, are dealt out evenly over the CTAs;
 // a CTA takes its range in chunks of up to sixteen groups of one expert.  A chunk's MMA has N = 16 columns per group:
-// first the chunk's gate rows, then its up rows; a thread of the epilogue (a token) reads both of each pair.
-//   warp 0  TMA: per stage one or two k blocks of X and of the weights, 8 g rows of each matrix as boxes of 64, 32, 16
-//           and 8 rows, a lane per box (boxes of 8 rows alone would cap the stream at 4 TB/s, those of 16 at 6.5: measured).
-//   warp 1  MMA, two accumulators in turn.   warps 2-5  epilogue: silu, product, routing weight, rounding.
-constexpr int UP_GROUPS = 16;
+// first the chunk's gate rows, then its up rows.
+//   warp 0  TMA: per stage one, two or four k blocks of X and of the weights, 8 g rows of each matrix as boxes of 64, 32,
+//           16 and 8 rows, a lane per box (boxes of 8 rows alone would cap the stream at 4 TB/s, those of 16 at 6.5: measured).
+//   warp 1  MMA, two accumulators in turn.
+//   warps 2-5  epilogue: silu, product, routing weight, rounding.  Only the tokens that chose the expert count, one lane
+//           of 64 for a single token, so 32 pairs of columns at a time go through shared memory, where all 128 threads
+//           share them (a thread per token took 1.2 us per group: 15 us after the last weight, 8 of 4096 x 14336).
+constexpr int UP_GROUPS = 16, UP_PAIRS = 32;
+constexpr uint32_t UP_PITCH = (2 * UP_PAIRS + 4) * 4;  // a token's pairs of one step: gate, up
 struct UpMaps {
     CUtensorMap gate[4], up[4];  // boxes of 64, 32, 16 and 8 rows
 };
-__device__ __forceinline__ int up_blocks(int groups) { return groups <= 8 ? 2 : 1; }  // k blocks per stage
+// k blocks per stage: what a stage of 2 token_rows + 256 rows holds.
+__device__ __forceinline__ int up_blocks(int groups, int token_rows) {
+    return groups > 8 ? 1 : (groups <= 4 && 4 * (token_rows + 16 * groups) <= 2 * token_rows + 256 ? 4 : 2);
+}
+
+__host__ __device__ __forceinline__ uint32_t up_step_bytes(int token_rows) { return (uint32_t(token_rows) * UP_PITCH + 1023u) & ~1023u; }
 
 // Calls f(expert's place in the list, first group, groups) for every chunk of this CTA; f returns false to stop.
 template <typename F>
@@ -228,7 +239,8 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     MoeHead &h = *reinterpret_cast<MoeHead *>(smem_raw + (base - raw));
-    const uint32_t ring = base + MOE_HEAD, x_bytes = uint32_t(p.token_rows) * 128u;
+    // The head, the epilogue's step, the ring.
+    const uint32_t pairs = base + MOE_HEAD, ring = pairs + up_step_bytes(p.token_rows), x_bytes = uint32_t(p.token_rows) * 128u;
     auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
     volatile uint32_t *abort_flag = &h.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k_blocks = (p.d + 63) / 64;
@@ -266,13 +278,15 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (ok)
             up_chunks(h, p, [&](int a, int g0, int groups) {
-                const int kps = up_blocks(groups), w_bytes = groups * 2048;
-                // Lanes 0-9 and 10-19 issue the boxes of a stage's two k blocks, five per matrix: two of 64 rows, then 32, 16, 8;
-                // lanes 30 and 31 the blocks of X.
-                const int kk = lane < 20 ? lane / 10 : lane & 1, up = lane % 10 / 5, box = lane % 5;
+                const int kps = up_blocks(groups, p.token_rows), w_bytes = groups * 2048;
+                // Lanes issue the boxes of a stage's k blocks, per matrix two of 64 rows, then 32, 16, 8 (up to four groups: from
+                // 32 on), and, from lane 28 or 30 on, the blocks of X.
+                const int boxes = kps == 4 ? 3 : 5, weights = kps == 4 ? 24 : 20;
+                const bool x_lane = lane >= 32 - (kps == 4 ? 4 : 2);
+                const int kk = x_lane ? lane - (32 - (kps == 4 ? 4 : 2)) : lane / (2 * boxes), up = lane / boxes % 2, box = lane % boxes + 5 - boxes;
                 const int size = box < 2 ? 64 : 128 >> box;
                 const int off = box < 2 ? 64 * box : (8 * groups) & ~(2 * size - 1);  // the larger boxes lie before it
-                const bool mine = lane < 20 && (box < 2 ? groups >= 8 * (box + 1) : (8 * groups & size) != 0);
+                const bool mine = lane < weights && (box < 2 ? groups >= 8 * (box + 1) : (8 * groups & size) != 0);
                 const CUtensorMap *map = (up ? maps.up : maps.gate) + (box < 2 ? 0 : box - 1);
                 const uint32_t to = uint32_t(kps) * x_bytes + uint32_t(kk * w_bytes + up * groups * 1024 + off * 128);
                 const int row = h.expert[a] * p.f + 8 * g0 + off;
@@ -285,7 +299,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
                     if (lane == 0) ptx::mbar_arrive_expect_tx(full, uint32_t(nk) * (x_bytes + uint32_t(w_bytes)));
                     __syncwarp();
                     if (mine && kk < nk) ptx::tma_load_2d(dst + to, map, full, (kb + kk) * 64, row);
-                    if (lane >= 30 && kk < nk) ptx::tma_load_2d(dst + uint32_t(kk) * x_bytes, &tmX, full, (kb + kk) * 64, 0);
+                    if (x_lane && kk < nk) ptx::tma_load_2d(dst + uint32_t(kk) * x_bytes, &tmX, full, (kb + kk) * 64, 0);
                     __syncwarp();
                     filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
                     if (++s == p.stages) s = 0, ph ^= 1u;
@@ -307,7 +321,7 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit)), issued = false;
         if (ok)
             up_chunks(h, p, [&](int, int, int groups) {
-                const int buf = it & 1, kps = up_blocks(groups);
+                const int buf = it & 1, kps = up_blocks(groups, p.token_rows);
                 const uint32_t idesc = make_idesc(p.bf16, 128, 16 * groups), d = tmem + uint32_t(buf) * 256u;
                 ok = __all_sync(0xffffffffu, wait_bar(bar(h.tempty[buf]), (uint32_t(it >> 1) & 1u) ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf), limit));
                 if (!ok) return false;
@@ -354,34 +368,52 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
             const bool ok = wait_bar(bar(h.tfull[buf]), uint32_t(it >> 1) & 1u, abort_flag, p.status, WHERE_EPILOGUE, uint32_t(buf), limit);
             if (!__all_sync(0xffffffffu, ok)) return false;
             ptx::tc_fence_after();
+            // The tokens that chose the expert, in order, and their weights.
             const int e = h.expert[a];
             const unsigned long long who = h.who[e];
-            if (q < 2 && uint32_t(who >> (32 * q)) != 0u) {
-                const bool mine = (who >> token) & 1ull;
-                float weight = 0.0f;
-                if (mine)
-                    for (int i = 0; i < p.top; i++)
-                        if (h.ids[token * p.top + i] == e) weight = h.weights[token * p.top + i];
-                uint16_t *out = p.h + (int64_t(a) * p.token_rows + token) * p.f + 8 * g0;
-                for (int g = 0; g < groups; g++) {
-                    uint32_t vg[8], vu[8];
-                    const uint32_t at = tmem + (uint32_t(32 * q) << 16) + uint32_t(256 * buf + 8 * g);
-                    ptx::tmem_ld_32x8(at, vg);
-                    ptx::tmem_ld_32x8(at + uint32_t(8 * groups), vu);
+            const int count = __popcll(who), thread = threadIdx.x - 64;
+            const bool mine = q < 2 && ((who >> (token & 63)) & 1ull);
+            const int place = __popcll(who & ((1ull << (token & 63)) - 1ull));
+            if (mine) {
+                h.row[place] = token;
+                for (int i = 0; i < p.top; i++)
+                    if (h.ids[token * p.top + i] == e) h.row_weight[place] = h.weights[token * p.top + i];
+            }
+            const int columns = 8 * groups;
+            for (int c0 = 0; c0 < columns; c0 += UP_PAIRS) {
+                const int pairs_here = min(UP_PAIRS, columns - c0);
+                if (q < 2 && uint32_t(who >> (32 * q)) != 0u) {
+                    uint32_t vg[32], vu[32];
+                    const uint32_t at = tmem + (uint32_t(32 * q) << 16) + uint32_t(256 * buf + c0);
+                    ptx::tmem_ld_32x32(at, vg);
+                    ptx::tmem_ld_32x32(at + uint32_t(columns), vu);
                     ptx::tmem_ld_wait_all();
-                    ptx::pin8(vg);
-                    ptx::pin8(vu);
-                    float o[8];
+                    ptx::pin(vg);
+                    ptx::pin(vu);
+                    if (mine) {
+                        const uint32_t dst = pairs + uint32_t(place) * UP_PITCH;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float gate = __uint_as_float(vg[j]), up = __uint_as_float(vu[j]);
-                        o[j] = weight * (gate / (1.0f + expf(-gate))) * up;
+                        for (int g = 0; g < 8; g++) {
+                            ptx::st_shared_v4(dst + 16u * g, vg[4 * g], vg[4 * g + 1], vg[4 * g + 2], vg[4 * g + 3]);
+                            ptx::st_shared_v4(dst + 128u + 16u * g, vu[4 * g], vu[4 * g + 1], vu[4 * g + 2], vu[4 * g + 3]);
+                        }
                     }
-                    // Rounded once, to the operands' type: the last product runs on 16-bit tensor-core operands.
-                    if (mine)
-                        *reinterpret_cast<uint4 *>(out + 8 * g) = make_uint4(pack_16(o[0], o[1], p.bf16), pack_16(o[2], o[3], p.bf16),
-                                                                            pack_16(o[4], o[5], p.bf16), pack_16(o[6], o[7], p.bf16));
                 }
+                ptx::named_barrier(1, 128);
+                // Two columns of one token per thread and turn.
+                for (int i = thread; i < count * (UP_PAIRS / 2); i += 128) {
+                    const int r = i / (UP_PAIRS / 2), c = i % (UP_PAIRS / 2) * 2;
+                    if (c >= pairs_here) continue;
+                    const float *v = reinterpret_cast<const float *>(smem_raw + (pairs - raw) + uint32_t(r) * UP_PITCH) + c;
+                    const float weight = h.row_weight[r];
+                    float o[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) o[j] = weight * (v[j] / (1.0f + expf(-v[j]))) * v[UP_PAIRS + j];
+                    // Rounded once, to the operands' type: the last product runs on 16-bit tensor-core operands.
+                    uint16_t *out = p.h + (int64_t(a) * p.token_rows + h.row[r]) * p.f + 8 * g0 + c0 + c;
+                    *reinterpret_cast<uint32_t *>(out) = pack_16(o[0], o[1], p.bf16);
+                }
+                ptx::named_barrier(1, 128);
             }
             ptx::tc_fence_before();
             __syncwarp();
@@ -637,8 +669,8 @@ Layout layout(const cute_b200_moe_desc &d) {
 }
 
 // Stages of `bytes` behind the head; an MMA reads 128 rows of 128 bytes from up to `last` bytes behind a stage's start.
-int ring_stages(uint32_t bytes, uint32_t last) {
-    const uint32_t ring = MOE_SMEM - MOE_HEAD - 1024, reach = last + 16384, over = bytes < reach ? reach - bytes : 0;
+int ring_stages(uint32_t bytes, uint32_t last, uint32_t before = 0) {
+    const uint32_t ring = MOE_SMEM - MOE_HEAD - 1024 - before, reach = last + 16384, over = bytes < reach ? reach - bytes : 0;
     const int stages = int((ring - over) / bytes);
     return stages < MOE_MAX_STAGES ? stages : MOE_MAX_STAGES;
 }
@@ -692,7 +724,7 @@ cute_b200_status moe_tn(const cute_b200_moe_desc &d, const uint64_t ptr[7], cuda
         CB_TRY(rows_tensor_map(&maps.up[i], ptr[3], p.bf16, uint64_t(d.experts) * d.f, d.d, d.d, 64 >> i));
     }
     p.stage_bytes = uint32_t(2 * p.token_rows + 16 * UP_GROUPS) * 128u;
-    p.stages = ring_stages(p.stage_bytes, 0);
+    p.stages = ring_stages(p.stage_bytes, 0, up_step_bytes(p.token_rows));
     CB_TRY(launch_dependent(moe_up_kernel, dim3(unsigned(dev.sm_count)), MOE_THREADS, MOE_SMEM, 1, stream, tmX, maps, p));
 
     p.bn = 16, p.kc = 1;
