@@ -132,14 +132,21 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
         uint32_t ph = 0, filled = 0, filled_parity = 0;
         bool ok = !(p.debug & 4);
         const uint32_t bytes = uint32_t(2 + low_boxes) * GRAD_BOX;
-        for (int b = b0; b < b1 && ok; b++) {
-            // Lanes 0-15 hold four rows of the block each; past the end of the list a row that no matrix has.
-            int row[4];
+        // Lanes 0-15 hold four rows of a block each, read one block ahead; past the end of the list a row that no matrix has.
+        int next[4];
+        auto read_rows = [&](int b) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int at = b * GRAD_ROWS + 4 * (lane & 15) + i;
-                row[i] = at < count ? p.list[begin + at] : p.m;
+                next[i] = b < b1 && at < count ? p.list[begin + at] : p.m;
             }
+        };
+        read_rows(b0);
+        for (int b = b0; b < b1 && ok; b++) {
+            int row[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) row[i] = next[i];
+            read_rows(b + 1);
             const int first_row = __shfl_sync(0xffffffffu, row[0], 0), last_row = __shfl_sync(0xffffffffu, row[3], 15);
             const bool run = last_row < p.m && last_row - first_row == GRAD_ROWS - 1;
             ok = wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit);
