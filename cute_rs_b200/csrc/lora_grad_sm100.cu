@@ -63,8 +63,15 @@ __global__ void __launch_bounds__(LIST_THREADS) row_list_kernel(const int32_t *i
 }
 
 constexpr int GRAD_THREADS = 192, GRAD_M = 128, GRAD_ROWS = 64, GRAD_STAGES = 4;
-constexpr uint32_t GRAD_BOX = GRAD_ROWS * 128, GRAD_RING = 96 * 1024, GRAD_HEAD = 1024;
-constexpr uint32_t GRAD_SMEM = 1024 + GRAD_HEAD + GRAD_RING;
+constexpr uint32_t GRAD_BOX = GRAD_ROWS * 128, GRAD_HEAD = 1024;
+
+// How a tile is cut by rank.  What bounds the kernel beside HBM is the way from L2 to the SMs (some 100 GB/s each): per 64
+// rows a tile fetches 8 KB per 64 columns of V and 8 KB per 64 columns of L, so a high rank takes two accumulators of 128
+// columns of V (rank 128, 8192 rows, 8192 + 2048 columns: 491 MB with one, 335 MB with two), and the SM to itself.
+__host__ __device__ constexpr int grad_halves(int rp) { return rp >= 64 ? 2 : 1; }
+__host__ __device__ constexpr int grad_low_boxes(int rp) { return (2 * rp + 63) / 64; }
+constexpr uint32_t grad_ring(int rp) { return (rp == 128 ? 192u : 96u) * 1024; }
+constexpr uint32_t grad_smem(int rp) { return 1024 + GRAD_HEAD + grad_ring(rp); }
 
 struct GradMaps {
     CUtensorMap wide[2], wide_rows[2], low[2], low_rows[2];  // [0] for dA: X and U, [1] for dB: dY and T; boxes of 64 rows, and of one
@@ -73,7 +80,7 @@ struct GradMaps {
 struct GradParams {
     float *out[2];
     const int32_t *first, *list;
-    int cols[2], tiles[2], m, rank, rp, kc, stages, vec;
+    int cols[2], tiles[2], m, rank, rp, halves, kc, stages, vec;
     uint32_t stage_bytes, idesc, tmem_cols;
     uint32_t *status;
     int debug;
@@ -97,7 +104,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
     int tile = unit - a * per;
     const int job = tile >= p.tiles[0] ? 1 : 0;
     if (job) tile -= p.tiles[0];
-    const int c0 = tile * GRAD_M, low_boxes = (2 * p.rp + 63) / 64;
+    const int c0 = tile * GRAD_M * p.halves, wide_boxes = 2 * p.halves, low_boxes = grad_low_boxes(p.rp);
     const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
 
     if (threadIdx.x == 0) {
@@ -131,7 +138,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
         int s = 0;
         uint32_t ph = 0, filled = 0, filled_parity = 0;
         bool ok = !(p.debug & 4);
-        const uint32_t bytes = uint32_t(2 + low_boxes) * GRAD_BOX;
+        const uint32_t bytes = uint32_t(wide_boxes + low_boxes) * GRAD_BOX;
         // Lanes 0-15 hold four rows of a block each, read one block ahead; past the end of the list a row that no matrix has.
         int next[4];
         auto read_rows = [&](int b) {
@@ -156,13 +163,13 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
             if (lane == 0) ptx::mbar_arrive_expect_tx(full, bytes);
             __syncwarp();
             if (run) {  // a lane per box
-                if (lane < 2) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.wide[job], full, c0 + 64 * lane, first_row);
-                else if (lane < 2 + low_boxes) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.low[job], full, 64 * (lane - 2), first_row);
+                if (lane < wide_boxes) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.wide[job], full, c0 + 64 * lane, first_row);
+                else if (lane < wide_boxes + low_boxes) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.low[job], full, 64 * (lane - wide_boxes), first_row);
             } else if (lane < 16) {
-                for (int x = 0; x < 2; x++)
+                for (int x = 0; x < wide_boxes; x++)
                     ptx::tma_gather4(dst + x * GRAD_BOX + 512u * lane, &maps.wide_rows[job], full, c0 + 64 * x, row[0], row[1], row[2], row[3]);
                 for (int x = 0; x < low_boxes; x++)
-                    ptx::tma_gather4(dst + (2 + x) * GRAD_BOX + 512u * lane, &maps.low_rows[job], full, 64 * x, row[0], row[1], row[2], row[3]);
+                    ptx::tma_gather4(dst + (wide_boxes + x) * GRAD_BOX + 512u * lane, &maps.low_rows[job], full, 64 * x, row[0], row[1], row[2], row[3]);
             }
             __syncwarp();
             filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
@@ -186,11 +193,15 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
             if (!ok) break;
             ptx::tc_fence_after();
             const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
-            const uint64_t wide = mn_desc(src, GRAD_BOX), low = mn_desc(src + 2 * GRAD_BOX, GRAD_BOX);
+            const uint64_t low = mn_desc(src + uint32_t(wide_boxes) * GRAD_BOX, GRAD_BOX);
             const uint32_t more = b > b0 ? 1u : 0u;
             if (leader) {
+                for (int x = 0; x < p.halves; x++) {
+                    const uint64_t wide = mn_desc(src + uint32_t(2 * x) * GRAD_BOX, GRAD_BOX);
 #pragma unroll
-                for (int j = 0; j < 4; j++) ptx::umma_f16<1>(tmem, wide + MN_K_STEP * j, low + MN_K_STEP * j, p.idesc, j > 0 ? 1u : more);
+                    for (int j = 0; j < 4; j++)
+                        ptx::umma_f16<1>(tmem + uint32_t(2 * x * p.rp), wide + MN_K_STEP * j, low + MN_K_STEP * j, p.idesc, j > 0 ? 1u : more);
+                }
                 ptx::umma_commit<1>(bar(h.empty[s]));
             }
             __syncwarp();
@@ -211,17 +222,20 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
     } else {
         const bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.done), 0, abort_flag, p.status, WHERE_EPILOGUE, 0u, limit));
         const int q = warp & 3;
-        const uint32_t pitch = uint32_t(p.rp + 4) * 4u, dst = ring + uint32_t(32 * q + lane) * pitch;
+        const uint32_t pitch = uint32_t(p.rp + 4) * 4u;
         if (ok) {
             ptx::tc_fence_after();
             ptx::fence_proxy_async_shared();
             // Columns j and rp + j belong to the two numbers of value j: their sum is the gradient's part.
-            for (int c = 0; c < p.rp; c += 16) {
+            for (int i = 0; i < p.halves * p.rp; i += 16) {
+                const int x = i / p.rp, c = i - x * p.rp;
+                const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(2 * x * p.rp + c);
+                const uint32_t dst = ring + uint32_t(GRAD_M * x + 32 * q + lane) * pitch;
                 float v[16];
                 if (b0 < b1) {
                     uint32_t hi[16], lo[16];
-                    ptx::tmem_ld_32x16(tmem + (uint32_t(32 * q) << 16) + uint32_t(c), hi);
-                    ptx::tmem_ld_32x16(tmem + (uint32_t(32 * q) << 16) + uint32_t(p.rp + c), lo);
+                    ptx::tmem_ld_32x16(from, hi);
+                    ptx::tmem_ld_32x16(from + uint32_t(p.rp), lo);
                     ptx::tmem_ld_wait_all();
                     ptx::pin16(hi);
                     ptx::pin16(lo);
@@ -250,10 +264,10 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
         const uint32_t pitch = uint32_t(p.rp + 4) * 4u;
         // Four ranks of one column of V per step.  Neighbouring threads write neighbouring addresses: of dA the columns, of dB
         // the ranks, 16 bytes at once.
-        const int cols = p.cols[job], wide = min(GRAD_M, cols - c0), quads = p.rank / 4, items = GRAD_M * quads;
+        const int cols = p.cols[job], columns = GRAD_M * p.halves, wide = min(columns, cols - c0), quads = p.rank / 4, items = columns * quads;
         float *out = p.out[job] + int64_t(a) * p.rank * cols;
         for (int i = int(rank) * GRAD_THREADS + int(threadIdx.x); i < items; i += p.kc * GRAD_THREADS) {
-            const int c = job ? i / quads : i % GRAD_M, j = 4 * (job ? i % quads : i / GRAD_M);
+            const int c = job ? i / quads : i % columns, j = 4 * (job ? i % quads : i / columns);
             if (c >= wide) continue;
             const float4 v = cluster_sum(ring + uint32_t(c) * pitch + uint32_t(j) * 4u, p.kc);
             if (job) {
@@ -286,7 +300,7 @@ cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const Devi
     for (int i = 0; i < 2; i++) {
         p.out[i] = g.out[i];
         p.cols[i] = g.cols[i];
-        p.tiles[i] = (g.cols[i] + GRAD_M - 1) / GRAD_M;
+        p.tiles[i] = (g.cols[i] + GRAD_M * grad_halves(g.rp) - 1) / (GRAD_M * grad_halves(g.rp));
         const uint64_t wide = reinterpret_cast<uint64_t>(g.wide[i]), low = reinterpret_cast<uint64_t>(g.low[i]);
         CB_TRY(rows_tensor_map(&maps.wide[i], wide, bf16, g.m, g.cols[i], g.pitch[i], GRAD_ROWS));
         CB_TRY(rows_tensor_map(&maps.wide_rows[i], wide, bf16, g.m, g.cols[i], g.pitch[i], 1));
@@ -295,25 +309,30 @@ cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const Devi
     }
     p.first = g.first, p.list = g.list;
     p.vec = reinterpret_cast<uint64_t>(g.out[1]) % 16 == 0;
-    p.m = g.m, p.rank = g.rank, p.rp = g.rp;
-    p.stage_bytes = uint32_t(2 + (2 * g.rp + 63) / 64) * GRAD_BOX;
-    p.stages = int(GRAD_RING / p.stage_bytes);
+    p.m = g.m, p.rank = g.rank, p.rp = g.rp, p.halves = grad_halves(g.rp);
+    p.stage_bytes = uint32_t(2 * p.halves + grad_low_boxes(g.rp)) * GRAD_BOX;
+    p.stages = int(grad_ring(g.rp) / p.stage_bytes);
     if (p.stages > GRAD_STAGES) p.stages = GRAD_STAGES;
     p.idesc = make_idesc(bf16, GRAD_M, 2 * g.rp) | IDESC_A_MN | IDESC_B_MN;
-    p.tmem_cols = uint32_t(2 * g.rp);
+    p.tmem_cols = uint32_t(2 * g.rp * p.halves);
     p.status = dev.status_word;
     p.debug = debug;
-    // The rows of a tile are shared by a cluster while that fills the GPU (two CTAs per SM) and leaves each CTA of an
-    // adapter of average size at least four blocks.
-    const int64_t units = int64_t(p.tiles[0] + p.tiles[1]) * g.adapters;
+    // The rows of a tile are shared by a cluster of kc CTAs: the least time for whole waves of CTAs, each the blocks of an
+    // adapter of average size and some twelve blocks' time to start, add up and store.
+    const int64_t units = int64_t(p.tiles[0] + p.tiles[1]) * g.adapters, slots = int64_t(dev.sm_count) * (g.rp == 128 ? 1 : 2);
+    const int blocks = int((int64_t(g.m) + int64_t(GRAD_ROWS) * g.adapters - 1) / (int64_t(GRAD_ROWS) * g.adapters));
     p.kc = 1;
-    while (p.kc < 8 && units * p.kc < 2 * dev.sm_count && int64_t(g.m) >= int64_t(8 * GRAD_ROWS) * p.kc * g.adapters) p.kc *= 2;
+    double best = 1e300;
+    for (int kc = 1; kc <= 8 && kc <= blocks; kc++) {
+        const double waves = double((units * kc + slots - 1) / slots), t = waves * ((blocks + kc - 1) / kc + 12.0);
+        if (t < best) best = t, p.kc = kc;
+    }
     if (units * p.kc > 0x7fffffff) return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "lora_tn_backward: the adapters are too large");
-    return launch_dependent(lora_grad_kernel, dim3(unsigned(units * p.kc)), GRAD_THREADS, GRAD_SMEM, p.kc, stream, maps, p);
+    return launch_dependent(lora_grad_kernel, dim3(unsigned(units * p.kc)), GRAD_THREADS, grad_smem(g.rp), p.kc, stream, maps, p);
 }
 
 cute_b200_status lora_grad_init() {
-    CB_CUDA(cudaFuncSetAttribute(lora_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GRAD_SMEM));
+    CB_CUDA(cudaFuncSetAttribute(lora_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, grad_smem(128)));
     return CUTE_B200_OK;
 }
 

@@ -27,7 +27,7 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 //           the plan of the GEMM's tile that starts at its rows), then the sum over the
 //           cluster, scale, split into two 16-bit numbers.
 // On the way back A is B[a] as it lies, (n, rank): rank is the fast index, so it is an MN-major operand.
-constexpr int SHRINK_THREADS = 192, X_STAGES = 3, A_STAGES = 3, X_BLOCKS = 2;
+constexpr int SHRINK_THREADS = 192, X_STAGES = 4, A_STAGES = 2, X_BLOCKS = 2;
 constexpr uint32_t X_BYTES = BM * BK * 2, A_BYTES = 32 * 1024, SHRINK_HEAD = 20 * 1024;
 constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + X_STAGES * X_BLOCKS * X_BYTES + A_STAGES * A_BYTES;
 
@@ -50,6 +50,7 @@ struct ShrinkHead {
     uint64_t xfull[X_STAGES], xempty[X_STAGES], afull[A_STAGES], aempty[A_STAGES], plan, done, drain;
     uint32_t tmem, abort;
     int32_t entries, entry_id[BM], id[BM];
+    float scale[BM];
     uint32_t off[BM][4];
     IdTable<128> rows;  // of this CTA's rows
     IdTable<P> tile;    // of the GEMM's tile
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             const int32_t ids[1] = {read_id(row0 + t)};
             int32_t mine[1];
             h.id[t] = ids[0];
+            h.scale[t] = ids[0] >= 0 ? __ldcg(p.scale + ids[0]) : 0.0f;
             for (int i = t; i < BM * 4; i += 128) h.off[i / 4][i % 4] = 0xffffffffu;
             const int total = distinct_ids<128>(ids, h.rows, t, mine, [&](int e, int id) { h.entry_id[e] = id; });
             if (mine[0] >= 0) atomicAnd(&h.off[mine[0]][t / 32], ~(1u << (t % 32)));
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (id >= 0 && col < p.rank) {  // lanes of rows without an adapter hold nothing; past the rank may lie another adapter's sums
                 v = cluster_sum(xring + uint32_t(row) * pitch + uint32_t(col) * 4u, p.kc);
-                const float s = __ldcg(p.scale + id);
+                const float s = h.scale[row];
                 v.x *= s, v.y *= s, v.z *= s, v.w *= s;
             }
             const uint32_t h0 = pack_16(v.x, v.y, p.bf16), h1 = pack_16(v.z, v.w, p.bf16);
