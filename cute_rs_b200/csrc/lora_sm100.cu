@@ -92,7 +92,7 @@ struct FewParams {
     void *y;
     int64_t ldy;
     int m, n, rank, rp, adapters, c_dtype, vec;
-    int k_blocks, bn, kc, xr, stages, kps, b_blocks;
+    int k_blocks, bn, kc, xr, stages, kps, b_blocks, parts;  // parts: accumulators the k range goes to in turn
     uint32_t stage_bytes, x_bytes, w_bytes, low_bytes, idesc, tmem_cols;
     const uint16_t *t, *b;
     bool bf16;
@@ -293,16 +293,20 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             __syncwarp();
             if (++s == p.stages) s = 0, ph ^= 1u;
         };
+        const int part_cols = (p.bn + 31) / 32 * 32;
+        int part = 0, part_end = kb0 + (kb1 - kb0 + p.parts - 1) / p.parts;  // the k block the next accumulator begins at
         for (int kb = kb0; kb < kb1; kb += p.kps) {
             if (!ready()) break;
             const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
             const int nk = min(p.kps, kb1 - kb);
             for (int kk = 0; kk < nk; kk++) {
                 const uint64_t a = sw128_desc(src + uint32_t(kk) * p.x_bytes), b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
-                const uint32_t more = kb > kb0 || kk > 0 ? 1u : 0u;
+                const bool next_part = kb + kk == part_end && part + 1 < p.parts;
+                if (next_part) part++, part_end = kb0 + ((kb1 - kb0) * (part + 1) + p.parts - 1) / p.parts;
+                const uint32_t more = (kb > kb0 || kk > 0) && !next_part ? 1u : 0u, d = tmem + uint32_t(part * part_cols);
                 if (leader) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) ptx::umma_f16<1>(tmem, a + 2u * j, b + 2u * j, p.idesc, j > 0 ? 1u : more);
+                    for (int j = 0; j < 4; j++) ptx::umma_f16<1>(d, a + 2u * j, b + 2u * j, p.idesc, j > 0 ? 1u : more);
                 }
                 __syncwarp();
             }
@@ -374,8 +378,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             ptx::fence_proxy_async_shared();
             for (int c = 0; c < p.bn; c += 32) {
                 uint32_t v[32];
-                ptx::tmem_ld_32x32(tmem + (uint32_t(32 * q) << 16) + uint32_t(c), v);
+                const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(c);
+                ptx::tmem_ld_32x32(from, v);
                 ptx::tmem_ld_wait(v);
+                for (int i = 1; i < p.parts; i++) {
+                    uint32_t o[32];
+                    ptx::tmem_ld_32x32(from + uint32_t(i * ((p.bn + 31) / 32 * 32)), o);
+                    ptx::tmem_ld_wait(o);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(o[j]));
+                }
                 if (32 * q + lane < p.m) {
                     const uint32_t dst = ring + uint32_t(32 * q + lane) * pitch + uint32_t(c) * 4u;
 #pragma unroll
@@ -462,7 +474,10 @@ cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int de
     f.stages = int((ring - over) / f.stage_bytes);
     if (f.stages > FEW_MAX_STAGES) f.stages = FEW_MAX_STAGES;
     f.idesc = make_idesc(BF16, 128, f.bn);
-    f.tmem_cols = f.bn <= 32 ? 32 : (f.bn <= 64 ? 64 : (f.bn <= 128 ? 128 : 256));
+    // An f32 result: two or four accumulators, added in f32 (the tensor core's own sums are cut off, not rounded).
+    f.parts = p.c_dtype != CUTE_B200_F32 ? 1 : (f.bn <= 128 ? 4 : 2);
+    while (f.parts > f.k_blocks / f.kc && f.parts > 1) f.parts /= 2;  // every one of them is written
+    for (f.tmem_cols = 32; f.tmem_cols < uint32_t(f.parts * ((f.bn + 31) / 32 * 32)); f.tmem_cols *= 2) {}
     f.status = dev.status_word;
     f.debug = debug;
     CUtensorMap tmX, tmW, tmT, tmB;

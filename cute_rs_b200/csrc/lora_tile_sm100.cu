@@ -27,8 +27,12 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 //           the plan of the GEMM's tile that starts at its rows), then the sum over the
 //           cluster, scale, split into two 16-bit numbers.
 // On the way back A is B[a] as it lies, (n, rank): rank is the fast index, so it is an MN-major operand.
+// A CTA's k range goes to T_PARTS accumulators in turn, added in f32 at the end: the tensor core cuts its sums off instead of
+// rounding them, an error of the same sign that grows with the products added into one accumulator (256 MMAs of 16: 5e-6
+// of the sum, measured), and T enters f32 gradients.
 constexpr int SHRINK_THREADS = 192, X_STAGES = 4, A_STAGES = 2, X_BLOCKS = 2;
 constexpr uint32_t X_BYTES = BM * BK * 2, A_BYTES = 32 * 1024, SHRINK_HEAD = 20 * 1024;
+constexpr int T_PARTS = 4;
 constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + X_STAGES * X_BLOCKS * X_BYTES + A_STAGES * A_BYTES;
 
 struct ShrinkParams {
@@ -39,11 +43,14 @@ struct ShrinkParams {
     int m, rank, rp, adapters, k_blocks, kc;
     int boxes;       // of A per adapter and k block
     uint32_t box_bytes;
-    uint32_t idesc, tmem_cols;
+    uint32_t idesc, part_cols;  // TMEM columns of one accumulator
     bool bf16, mn, early;
     uint32_t *status;
     int debug;
 };
+
+// Whether accumulator `part` of a range of `blocks` k blocks holds anything (block i goes to i * T_PARTS / blocks).
+__device__ __forceinline__ bool part_used(int part, int blocks) { return (part * blocks + T_PARTS - 1) / T_PARTS * T_PARTS / blocks == part; }
 
 template <int P>
 struct ShrinkHead {
@@ -90,7 +97,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         ptx::fence_mbar_init();
     }
     if (warp == 1) {
-        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), p.tmem_cols);
+        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), T_PARTS * p.part_cols);
         ptx::tmem_relinquish<1>();
     }
     ptx::tc_fence_before();
@@ -157,6 +164,10 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         uint32_t px = 0, pa = 0;
         for (int kb = kb0; kb < kb1 && ok && entries > 0; kb += X_BLOCKS) {
             const int items = min(X_BLOCKS, kb1 - kb) * entries;
+            // The accumulators of the block before these two and of the two.
+            int part[3];
+#pragma unroll
+            for (int i = 0; i < 3; i++) part[i] = kb + i > kb0 ? (kb + i - 1 - kb0) * T_PARTS / (kb1 - kb0) : -1;
             ok = __all_sync(0xffffffffu, wait_bar(bar(h.xfull[sx]), px, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(sx), limit));
             if (!ok) break;
             for (int i0 = 0; i0 < items; i0 += group) {
@@ -169,12 +180,13 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
                     const uint32_t src = aring + uint32_t(sa) * A_BYTES + uint32_t(i) * entry_bytes;
                     const uint64_t a = sw128_desc(xring + uint32_t(sx * X_BLOCKS + second) * X_BYTES);
                     const uint64_t b = p.mn ? mn_desc(src, p.box_bytes) : sw128_desc(src);
-                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u, more = kb > kb0 || second ? 1u : 0u;
+                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u, d = tmem + uint32_t(part[1 + second]) * p.part_cols;
+                    const uint32_t more = part[second] == part[1 + second] ? 1u : 0u;
                     const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
                     if (leader) {
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            ptx::umma_f16_lanes(tmem, a + 2u * j, b + k_step * j, p.idesc, j > 0 ? 1u : more, o0, o1, o2, o3);
+                            ptx::umma_f16_lanes(d, a + 2u * j, b + k_step * j, p.idesc, j > 0 ? 1u : more, o0, o1, o2, o3);
                     }
                     __syncwarp();
                 }
@@ -239,10 +251,20 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         if (ok) {
             ptx::tc_fence_after();
             ptx::fence_proxy_async_shared();
+            const int parts = min(T_PARTS, kb1 - kb0);  // those that hold something
             for (int c = 0; c < p.rp; c += 32) {
                 uint32_t v[32];
-                ptx::tmem_ld_32x32(tmem + (uint32_t(32 * q) << 16) + uint32_t(c), v);
+                const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(c);
+                ptx::tmem_ld_32x32(from, v);
                 ptx::tmem_ld_wait(v);
+                for (int i = 1; i < T_PARTS; i++) {
+                    if (parts < T_PARTS && !part_used(i, kb1 - kb0)) continue;
+                    uint32_t o[32];
+                    ptx::tmem_ld_32x32(from + uint32_t(i) * p.part_cols, o);
+                    ptx::tmem_ld_wait(o);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(o[j]));
+                }
                 const uint32_t dst = xring + uint32_t(32 * q + lane) * pitch + uint32_t(c) * 4u;
 #pragma unroll
                 for (int g = 0; g < 8; g++)
@@ -284,7 +306,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         ptx::cluster_arrive();
         ptx::cluster_wait();
     }
-    if (warp == 1) ptx::tmem_dealloc<1>(tmem, p.tmem_cols);
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, T_PARTS * p.part_cols);
 }
 
 // ---- Y --------------------------------------------------------------------------
@@ -294,6 +316,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
 // masked to the lanes of the adapter's rows.  One adapter of rank 64 costs 1 block (2 for
 // an f32 result) beside the 64 of k = 4096.
 // On the way back B is A[a] as it lies, (rank, k): an MN-major operand, in boxes of 64 columns by up to 64 ranks.
+// An f32 result of a long k is summed in `parts` accumulators (see T_PARTS), one set instead of two.
 constexpr uint32_t RING_BYTES = 192 * 1024;
 constexpr int TILE_THREADS = 64 + 256;
 
@@ -305,7 +328,7 @@ struct Tile {
     static constexpr uint32_t STAGE_BYTES = KPS * KB_BYTES;
     static constexpr int STAGES = int(RING_BYTES / STAGE_BYTES);
     static constexpr int ACC_COLS = MH * BN, ACC_BUFS = 2 * ACC_COLS <= 512 ? 2 : 1;
-    static constexpr uint32_t TMEM_COLS = ACC_COLS * ACC_BUFS;
+    static constexpr uint32_t TMEM_COLS = MH == 1 ? 512 : ACC_COLS * ACC_BUFS;
     static constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512;
     static constexpr uint32_t EXPECT = G * KB_BYTES;
     static constexpr int CH = BN / 64;  // 32-column chunks of an accumulator per epilogue warp
@@ -317,7 +340,7 @@ struct TileParams {
     void *y;
     int64_t ldy;
     int m, n, rank, rp, adapters, c_dtype, vec;
-    int k_blocks, m_tiles, n_tiles, group_m;
+    int k_blocks, m_tiles, n_tiles, group_m, parts;
     uint32_t idesc, low_idesc, low_box;  // low_box: bytes of an MN-major box of B, 0 = B is K-major
     uint32_t *status;
     int debug;
@@ -390,6 +413,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
     const uint64_t stride = plan_stride(C::ROWS, p.adapters);
     constexpr int ENTRY = 4 + C::ROWS / 32;
+    const int bufs = p.parts > 1 ? 1 : C::ACC_BUFS;
     const bool whole = whole_t(p.c_dtype);
     const int q_blocks = ext_blocks(p.rp, whole);
 
@@ -523,8 +547,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             };
             for (int t = first; t < tiles && ok; t += step, it++) {
                 const TileAt at = tile_at(t, p);
-                const int buf = it % C::ACC_BUFS;
-                const uint32_t aph = uint32_t(it / C::ACC_BUFS) & 1u, d = tmem + uint32_t(buf * C::ACC_COLS);
+                const int buf = it % bufs;
+                const uint32_t aph = uint32_t(it / bufs) & 1u, d0 = tmem + uint32_t(buf * C::ACC_COLS);
+                uint32_t d = d0;
+                int part = 0, part_end = (p.k_blocks + p.parts - 1) / p.parts;  // the k block the next accumulator begins at
                 const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
                 // Lane l holds word l of an entry's masks, read one entry ahead.
                 int entries = 0;
@@ -541,12 +567,18 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll
                     for (int kk = 0; kk < C::KPS; kk++) {
                         if (k0 + kk >= p.k_blocks) break;
-                        const bool fresh = k0 == 0 && kk == 0;
+                        bool fresh = k0 == 0 && kk == 0;
+                        if (k0 + kk == part_end && part + 1 < p.parts) {
+                            part++;
+                            part_end = (p.k_blocks * (part + 1) + p.parts - 1) / p.parts;
+                            d = d0 + uint32_t(part * C::ACC_COLS);
+                            fresh = true;
+                        }
                         const uint32_t src = stage + kk * C::KB_BYTES;
                         const uint64_t b = sw128_desc(src + C::A_BYTES);
 #pragma unroll
                         for (int h = 0; h < MH; h++) {
-                            if (fresh) {  // the epilogue must have drained this half of the buffer
+                            if (fresh && part == 0) {  // the epilogue must have drained this half of the buffer
                                 ok = __all_sync(0xffffffffu, wait_bar(tempty_bar(buf, h), aph ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf * 2 + h), limit));
                                 if (!ok) break;
                                 ptx::tc_fence_after();
@@ -593,8 +625,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                             if (leader && all != 0xffffffffu)  // else no row of these accumulators
                                 for (int j = 0; j < x.steps; j++) {
                                     const uint64_t bj = b + uint64_t(k_step * uint32_t(j & x.b_mask));
-                                    if constexpr (G == 1) ptx::umma_f16_lanes(d + uint32_t(h * BN), a + 2u * j, bj, p.low_idesc, 1u, m[0], m[1], m[2], m[3]);
-                                    else ptx::umma_f16_lanes_pair(d + uint32_t(h * BN), a + 2u * j, bj, p.low_idesc, 1u, m);
+                                    if constexpr (G == 1) ptx::umma_f16_lanes(d0 + uint32_t(h * BN), a + 2u * j, bj, p.low_idesc, 1u, m[0], m[1], m[2], m[3]);
+                                    else ptx::umma_f16_lanes_pair(d0 + uint32_t(h * BN), a + 2u * j, bj, p.low_idesc, 1u, m);
                                 }
                             __syncwarp();
                         }
@@ -622,8 +654,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         int it = 0;
         for (int t = first; t < tiles; t += step, it++) {
             const TileAt at = tile_at(t, p);
-            const int buf = it % C::ACC_BUFS;
-            const bool ok = wait_bar(tfull_bar(buf), uint32_t(it / C::ACC_BUFS) & 1u, abort_flag, p.status, WHERE_EPILOGUE, uint32_t(buf), limit);
+            const int buf = it % bufs;
+            const bool ok = wait_bar(tfull_bar(buf), uint32_t(it / bufs) & 1u, abort_flag, p.status, WHERE_EPILOGUE, uint32_t(buf), limit);
             if (!__all_sync(0xffffffffu, ok)) break;
             ptx::tc_fence_after();
             const int row0 = at.tm * C::ROWS + int(rank) * C::CTA_ROWS + int(q) * 32 + lane;
@@ -638,6 +670,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 ptx::tmem_ld_wait_all();
 #pragma unroll
                 for (int c = 0; c < C::CH; c++) ptx::pin(v[c]);
+                if constexpr (MH == 1)
+                    for (int i = 1; i < p.parts; i++) {
+#pragma unroll
+                        for (int c = 0; c < C::CH; c++) {
+                            uint32_t o[32];
+                            ptx::tmem_ld_32x32(taddr + uint32_t(i * C::ACC_COLS + (2 * c + e) * 32), o);
+                            ptx::tmem_ld_wait(o);
+#pragma unroll
+                            for (int j = 0; j < 32; j++) v[c][j] = __float_as_uint(__uint_as_float(v[c][j]) + __uint_as_float(o[j]));
+                        }
+                    }
                 ptx::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
@@ -674,7 +717,7 @@ cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceS
     s.box_bytes = p.low_mn ? BK * 128 : uint32_t(p.rp) * 128u;
     s.bf16 = bf16;
     s.idesc = make_idesc(bf16, 128, p.rp) | (p.low_mn ? IDESC_B_MN : 0u);
-    s.tmem_cols = p.rp <= 32 ? 32 : uint32_t(p.rp);
+    s.part_cols = p.rp <= 32 ? 32 : uint32_t(p.rp);
     s.status = dev.status_word;
     s.debug = debug;
     const int tiles = (p.m + BM - 1) / BM;
@@ -691,6 +734,9 @@ cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceS
     return launch_dependent(shrink_tile_kernel<P>, dim3(unsigned(tiles * s.kc)), SHRINK_THREADS, SHRINK_SMEM, s.kc, stream, tmX, tmA, s);
 }
 
+// Accumulators an f32 result of this k asks for: 4096 of k in one cost 5e-6 of the sum.
+int result_parts(int k, int c_dtype) { return c_dtype != CUTE_B200_F32 || k <= 4096 ? 1 : (k <= 8192 ? 2 : 4); }
+
 template <int G, int BN, int MH>
 cute_b200_status launch_tile(const LoraParams &p, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream) {
     using C = Tile<G, BN, MH>;
@@ -700,6 +746,8 @@ cute_b200_status launch_tile(const LoraParams &p, bool bf16, int debug, const De
     const uint64_t esize = p.c_dtype == CUTE_B200_F32 ? 4 : 2, y = reinterpret_cast<uint64_t>(p.y);
     t.vec = y % 32 == 0 && uint64_t(p.ldy) * esize % 32 == 0 ? 2 : (y % 16 == 0 && uint64_t(p.ldy) * esize % 16 == 0 ? 1 : 0);
     t.k_blocks = (p.k + BK - 1) / BK;
+    t.parts = result_parts(p.k, p.c_dtype);
+    if (t.parts > 512 / C::ACC_COLS) t.parts = 512 / C::ACC_COLS;
     t.m_tiles = (p.m + C::ROWS - 1) / C::ROWS;
     t.n_tiles = (p.n + BN - 1) / BN;
     const int64_t tiles = int64_t(t.m_tiles) * t.n_tiles;
@@ -732,10 +780,11 @@ struct Cut {
 };
 constexpr int NUM_CUTS = 4;
 constexpr Cut CUTS[NUM_CUTS] = {{512, 256, 1.0}, {256, 256, 0.92}, {128, 256, 0.86}, {128, 128, 0.7}};
-int choose_cut(int m, int n, int k, int sm_count) {
+int choose_cut(int m, int n, int k, int c_dtype, int sm_count) {
     int best = 0;
     double best_t = 1e300;
     for (int i = 0; i < NUM_CUTS; i++) {
+        if (result_parts(k, c_dtype) * CUTS[i].cols * (CUTS[i].rows == 512 ? 2 : 1) > 512) continue;
         const int pair = CUTS[i].rows >= 256 ? 2 : 1;
         const int64_t tiles = int64_t((m + CUTS[i].rows - 1) / CUTS[i].rows) * ((n + CUTS[i].cols - 1) / CUTS[i].cols);
         const int64_t at_once = sm_count / pair, waves = (tiles + at_once - 1) / at_once;
@@ -758,7 +807,7 @@ uint64_t lora_plan_bytes(int m, int adapters) {
 }
 
 cute_b200_status lora_tiled(const LoraParams &p, bool bf16, int cut, int debug, const DeviceState &dev, cudaStream_t stream) {
-    if (cut < 0) cut = choose_cut(p.m, p.n, p.k, dev.sm_count);
+    if (cut < 0) cut = choose_cut(p.m, p.n, p.k, p.c_dtype, dev.sm_count);
     if (CUTS[cut].rows == 512) CB_TRY(shrink<512>(p, bf16, debug, dev, stream));
     else if (CUTS[cut].rows == 256) CB_TRY(shrink<256>(p, bf16, debug, dev, stream));
     else CB_TRY(shrink<128>(p, bf16, debug, dev, stream));
