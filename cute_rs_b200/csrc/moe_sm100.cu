@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoePar
 // ---- which experts are chosen, and by whom ----------------------------------------
 struct MoeHead {
     uint64_t full[16], empty[16], tfull[2], tempty[2], plan, zeroed, done, drain;
-    uint32_t tmem, abort;
+    uint32_t tmem, abort, stop;
     int32_t active, before[4];
     int32_t expert[MAX_EXPERTS];                     // the chosen experts, ascending
     unsigned long long who[MAX_EXPERTS];             // by expert: which tokens chose it
@@ -365,8 +365,12 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
         int it = 0;
         up_chunks(h, p, [&](int a, int g0, int groups) {
             const int buf = it & 1;
-            const bool ok = wait_bar(bar(h.tfull[buf]), uint32_t(it >> 1) & 1u, abort_flag, p.status, WHERE_EPILOGUE, uint32_t(buf), limit);
-            if (!__all_sync(0xffffffffu, ok)) return false;
+            wait_bar(bar(h.tfull[buf]), uint32_t(it >> 1) & 1u, abort_flag, p.status, WHERE_EPILOGUE, uint32_t(buf), limit);
+            // The four warps go on or stop together: the barriers below count all of them.
+            ptx::named_barrier(1, 128);
+            if (threadIdx.x == 64) h.stop = *abort_flag;
+            ptx::named_barrier(1, 128);
+            if (h.stop) return false;
             ptx::tc_fence_after();
             // The tokens that chose the expert, in order, and their weights.
             const int e = h.expert[a];

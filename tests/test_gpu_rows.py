@@ -547,6 +547,36 @@ def test_moe_on_two_streams_at_once(lib, gpu):
         assert all(torch.equal(w, y) for y in g)
 
 
+# ---- bounded waits -------------------------------------------------------------------
+
+
+def test_waits_that_run_out_are_reported(lib, gpu):
+    """The producers issue nothing (a test knob): every wait gives up after 20 ms, the kernels return, the report names it,
+    and the next call on the same device is right."""
+    few, tiled, moe = Lora(lib, 20, 264, 136, 72, 6, BF16, F32), Lora(lib, 700, 264, 136, 16, 6, BF16, F32), Moe(lib, 12, 24, 4, 256, 136, BF16)
+    calls = [lambda: few.run((1, 12))] + [lambda c=c: tiled.run((c, 12)) for c in (3, 4, 5, 6)] + [lambda: moe.run(tuning=12)]
+    for call in calls:
+        call()
+        with pytest.raises(lib.CuteB200Error) as e:
+            lib.synchronize()
+        assert e.value.status == lib.ERR_DEVICE_TIMEOUT
+        assert lib.device_status() == (0, 0, 0, 0)
+    few.check(few.run())
+    tiled.check(tiled.run())
+    d = tiled.desc((0, 12))
+    da, db, work = torch.empty_like(tiled.a, dtype=F32), torch.empty_like(tiled.b, dtype=F32), tiled.workspace(lib.lora_backward_workspace(d))
+    wt = tiled.w.t().contiguous()
+    lib.lora_tn_backward(d, tiled.x.data_ptr(), wt.data_ptr(), tiled.a.data_ptr(), tiled.b.data_ptr(), tiled.ids.data_ptr(),
+                         tiled.scale.data_ptr(), tiled.dy.data_ptr(), tiled.work.data_ptr(), 0, da.data_ptr(), db.data_ptr(),
+                         work.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    with pytest.raises(lib.CuteB200Error) as e:
+        lib.synchronize()
+    assert e.value.status == lib.ERR_DEVICE_TIMEOUT
+    tiled.check_back(*tiled.back())
+    moe.check(moe.run())
+    assert lib.device_status() == (0, 0, 0, 0)
+
+
 # ---- together ------------------------------------------------------------------------
 
 
