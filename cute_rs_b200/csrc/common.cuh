@@ -36,6 +36,9 @@ struct DeviceState {
     bool ready = false;
     int sm_count = 0;
     uint32_t *status_word = nullptr;  // 4 x u32 in device memory, zero when healthy
+    // Clusters of 1, 2, 4, 8 CTAs of the kernels that stream weights past few rows, and of the one that computes T, that
+    // this device can hold at once.
+    int few_clusters[4] = {}, shrink_clusters[4] = {}, down_clusters[4] = {};
 };
 
 // State of the current device, initialising it on first use.
@@ -77,11 +80,11 @@ cute_b200_status lora_tn_check(const cute_b200_lora_desc &desc, const uint64_t p
 cute_b200_status lora_tn(const cute_b200_lora_desc &desc, const uint64_t ptr[8], cudaStream_t stream, const DeviceState &dev);
 cute_b200_status lora_tn_backward_check(const cute_b200_lora_desc &desc, const uint64_t ptr[12]);
 cute_b200_status lora_tn_backward(const cute_b200_lora_desc &desc, const uint64_t ptr[12], cudaStream_t stream, const DeviceState &dev);
-cute_b200_status lora_init(const DeviceState &dev);
+cute_b200_status lora_init(DeviceState &dev);
 cute_b200_status moe_workspace(const cute_b200_moe_desc &desc, uint64_t *bytes);
 cute_b200_status moe_tn_check(const cute_b200_moe_desc &desc, const uint64_t ptr[7]);
 cute_b200_status moe_tn(const cute_b200_moe_desc &desc, const uint64_t ptr[7], cudaStream_t stream, const DeviceState &dev);
-cute_b200_status moe_init(const DeviceState &dev);
+cute_b200_status moe_init(DeviceState &dev);
 // The launcher for several GPUs (multi_gpu.cu).
 cute_b200_status comm_create(int ngpus, const int *ordinals, void **comm_out);
 cute_b200_status comm_destroy(void *comm);

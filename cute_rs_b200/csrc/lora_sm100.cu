@@ -10,55 +10,84 @@ namespace cb {
 namespace {
 
 // ---- few rows (m <= 128) ------------------------------------------------------
-// T: a CTA takes one row and four of its adapter's `rank` rows; its 256 threads
-// walk k in 16-byte pieces.  It is over before the weights have streamed past
-// (below), so it is kept simple.
-constexpr int SHRINK_THREADS = 256, SHRINK_J = 4;
+// T: a CTA takes J of an adapter's `rank` rows and up to four rows of X that name it; its 256 threads walk k in 16-byte pieces.
+// Of the rows that share an adapter every fourth brings its CTA to work, on itself and the next three; the others return.
+// Both operands come from L2 but for the first time (100 rows of 4 adapters, rank 128, k = 8192: 90 MB; a CTA per row and
+// four ranks read 256 MB).  It is over before the weights have streamed past (below).
+constexpr int FEW_ROWS = 128, SHRINK_THREADS = 256, SHRINK_ROWS = 4;
 
-template <bool BF16>
+template <bool BF16, int J>
 __global__ void __launch_bounds__(SHRINK_THREADS) shrink_rows_kernel(const LoraParams p) {
-    __shared__ float part[SHRINK_THREADS / 32][SHRINK_J];
+    __shared__ float part[SHRINK_THREADS / 32][SHRINK_ROWS * J];
+    __shared__ int rows[SHRINK_ROWS], counts[4], before;
     ptx::griddep_wait();
     ptx::griddep_launch_dependents();
-    const int row = blockIdx.x, j0 = blockIdx.y * SHRINK_J, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int id = p.ids[row];
-    const bool has = id >= 0 && id < p.adapters && j0 < p.rank;
-    float acc[SHRINK_J] = {};
-    if (has) {
-        const uint16_t *x = p.x + row * p.ldx;
-        const uint16_t *a = p.a + (int64_t(id) * p.rank + j0) * p.k;
-        const int vecs = p.k / 8;
-#pragma unroll 2
-        for (int c = threadIdx.x; c < vecs; c += SHRINK_THREADS) {
-            const uint4 xv = *reinterpret_cast<const uint4 *>(x + 8 * c);
-            uint4 av[SHRINK_J];
+    const int j0 = blockIdx.y * J, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int id = p.ids[blockIdx.x];
+    if (id < 0 || id >= p.adapters) return;
+    // Place of every row among those that share this adapter; `first` is this CTA's.
+    const bool same = tid < p.m && p.ids[tid] == id;
+    const uint32_t votes = __ballot_sync(0xffffffffu, same);
+    if (warp < 4 && lane == 0) counts[warp] = __popc(votes);
+    if (tid < SHRINK_ROWS) rows[tid] = blockIdx.x;  // a batch of fewer rows takes this one once more
+    __syncthreads();
+    int at = __popc(votes & ((1u << lane) - 1u)), count = 0;
+    for (int i = 0; i < 4; i++) {
+        if (i < warp) at += counts[i];
+        count += counts[i];
+    }
+    if (tid == int(blockIdx.x)) before = at;
+    __syncthreads();
+    const int first = before;
+    if (first % SHRINK_ROWS) return;
+    if (same && at >= first && at < first + SHRINK_ROWS) rows[at - first] = tid;
+    __syncthreads();
+    const bool live = j0 < p.rank;  // else the padding of the rank: zeros
+    const float scale = p.scale[id];
+    const uint16_t *a = p.a + (int64_t(id) * p.rank + j0) * p.k;
+    const int vecs = live ? p.k / 8 : 0, batch = min(SHRINK_ROWS, count - first);
+    const uint16_t *x[SHRINK_ROWS];
 #pragma unroll
-            for (int j = 0; j < SHRINK_J; j++) av[j] = __ldg(reinterpret_cast<const uint4 *>(a + int64_t(j) * p.k + 8 * c));
-            const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+    for (int r = 0; r < SHRINK_ROWS; r++) x[r] = p.x + rows[r] * p.ldx;
+    float acc[SHRINK_ROWS][J] = {};
+#pragma unroll 1
+    for (int c = tid; c < vecs; c += SHRINK_THREADS) {
+        uint4 av[J], xv[SHRINK_ROWS];
+#pragma unroll
+        for (int j = 0; j < J; j++) av[j] = __ldg(reinterpret_cast<const uint4 *>(a + int64_t(j) * p.k + 8 * c));
+#pragma unroll
+        for (int r = 0; r < SHRINK_ROWS; r++)
+            if (r == 0 || batch > 1) xv[r] = *reinterpret_cast<const uint4 *>(x[r] + 8 * c);
+#pragma unroll
+        for (int r = 0; r < SHRINK_ROWS; r++) {
+            if (r > 0 && batch == 1) break;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float2 xf = pair_f32<BF16>(xw[i]);
+                const float2 xf = pair_f32<BF16>(i == 0 ? xv[r].x : (i == 1 ? xv[r].y : (i == 2 ? xv[r].z : xv[r].w)));
 #pragma unroll
-                for (int j = 0; j < SHRINK_J; j++) {
-                    const uint32_t w = i == 0 ? av[j].x : (i == 1 ? av[j].y : (i == 2 ? av[j].z : av[j].w));
-                    const float2 af = pair_f32<BF16>(w);
-                    acc[j] = fmaf(af.y, xf.y, fmaf(af.x, xf.x, acc[j]));
+                for (int j = 0; j < J; j++) {
+                    const float2 af = pair_f32<BF16>(i == 0 ? av[j].x : (i == 1 ? av[j].y : (i == 2 ? av[j].z : av[j].w)));
+                    acc[r][j] = fmaf(af.y, xf.y, fmaf(af.x, xf.x, acc[r][j]));
                 }
             }
         }
     }
 #pragma unroll
-    for (int j = 0; j < SHRINK_J; j++) {
-        acc[j] = warp_sum(acc[j]);
-        if (lane == 0) part[warp][j] = acc[j];
+    for (int r = 0; r < SHRINK_ROWS; r++) {
+        if (r > 0 && batch == 1) break;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const float sum = warp_sum(acc[r][j]);
+            if (lane == 0) part[warp][r * J + j] = sum;
+        }
     }
     __syncthreads();
-    if (threadIdx.x < SHRINK_J) {
+    if (tid < batch * J) {
         float sum = 0.0f;
-        for (int w = 0; w < SHRINK_THREADS / 32; w++) sum += part[w][threadIdx.x];
-        if (has) sum *= p.scale[id];
+        for (int w = 0; w < SHRINK_THREADS / 32; w++) sum += part[w][tid];
+        sum = live ? sum * scale : 0.0f;
         const uint16_t hi = from_f32<BF16>(sum);
-        uint16_t *t = p.t + int64_t(row) * 2 * p.rp + j0 + threadIdx.x;
+        uint16_t *t = p.t + int64_t(rows[tid / J]) * 2 * p.rp + j0 + tid % J;
         t[0] = hi;
         t[p.rp] = from_f32<BF16>(sum - to_f32<BF16>(hi));
     }
@@ -84,7 +113,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS) shrink_rows_kernel(const LoraP
 //           and the stores.
 // W and X do not depend on the kernel that computes T, which has waited for all
 // before it: they are loaded before griddepcontrol.wait, T and the ids after.
-constexpr int FEW_THREADS = 192, FEW_MAX_STAGES = 16, FEW_ROWS = 128;
+constexpr int FEW_THREADS = 192, FEW_MAX_STAGES = 16;
 constexpr uint32_t FEW_HEAD = 8192;  // barriers, masks and ids, ahead of the ring
 
 struct FewParams {
@@ -161,7 +190,7 @@ __device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, 
     for (int i = thread; i < rows * p.rp; i += 128) {
         const int r = i / p.rp, j = i - r * p.rp;
         const uint16_t *src = p.t + int64_t(rank + r * p.kc) * 2 * p.rp + j;
-        t[i] = to_f32<BF16>(src[0]) + to_f32<BF16>(src[p.rp]);
+        t[i] = id[rank + r * p.kc] >= 0 ? to_f32<BF16>(src[0]) + to_f32<BF16>(src[p.rp]) : 0.0f;
     }
     ptx::named_barrier(1, 128);
     if (p.rank == 8) few_dots<BF16, 1, 8>(p, id, t, out, rank, rows, n0, thread);
@@ -408,26 +437,37 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     if (!*abort_flag) {
         const int quads = p.bn / 4, items = p.m * quads;
         const uint32_t pitch = uint32_t(p.bn + 4) * 4u;
-        for (int i = int(rank) * FEW_THREADS + int(threadIdx.x); i < items; i += p.kc * FEW_THREADS) {
-            const int row = i / quads, col = (i - row * quads) * 4;
-            const uint32_t at = ring + uint32_t(row) * pitch + uint32_t(col) * 4u;
-            float4 v = cluster_sum(at, p.kc);
-            if (b_blocks == 0) {  // the dot products of this row were taken by CTA row % kc
-                const uint32_t dots = low + uint32_t((p.m + p.kc - 1) / p.kc * p.rp + row / p.kc * p.bn + col) * 4u;
-                const float4 o = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(dots, uint32_t(row % p.kc)) : dots);
-                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-            }
-            const int64_t gcol = n0 + col, out = int64_t(row) * p.ldy + gcol;
-            if (p.vec && gcol + 4 <= p.n) {
-                if (p.c_dtype == CUTE_B200_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.y) + out) = v;
-                else {
-                    const bool bf16 = p.c_dtype == CUTE_B200_BF16;
-                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + out) = make_uint2(pack_16(v.x, v.y, bf16), pack_16(v.z, v.w, bf16));
+        // Two places per turn: their loads from the cluster's shared memories are on their way together.
+        const int stride = p.kc * FEW_THREADS;
+        for (int i0 = int(rank) * FEW_THREADS + int(threadIdx.x); i0 < items; i0 += 2 * stride) {
+            float4 v[2], dot[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int i = min(i0 + u * stride, items - 1), row = i / quads, col = (i - row * quads) * 4;
+                v[u] = cluster_sum(ring + uint32_t(row) * pitch + uint32_t(col) * 4u, p.kc);
+                if (b_blocks == 0) {  // the dot products of this row were taken by CTA row % kc
+                    const uint32_t dots = low + uint32_t((p.m + p.kc - 1) / p.kc * p.rp + row / p.kc * p.bn + col) * 4u;
+                    dot[u] = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(dots, uint32_t(row % p.kc)) : dots);
                 }
-            } else {
-                const float f[4] = {v.x, v.y, v.z, v.w};
-                for (int j = 0; j < 4; j++)
-                    if (gcol + j < p.n) store_c(p.y, p.c_dtype, size_t(out + j), f[j]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int i = i0 + u * stride, row = i / quads, col = (i - row * quads) * 4;
+                if (i >= items) break;
+                if (b_blocks == 0) v[u].x += dot[u].x, v[u].y += dot[u].y, v[u].z += dot[u].z, v[u].w += dot[u].w;
+                const int64_t gcol = n0 + col, out = int64_t(row) * p.ldy + gcol;
+                if (p.vec && gcol + 4 <= p.n) {
+                    if (p.c_dtype == CUTE_B200_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.y) + out) = v[u];
+                    else {
+                        const bool bf16 = p.c_dtype == CUTE_B200_BF16;
+                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + out) =
+                            make_uint2(pack_16(v[u].x, v[u].y, bf16), pack_16(v[u].z, v[u].w, bf16));
+                    }
+                } else {
+                    const float f[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+                    for (int j = 0; j < 4; j++)
+                        if (gcol + j < p.n) store_c(p.y, p.c_dtype, size_t(out + j), f[j]);
+                }
             }
         }
     }
@@ -443,11 +483,10 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 // they are gone.
 constexpr uint32_t FEW_SMEM = 216 * 1024;
 
-int g_few_clusters[64][4];  // clusters of 1, 2, 4, 8 CTAs of the few-row kernel that fit each device at once
-
 template <bool BF16>
 cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int debug, cudaStream_t stream) {
-    CB_TRY(launch_dependent(shrink_rows_kernel<BF16>, dim3(unsigned(p.m), unsigned(p.rp / SHRINK_J)), SHRINK_THREADS, 0, 1, stream, p));
+    if (p.rank >= 64) CB_TRY(launch_dependent(shrink_rows_kernel<BF16, 8>, dim3(unsigned(p.m), unsigned(p.rp / 8)), SHRINK_THREADS, 0, 1, stream, p));
+    else CB_TRY(launch_dependent(shrink_rows_kernel<BF16, 4>, dim3(unsigned(p.m), unsigned(p.rp / 4)), SHRINK_THREADS, 0, 1, stream, p));
     if (!p.y) return CUTE_B200_OK;
     FewParams f = {};
     f.ids = p.ids, f.y = p.y, f.ldy = p.ldy;
@@ -456,9 +495,7 @@ cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int de
     f.vec = reinterpret_cast<uint64_t>(p.y) % (4 * esize) == 0 && p.ldy % 4 == 0;
     f.k_blocks = (p.k + 63) / 64;
     f.bn = 16, f.kc = 1;
-    int device = 0;
-    CB_CUDA(cudaGetDevice(&device));
-    stream_cut(p.n, (p.k + 63) / 64, g_few_clusters[device], &f.bn, &f.kc);
+    stream_cut(p.n, (p.k + 63) / 64, dev.few_clusters, &f.bn, &f.kc);
     f.xr = (p.m + 7) / 8 * 8;
     f.x_bytes = uint32_t(f.xr) * 128u;
     f.w_bytes = uint32_t(f.bn) * 128u;
@@ -480,11 +517,13 @@ cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int de
     for (f.tmem_cols = 32; f.tmem_cols < uint32_t(f.parts * ((f.bn + 31) / 32 * 32)); f.tmem_cols *= 2) {}
     f.status = dev.status_word;
     f.debug = debug;
-    CUtensorMap tmX, tmW, tmT, tmB;
+    CUtensorMap tmX, tmW, tmT = {}, tmB = {};
     CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), BF16, p.m, p.k, p.ldx, f.xr));
     CB_TRY(rows_tensor_map(&tmW, reinterpret_cast<uint64_t>(p.w), BF16, p.n, p.k, p.k, f.bn));
-    CB_TRY(rows_tensor_map(&tmT, reinterpret_cast<uint64_t>(p.t), BF16, p.m, 2 * p.rp, 2 * p.rp, f.xr));
-    CB_TRY(rows_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), BF16, uint64_t(p.adapters) * p.n, p.rank, p.rank, f.bn));
+    if (f.b_blocks > 0) {
+        CB_TRY(rows_tensor_map(&tmT, reinterpret_cast<uint64_t>(p.t), BF16, p.m, 2 * p.rp, 2 * p.rp, f.xr));
+        CB_TRY(rows_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), BF16, uint64_t(p.adapters) * p.n, p.rank, p.rank, f.bn));
+    }
     const unsigned grid = unsigned((p.n + f.bn - 1) / f.bn) * unsigned(f.kc);
     return launch_dependent(lora_few_kernel, dim3(grid), FEW_THREADS, FEW_SMEM, f.kc, stream, tmX, tmW, tmT, tmB, f);
 }
@@ -654,12 +693,10 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
     return CUTE_B200_OK;
 }
 
-cute_b200_status lora_init(const DeviceState &) {
-    int device = 0;
-    CB_CUDA(cudaGetDevice(&device));
+cute_b200_status lora_init(DeviceState &dev) {
     CB_CUDA(cudaFuncSetAttribute(lora_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
-    for (int c = 0; c < 4; c++) CB_TRY(max_clusters(lora_few_kernel, FEW_THREADS, FEW_SMEM, 1 << c, &g_few_clusters[device][c]));
-    CB_TRY(lora_tiled_init());
+    for (int c = 0; c < 4; c++) CB_TRY(max_clusters(lora_few_kernel, FEW_THREADS, FEW_SMEM, 1 << c, &dev.few_clusters[c]));
+    CB_TRY(lora_tiled_init(dev));
     CB_TRY(lora_grad_init());
     return CUTE_B200_OK;
 }

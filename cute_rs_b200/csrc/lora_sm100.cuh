@@ -22,7 +22,7 @@ struct LoraParams {
 // The tiled forward product (any m; cut 0..3 names a tile, a negative one chooses) and the bytes of its plan.
 cute_b200_status lora_tiled(const LoraParams &p, bool bf16, int cut, int debug, const DeviceState &dev, cudaStream_t stream);
 uint64_t lora_plan_bytes(int m, int adapters);
-cute_b200_status lora_tiled_init();
+cute_b200_status lora_tiled_init(DeviceState &dev);
 
 // The adapters' gradients: [0] dA from X and U, [1] dB from dY and T.  `first` (adapters + 1) and `list` (m) are the row lists.
 struct LoraGrads {
@@ -50,7 +50,8 @@ __host__ __device__ constexpr int padded_rank(int rank) { return rank <= 16 ? 16
 // First occurrences of ids by a hash table in shared memory.
 template <int ROWS>
 struct IdTable {
-    static constexpr int SIZE = 2 * ROWS;  // a power of two: at most half full, so a probe ends
+    static constexpr int SIZE = 2 * ROWS;  // 256, 512 or 1024: at most half full, so a probe ends
+    static_assert(ROWS == 128 || ROWS == 256 || ROWS == 512, "the hash keeps log2(SIZE) bits");
     int32_t key[SIZE], first[SIZE], entry[SIZE], before[4];
 };
 
@@ -66,7 +67,7 @@ __device__ __forceinline__ int distinct_ids(const int32_t (&id)[ROWS / 128], IdT
     uint32_t slot[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        slot[i] = (uint32_t(id[i]) * 2654435761u) & uint32_t(h.SIZE - 1);
+        slot[i] = (uint32_t(id[i]) * 2654435761u) >> (ROWS == 128 ? 24 : (ROWS == 256 ? 23 : 22));  // SIZE slots
         if (id[i] >= 0) {
             for (;;) {
                 const int old = atomicCAS(&h.key[slot[i]], -1, id[i]);

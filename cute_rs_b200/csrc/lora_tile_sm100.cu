@@ -704,8 +704,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 }
 
 // ---- host -------------------------------------------------------------------------
-int g_shrink_clusters[64][4];  // clusters of 1, 2, 4, 8 CTAs of the T kernel that fit each device at once
-
 template <int P>
 cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream) {
     ShrinkParams s = {};
@@ -722,11 +720,9 @@ cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceS
     s.debug = debug;
     const int tiles = (p.m + BM - 1) / BM;
     // k is cut while that puts more CTAs to work and leaves each at least two blocks.
-    int device = 0;
-    CB_CUDA(cudaGetDevice(&device));
     s.kc = 1;
     for (int c = 1; c < 4; c++)
-        if (tiles <= g_shrink_clusters[device][c] && s.k_blocks >= (2 << c)) s.kc = 1 << c;
+        if (tiles <= dev.shrink_clusters[c] && s.k_blocks >= (2 << c)) s.kc = 1 << c;
     CUtensorMap tmX, tmA;
     CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), bf16, p.m, p.k, p.ldx, BM));
     if (p.low_mn) CB_TRY(stack_tensor_map(&tmA, reinterpret_cast<uint64_t>(p.a), bf16, p.adapters, p.k, p.rank, BK));
@@ -751,7 +747,7 @@ cute_b200_status launch_tile(const LoraParams &p, bool bf16, int debug, const De
     t.m_tiles = (p.m + C::ROWS - 1) / C::ROWS;
     t.n_tiles = (p.n + BN - 1) / BN;
     const int64_t tiles = int64_t(t.m_tiles) * t.n_tiles;
-    if (tiles > 0x7fffffff) return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "lora_tn: %d x %d is more than 2^31 tiles", p.m, p.n);
+    if (tiles > (1 << 30)) return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "lora_tn: %d x %d is more than 2^30 tiles", p.m, p.n);
     int clusters = dev.sm_count / G;
     if (tiles < clusters) clusters = int(tiles);
     int gm = 1;
@@ -818,9 +814,7 @@ cute_b200_status lora_tiled(const LoraParams &p, bool bf16, int cut, int debug, 
     return launch_tile<1, 128, 1>(p, bf16, debug, dev, stream);
 }
 
-cute_b200_status lora_tiled_init() {
-    int device = 0;
-    CB_CUDA(cudaGetDevice(&device));
+cute_b200_status lora_tiled_init(DeviceState &dev) {
     CB_CUDA(cudaFuncSetAttribute(shrink_tile_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHRINK_SMEM));
     CB_CUDA(cudaFuncSetAttribute(shrink_tile_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHRINK_SMEM));
     CB_CUDA(cudaFuncSetAttribute(shrink_tile_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHRINK_SMEM));
@@ -829,7 +823,7 @@ cute_b200_status lora_tiled_init() {
     CB_CUDA(cudaFuncSetAttribute(lora_tile_kernel<1, 256, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<1, 256, 1>::SMEM_BYTES));
     CB_CUDA(cudaFuncSetAttribute(lora_tile_kernel<1, 128, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<1, 128, 1>::SMEM_BYTES));
     for (int c = 0; c < 4; c++)
-        CB_TRY(max_clusters(shrink_tile_kernel<128>, SHRINK_THREADS, SHRINK_SMEM, 1 << c, &g_shrink_clusters[device][c]));
+        CB_TRY(max_clusters(shrink_tile_kernel<128>, SHRINK_THREADS, SHRINK_SMEM, 1 << c, &dev.shrink_clusters[c]));
     return CUTE_B200_OK;
 }
 

@@ -635,8 +635,6 @@ __global__ void __launch_bounds__(MOE_THREADS, 1)
     if (warp == 1) ptx::tmem_dealloc<1>(tmem, p.tmem_cols);
 }
 
-int g_down_clusters[64][4];
-
 constexpr uint64_t kAlign = 256;
 uint64_t round_up(uint64_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
 
@@ -703,8 +701,6 @@ cute_b200_status moe_tn_check(const cute_b200_moe_desc &d, const uint64_t ptr[7]
 cute_b200_status moe_tn(const cute_b200_moe_desc &d, const uint64_t ptr[7], cudaStream_t stream, const DeviceState &dev) {
     if (d.tokens == 0) return CUTE_B200_OK;
     const Layout l = layout(d);
-    int device = 0;
-    CB_CUDA(cudaGetDevice(&device));
     MoeParams p = {};
     p.x = reinterpret_cast<const uint16_t *>(ptr[0]);
     p.r = reinterpret_cast<const uint16_t *>(ptr[1]);
@@ -734,7 +730,7 @@ cute_b200_status moe_tn(const cute_b200_moe_desc &d, const uint64_t ptr[7], cuda
     p.bn = 16, p.kc = 1;
     const int f_blocks = (d.f + 63) / 64, expected = most_active(d);
     int fits[4];
-    for (int c = 0; c < 4; c++) fits[c] = (1 << c) <= f_blocks ? g_down_clusters[device][c] : 0;  // every CTA has a block of one expert at least
+    for (int c = 0; c < 4; c++) fits[c] = (1 << c) <= f_blocks ? dev.down_clusters[c] : 0;  // every CTA has a block of one expert at least
     stream_cut(d.d, f_blocks * expected, fits, &p.bn, &p.kc);
     p.kps = stream_blocks(p.bn, p.token_rows, MOE_SMEM - MOE_HEAD - 1024);
     p.stage_bytes = uint32_t(p.kps * (p.token_rows + p.bn)) * 128u;
@@ -745,12 +741,10 @@ cute_b200_status moe_tn(const cute_b200_moe_desc &d, const uint64_t ptr[7], cuda
     return launch_dependent(moe_down_kernel, dim3(unsigned((d.d + p.bn - 1) / p.bn * p.kc)), MOE_THREADS, MOE_SMEM, p.kc, stream, tmH, tmD, p);
 }
 
-cute_b200_status moe_init(const DeviceState &) {
-    int device = 0;
-    CB_CUDA(cudaGetDevice(&device));
+cute_b200_status moe_init(DeviceState &dev) {
     CB_CUDA(cudaFuncSetAttribute(moe_up_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOE_SMEM));
     CB_CUDA(cudaFuncSetAttribute(moe_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOE_SMEM));
-    for (int c = 0; c < 4; c++) CB_TRY(max_clusters(moe_down_kernel, MOE_THREADS, MOE_SMEM, 1 << c, &g_down_clusters[device][c]));
+    for (int c = 0; c < 4; c++) CB_TRY(max_clusters(moe_down_kernel, MOE_THREADS, MOE_SMEM, 1 << c, &dev.down_clusters[c]));
     return CUTE_B200_OK;
 }
 

@@ -196,8 +196,8 @@ cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint6
  *   adapters * n, adapters * k and adapters * rank below 2^31.
  *   Before it is multiplied by B, scale[a] * A[a] x is rounded to the operands'
  *   type for a 16-bit Y, and to the sum of two such numbers (16 significant bits
- *   for bf16, 22 for f16) for an f32 Y and for the gradients; an f16 value past
- *   +-65504 becomes infinite.
+ *   for bf16, 22 for f16) for an f32 Y and for the gradients; where an f16 value
+ *   passes +-65504 its row of Y is not finite.
  *   The workspace begins with these numbers, which the backward pass reads.
  *
  * cute_b200_lora_tn_backward: the gradients for dY (m, n) in the operands' type
