@@ -221,7 +221,7 @@ def shard_rows(m: int, world: int, rank: int) -> tuple[int, int]:
 
 
 def lora_desc(m, n, k, rank, adapters, ab_dtype, c_dtype, ldx=0, ldy=0) -> LoraDesc:
-    return LoraDesc(m, n, k, rank, adapters, ab_dtype, c_dtype, ldx, ldy, (ctypes.c_int32 * 2)(0, 0))
+    return LoraDesc(m, n, k, rank, adapters, ab_dtype, c_dtype, ldx, ldy)
 
 
 def lora_workspace(desc: LoraDesc) -> int:
@@ -252,7 +252,7 @@ def lora_tn_backward(desc: LoraDesc, dX: int, dWt: int, dA: int, dB: int, dIds: 
 
 
 def moe_desc(tokens, experts, top, d, f, dtype, renormalise=True) -> MoeDesc:
-    return MoeDesc(tokens, experts, top, d, f, dtype, int(renormalise), (ctypes.c_int32 * 2)(0, 0))
+    return MoeDesc(tokens, experts, top, d, f, dtype, int(renormalise))
 
 
 def moe_workspace(desc: MoeDesc) -> int:

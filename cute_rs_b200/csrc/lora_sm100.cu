@@ -56,8 +56,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS) shrink_rows_kernel(const LoraP
 #pragma unroll
         for (int j = 0; j < J; j++) av[j] = __ldg(reinterpret_cast<const uint4 *>(a + int64_t(j) * p.k + 8 * c));
 #pragma unroll
-        for (int r = 0; r < SHRINK_ROWS; r++)
-            if (r == 0 || batch > 1) xv[r] = *reinterpret_cast<const uint4 *>(x[r] + 8 * c);
+        for (int r = 0; r < SHRINK_ROWS; r++) xv[r] = *reinterpret_cast<const uint4 *>(x[r] + 8 * c);  // no branch between the loads
 #pragma unroll
         for (int r = 0; r < SHRINK_ROWS; r++) {
             if (r > 0 && batch == 1) break;
