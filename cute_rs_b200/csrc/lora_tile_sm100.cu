@@ -21,8 +21,9 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 // the lanes of its rows, so one accumulator serves all of them.  Bound by reading X
 // (and, where nearly every row has an adapter of its own, A).
 //   warp 0  TMA: two (128 x 64) blocks of X per stage of one ring, then the blocks of A
-//           of the tile's adapters for them through another, 32 KB per stage, a lane each
-//           (with 16 KB per stage of either the issuing warp was the bound: 0.3 us a stage).
+//           of the tile's adapters for them through another, a lane each (with one block
+//           per stage the issuing warp was the bound: 0.3 us a stage).  Both rings are three
+//           or four stages deep, as the rank allows: the shorter one is what keeps X coming.
 //   warp 1  MMA.   warps 2-5  the adapters the rows name (and, by the cluster's first CTA,
 //           the plan of the GEMM's tile that starts at its rows), then the sum over the
 //           cluster, scale, split into two 16-bit numbers.
@@ -30,10 +31,10 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 // A CTA's k range goes to T_PARTS accumulators in turn, added in f32 at the end: the tensor core cuts its sums off instead of
 // rounding them, an error of the same sign that grows with the products added into one accumulator (256 MMAs of 16: 5e-6
 // of the sum, measured), and T enters f32 gradients.
-constexpr int SHRINK_THREADS = 192, X_STAGES = 4, A_STAGES = 2, X_BLOCKS = 2;
-constexpr uint32_t X_BYTES = BM * BK * 2, A_BYTES = 32 * 1024, SHRINK_HEAD = 20 * 1024;
+constexpr int SHRINK_THREADS = 192, MAX_X_STAGES = 4, MAX_A_STAGES = 4, X_BLOCKS = 2;
+constexpr uint32_t X_BYTES = BM * BK * 2, SHRINK_HEAD = 20 * 1024, SHRINK_RINGS = 192 * 1024;
 constexpr int T_PARTS = 4;
-constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + X_STAGES * X_BLOCKS * X_BYTES + A_STAGES * A_BYTES;
+constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + SHRINK_RINGS;
 
 struct ShrinkParams {
     const int32_t *ids;
@@ -42,7 +43,8 @@ struct ShrinkParams {
     uint32_t *plan;
     int m, rank, rp, adapters, k_blocks, kc;
     int boxes;       // of A per adapter and k block
-    uint32_t box_bytes;
+    uint32_t box_bytes, a_bytes;  // a_bytes: of a stage of A
+    int x_stages, a_stages;
     uint32_t idesc, part_cols;  // TMEM columns of one accumulator
     bool bf16, mn, early;
     uint32_t *status;
@@ -54,7 +56,7 @@ __device__ __forceinline__ bool part_used(int part, int blocks) { return (part *
 
 template <int P>
 struct ShrinkHead {
-    uint64_t xfull[X_STAGES], xempty[X_STAGES], afull[A_STAGES], aempty[A_STAGES], plan, done, drain;
+    uint64_t xfull[MAX_X_STAGES], xempty[MAX_X_STAGES], afull[MAX_A_STAGES], aempty[MAX_A_STAGES], plan, done, drain;
     uint32_t tmem, abort;
     int32_t entries, entry_id[BM], id[BM];
     float scale[BM];
@@ -70,7 +72,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     ShrinkHead<P> &h = *reinterpret_cast<ShrinkHead<P> *>(smem_raw + (base - raw));
-    const uint32_t xring = base + SHRINK_HEAD, aring = xring + X_STAGES * X_BLOCKS * X_BYTES;
+    const uint32_t xring = base + SHRINK_HEAD, aring = xring + uint32_t(p.x_stages * X_BLOCKS) * X_BYTES;
     auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
     volatile uint32_t *abort_flag = &h.abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -78,15 +80,15 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
     const int row0 = int(blockIdx.x) / p.kc * BM;
     const int kb0 = int(int64_t(p.k_blocks) * rank / p.kc), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / p.kc);
     const uint32_t entry_bytes = uint32_t(p.boxes) * p.box_bytes;
-    const int group = min(int(A_BYTES / entry_bytes), 32 / p.boxes);  // (k block, adapter) pairs per stage of A: 2 to 16
+    const int group = min(int(p.a_bytes / entry_bytes), 32 / p.boxes);  // (k block, adapter) pairs per stage of A: 2 to 16
     const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < X_STAGES; s++) {
+        for (int s = 0; s < p.x_stages; s++) {
             ptx::mbar_init(bar(h.xfull[s]), 1);
             ptx::mbar_init(bar(h.xempty[s]), 1);
         }
-        for (int s = 0; s < A_STAGES; s++) {
+        for (int s = 0; s < p.a_stages; s++) {
             ptx::mbar_init(bar(h.afull[s]), 1);
             ptx::mbar_init(bar(h.aempty[s]), 1);
         }
@@ -127,7 +129,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             if (lane < nk) ptx::tma_load_2d(xring + uint32_t(sx * X_BLOCKS + lane) * X_BYTES, &tmX, bar(h.xfull[sx]), (kb + lane) * BK, row0);
             __syncwarp();
             xfilled |= 1u << sx, xparity = (xparity & ~(1u << sx)) | (px << sx);
-            if (++sx == X_STAGES) sx = 0, px ^= 1u;
+            if (++sx == p.x_stages) sx = 0, px ^= 1u;
             for (int i0 = 0; i0 < items; i0 += group) {
                 ok = __all_sync(0xffffffffu, wait_bar(bar(h.aempty[sa]), pa ^ 1u, abort_flag, p.status, WHERE_PRODUCER, 32u + uint32_t(sa), limit));
                 if (!ok) break;
@@ -136,21 +138,21 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
                 __syncwarp();
                 if (my_item < count) {
                     const int second = i0 + my_item >= entries ? 1 : 0, id = h.entry_id[i0 + my_item - second * entries];
-                    const uint32_t dst = aring + uint32_t(sa) * A_BYTES + uint32_t(lane) * p.box_bytes;
+                    const uint32_t dst = aring + uint32_t(sa) * p.a_bytes + uint32_t(lane) * p.box_bytes;
                     if (p.mn) ptx::tma_load_3d(dst, &tmA, bar(h.afull[sa]), 64 * my_box, (kb + second) * BK, id);
                     else ptx::tma_load_2d(dst, &tmA, bar(h.afull[sa]), (kb + second) * BK, id * p.rank);
                 }
                 __syncwarp();
                 afilled |= 1u << sa, aparity = (aparity & ~(1u << sa)) | (pa << sa);
-                if (++sa == A_STAGES) sa = 0, pa ^= 1u;
+                if (++sa == p.a_stages) sa = 0, pa ^= 1u;
             }
         }
         if (!ok && lane == 0) {  // giving up: let the copies in flight land (bounded)
             const uint64_t t0 = ptx::globaltimer_ns();
-            for (int i = 0; i < X_STAGES; i++)
+            for (int i = 0; i < p.x_stages; i++)
                 while ((xfilled >> i & 1u) && !ptx::mbar_try_wait(bar(h.xfull[i]), (xparity >> i) & 1u))
                     if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
-            for (int i = 0; i < A_STAGES; i++)
+            for (int i = 0; i < p.a_stages; i++)
                 while ((afilled >> i & 1u) && !ptx::mbar_try_wait(bar(h.afull[i]), (aparity >> i) & 1u))
                     if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
         }
@@ -160,14 +162,13 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         const bool leader = ptx::elect_one();
         bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit)), issued = false;
         const int entries = ok ? h.entries : 0;
+        // The blocks at which the second to fourth accumulator begin (part_used tells which of them get any).
+        static_assert(T_PARTS == 4, "three beginnings");
+        const int blocks = kb1 - kb0, begin1 = (blocks + 3) / 4, begin2 = (2 * blocks + 3) / 4, begin3 = (3 * blocks + 3) / 4;
         int sx = 0, sa = 0;
         uint32_t px = 0, pa = 0;
         for (int kb = kb0; kb < kb1 && ok && entries > 0; kb += X_BLOCKS) {
             const int items = min(X_BLOCKS, kb1 - kb) * entries;
-            // The accumulators of the block before these two and of the two.
-            int part[3];
-#pragma unroll
-            for (int i = 0; i < 3; i++) part[i] = kb + i > kb0 ? (kb + i - 1 - kb0) * T_PARTS / (kb1 - kb0) : -1;
             ok = __all_sync(0xffffffffu, wait_bar(bar(h.xfull[sx]), px, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(sx), limit));
             if (!ok) break;
             for (int i0 = 0; i0 < items; i0 += group) {
@@ -177,11 +178,13 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
                 const int count = min(group, items - i0);
                 for (int i = 0; i < count; i++) {
                     const int second = i0 + i >= entries ? 1 : 0, e = i0 + i - second * entries;
-                    const uint32_t src = aring + uint32_t(sa) * A_BYTES + uint32_t(i) * entry_bytes;
+                    const uint32_t src = aring + uint32_t(sa) * p.a_bytes + uint32_t(i) * entry_bytes;
                     const uint64_t a = sw128_desc(xring + uint32_t(sx * X_BLOCKS + second) * X_BYTES);
                     const uint64_t b = p.mn ? mn_desc(src, p.box_bytes) : sw128_desc(src);
-                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u, d = tmem + uint32_t(part[1 + second]) * p.part_cols;
-                    const uint32_t more = part[second] == part[1 + second] ? 1u : 0u;
+                    const int at = kb + second - kb0;
+                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u;
+                    const uint32_t d = tmem + (uint32_t(at >= begin1) + uint32_t(at >= begin2) + uint32_t(at >= begin3)) * p.part_cols;
+                    const uint32_t more = at != 0 && at != begin1 && at != begin2 && at != begin3 ? 1u : 0u;
                     const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
                     if (leader) {
 #pragma unroll
@@ -193,12 +196,12 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
                 issued = true;
                 if (leader) ptx::umma_commit<1>(bar(h.aempty[sa]));
                 __syncwarp();
-                if (++sa == A_STAGES) sa = 0, pa ^= 1u;
+                if (++sa == p.a_stages) sa = 0, pa ^= 1u;
             }
             if (!ok) break;
             if (leader) ptx::umma_commit<1>(bar(h.xempty[sx]));
             __syncwarp();
-            if (++sx == X_STAGES) sx = 0, px ^= 1u;
+            if (++sx == p.x_stages) sx = 0, px ^= 1u;
         }
         if (leader) {
             if (ok) {
@@ -255,15 +258,18 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             for (int c = 0; c < p.rp; c += 32) {
                 uint32_t v[32];
                 const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(c);
+                uint32_t o[T_PARTS - 1][32];
                 ptx::tmem_ld_32x32(from, v);
-                ptx::tmem_ld_wait(v);
-                for (int i = 1; i < T_PARTS; i++) {
-                    if (parts < T_PARTS && !part_used(i, kb1 - kb0)) continue;
-                    uint32_t o[32];
-                    ptx::tmem_ld_32x32(from + uint32_t(i) * p.part_cols, o);
-                    ptx::tmem_ld_wait(o);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(o[j]));
+                for (int i = 1; i < T_PARTS; i++) ptx::tmem_ld_32x32(from + uint32_t(i) * p.part_cols, o[i - 1]);
+                ptx::tmem_ld_wait_all();
+                ptx::pin(v);
+#pragma unroll
+                for (int i = 1; i < T_PARTS; i++) {
+                    ptx::pin(o[i - 1]);
+                    if (parts < T_PARTS && !part_used(i, kb1 - kb0)) continue;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(o[i - 1][j]));
                 }
                 const uint32_t dst = xring + uint32_t(32 * q + lane) * pitch + uint32_t(c) * 4u;
 #pragma unroll
@@ -283,21 +289,28 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
     if (!*abort_flag) {
         const int quads = p.rp / 4;
         const uint32_t pitch = uint32_t(p.rp + 4) * 4u;
-        for (int i = int(rank) * SHRINK_THREADS + int(threadIdx.x); i < BM * quads; i += p.kc * SHRINK_THREADS) {
-            const int row = i / quads, col = (i - row * quads) * 4;
-            if (row0 + row >= p.m) break;
-            const int id = h.id[row];
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (id >= 0 && col < p.rank) {  // lanes of rows without an adapter hold nothing; past the rank may lie another adapter's sums
-                v = cluster_sum(xring + uint32_t(row) * pitch + uint32_t(col) * 4u, p.kc);
-                const float s = h.scale[row];
-                v.x *= s, v.y *= s, v.z *= s, v.w *= s;
+        const int stride = p.kc * SHRINK_THREADS, items = min(BM, p.m - row0) * quads;
+        for (int i0 = int(rank) * SHRINK_THREADS + int(threadIdx.x); i0 < items; i0 += 2 * stride) {
+            float4 v[2];  // two places per turn: their loads are on their way together
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int i = min(i0 + u * stride, items - 1), row = i / quads, col = (i - row * quads) * 4;
+                v[u] = cluster_sum(xring + uint32_t(row) * pitch + uint32_t(col) * 4u, p.kc);
             }
-            const uint32_t h0 = pack_16(v.x, v.y, p.bf16), h1 = pack_16(v.z, v.w, p.bf16);
-            const float2 f0 = p.bf16 ? pair_f32<true>(h0) : pair_f32<false>(h0), f1 = p.bf16 ? pair_f32<true>(h1) : pair_f32<false>(h1);
-            uint16_t *t = p.t + int64_t(row0 + row) * 2 * p.rp + col;
-            *reinterpret_cast<uint2 *>(t) = make_uint2(h0, h1);
-            *reinterpret_cast<uint2 *>(t + p.rp) = make_uint2(pack_16(v.x - f0.x, v.y - f0.y, p.bf16), pack_16(v.z - f1.x, v.w - f1.y, p.bf16));
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int i = i0 + u * stride, row = i / quads, col = (i - row * quads) * 4;
+                if (i >= items) break;
+                // Lanes of rows without an adapter hold nothing, and past the rank may lie another adapter's sums.
+                const float s = h.scale[row];
+                const bool has = h.id[row] >= 0 && col < p.rank;
+                const float4 w = has ? make_float4(v[u].x * s, v[u].y * s, v[u].z * s, v[u].w * s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const uint32_t h0 = pack_16(w.x, w.y, p.bf16), h1 = pack_16(w.z, w.w, p.bf16);
+                const float2 f0 = p.bf16 ? pair_f32<true>(h0) : pair_f32<false>(h0), f1 = p.bf16 ? pair_f32<true>(h1) : pair_f32<false>(h1);
+                uint16_t *t = p.t + int64_t(row0 + row) * 2 * p.rp + col;
+                *reinterpret_cast<uint2 *>(t) = make_uint2(h0, h1);
+                *reinterpret_cast<uint2 *>(t + p.rp) = make_uint2(pack_16(w.x - f0.x, w.y - f0.y, p.bf16), pack_16(w.z - f1.x, w.w - f1.y, p.bf16));
+            }
         }
     }
     if (p.early) ptx::griddep_wait();
@@ -713,6 +726,12 @@ cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceS
     s.mn = s.early = p.low_mn;
     s.boxes = p.low_mn ? (p.rp + 63) / 64 : 1;
     s.box_bytes = p.low_mn ? BK * 128 : uint32_t(p.rp) * 128u;
+    // A stage of A holds the blocks of two k blocks of one adapter, or 16 KB of them.
+    s.a_bytes = 2 * uint32_t(s.boxes) * s.box_bytes;
+    if (s.a_bytes < 16 * 1024) s.a_bytes = 16 * 1024;
+    s.x_stages = s.a_bytes > 16 * 1024 ? 3 : 4;
+    s.a_stages = int((SHRINK_RINGS - uint32_t(s.x_stages * X_BLOCKS) * X_BYTES) / s.a_bytes);
+    if (s.a_stages > MAX_A_STAGES) s.a_stages = MAX_A_STAGES;
     s.bf16 = bf16;
     s.idesc = make_idesc(bf16, 128, p.rp) | (p.low_mn ? IDESC_B_MN : 0u);
     s.part_cols = p.rp <= 32 ? 32 : uint32_t(p.rp);
