@@ -482,8 +482,41 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 // they are gone.
 constexpr uint32_t FEW_SMEM = 216 * 1024;
 
+// How the few-row kernels would run a problem, and in what time.  The terms are fitted to measurements of both ways (graphs of
+// 60 calls, us, few / tiled; rows with one of a adapters each):
+//   n 4096 k 4096 rank 16 a 64: 8 rows 12 / 23, 64 rows 18 / 66, 128 rows 24 / 91
+//   n 8192 k 4096 rank 16 a 4: 8 rows 18 / 23, 32 rows 20 / 23, 64 rows 26 / 23, 128 rows 33 / 23
+//   n 16384 k 2048 rank 32 a 8: 8 rows 17 / 24, 32 rows 26 / 20, 128 rows 29 / 20
+//   n 1000 k 8192 rank 128 a 4: 8 rows 15 / 33, 128 rows 29 / 35
+// The tiled kernels read every adapter's weights tile by tile and do not cut k; the few-row kernels pay for every row: its
+// part of X per k block, its dot products (or its adapter's masked product), its place in the final sum.
+struct FewPlan {
+    int bn = 16, kc = 1;
+    bool dots = false;  // the adapters' part as dot products
+    double time = 0.0;
+};
+FewPlan few_plan(const LoraParams &p, const DeviceState &dev) {
+    FewPlan f;
+    const int k_blocks = (p.k + 63) / 64, entries = p.adapters < p.m ? p.adapters : p.m;
+    stream_cut(p.n, k_blocks, dev.few_clusters, &f.bn, &f.kc);
+    const int own = (p.m + f.kc - 1) / f.kc, at_once = p.rank <= 16 ? 8 : 4;
+    const double dots = (own + at_once - 1) / at_once * ((f.bn + 127) / 128) * 0.8e-6;
+    const double masked = (entries + f.kc - 1) / f.kc * (p.rp <= 64 ? 1 : 2) * 0.5e-6;
+    f.dots = p.rp <= 32 && uint64_t(own) * uint64_t(p.rp + f.bn) * 4 <= FEW_DOTS && dots <= masked;
+    const double stream = double(p.n) * p.k * 2 / 6.0e12 + double(k_blocks) / f.kc * p.m * 128 / 9.0e10;
+    const double low = 2.5e-6 + double(p.m) / SHRINK_ROWS * p.rp / (p.rank >= 64 ? 8 : 4) / (2.0 * dev.sm_count) * (p.k / 2048.0 * 1.0e-6 + 1.5e-6);
+    f.time = 5.5e-6 + (stream > low ? stream : low) + (f.dots ? dots : masked) + double(p.m) * f.bn / (4.0 * f.kc * 2 * FEW_THREADS) * 0.6e-6;
+    return f;
+}
+double tiled_time(const LoraParams &p, const DeviceState &dev) {
+    const int k_blocks = (p.k + 63) / 64, entries = p.adapters < p.m ? p.adapters : p.m;
+    const double waves = double(((p.n + 127) / 128 + dev.sm_count - 1) / dev.sm_count), weight = double(p.n) * p.k * 2 / 5.5e12;
+    const double product = waves * k_blocks * 0.19e-6;
+    return 8.0e-6 + (weight > product ? weight : product) + entries * (0.17e-6 * p.k / 1024 + 0.3e-6 * ext_blocks(p.rp, whole_t(p.c_dtype)));
+}
+
 template <bool BF16>
-cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int debug, cudaStream_t stream) {
+cute_b200_status forward_few(const LoraParams &p, const FewPlan &plan, const DeviceState &dev, int debug, cudaStream_t stream) {
     if (p.rank >= 64) CB_TRY(launch_dependent(shrink_rows_kernel<BF16, 8>, dim3(unsigned(p.m), unsigned(p.rp / 8)), SHRINK_THREADS, 0, 1, stream, p));
     else CB_TRY(launch_dependent(shrink_rows_kernel<BF16, 4>, dim3(unsigned(p.m), unsigned(p.rp / 4)), SHRINK_THREADS, 0, 1, stream, p));
     if (!p.y) return CUTE_B200_OK;
@@ -493,14 +526,13 @@ cute_b200_status forward_few(const LoraParams &p, const DeviceState &dev, int de
     const uint64_t esize = p.c_dtype == CUTE_B200_F32 ? 4 : 2;
     f.vec = reinterpret_cast<uint64_t>(p.y) % (4 * esize) == 0 && p.ldy % 4 == 0;
     f.k_blocks = (p.k + 63) / 64;
-    f.bn = 16, f.kc = 1;
-    stream_cut(p.n, (p.k + 63) / 64, dev.few_clusters, &f.bn, &f.kc);
+    f.bn = plan.bn, f.kc = plan.kc;
     f.xr = (p.m + 7) / 8 * 8;
     f.x_bytes = uint32_t(f.xr) * 128u;
     f.w_bytes = uint32_t(f.bn) * 128u;
     // The head, T, the ring, and behind the last stage as much as an MMA reads past its rows of X.
     const uint64_t dots = uint64_t((p.m + f.kc - 1) / f.kc) * uint64_t(p.rp + f.bn) * 4;
-    f.b_blocks = p.rp <= 32 && dots <= FEW_DOTS ? 0 : (p.rp <= 64 ? 1 : 2);
+    f.b_blocks = plan.dots ? 0 : (p.rp <= 64 ? 1 : 2);
     f.low_bytes = f.b_blocks == 0 ? uint32_t((dots + 1023) / 1024 * 1024) : uint32_t(ext_blocks(p.rp, whole_t(p.c_dtype))) * f.x_bytes;
     f.t = p.t, f.b = p.b, f.bf16 = BF16;
     const uint32_t ring = FEW_SMEM - FEW_HEAD - 1024 - f.low_bytes;
@@ -581,8 +613,11 @@ uint64_t elem_bytes(int dtype) { return dtype == CUTE_B200_F32 ? 4 : 2; }
 
 cute_b200_status forward(const LoraParams &p, bool bf16, const int32_t (&tuning)[2], const DeviceState &dev, cudaStream_t stream) {
     if (p.m == 0) return CUTE_B200_OK;
-    if (tuning[0] == 1 || (tuning[0] == 0 && p.m <= FEW_ROWS))
-        return bf16 ? forward_few<true>(p, dev, tuning[1], stream) : forward_few<false>(p, dev, tuning[1], stream);
+    if (tuning[0] == 1 || (tuning[0] == 0 && p.m <= FEW_ROWS)) {
+        const FewPlan plan = few_plan(p, dev);
+        if (tuning[0] == 1 || plan.time <= tiled_time(p, dev))
+            return bf16 ? forward_few<true>(p, plan, dev, tuning[1], stream) : forward_few<false>(p, plan, dev, tuning[1], stream);
+    }
     return lora_tiled(p, bf16, tuning[0] - 3, tuning[1], dev, stream);
 }
 
