@@ -17,8 +17,11 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 
 // ---- T --------------------------------------------------------------------------
 // T[i] = scale * A[ids[i]] x_i for 128 rows per CTA, the k range of a tile shared by
-// a cluster.  M = the rows, N = the padded rank: every adapter's MMAs are masked to
-// the lanes of its rows, so one accumulator serves all of them.  Bound by reading X
+// a cluster.  M = the rows, N = the padded ranks of several adapters side by side (an
+// MMA of N = 128 takes the 65 clocks that one of N = 16 takes); each row reads its own
+// adapter's columns of the accumulator.  Entry e of the tile's adapters has the columns
+// of slot e % slots; where there are more entries than slots, the MMAs of entries g slots
+// to (g + 1) slots - 1 are masked to the lanes of those entries' rows.  Bound by reading X
 // (and, where nearly every row has an adapter of its own, A).
 //   warp 0  TMA: two (128 x 64) blocks of X per stage of one ring, then the blocks of A
 //           of the tile's adapters for them through another, a lane each (with one block
@@ -28,12 +31,12 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 //           the plan of the GEMM's tile that starts at its rows), then the sum over the
 //           cluster, scale, split into two 16-bit numbers.
 // On the way back A is B[a] as it lies, (n, rank): rank is the fast index, so it is an MN-major operand.
-// A CTA's k range goes to T_PARTS accumulators in turn, added in f32 at the end: the tensor core cuts its sums off instead of
-// rounding them, an error of the same sign that grows with the products added into one accumulator (256 MMAs of 16: 5e-6
+// A CTA's k range goes to 1, 2 or 4 accumulators in turn, added in f32 at the end: the tensor core cuts its sums off instead
+// of rounding them, an error of the same sign that grows with the products added into one accumulator (256 MMAs of 16: 5e-6
 // of the sum, measured), and T enters f32 gradients.
 constexpr int SHRINK_THREADS = 192, MAX_X_STAGES = 4, MAX_A_STAGES = 4, X_BLOCKS = 2;
 constexpr uint32_t X_BYTES = BM * BK * 2, SHRINK_HEAD = 20 * 1024, SHRINK_RINGS = 192 * 1024;
-constexpr int T_PARTS = 4;
+constexpr int T_PARTS = 4, T_COLS = 512;  // at most; TMEM columns of all accumulators
 constexpr uint32_t SHRINK_SMEM = 1024 + SHRINK_HEAD + SHRINK_RINGS;
 
 struct ShrinkParams {
@@ -45,22 +48,20 @@ struct ShrinkParams {
     int boxes;       // of A per adapter and k block
     uint32_t box_bytes, a_bytes;  // a_bytes: of a stage of A
     int x_stages, a_stages;
-    uint32_t idesc, part_cols;  // TMEM columns of one accumulator
+    uint32_t idesc;  // without N
+    int parts, slot_shift, slot_cols;  // slot_cols: of an entry; an accumulator has slot_cols << slot_shift columns
     bool bf16, mn, early;
     uint32_t *status;
     int debug;
 };
 
-// Whether accumulator `part` of a range of `blocks` k blocks holds anything (block i goes to i * T_PARTS / blocks).
-__device__ __forceinline__ bool part_used(int part, int blocks) { return (part * blocks + T_PARTS - 1) / T_PARTS * T_PARTS / blocks == part; }
-
 template <int P>
 struct ShrinkHead {
     uint64_t xfull[MAX_X_STAGES], xempty[MAX_X_STAGES], afull[MAX_A_STAGES], aempty[MAX_A_STAGES], plan, done, drain;
     uint32_t tmem, abort;
-    int32_t entries, entry_id[BM], id[BM];
+    int32_t entries, entry_id[BM], id[BM], entry[BM];  // entry: of a row, -1 = none
     float scale[BM];
-    uint32_t off[BM][4];
+    uint32_t off[BM][4];  // by group of slots: lanes of other rows
     IdTable<128> rows;  // of this CTA's rows
     IdTable<P> tile;    // of the GEMM's tile
 };
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         ptx::fence_mbar_init();
     }
     if (warp == 1) {
-        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), T_PARTS * p.part_cols);
+        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), T_COLS);
         ptx::tmem_relinquish<1>();
     }
     ptx::tc_fence_before();
@@ -162,9 +163,13 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         const bool leader = ptx::elect_one();
         bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.plan), 0, abort_flag, p.status, WHERE_MMA_TMEM, 100u, limit)), issued = false;
         const int entries = ok ? h.entries : 0;
-        // The blocks at which the second to fourth accumulator begin (part_used tells which of them get any).
+        // The blocks at which the second to fourth accumulator begin.
         static_assert(T_PARTS == 4, "three beginnings");
-        const int blocks = kb1 - kb0, begin1 = (blocks + 3) / 4, begin2 = (2 * blocks + 3) / 4, begin3 = (3 * blocks + 3) / 4;
+        const int blocks = kb1 - kb0, never = 0x7fffffff;
+        const int begin1 = p.parts > 1 ? (blocks + p.parts - 1) / p.parts : never, begin2 = p.parts > 2 ? (blocks + 1) / 2 : never,
+                  begin3 = p.parts > 2 ? (3 * blocks + 3) / 4 : never;
+        const int slots = 1 << p.slot_shift;
+        const uint32_t part_cols = uint32_t(p.slot_cols) << p.slot_shift;
         int sx = 0, sa = 0;
         uint32_t px = 0, pa = 0;
         for (int kb = kb0; kb < kb1 && ok && entries > 0; kb += X_BLOCKS) {
@@ -176,22 +181,25 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
                 if (!ok) break;
                 ptx::tc_fence_after();
                 const int count = min(group, items - i0);
-                for (int i = 0; i < count; i++) {
-                    const int second = i0 + i >= entries ? 1 : 0, e = i0 + i - second * entries;
+                for (int i = 0; i < count;) {
+                    // As many adapters as lie side by side: in this stage, of one k block and one group of slots.
+                    const int second = i0 + i >= entries ? 1 : 0, e = i0 + i - second * entries, slot = e & (slots - 1);
+                    const int run = min(min(count - i, entries - e), slots - slot), at = kb + second - kb0;
                     const uint32_t src = aring + uint32_t(sa) * p.a_bytes + uint32_t(i) * entry_bytes;
                     const uint64_t a = sw128_desc(xring + uint32_t(sx * X_BLOCKS + second) * X_BYTES);
                     const uint64_t b = p.mn ? mn_desc(src, p.box_bytes) : sw128_desc(src);
-                    const int at = kb + second - kb0;
-                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u;
-                    const uint32_t d = tmem + (uint32_t(at >= begin1) + uint32_t(at >= begin2) + uint32_t(at >= begin3)) * p.part_cols;
+                    const uint32_t k_step = p.mn ? MN_K_STEP : 2u, idesc = p.idesc | uint32_t(run * p.slot_cols / 8) << 17;
+                    const uint32_t d = tmem + (uint32_t(at >= begin1) + uint32_t(at >= begin2) + uint32_t(at >= begin3)) * part_cols + uint32_t(slot * p.slot_cols);
                     const uint32_t more = at != 0 && at != begin1 && at != begin2 && at != begin3 ? 1u : 0u;
-                    const uint32_t o0 = h.off[e][0], o1 = h.off[e][1], o2 = h.off[e][2], o3 = h.off[e][3];
+                    const uint32_t *off = h.off[e >> p.slot_shift];
+                    const uint32_t o0 = off[0], o1 = off[1], o2 = off[2], o3 = off[3];
                     if (leader) {
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            ptx::umma_f16_lanes(d, a + 2u * j, b + k_step * j, p.idesc, j > 0 ? 1u : more, o0, o1, o2, o3);
+                            ptx::umma_f16_lanes(d, a + 2u * j, b + k_step * j, idesc, j > 0 ? 1u : more, o0, o1, o2, o3);
                     }
                     __syncwarp();
+                    i += run;
                 }
                 issued = true;
                 if (leader) ptx::umma_commit<1>(bar(h.aempty[sa]));
@@ -227,7 +235,8 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             h.scale[t] = ids[0] >= 0 ? __ldcg(p.scale + ids[0]) : 0.0f;
             for (int i = t; i < BM * 4; i += 128) h.off[i / 4][i % 4] = 0xffffffffu;
             const int total = distinct_ids<128>(ids, h.rows, t, mine, [&](int e, int id) { h.entry_id[e] = id; });
-            if (mine[0] >= 0) atomicAnd(&h.off[mine[0]][t / 32], ~(1u << (t % 32)));
+            h.entry[t] = mine[0];
+            if (mine[0] >= 0) atomicAnd(&h.off[mine[0] >> p.slot_shift][t / 32], ~(1u << (t % 32)));
             if (t == 0) h.entries = total;
             ptx::named_barrier(1, 128);
             if (t == 0) ptx::mbar_arrive(bar(h.plan));
@@ -254,27 +263,33 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         if (ok) {
             ptx::tc_fence_after();
             ptx::fence_proxy_async_shared();
-            const int parts = min(T_PARTS, kb1 - kb0);  // those that hold something
-            for (int c = 0; c < p.rp; c += 32) {
-                uint32_t v[32];
-                const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(c);
-                uint32_t o[T_PARTS - 1][32];
-                ptx::tmem_ld_32x32(from, v);
+            const int entry = h.entry[32 * q + lane], slots = 1 << p.slot_shift, used = min(slots, h.entries);
+            const uint32_t part_cols = uint32_t(p.slot_cols) << p.slot_shift;
+            for (int slot = 0; slot < used; slot++) {
+                const bool here = entry >= 0 && (entry & (slots - 1)) == slot;
+                if (!__any_sync(0xffffffffu, here)) continue;
+                for (int c = 0; c < p.rp; c += 16) {
+                    uint32_t v[T_PARTS][16];
+                    const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(slot * p.slot_cols + c);
 #pragma unroll
-                for (int i = 1; i < T_PARTS; i++) ptx::tmem_ld_32x32(from + uint32_t(i) * p.part_cols, o[i - 1]);
-                ptx::tmem_ld_wait_all();
-                ptx::pin(v);
+                    for (int i = 0; i < T_PARTS; i++)
+                        if (i < p.parts) ptx::tmem_ld_32x16(from + uint32_t(i) * part_cols, v[i]);
+                    ptx::tmem_ld_wait_all();
+                    ptx::pin16(v[0]);
 #pragma unroll
-                for (int i = 1; i < T_PARTS; i++) {
-                    ptx::pin(o[i - 1]);
-                    if (parts < T_PARTS && !part_used(i, kb1 - kb0)) continue;
+                    for (int i = 1; i < T_PARTS; i++) {
+                        if (i >= p.parts) continue;
+                        ptx::pin16(v[i]);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(o[i - 1][j]));
+                        for (int j = 0; j < 16; j++) v[0][j] = __float_as_uint(__uint_as_float(v[0][j]) + __uint_as_float(v[i][j]));
+                    }
+                    const uint32_t dst = xring + uint32_t(32 * q + lane) * pitch + uint32_t(c) * 4u;
+                    if (here) {
+#pragma unroll
+                        for (int g = 0; g < 4; g++) ptx::st_shared_v4(dst + 16u * g, v[0][4 * g], v[0][4 * g + 1], v[0][4 * g + 2], v[0][4 * g + 3]);
+                    }
+                    __syncwarp();
                 }
-                const uint32_t dst = xring + uint32_t(32 * q + lane) * pitch + uint32_t(c) * 4u;
-#pragma unroll
-                for (int g = 0; g < 8; g++)
-                    if (c + 4 * g < p.rp) ptx::st_shared_v4(dst + 16u * g, v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
             }
         }
         __syncwarp();
@@ -301,7 +316,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             for (int u = 0; u < 2; u++) {
                 const int i = i0 + u * stride, row = i / quads, col = (i - row * quads) * 4;
                 if (i >= items) break;
-                // Lanes of rows without an adapter hold nothing, and past the rank may lie another adapter's sums.
+                // Rows without an adapter have nothing there, and past the rank may lie another adapter's sums.
                 const float s = h.scale[row];
                 const bool has = h.id[row] >= 0 && col < p.rank;
                 const float4 w = has ? make_float4(v[u].x * s, v[u].y * s, v[u].z * s, v[u].w * s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -319,7 +334,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
         ptx::cluster_arrive();
         ptx::cluster_wait();
     }
-    if (warp == 1) ptx::tmem_dealloc<1>(tmem, T_PARTS * p.part_cols);
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, T_COLS);
 }
 
 // ---- Y --------------------------------------------------------------------------
@@ -733,8 +748,7 @@ cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceS
     s.a_stages = int((SHRINK_RINGS - uint32_t(s.x_stages * X_BLOCKS) * X_BYTES) / s.a_bytes);
     if (s.a_stages > MAX_A_STAGES) s.a_stages = MAX_A_STAGES;
     s.bf16 = bf16;
-    s.idesc = make_idesc(bf16, 128, p.rp) | (p.low_mn ? IDESC_B_MN : 0u);
-    s.part_cols = p.rp <= 32 ? 32 : uint32_t(p.rp);
+    s.idesc = make_idesc(bf16, 128, 0) | (p.low_mn ? IDESC_B_MN : 0u);
     s.status = dev.status_word;
     s.debug = debug;
     const int tiles = (p.m + BM - 1) / BM;
@@ -742,6 +756,11 @@ cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceS
     s.kc = 1;
     for (int c = 1; c < 4; c++)
         if (tiles <= dev.shrink_clusters[c] && s.k_blocks >= (2 << c)) s.kc = 1 << c;
+    // At most 8 k blocks (32 MMAs of 16) per accumulator where one or two are enough: fewer of them have more slots.
+    const int blocks = (s.k_blocks + s.kc - 1) / s.kc;
+    s.parts = blocks <= 8 ? 1 : (blocks <= 16 ? 2 : T_PARTS);
+    s.slot_cols = p.low_mn ? 64 * s.boxes : p.rp;
+    while ((s.slot_cols << (s.slot_shift + 1)) * s.parts <= T_COLS) s.slot_shift++;
     CUtensorMap tmX, tmA;
     CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), bf16, p.m, p.k, p.ldx, BM));
     if (p.low_mn) CB_TRY(stack_tensor_map(&tmA, reinterpret_cast<uint64_t>(p.a), bf16, p.adapters, p.k, p.rank, BK));
