@@ -342,7 +342,9 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
 // ring of 192 KiB.  G: CTAs per MMA; BN: columns per tile; MH: 128-row accumulators per CTA.  Behind a tile's k blocks
 // of W come, for every adapter its rows name, the blocks of T (in place of X) and of B[a] (in place of W), their MMAs
 // masked to the lanes of the adapter's rows.  One adapter of rank 64 costs 1 block (2 for
-// an f32 result) beside the 64 of k = 4096.
+// an f32 result) beside the 64 of k = 4096.  A block of T serves all adapters of the tile: it
+// keeps its stage until the last of them, and their blocks of B fill the rest of that stage and
+// the others, as many as fit into each (a stage costs its issuing warps 0.3 us).
 // On the way back B is A[a] as it lies, (rank, k): an MN-major operand, in boxes of 64 columns by up to 64 ranks.
 // An f32 result of a long k is summed in `parts` accumulators (see T_PARTS), one set instead of two.
 constexpr uint32_t RING_BYTES = 192 * 1024;
@@ -360,6 +362,9 @@ struct Tile {
     static constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512;
     static constexpr uint32_t EXPECT = G * KB_BYTES;
     static constexpr int CH = BN / 64;  // 32-column chunks of an accumulator per epilogue warp
+    // Blocks of B in the stage that holds T, and in one without it.
+    static constexpr int FIRST = int((STAGE_BYTES - A_BYTES) / B_BYTES), REST = int(STAGE_BYTES / B_BYTES);
+    static constexpr int WORDS = ROWS / 32, BATCH = 32 / WORDS;  // mask words of an entry; entries whose words a warp reads at once
     static_assert(STAGES >= 3 && TMEM_COLS <= 512 && SMEM_BYTES <= 227 * 1024 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
 };
 
@@ -479,20 +484,22 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             ptx::prefetch_tensormap(&tmT);
             ptx::prefetch_tensormap(&tmB);
         }
-        int s = 0;
-        uint32_t ph = 0, filled = 0, filled_parity = 0;
+        int s = 0, held = -1;  // held: the stage that keeps a block of T, passed over until its adapters are done
+        uint32_t phases = 0, filled = 0, filled_parity = 0;  // phases: bit s = the parity of stage s's next use
         bool ok = !(p.debug & 4), waited = false;
         // Waits for the next stage and announces `bytes` per CTA.
         auto next = [&](uint32_t bytes) {
-            ok = __all_sync(0xffffffffu, wait_bar(empty_bar(s), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit));
+            if (s == held) s = s + 1 == C::STAGES ? 0 : s + 1;
+            ok = __all_sync(0xffffffffu, wait_bar(empty_bar(s), ~(phases >> s) & 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit));
             if (ok && lane == 0 && rank == 0) ptx::mbar_arrive_expect_tx(full_bar(s), uint32_t(G) * bytes);
             __syncwarp();
             return ok;
         };
         auto issued = [&] {
             __syncwarp();
-            filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
-            if (++s == C::STAGES) s = 0, ph ^= 1u;
+            filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (phases & 1u << s);
+            phases ^= 1u << s;
+            if (++s == C::STAGES) s = 0;
         };
         auto load = [&](uint32_t dst, const CUtensorMap *map, int x, int y) {
             if constexpr (G == 1) ptx::tma_load_2d(dst, map, full_bar(s), x, y);
@@ -525,23 +532,33 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 waited = true;
                 read_plan();
             }
-            for (int e = 0; e < entries && ok; e++) {
-                if (e > 0 && e % 32 == 0) read_ids(e);
-                const int id = __shfl_sync(0xffffffffu, ids, e % 32);
-                for (int q = 0; q < q_blocks; q++) {
-                    const ExtBlock b = ext_block(q, p.rp, p.rank, whole);
-                    if (!next(C::A_BYTES + low_bytes)) break;
-                    const uint32_t dst = ring + uint32_t(s) * C::STAGE_BYTES;
-                    if (lane == 0) load(dst, &tmT, b.t_col, row);
-                    if (p.low_box == 0) {
-                        if (lane == 1) load(dst + C::A_BYTES, &tmB, b.b_col, id * p.n + col);
-                    } else if (lane >= 1 && lane <= C::B_ROWS / 64) {
-                        const uint32_t to = dst + C::A_BYTES + uint32_t(lane - 1) * p.low_box;
-                        if constexpr (G == 1) ptx::tma_load_3d(to, &tmB, full_bar(s), col + 64 * (lane - 1), b.b_col, id);
-                        else ptx::tma_load_3d_pair(to, &tmB, ptx::mapa(full_bar(s), 0), col + 64 * (lane - 1), b.b_col, id);
+            const int boxes = p.low_box ? C::B_ROWS / 64 : 1;  // of B per adapter
+            for (int q = 0; q < q_blocks && entries > 0 && ok; q++) {
+                const ExtBlock b = ext_block(q, p.rp, p.rank, whole);
+                if (q > 0 && entries > 32) read_ids(0);
+                for (int e = 0; e < entries && ok;) {
+                    if (e > 0 && e % 32 == 0) read_ids(e);
+                    // Entries of one stage, all of one reading of the ids.
+                    const int count = min(min(e == 0 ? C::FIRST : C::REST, entries - e), 32 - e % 32);
+                    const int item = e == 0 ? lane - 1 : lane, mine = item / boxes, box = item % boxes;  // lane 0 issues T
+                    const int id = __shfl_sync(0xffffffffu, ids, (e + mine) % 32);
+                    if (!next((e == 0 ? C::A_BYTES : 0u) + uint32_t(count) * low_bytes)) break;
+                    const uint32_t dst = ring + uint32_t(s) * C::STAGE_BYTES, low = dst + (e == 0 ? C::A_BYTES : 0u) + uint32_t(mine) * C::B_BYTES;
+                    if (e == 0 && lane == 0) load(dst, &tmT, b.t_col, row);
+                    if (item >= 0 && mine < count) {
+                        if (p.low_box == 0) {
+                            load(low, &tmB, b.b_col, id * p.n + col);
+                        } else {
+                            const uint32_t to = low + uint32_t(box) * p.low_box;
+                            if constexpr (G == 1) ptx::tma_load_3d(to, &tmB, full_bar(s), col + 64 * box, b.b_col, id);
+                            else ptx::tma_load_3d_pair(to, &tmB, ptx::mapa(full_bar(s), 0), col + 64 * box, b.b_col, id);
+                        }
                     }
+                    if (e == 0) held = s;
                     issued();
+                    e += count;
                 }
+                held = -1;
             }
         }
         if (!ok && rank == 0 && lane == 0) {  // giving up: let the copies in flight land (bounded)
@@ -556,22 +573,26 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         if (rank == 0) {
             // The whole warp runs the loop and one thread issues: see lora_few_kernel.
             const bool leader = ptx::elect_one();
-            int s = 0, it = 0;
-            uint32_t ph = 0;
+            int s = 0, it = 0, held = -1;
+            uint32_t phases = 0;
             bool ok = true, issued = false, waited = false;
             auto ready = [&] {
-                ok = __all_sync(0xffffffffu, wait_bar(full_bar(s), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
+                if (s == held) s = s + 1 == C::STAGES ? 0 : s + 1;
+                ok = __all_sync(0xffffffffu, wait_bar(full_bar(s), phases >> s & 1u, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
                 ptx::tc_fence_after();
                 return ok;
             };
-            auto free_stage = [&] {
-                issued = true;
+            auto release = [&](int stage) {
                 if (leader) {
-                    ptx::umma_commit<G>(empty_bar(s));
-                    if constexpr (G == 2) ptx::umma_commit<G>(ptx::mapa(empty_bar(s), 1));
+                    ptx::umma_commit<G>(empty_bar(stage));
+                    if constexpr (G == 2) ptx::umma_commit<G>(ptx::mapa(empty_bar(stage), 1));
                 }
                 __syncwarp();
-                if (++s == C::STAGES) s = 0, ph ^= 1u;
+            };
+            auto advance = [&] {
+                issued = true;
+                phases ^= 1u << s;
+                if (++s == C::STAGES) s = 0;
             };
             for (int t = first; t < tiles && ok; t += step, it++) {
                 const TileAt at = tile_at(t, p);
@@ -580,10 +601,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 uint32_t d = d0;
                 int part = 0, part_end = (p.k_blocks + p.parts - 1) / p.parts;  // the k block the next accumulator begins at
                 const uint32_t *plan = p.plan + uint64_t(at.tm) * stride;
-                // Lane l holds word l of an entry's masks, read one entry ahead.
+                // Lane l holds word l % WORDS of the masks of entry l / WORDS of a batch, read one batch ahead.
                 int entries = 0;
                 uint32_t ahead = 0;
-                auto read_off = [&](int e) { ahead = e < entries && lane < C::ROWS / 32 ? plan[4 + e * ENTRY + 4 + lane] : 0u; };
+                auto read_off = [&](int e0) {
+                    const int e = e0 + lane / C::WORDS;
+                    ahead = e < entries ? plan[4 + e * ENTRY + 4 + lane % C::WORDS] : 0u;
+                };
                 auto read_plan = [&] {
                     entries = int(plan[0]);
                     read_off(0);
@@ -622,7 +646,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                         if (!ok) break;
                     }
                     if (!ok) break;
-                    free_stage();
+                    release(s);
+                    advance();
                 }
                 if (!ok) break;
                 if (!waited) {
@@ -631,25 +656,32 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     read_plan();
                 }
                 const uint32_t k_step = p.low_box ? MN_K_STEP : 2u;
-                for (int e = 0; e < entries && ok; e++) {
-                    uint32_t off[C::ROWS / 32];
-#pragma unroll
-                    for (int i = 0; i < C::ROWS / 32; i++) off[i] = __shfl_sync(0xffffffffu, ahead, i);
-                    read_off(e + 1);
-                    for (int q = 0; q < q_blocks; q++) {
-                        const ExtBlock x = ext_block(q, p.rp, p.rank, whole);
-                        if (!ready()) break;
-                        const uint32_t src = ring + uint32_t(s) * C::STAGE_BYTES;
-                        const uint64_t b = p.low_box ? mn_desc(src + C::A_BYTES, p.low_box) : sw128_desc(src + C::A_BYTES);
+                for (int q = 0; q < q_blocks && entries > 0 && ok; q++) {
+                    const ExtBlock x = ext_block(q, p.rp, p.rank, whole);
+                    uint32_t words = 0, t_block = 0, b_block = 0;
+                    int first_stage = 0, left = 0;  // left: entries of this stage still to come
+                    if (q > 0 && entries > C::BATCH) read_off(0);
+                    for (int e = 0; e < entries; e++) {
+                        if (e % C::BATCH == 0) {
+                            words = ahead;
+                            if (entries > C::BATCH) read_off(e + C::BATCH);
+                        }
+                        if (left == 0) {
+                            if (!ready()) break;
+                            left = min(min(e == 0 ? C::FIRST : C::REST, entries - e), 32 - e % 32);
+                            b_block = ring + uint32_t(s) * C::STAGE_BYTES;
+                            if (e == 0) t_block = b_block, b_block += C::A_BYTES, first_stage = s;
+                        }
+                        const uint64_t b = p.low_box ? mn_desc(b_block, p.low_box) : sw128_desc(b_block);
 #pragma unroll
                         for (int h = 0; h < MH; h++) {
-                            const uint64_t a = sw128_desc(src + uint32_t(h) * (BM * BK * 2));
-                            uint32_t m[4 * G];
+                            const uint64_t a = sw128_desc(t_block + uint32_t(h) * (BM * BK * 2));
+                            uint32_t m[4 * G], all = 0xffffffffu;
 #pragma unroll
-                            for (int i = 0; i < 4 * G; i++) m[i] = off[(i / 4) * (C::CTA_ROWS / 32) + 4 * h + i % 4];
-                            uint32_t all = 0xffffffffu;
-#pragma unroll
-                            for (int i = 0; i < 4 * G; i++) all &= m[i];
+                            for (int i = 0; i < 4 * G; i++) {
+                                m[i] = __shfl_sync(0xffffffffu, words, e % C::BATCH * C::WORDS + (i / 4) * (C::CTA_ROWS / 32) + 4 * h + i % 4);
+                                all &= m[i];
+                            }
                             if (leader && all != 0xffffffffu)  // else no row of these accumulators
                                 for (int j = 0; j < x.steps; j++) {
                                     const uint64_t bj = b + uint64_t(k_step * uint32_t(j & x.b_mask));
@@ -658,8 +690,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                                 }
                             __syncwarp();
                         }
-                        free_stage();
+                        b_block += C::B_BYTES;
+                        if (--left == 0) {  // T's stage keeps until the last entry
+                            if (e >= C::FIRST) release(s);
+                            if (e < C::FIRST) held = s;
+                            advance();
+                        }
                     }
+                    if (!ok) break;
+                    release(first_stage);
+                    held = -1;
                 }
                 if (!ok) break;
                 if (leader) {
