@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
 // On the way back B is A[a] as it lies, (rank, k): an MN-major operand, in boxes of 64 columns by up to 64 ranks.
 // An f32 result of a long k is summed in `parts` accumulators (see T_PARTS), one set instead of two.
 constexpr uint32_t RING_BYTES = 192 * 1024;
-constexpr int TILE_THREADS = 64 + 256;
+constexpr int TILE_THREADS = 64 + 256, TURN_PITCH = 33;  // words per row of a warp's piece of Y in shared memory, see store_32
 
 template <int G, int BN, int MH>
 struct Tile {
@@ -359,7 +359,7 @@ struct Tile {
     static constexpr int STAGES = int(RING_BYTES / STAGE_BYTES);
     static constexpr int ACC_COLS = MH * BN, ACC_BUFS = 2 * ACC_COLS <= 512 ? 2 : 1;
     static constexpr uint32_t TMEM_COLS = MH == 1 ? 512 : ACC_COLS * ACC_BUFS;
-    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512;
+    static constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512 + 8 * 32 * TURN_PITCH * 4;
     static constexpr uint32_t EXPECT = G * KB_BYTES;
     static constexpr int CH = BN / 64;  // 32-column chunks of an accumulator per epilogue warp
     // Blocks of B in the stage that holds T, and in one without it.
@@ -388,10 +388,15 @@ __device__ __forceinline__ TileAt tile_at(int t, const TileParams &p) {
     return {first + r % gm, r / gm};
 }
 
-__device__ __forceinline__ void store_32(const TileParams &p, int row, int col, const uint32_t (&v)[32]) {
-    if (row >= p.m || col >= p.n) return;
-    const int64_t at = int64_t(row) * p.ldy + col;
+// A warp's 32 x 32 piece of Y from row row0 and column col on, a row per lane.  Lanes that hold whole aligned vectors store
+// them as they are; others turn the piece through shared memory, so that a row is stored by neighbouring lanes (from a row
+// per lane, stores of 4 bytes took 10 us of 777 x 2050 values in f32: each touches 32 sectors).
+__device__ __forceinline__ void store_32(const TileParams &p, int row0, int col, const uint32_t (&v)[32], float *turn) {
+    if (col >= p.n || row0 >= p.m) return;
+    const int lane = int(threadIdx.x) & 31;
     if (p.vec && col + 32 <= p.n) {
+        if (row0 + lane >= p.m) return;
+        const int64_t at = int64_t(row0 + lane) * p.ldy + col;
         if (p.c_dtype == CUTE_B200_F32) {
             float *c = static_cast<float *>(p.y) + at;
             if (p.vec == 2) {
@@ -417,9 +422,15 @@ __device__ __forceinline__ void store_32(const TileParams &p, int row, int col, 
             }
         }
     } else {
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; j++)
-            if (col + j < p.n) store_c(p.y, p.c_dtype, size_t(at + j), __uint_as_float(v[j]));
+        for (int j = 0; j < 32; j++) turn[lane * TURN_PITCH + j] = __uint_as_float(v[j]);
+        __syncwarp();
+        const int rows = min(32, p.m - row0);
+        if (col + lane < p.n)
+#pragma unroll 8
+            for (int r = 0; r < rows; r++) store_c(p.y, p.c_dtype, size_t(int64_t(row0 + r) * p.ldy + col + lane), turn[r * TURN_PITCH + lane]);
+        __syncwarp();
     }
 }
 
@@ -718,6 +729,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         __syncwarp();
     } else {
         const uint32_t q = uint32_t(warp) & 3u;
+        float *turn = reinterpret_cast<float *>(smem_raw + (bars - raw) + 512) + (warp - 2) * 32 * TURN_PITCH;
         const int e = (warp - 2) >> 2;  // of two groups of four warps, each takes every other 32-column chunk
         int it = 0;
         for (int t = first; t < tiles; t += step, it++) {
@@ -726,7 +738,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             const bool ok = wait_bar(tfull_bar(buf), uint32_t(it / bufs) & 1u, abort_flag, p.status, WHERE_EPILOGUE, uint32_t(buf), limit);
             if (!__all_sync(0xffffffffu, ok)) break;
             ptx::tc_fence_after();
-            const int row0 = at.tm * C::ROWS + int(rank) * C::CTA_ROWS + int(q) * 32 + lane;
+            const int row0 = at.tm * C::ROWS + int(rank) * C::CTA_ROWS + int(q) * 32;
             const uint32_t taddr = tmem + ((q * 32u) << 16) + uint32_t(buf * C::ACC_COLS);
 #pragma unroll 1
             for (int h = 0; h < MH; h++) {
@@ -756,7 +768,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     else ptx::mbar_arrive_cluster(ptx::mapa(tempty_bar(buf, h), 0));
                 }
 #pragma unroll
-                for (int c = 0; c < C::CH; c++) store_32(p, row0 + h * BM, at.tn * BN + (2 * c + e) * 32, v[c]);
+                for (int c = 0; c < C::CH; c++) store_32(p, row0 + h * BM, at.tn * BN + (2 * c + e) * 32, v[c], turn);
             }
         }
         __syncwarp();
