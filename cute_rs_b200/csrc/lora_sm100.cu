@@ -484,10 +484,10 @@ constexpr uint32_t FEW_SMEM = 216 * 1024;
 
 // How the few-row kernels would run a problem, and in what time.  The terms are fitted to measurements of both ways (graphs of
 // 60 calls, us, few / tiled; rows with one of a adapters each):
-//   n 4096 k 4096 rank 16 a 64: 8 rows 12 / 23, 64 rows 18 / 66, 128 rows 24 / 91
-//   n 8192 k 4096 rank 16 a 4: 8 rows 18 / 23, 32 rows 20 / 23, 64 rows 26 / 23, 128 rows 33 / 23
-//   n 16384 k 2048 rank 32 a 8: 8 rows 17 / 24, 32 rows 26 / 20, 128 rows 29 / 20
-//   n 1000 k 8192 rank 128 a 4: 8 rows 15 / 33, 128 rows 29 / 35
+//   n 4096 k 4096 rank 16 a 64: 8 rows 12 / 24, 64 rows 18 / 41, 128 rows 24 / 51
+//   n 8192 k 4096 rank 16 a 4: 8 rows 18 / 32, 32 rows 20 / 22, 64 rows 23 / 23, 128 rows 28 / 23
+//   n 16384 k 2048 rank 32 a 8: 8 rows 17 / 22, 32 rows 21 / 18, 128 rows 29 / 19
+//   n 1000 k 8192 rank 128 a 4: 8 rows 14 / 32, 128 rows 29 / 34
 // The tiled kernels read every adapter's weights tile by tile and do not cut k; the few-row kernels pay for every row: its
 // part of X per k block, its dot products (or its adapter's masked product), its place in the final sum.
 struct FewPlan {
@@ -512,7 +512,7 @@ double tiled_time(const LoraParams &p, const DeviceState &dev) {
     const int k_blocks = (p.k + 63) / 64, entries = p.adapters < p.m ? p.adapters : p.m;
     const double waves = double(((p.n + 127) / 128 + dev.sm_count - 1) / dev.sm_count), weight = double(p.n) * p.k * 2 / 5.5e12;
     const double product = waves * k_blocks * 0.19e-6;
-    return 8.0e-6 + (weight > product ? weight : product) + entries * (0.17e-6 * p.k / 1024 + 0.3e-6 * ext_blocks(p.rp, whole_t(p.c_dtype)));
+    return 8.0e-6 + (weight > product ? weight : product) + entries * (0.05e-6 * p.k / 1024 * p.rp / 16 + 0.3e-6 * ext_blocks(p.rp, whole_t(p.c_dtype)));
 }
 
 template <bool BF16>
