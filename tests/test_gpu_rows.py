@@ -158,6 +158,7 @@ SHAPES = [  # m, n, k, rank, adapters, ids
     (64, 500, 264, 64, 64, "mixed"), (127, 130, 136, 40, 9, "packed"), (128, 257, 520, 128, 4, "mixed"),
     (129, 130, 72, 8, 2, "packed"), (300, 520, 1000, 32, 6, "mixed"), (513, 1025, 264, 72, 40, "mixed"),
     (1025, 384, 640, 16, 3, "packed"), (2050, 264, 4104, 128, 2, "packed"), (600, 2050, 64, 112, 600, "mixed"),
+    (300, 264, 4104, 16, 100, "mixed"), (530, 513, 2056, 48, 90, "mixed"),
 ]
 
 
@@ -224,6 +225,24 @@ def test_lora_rows_do_not_touch_one_another(lib, gpu, m):
             assert dirty[0].isnan().all() and not dirty[3].isfinite().any()
 
 
+@pytest.mark.parametrize("rank", [16, 40, 128])
+def test_lora_adapters_side_by_side_do_not_touch_one_another(lib, gpu, rank):
+    # Many adapters per tile share T's accumulators: only the rows of the bad ones differ.
+    m, adapters = 260, 90
+    ids = torch.arange(m) % (adapters + 1) - 1
+    bad = (ids % 7 == 3).cuda()
+    p = Lora(lib, m, 264, 520, rank, adapters, BF16, F32, ids)
+    q = Lora(lib, m, 264, 520, rank, adapters, BF16, F32, ids)
+    q.a[3::7] = float("nan")
+    q.b[3::7] = float("inf")
+    for tuning in variants(m):
+        clean, dirty = p.run(tuning)[:m], q.run(tuning)[:m]
+        assert torch.equal(clean[~bad], dirty[~bad])
+        assert not dirty[bad].isfinite().any()
+        dx, dx_bad = p.back(tuning=tuning)[0][:m], q.back(tuning=tuning)[0][:m]
+        assert torch.equal(dx[~bad], dx_bad[~bad])
+
+
 def test_gradients_leave_masked_rows_out(lib, gpu):
     m = 500
     ids = torch.arange(m) // 7 % 5 - 1
@@ -258,7 +277,7 @@ def test_lora_pitches(lib, gpu, m, ab, c):
 BACK = [
     (1, 8, 8, 8, 1, "packed"), (3, 72, 136, 16, 2, "mixed"), (64, 264, 520, 64, 9, "mixed"), (127, 128, 64, 40, 3, "packed"),
     (129, 520, 72, 128, 2, "mixed"), (777, 264, 1000, 24, 5, "packed"), (1500, 1032, 648, 16, 70, "mixed"),
-    (2050, 136, 128, 8, 1, "packed"),
+    (2050, 136, 128, 8, 1, "packed"), (300, 4104, 264, 16, 100, "mixed"), (530, 1032, 520, 96, 90, "mixed"),
 ]
 
 
