@@ -268,26 +268,38 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
             for (int slot = 0; slot < used; slot++) {
                 const bool here = entry >= 0 && (entry & (slots - 1)) == slot;
                 if (!__any_sync(0xffffffffu, here)) continue;
-                for (int c = 0; c < p.rp; c += 16) {
+                // Four pieces of 16 columns at a time: `parts` accumulators of 4 / parts pieces of the row.
+                const int width = 16 * T_PARTS / p.parts;
+                const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(slot * p.slot_cols);
+                for (int c = 0; c < p.rp; c += width) {
                     uint32_t v[T_PARTS][16];
-                    const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(slot * p.slot_cols + c);
+                    auto piece = [&](int i) { return c + 16 * (p.parts == 1 ? i : (p.parts == 2 ? i >> 1 : 0)); };
 #pragma unroll
                     for (int i = 0; i < T_PARTS; i++)
-                        if (i < p.parts) ptx::tmem_ld_32x16(from + uint32_t(i) * part_cols, v[i]);
+                        if (piece(i) < p.rp) ptx::tmem_ld_32x16(from + uint32_t(i & (p.parts - 1)) * part_cols + uint32_t(piece(i)), v[i]);
                     ptx::tmem_ld_wait_all();
-                    ptx::pin16(v[0]);
 #pragma unroll
-                    for (int i = 1; i < T_PARTS; i++) {
-                        if (i >= p.parts) continue;
-                        ptx::pin16(v[i]);
+                    for (int i = 0; i < T_PARTS; i++)
+                        if (piece(i) < p.rp) ptx::pin16(v[i]);
+                    auto add = [&](uint32_t (&to)[16], const uint32_t (&w)[16]) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) v[0][j] = __float_as_uint(__uint_as_float(v[0][j]) + __uint_as_float(v[i][j]));
+                        for (int j = 0; j < 16; j++) to[j] = __float_as_uint(__uint_as_float(to[j]) + __uint_as_float(w[j]));
+                    };
+                    if (p.parts == 2) {
+                        add(v[0], v[1]);
+                        if (piece(2) < p.rp) add(v[2], v[3]);
+                    } else if (p.parts == 4) {
+                        add(v[0], v[1]);
+                        add(v[0], v[2]);
+                        add(v[0], v[3]);
                     }
-                    const uint32_t dst = xring + uint32_t(32 * q + lane) * pitch + uint32_t(c) * 4u;
-                    if (here) {
+                    const uint32_t dst = xring + uint32_t(32 * q + lane) * pitch;
 #pragma unroll
-                        for (int g = 0; g < 4; g++) ptx::st_shared_v4(dst + 16u * g, v[0][4 * g], v[0][4 * g + 1], v[0][4 * g + 2], v[0][4 * g + 3]);
-                    }
+                    for (int i = 0; i < T_PARTS; i++)
+                        if (here && (i & (p.parts - 1)) == 0 && piece(i) < p.rp) {
+#pragma unroll
+                            for (int g = 0; g < 4; g++) ptx::st_shared_v4(dst + uint32_t(piece(i)) * 4u + 16u * g, v[i][4 * g], v[i][4 * g + 1], v[i][4 * g + 2], v[i][4 * g + 3]);
+                        }
                     __syncwarp();
                 }
             }
@@ -785,7 +797,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 
 // ---- host -------------------------------------------------------------------------
 template <int P>
-cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream) {
+cute_b200_status shrink(const LoraParams &p, int product_ctas, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream) {
     ShrinkParams s = {};
     s.ids = p.ids, s.scale = p.scale, s.t = p.t, s.plan = p.y ? p.plan : nullptr;
     s.m = p.m, s.rank = p.rank, s.rp = p.rp, s.adapters = p.adapters;
@@ -808,6 +820,16 @@ cute_b200_status shrink(const LoraParams &p, bool bf16, int debug, const DeviceS
     s.kc = 1;
     for (int c = 1; c < 4; c++)
         if (tiles <= dev.shrink_clusters[c] && s.k_blocks >= (2 << c)) s.kc = 1 << c;
+    // Where the product's CTAs (an SM each, like these) leave SMs free, T's kernel keeps to those, so that the product's k loop
+    // over W runs beside it; unless that takes longer than both one after the other, at 0.25 us per k block of the product
+    // and, per k block of T, 0.2 us and 0.25 per 128 rows of A.
+    const int free = dev.sm_count - product_ctas, entries = p.adapters < BM ? p.adapters : BM;
+    if (p.y && free >= tiles && tiles * s.kc > free) {
+        int kc = s.kc;
+        while (tiles * kc > free) kc /= 2;
+        const double block = 0.2 + 0.25 * entries * p.rp / 128.0;
+        if (block * s.k_blocks / kc <= block * s.k_blocks / s.kc + 0.25 * s.k_blocks) s.kc = kc;
+    }
     // At most 8 k blocks (32 MMAs of 16) per accumulator where one or two are enough: fewer of them have more slots.
     const int blocks = (s.k_blocks + s.kc - 1) / s.kc;
     s.parts = blocks <= 8 ? 1 : (blocks <= 16 ? 2 : T_PARTS);
@@ -894,9 +916,11 @@ uint64_t lora_plan_bytes(int m, int adapters) {
 
 cute_b200_status lora_tiled(const LoraParams &p, bool bf16, int cut, int debug, const DeviceState &dev, cudaStream_t stream) {
     if (cut < 0) cut = choose_cut(p.m, p.n, p.k, p.c_dtype, dev.sm_count);
-    if (CUTS[cut].rows == 512) CB_TRY(shrink<512>(p, bf16, debug, dev, stream));
-    else if (CUTS[cut].rows == 256) CB_TRY(shrink<256>(p, bf16, debug, dev, stream));
-    else CB_TRY(shrink<128>(p, bf16, debug, dev, stream));
+    const int64_t tiles = int64_t((p.m + CUTS[cut].rows - 1) / CUTS[cut].rows) * ((p.n + CUTS[cut].cols - 1) / CUTS[cut].cols);
+    const int pair = CUTS[cut].rows >= 256 ? 2 : 1, ctas = tiles * pair < dev.sm_count ? int(tiles) * pair : dev.sm_count;
+    if (CUTS[cut].rows == 512) CB_TRY(shrink<512>(p, ctas, bf16, debug, dev, stream));
+    else if (CUTS[cut].rows == 256) CB_TRY(shrink<256>(p, ctas, bf16, debug, dev, stream));
+    else CB_TRY(shrink<128>(p, ctas, bf16, debug, dev, stream));
     if (!p.y) return CUTE_B200_OK;
     if (cut == 0) return launch_tile<2, 256, 2>(p, bf16, debug, dev, stream);
     if (cut == 1) return launch_tile<2, 256, 1>(p, bf16, debug, dev, stream);
