@@ -374,8 +374,11 @@ struct Tile {
     static constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512 + 8 * 32 * TURN_PITCH * 4;
     static constexpr uint32_t EXPECT = G * KB_BYTES;
     static constexpr int CH = BN / 64;  // 32-column chunks of an accumulator per epilogue warp
-    // Blocks of B in the stage that holds T, and in one without it.
-    static constexpr int FIRST = int((STAGE_BYTES - A_BYTES) / B_BYTES), REST = int(STAGE_BYTES / B_BYTES);
+    // Blocks of B in a stage that holds one or two blocks of T, and in one without.  Two of them, the values' two numbers,
+    // where they fit: they are multiplied by the same block of B.
+    static constexpr bool PAIRS = 2 * A_BYTES <= STAGE_BYTES;
+    static constexpr int FIRST = int((STAGE_BYTES - A_BYTES) / B_BYTES), FIRST_PAIR = PAIRS ? int((STAGE_BYTES - 2 * A_BYTES) / B_BYTES) : 0;
+    static constexpr int REST = int(STAGE_BYTES / B_BYTES);
     static constexpr int WORDS = ROWS / 32, BATCH = 32 / WORDS;  // mask words of an entry; entries whose words a warp reads at once
     static_assert(STAGES >= 3 && TMEM_COLS <= 512 && SMEM_BYTES <= 227 * 1024 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
 };
@@ -471,7 +474,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     constexpr int ENTRY = 4 + C::ROWS / 32;
     const int bufs = p.parts > 1 ? 1 : C::ACC_BUFS;
     const bool whole = whole_t(p.c_dtype);
-    const int q_blocks = ext_blocks(p.rp, whole);
+    const int t_blocks = C::PAIRS && whole && p.rp > 32 ? 2 : 1, q_blocks = ext_blocks(p.rp, whole);  // t_blocks: of T taken together
+    const int first_blocks = t_blocks == 2 ? C::FIRST_PAIR : C::FIRST;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) {
@@ -556,18 +560,20 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 read_plan();
             }
             const int boxes = p.low_box ? C::B_ROWS / 64 : 1;  // of B per adapter
-            for (int q = 0; q < q_blocks && entries > 0 && ok; q++) {
+            for (int q = 0; q < q_blocks && entries > 0 && ok; q += t_blocks) {
                 const ExtBlock b = ext_block(q, p.rp, p.rank, whole);
                 if (q > 0 && entries > 32) read_ids(0);
-                for (int e = 0; e < entries && ok;) {
+                bool head = true;  // this stage begins with T
+                for (int e = 0; e < entries && ok; head = false) {
                     if (e > 0 && e % 32 == 0) read_ids(e);
                     // Entries of one stage, all of one reading of the ids.
-                    const int count = min(min(e == 0 ? C::FIRST : C::REST, entries - e), 32 - e % 32);
-                    const int item = e == 0 ? lane - 1 : lane, mine = item / boxes, box = item % boxes;  // lane 0 issues T
-                    const int id = __shfl_sync(0xffffffffu, ids, (e + mine) % 32);
-                    if (!next((e == 0 ? C::A_BYTES : 0u) + uint32_t(count) * low_bytes)) break;
-                    const uint32_t dst = ring + uint32_t(s) * C::STAGE_BYTES, low = dst + (e == 0 ? C::A_BYTES : 0u) + uint32_t(mine) * C::B_BYTES;
-                    if (e == 0 && lane == 0) load(dst, &tmT, b.t_col, row);
+                    const int count = min(min(head ? first_blocks : C::REST, entries - e), 32 - e % 32);
+                    const int item = head ? lane - t_blocks : lane, mine = item / boxes, box = item % boxes;  // the first lanes issue T
+                    const int id = __shfl_sync(0xffffffffu, ids, (e + mine) & 31);
+                    const uint32_t t_bytes = head ? uint32_t(t_blocks) * C::A_BYTES : 0u;
+                    if (!next(t_bytes + uint32_t(count) * low_bytes)) break;
+                    const uint32_t dst = ring + uint32_t(s) * C::STAGE_BYTES, low = dst + t_bytes + uint32_t(mine) * C::B_BYTES;
+                    if (head && lane < t_blocks) load(dst + uint32_t(lane) * C::A_BYTES, &tmT, b.t_col + lane * p.rp, row);
                     if (item >= 0 && mine < count) {
                         if (p.low_box == 0) {
                             load(low, &tmB, b.b_col, id * p.n + col);
@@ -577,7 +583,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                             else ptx::tma_load_3d_pair(to, &tmB, ptx::mapa(full_bar(s), 0), col + 64 * box, b.b_col, id);
                         }
                     }
-                    if (e == 0) held = s;
+                    if (head) held = s;
                     issued();
                     e += count;
                 }
@@ -679,21 +685,31 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     read_plan();
                 }
                 const uint32_t k_step = p.low_box ? MN_K_STEP : 2u;
-                for (int q = 0; q < q_blocks && entries > 0 && ok; q++) {
+                for (int q = 0; q < q_blocks && entries > 0 && ok; q += t_blocks) {
                     const ExtBlock x = ext_block(q, p.rp, p.rank, whole);
                     uint32_t words = 0, t_block = 0, b_block = 0;
                     int first_stage = 0, left = 0;  // left: entries of this stage still to come
+                    bool head = false;              // this stage holds T
                     if (q > 0 && entries > C::BATCH) read_off(0);
                     for (int e = 0; e < entries; e++) {
                         if (e % C::BATCH == 0) {
                             words = ahead;
                             if (entries > C::BATCH) read_off(e + C::BATCH);
                         }
+                        if (e == 0) {
+                            if (!ready()) break;
+                            first_stage = s, t_block = ring + uint32_t(s) * C::STAGE_BYTES, b_block = t_block + uint32_t(t_blocks) * C::A_BYTES;
+                            left = min(min(first_blocks, entries), 32);
+                            head = true;
+                            if (left == 0) {
+                                held = s, head = false;
+                                advance();
+                            }
+                        }
                         if (left == 0) {
                             if (!ready()) break;
-                            left = min(min(e == 0 ? C::FIRST : C::REST, entries - e), 32 - e % 32);
+                            left = min(min(C::REST, entries - e), 32 - e % 32);
                             b_block = ring + uint32_t(s) * C::STAGE_BYTES;
-                            if (e == 0) t_block = b_block, b_block += C::A_BYTES, first_stage = s;
                         }
                         const uint64_t b = p.low_box ? mn_desc(b_block, p.low_box) : sw128_desc(b_block);
 #pragma unroll
@@ -705,18 +721,23 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                                 m[i] = __shfl_sync(0xffffffffu, words, e % C::BATCH * C::WORDS + (i / 4) * (C::CTA_ROWS / 32) + 4 * h + i % 4);
                                 all &= m[i];
                             }
-                            if (leader && all != 0xffffffffu)  // else no row of these accumulators
-                                for (int j = 0; j < x.steps; j++) {
-                                    const uint64_t bj = b + uint64_t(k_step * uint32_t(j & x.b_mask));
-                                    if constexpr (G == 1) ptx::umma_f16_lanes(d0 + uint32_t(h * BN), a + 2u * j, bj, p.low_idesc, 1u, m[0], m[1], m[2], m[3]);
-                                    else ptx::umma_f16_lanes_pair(d0 + uint32_t(h * BN), a + 2u * j, bj, p.low_idesc, 1u, m);
-                                }
+                            if (leader && all != 0xffffffffu) {  // else no row of these accumulators
+                                auto multiply = [&](uint64_t from) {
+                                    for (int j = 0; j < x.steps; j++) {
+                                        const uint64_t bj = b + uint64_t(k_step * uint32_t(j & x.b_mask));
+                                        if constexpr (G == 1) ptx::umma_f16_lanes(d0 + uint32_t(h * BN), from + 2u * j, bj, p.low_idesc, 1u, m[0], m[1], m[2], m[3]);
+                                        else ptx::umma_f16_lanes_pair(d0 + uint32_t(h * BN), from + 2u * j, bj, p.low_idesc, 1u, m);
+                                    }
+                                };
+                                multiply(a);
+                                if (t_blocks == 2) multiply(a + (C::A_BYTES >> 4));
+                            }
                             __syncwarp();
                         }
                         b_block += C::B_BYTES;
-                        if (--left == 0) {  // T's stage keeps until the last entry
-                            if (e >= C::FIRST) release(s);
-                            if (e < C::FIRST) held = s;
+                        if (--left == 0) {  // T's stage is kept until the last entry
+                            if (head) held = s, head = false;
+                            else release(s);
                             advance();
                         }
                     }
