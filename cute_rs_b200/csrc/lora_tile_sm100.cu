@@ -688,6 +688,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 for (int q = 0; q < q_blocks && entries > 0 && ok; q += t_blocks) {
                     const ExtBlock x = ext_block(q, p.rp, p.rank, whole);
                     uint32_t words = 0, t_block = 0, b_block = 0;
+                    uint32_t step[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) step[j] = k_step * uint32_t(j & x.b_mask);
                     int first_stage = 0, left = 0;  // left: entries of this stage still to come
                     bool head = false;              // this stage holds T
                     if (q > 0 && entries > C::BATCH) read_off(0);
@@ -723,8 +726,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                             }
                             if (leader && all != 0xffffffffu) {  // else no row of these accumulators
                                 auto multiply = [&](uint64_t from) {
-                                    for (int j = 0; j < x.steps; j++) {
-                                        const uint64_t bj = b + uint64_t(k_step * uint32_t(j & x.b_mask));
+#pragma unroll
+                                    for (int j = 0; j < 4; j++) {
+                                        if (j >= x.steps) continue;
+                                        const uint64_t bj = b + uint64_t(step[j]);
                                         if constexpr (G == 1) ptx::umma_f16_lanes(d0 + uint32_t(h * BN), from + 2u * j, bj, p.low_idesc, 1u, m[0], m[1], m[2], m[3]);
                                         else ptx::umma_f16_lanes_pair(d0 + uint32_t(h * BN), from + 2u * j, bj, p.low_idesc, 1u, m);
                                     }
