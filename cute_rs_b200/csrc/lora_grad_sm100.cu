@@ -266,19 +266,24 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
         // the ranks, 16 bytes at once.
         const int cols = p.cols[job], columns = GRAD_M * p.halves, wide = min(columns, cols - c0), quads = p.rank / 4, items = columns * quads;
         float *out = p.out[job] + int64_t(a) * p.rank * cols;
-        for (int i = int(rank) * GRAD_THREADS + int(threadIdx.x); i < items; i += p.kc * GRAD_THREADS) {
-            const int c = job ? i / quads : i % columns, j = 4 * (job ? i % quads : i / columns);
-            if (c >= wide) continue;
-            const float4 v = cluster_sum(ring + uint32_t(c) * pitch + uint32_t(j) * 4u, p.kc);
-            if (job) {
-                float *to = out + int64_t(c0 + c) * p.rank + j;
-                if (p.vec) *reinterpret_cast<float4 *>(to) = v;
-                else to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
-            } else {
-                float *to = out + int64_t(j) * cols + c0 + c;
-                to[0] = v.x, to[cols] = v.y, to[2 * int64_t(cols)] = v.z, to[3 * int64_t(cols)] = v.w;
-            }
-        }
+        const Divider by_quads(quads);
+        const int shift = __ffs(columns) - 1;  // a power of two
+        auto column = [&](int i) { return job ? by_quads(i) : i & (columns - 1); };
+        auto first_rank = [&](int i) { return 4 * (job ? i - by_quads(i) * quads : i >> shift); };
+        cluster_sums<2>(
+            items, int(rank), p.kc, GRAD_THREADS, [&](int i) { return ring + uint32_t(column(i)) * pitch + uint32_t(first_rank(i)) * 4u; },
+            [&](int i, const float4 &v) {
+                const int c = column(i), j = first_rank(i);
+                if (c >= wide) return;
+                if (job) {
+                    float *to = out + int64_t(c0 + c) * p.rank + j;
+                    if (p.vec) *reinterpret_cast<float4 *>(to) = v;
+                    else to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+                } else {
+                    float *to = out + int64_t(j) * cols + c0 + c;
+                    to[0] = v.x, to[cols] = v.y, to[2 * int64_t(cols)] = v.z, to[3 * int64_t(cols)] = v.w;
+                }
+            });
     }
     __syncthreads();
     if (p.kc > 1) {

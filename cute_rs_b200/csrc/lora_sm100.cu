@@ -436,22 +436,26 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     if (!*abort_flag) {
         const int quads = p.bn / 4, items = p.m * quads;
         const uint32_t pitch = uint32_t(p.bn + 4) * 4u;
-        // Two places per turn: their loads from the cluster's shared memories are on their way together.
-        const int stride = p.kc * FEW_THREADS;
-        for (int i0 = int(rank) * FEW_THREADS + int(threadIdx.x); i0 < items; i0 += 2 * stride) {
-            float4 v[2], dot[2];
+        const Divider by_quads(quads);
+        constexpr int TURN = 4;
+        const int shift = __ffs(p.kc) - 1, stride = p.kc * FEW_THREADS;
+        const uint32_t dots = low + uint32_t(((p.m + p.kc - 1) >> shift) * p.rp) * 4u;
+        for (int first = int(rank) * FEW_THREADS; first < items; first += TURN * stride) {  // as in cluster_sums
+            const int i0 = first + int(threadIdx.x);
+            float4 v[TURN], dot[TURN];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int i = min(i0 + u * stride, items - 1), row = i / quads, col = (i - row * quads) * 4;
+            for (int u = 0; u < TURN; u++) {
+                if (first + u * stride >= items) continue;
+                const int i = min(i0 + u * stride, items - 1), row = by_quads(i), col = (i - row * quads) * 4;
                 v[u] = cluster_sum(ring + uint32_t(row) * pitch + uint32_t(col) * 4u, p.kc);
                 if (b_blocks == 0) {  // the dot products of this row were taken by CTA row % kc
-                    const uint32_t dots = low + uint32_t((p.m + p.kc - 1) / p.kc * p.rp + row / p.kc * p.bn + col) * 4u;
-                    dot[u] = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(dots, uint32_t(row % p.kc)) : dots);
+                    const uint32_t from = dots + uint32_t((row >> shift) * p.bn + col) * 4u;
+                    dot[u] = ptx::ld_shared_cluster_v4(p.kc > 1 ? ptx::mapa(from, uint32_t(row & (p.kc - 1))) : from);
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int i = i0 + u * stride, row = i / quads, col = (i - row * quads) * 4;
+            for (int u = 0; u < TURN; u++) {
+                const int i = i0 + u * stride, row = by_quads(i), col = (i - row * quads) * 4;
                 if (i >= items) break;
                 if (b_blocks == 0) v[u].x += dot[u].x, v[u].y += dot[u].y, v[u].z += dot[u].z, v[u].w += dot[u].w;
                 const int64_t gcol = n0 + col, out = int64_t(row) * p.ldy + gcol;

@@ -325,29 +325,22 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
     if (!*abort_flag) {
         const int quads = p.rp / 4;
         const uint32_t pitch = uint32_t(p.rp + 4) * 4u;
-        const int stride = p.kc * SHRINK_THREADS, items = min(BM, p.m - row0) * quads;
-        for (int i0 = int(rank) * SHRINK_THREADS + int(threadIdx.x); i0 < items; i0 += 2 * stride) {
-            float4 v[2];  // two places per turn: their loads are on their way together
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int i = min(i0 + u * stride, items - 1), row = i / quads, col = (i - row * quads) * 4;
-                v[u] = cluster_sum(xring + uint32_t(row) * pitch + uint32_t(col) * 4u, p.kc);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int i = i0 + u * stride, row = i / quads, col = (i - row * quads) * 4;
-                if (i >= items) break;
+        const int shift = __ffs(quads) - 1;  // a power of two, as rp is
+        cluster_sums<2>(
+            min(BM, p.m - row0) * quads, int(rank), p.kc, SHRINK_THREADS,
+            [&](int i) { return xring + uint32_t(i >> shift) * pitch + uint32_t(i & (quads - 1)) * 16u; },
+            [&](int i, const float4 &v) {
+                const int row = i >> shift, col = (i & (quads - 1)) * 4;
                 // Rows without an adapter have nothing there, and past the rank may lie another adapter's sums.
                 const float s = h.scale[row];
                 const bool has = h.id[row] >= 0 && col < p.rank;
-                const float4 w = has ? make_float4(v[u].x * s, v[u].y * s, v[u].z * s, v[u].w * s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 w = has ? make_float4(v.x * s, v.y * s, v.z * s, v.w * s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 const uint32_t h0 = pack_16(w.x, w.y, p.bf16), h1 = pack_16(w.z, w.w, p.bf16);
                 const float2 f0 = p.bf16 ? pair_f32<true>(h0) : pair_f32<false>(h0), f1 = p.bf16 ? pair_f32<true>(h1) : pair_f32<false>(h1);
                 uint16_t *t = p.t + int64_t(row0 + row) * 2 * p.rp + col;
                 *reinterpret_cast<uint2 *>(t) = make_uint2(h0, h1);
                 *reinterpret_cast<uint2 *>(t + p.rp) = make_uint2(pack_16(w.x - f0.x, w.y - f0.y, p.bf16), pack_16(w.z - f1.x, w.w - f1.y, p.bf16));
-            }
-        }
+            });
     }
     if (p.early) ptx::griddep_wait();
     __syncthreads();

@@ -56,6 +56,30 @@ __device__ __forceinline__ float4 cluster_sum(uint32_t at, int kc) {
     return v;
 }
 
+// The final sums of a cluster: out(i, sum of the CTAs' floats at at(i)) for items i of 0 .. items - 1, shared by the cluster's
+// threads.  TURN items per turn: their loads are on their way together (a turn takes some 0.8 us with any number of them).
+template <int TURN, typename At, typename Out>
+__device__ __forceinline__ void cluster_sums(int items, int rank, int kc, int threads, At at, Out out) {
+    const int stride = kc * threads;
+    for (int first = rank * threads; first < items; first += TURN * stride) {  // the same for the whole CTA
+        const int i0 = first + int(threadIdx.x);
+        float4 v[TURN];
+#pragma unroll
+        for (int u = 0; u < TURN; u++)
+            if (first + u * stride < items) v[u] = cluster_sum(at(min(i0 + u * stride, items - 1)), kc);
+#pragma unroll
+        for (int u = 0; u < TURN; u++)
+            if (i0 + u * stride < items) out(i0 + u * stride, v[u]);
+    }
+}
+
+// i / n by a product, for i * n < 2^20.
+struct Divider {
+    uint32_t factor;
+    __device__ __forceinline__ explicit Divider(int n) : factor((1u << 20) / uint32_t(n) + 1u) {}
+    __device__ __forceinline__ int operator()(int i) const { return int((uint32_t(i) * factor) >> 20); }
+};
+
 // Tensor map of a row-major 16-bit matrix of `rows` x `cols`, `pitch` elements between rows, in boxes of 64 columns
 // (one 128-byte swizzled row) by box_rows; what lies outside reads as zero.  Encoded anew for every call: it takes
 // a fraction of a microsecond on the host, and nothing is kept by an operand's address.
