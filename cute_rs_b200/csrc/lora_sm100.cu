@@ -486,6 +486,298 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
 // they are gone.
 constexpr uint32_t FEW_SMEM = 216 * 1024;
 
+// ---- one row of a rank up to 16 ---------------------------------------------------
+// T and Y by one kernel: the 16 rows of the row's A lie behind the tile's rows of W as further columns of the same MMA, so T
+// comes out of the stream that Y comes out of (every cluster computes it anew; A comes from L2 but for the first time), and
+// the adapter's part is dot products with rows of B fetched meanwhile, by the first CTA of a cluster.  A second kernel's launch
+// falls away, 2 us on the host; on the device 4096 x 4096 takes 11.3 us (11.6 by two kernels), 32000 x 2048 24.6 (26.4), 1024 x 1024
+// 6.1 (6.7), 512 x 8192 8.6 (8.4).  With more rows or ranks the stream of A costs what the launch saves (64 columns of A: 13.9
+// and 11.8).  Bound by latency, then HBM.
+//   warp 0  TMA: W, X and, once the id is there, A.   warp 1  MMA, M 128, N = bn + 16.
+//   warps 2-5  the slice of B to shared memory; then the accumulators' row.  All: T, the sums over the cluster, Y.
+// T is rounded to the sum of two 16-bit numbers, as everywhere.
+constexpr int ONE_RANK = 16;
+constexpr uint32_t ONE_HEAD = 2048;
+
+struct OneParams {
+    const int32_t *ids;
+    const float *scale;
+    const uint16_t *b;
+    uint16_t *t;
+    void *y;
+    int n, rank, adapters, c_dtype, vec;
+    int k_blocks, bn, kc, cols, stages, kps, parts;  // cols: bn + ONE_RANK
+    uint32_t stage_bytes, w_bytes, b_bytes, idesc, tmem_cols;
+    bool bf16;
+    uint32_t *status;
+    int debug;
+};
+constexpr uint32_t ONE_X_BYTES = 8 * 128;
+
+struct OneHead {
+    uint64_t full[FEW_MAX_STAGES], empty[FEW_MAX_STAGES], done, drain;
+    uint32_t tmem, abort;
+    int32_t id;  // -1 = none
+    float scale, t[ONE_RANK];
+};
+static_assert(sizeof(OneHead) <= ONE_HEAD, "head");
+
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+    lora_one_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
+                    const OneParams p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    OneHead &h = *reinterpret_cast<OneHead *>(smem_raw + (base - raw));
+    const uint32_t slice = base + ONE_HEAD, ring = slice + p.b_bytes;
+    auto bar = [&](uint64_t &b) { return ptx::smem_u32(&b); };
+    volatile uint32_t *abort_flag = &h.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = p.kc > 1 ? ptx::cluster_ctarank() : 0u;
+    const int n0 = int(blockIdx.x) / p.kc * p.bn;
+    const int kb0 = int(int64_t(p.k_blocks) * rank / p.kc), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / p.kc);
+    const int part_cols = (p.cols + 31) / 32 * 32;
+    const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            ptx::mbar_init(bar(h.full[s]), 1);
+            ptx::mbar_init(bar(h.empty[s]), 1);
+        }
+        ptx::mbar_init(bar(h.done), 1);
+        ptx::mbar_init(bar(h.drain), 1);
+        h.abort = 0u;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tmX);
+        ptx::prefetch_tensormap(&tmW);
+        ptx::prefetch_tensormap(&tmA);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), p.tmem_cols);
+        ptx::tmem_relinquish<1>();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&h.tmem);
+    ptx::griddep_wait();
+    if (threadIdx.x == 0) ptx::griddep_launch_dependents();
+
+    const uint32_t w0 = uint32_t(p.kps) * ONE_X_BYTES;
+    if (warp == 0) {
+        // Lanes 0-3 issue blocks of W, 8-11 of X, 16-19 of A (some adapter's, where the row has none: nothing reads those
+        // columns).  One instruction for all of them: a step costs 0.3 us per instruction.
+        const bool w_lane = lane < 8, a_lane = lane >= 16;
+        const int kk = lane & 7;
+        const bool mine = kk < p.kps && lane < 24;
+        const CUtensorMap *map = a_lane ? &tmA : (w_lane ? &tmW : &tmX);
+        const uint32_t to = ring + (a_lane || w_lane ? w0 + uint32_t(kk) * p.w_bytes + (a_lane ? uint32_t(p.bn) * 128u : 0u) : uint32_t(kk) * ONE_X_BYTES);
+        const int id = a_lane ? __ldcg(p.ids) : 0;
+        int y = w_lane ? n0 : 0;
+        bool ok = !(p.debug & 4);
+        int s = 0;
+        uint32_t ph = 0, filled = 0, filled_parity = 0;
+        const int steps = (kb1 - kb0 + p.kps - 1) / p.kps, early = min(2, steps);  // early: steps issued before the id is there
+        auto issue = [&](int i, int stage, bool go) {
+            const int kb = kb0 + i * p.kps + kk;
+            if (go && mine && kb < kb1) ptx::tma_load_2d(to + uint32_t(stage) * p.stage_bytes, map, bar(h.full[stage]), kb * 64, y);
+            __syncwarp();
+        };
+        for (int i = 0; i < steps && ok; i++) {
+            if (i >= p.stages) ok = __all_sync(0xffffffffu, wait_bar(bar(h.empty[s]), ph ^ 1u, abort_flag, p.status, WHERE_PRODUCER, uint32_t(s), limit));
+            if (!ok) break;
+            if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.full[s]), uint32_t(min(p.kps, kb1 - kb0 - i * p.kps)) * (ONE_X_BYTES + p.w_bytes));
+            __syncwarp();
+            issue(i, s, i >= early || !a_lane);
+            filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
+            if (++s == p.stages) s = 0, ph ^= 1u;
+            if (i + 1 == early) {  // stages 0 and 1
+                if (a_lane) y = id >= 0 && id < p.adapters ? id * p.rank : 0;
+                for (int e = 0; e < early; e++) issue(e, e, a_lane);
+            }
+        }
+        if (!ok && lane == 0) {  // giving up: let the copies in flight land (bounded)
+            const uint64_t t0 = ptx::globaltimer_ns();
+            for (int i = 0; i < p.stages; i++)
+                while ((filled >> i & 1u) && !ptx::mbar_try_wait(bar(h.full[i]), (filled_parity >> i) & 1u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const bool leader = ptx::elect_one();  // see lora_few_kernel
+        int s = 0, part = 0, part_end = kb0 + (kb1 - kb0 + p.parts - 1) / p.parts;
+        uint32_t ph = 0;
+        bool ok = true, issued = false;
+        for (int kb = kb0; kb < kb1; kb += p.kps) {
+            ok = __all_sync(0xffffffffu, wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
+            const int nk = min(p.kps, kb1 - kb);
+            for (int kk = 0; kk < nk; kk++) {
+                const uint64_t a = sw128_desc(src + uint32_t(kk) * ONE_X_BYTES), b = sw128_desc(src + w0 + uint32_t(kk) * p.w_bytes);
+                const bool next_part = kb + kk == part_end && part + 1 < p.parts;
+                if (next_part) part++, part_end = kb0 + ((kb1 - kb0) * (part + 1) + p.parts - 1) / p.parts;
+                const uint32_t more = (kb > kb0 || kk > 0) && !next_part ? 1u : 0u, d = tmem + uint32_t(part * part_cols);
+                if (leader) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) ptx::umma_f16<1>(d, a + 2u * j, b + 2u * j, p.idesc, j > 0 ? 1u : more);
+                }
+                __syncwarp();
+            }
+            issued = true;
+            if (leader) ptx::umma_commit<1>(bar(h.empty[s]));
+            __syncwarp();
+            if (++s == p.stages) s = 0, ph ^= 1u;
+        }
+        if (leader) {
+            if (ok) {
+                ptx::umma_commit<1>(bar(h.done));
+            } else if (issued) {
+                ptx::umma_commit<1>(bar(h.drain));
+                const uint64_t t0 = ptx::globaltimer_ns();
+                while (!ptx::mbar_try_wait(bar(h.drain), 0u))
+                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        const int t = threadIdx.x - 64, named = __ldcg(p.ids), id = named >= 0 && named < p.adapters ? named : -1;
+        if (t == 0) h.id = id, h.scale = id >= 0 ? __ldcg(p.scale + id) : 0.0f;
+        if (id >= 0) {  // the tile's rows of B lie one after another
+            const int pieces = min(p.bn, p.n - n0) * p.rank / 8;
+            const uint4 *src = reinterpret_cast<const uint4 *>(p.b + (int64_t(id) * p.n + n0) * p.rank);
+#pragma unroll 4
+            for (int i = t; i < pieces; i += 128) {
+                const uint4 v = __ldg(src + i);
+                ptx::st_shared_v4(slice + uint32_t(i) * 16u, v.x, v.y, v.z, v.w);
+            }
+        }
+        const bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.done), 0, abort_flag, p.status, WHERE_EPILOGUE, 0u, limit));
+        if (ok && (warp & 3) == 0) {  // the warp that may read row 0
+            ptx::tc_fence_after();
+            ptx::fence_proxy_async_shared();
+            for (int c = 0; c < p.cols; c += 16) {
+                uint32_t v[4][16];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i < p.parts) ptx::tmem_ld_32x16(tmem + uint32_t(i * part_cols + c), v[i]);
+                ptx::tmem_ld_wait_all();
+                ptx::pin16(v[0]);
+#pragma unroll
+                for (int i = 1; i < 4; i++) {
+                    if (i >= p.parts) continue;
+                    ptx::pin16(v[i]);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[0][j] = __float_as_uint(__uint_as_float(v[0][j]) + __uint_as_float(v[i][j]));
+                }
+                if (lane == 0) {
+#pragma unroll
+                    for (int g = 0; g < 4; g++) ptx::st_shared_v4(ring + uint32_t(c) * 4u + 16u * g, v[0][4 * g], v[0][4 * g + 1], v[0][4 * g + 2], v[0][4 * g + 3]);
+                }
+                __syncwarp();
+            }
+        }
+        __syncwarp();
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (p.kc > 1) {
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    const bool good = !*abort_flag;
+    if (good && rank == 0 && threadIdx.x < ONE_RANK / 4) {  // T; the first cluster stores it
+        const int j = 4 * int(threadIdx.x);
+        const float4 v = cluster_sum(ring + uint32_t(p.bn + j) * 4u, p.kc);
+        const float s = h.scale;
+        const bool has = h.id >= 0 && j < p.rank;  // past the rank may lie another adapter's sums
+        const float4 w = has ? make_float4(v.x * s, v.y * s, v.z * s, v.w * s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const uint32_t h0 = pack_16(w.x, w.y, p.bf16), h1 = pack_16(w.z, w.w, p.bf16);
+        const float2 f0 = p.bf16 ? pair_f32<true>(h0) : pair_f32<false>(h0), f1 = p.bf16 ? pair_f32<true>(h1) : pair_f32<false>(h1);
+        const uint32_t l0 = pack_16(w.x - f0.x, w.y - f0.y, p.bf16), l1 = pack_16(w.z - f1.x, w.w - f1.y, p.bf16);
+        const float2 g0 = p.bf16 ? pair_f32<true>(l0) : pair_f32<false>(l0), g1 = p.bf16 ? pair_f32<true>(l1) : pair_f32<false>(l1);
+        h.t[j] = f0.x + g0.x, h.t[j + 1] = f0.y + g0.y, h.t[j + 2] = f1.x + g1.x, h.t[j + 3] = f1.y + g1.y;
+        if (blockIdx.x == 0) {
+            *reinterpret_cast<uint2 *>(p.t + j) = make_uint2(h0, h1);
+            *reinterpret_cast<uint2 *>(p.t + ONE_RANK + j) = make_uint2(l0, l1);
+        }
+    }
+    __syncthreads();
+    const int i = int(threadIdx.x);  // four columns; bn / 4 is less than the CTA's threads
+    if (good && rank == 0 && i < p.bn / 4) {
+        const float4 v = cluster_sum(ring + uint32_t(i) * 16u, p.kc);
+        float f[4] = {v.x, v.y, v.z, v.w};
+        const int gcol = n0 + 4 * i;
+        if (h.id >= 0) {
+            const uint4 *b = reinterpret_cast<const uint4 *>(smem_raw + (slice - raw)) + 4 * i * p.rank / 8;
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                float dot = 0.0f;
+                for (int j = 0; j < p.rank; j += 8) {
+                    const uint4 q = b[(c * p.rank + j) / 8];
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float2 x = p.bf16 ? pair_f32<true>(w[e]) : pair_f32<false>(w[e]);
+                        dot = fmaf(x.y, h.t[j + 2 * e + 1], fmaf(x.x, h.t[j + 2 * e], dot));
+                    }
+                }
+                f[c] += dot;
+            }
+        }
+        if (p.vec && gcol + 4 <= p.n) {
+            if (p.c_dtype == CUTE_B200_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.y) + gcol) = make_float4(f[0], f[1], f[2], f[3]);
+            else {
+                const bool bf16 = p.c_dtype == CUTE_B200_BF16;
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.y) + gcol) = make_uint2(pack_16(f[0], f[1], bf16), pack_16(f[2], f[3], bf16));
+            }
+        } else {
+            for (int c = 0; c < 4; c++)
+                if (gcol + c < p.n) store_c(p.y, p.c_dtype, size_t(gcol + c), f[c]);
+        }
+    }
+    __syncthreads();
+    if (p.kc > 1) {  // until every CTA has read its peers' shared memory
+        ptx::cluster_arrive();
+        ptx::cluster_wait();
+    }
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, p.tmem_cols);
+}
+
+cute_b200_status forward_one(const LoraParams &p, bool bf16, const DeviceState &dev, int debug, cudaStream_t stream) {
+    OneParams f = {};
+    f.ids = p.ids, f.scale = p.scale, f.b = p.b, f.t = p.t, f.y = p.y;
+    f.n = p.n, f.rank = p.rank, f.adapters = p.adapters, f.c_dtype = p.c_dtype;
+    f.vec = reinterpret_cast<uint64_t>(p.y) % (p.c_dtype == CUTE_B200_F32 ? 16 : 8) == 0;
+    f.k_blocks = (p.k + 63) / 64;
+    f.bn = 16, f.kc = 1;
+    stream_cut(p.n, f.k_blocks, dev.few_clusters, &f.bn, &f.kc, ONE_RANK);
+    f.cols = f.bn + ONE_RANK;
+    f.w_bytes = uint32_t(f.cols) * 128u;
+    f.b_bytes = (uint32_t(f.bn * p.rank) * 2u + 1023u) / 1024u * 1024u;
+    // The head, B, the ring, and behind the last stage as much as an MMA reads past its rows of X.
+    const uint32_t ring = FEW_SMEM - ONE_HEAD - 1024 - f.b_bytes;
+    f.kps = stream_blocks(f.cols, 8, ring, 320);
+    f.stage_bytes = uint32_t(f.kps) * (ONE_X_BYTES + f.w_bytes);
+    const uint32_t reach = uint32_t(f.kps - 1) * ONE_X_BYTES + 16384, over = f.stage_bytes < reach ? reach - f.stage_bytes : 0;
+    f.stages = int((ring - over) / f.stage_bytes);
+    if (f.stages > FEW_MAX_STAGES) f.stages = FEW_MAX_STAGES;
+    f.idesc = make_idesc(bf16, 128, f.cols);
+    f.parts = f.cols <= 128 ? 4 : 2;  // accumulators added in f32: see T_PARTS of the tiled kernels
+    while (f.parts > f.k_blocks / f.kc && f.parts > 1) f.parts /= 2;
+    for (f.tmem_cols = 32; f.tmem_cols < uint32_t(f.parts * ((f.cols + 31) / 32 * 32)); f.tmem_cols *= 2) {}
+    f.bf16 = bf16;
+    f.status = dev.status_word;
+    f.debug = debug;
+    CUtensorMap tmX, tmW, tmA;
+    CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), bf16, p.m, p.k, p.ldx, 8));
+    CB_TRY(rows_tensor_map(&tmW, reinterpret_cast<uint64_t>(p.w), bf16, p.n, p.k, p.k, f.bn));
+    CB_TRY(rows_tensor_map(&tmA, reinterpret_cast<uint64_t>(p.a), bf16, uint64_t(p.adapters) * p.rank, p.k, p.k, ONE_RANK));
+    const unsigned grid = unsigned((p.n + f.bn - 1) / f.bn) * unsigned(f.kc);
+    return launch_dependent(lora_one_kernel, dim3(grid), FEW_THREADS, FEW_SMEM, f.kc, stream, tmX, tmW, tmA, f);
+}
+
 // How the few-row kernels would run a problem, and in what time.  The terms are fitted to measurements of both ways (graphs of
 // 60 calls, us, few / tiled; rows with one of a adapters each):
 //   n 4096 k 4096 rank 16 a 64: 8 rows 12 / 24, 64 rows 18 / 41, 128 rows 24 / 51
@@ -618,6 +910,7 @@ uint64_t elem_bytes(int dtype) { return dtype == CUTE_B200_F32 ? 4 : 2; }
 cute_b200_status forward(const LoraParams &p, bool bf16, const int32_t (&tuning)[2], const DeviceState &dev, cudaStream_t stream) {
     if (p.m == 0) return CUTE_B200_OK;
     if (tuning[0] == 1 || (tuning[0] == 0 && p.m <= FEW_ROWS)) {
+        if (p.m == 1 && p.rp == ONE_RANK) return forward_one(p, bf16, dev, tuning[1], stream);
         const FewPlan plan = few_plan(p, dev);
         if (tuning[0] == 1 || plan.time <= tiled_time(p, dev))
             return bf16 ? forward_few<true>(p, plan, dev, tuning[1], stream) : forward_few<false>(p, plan, dev, tuning[1], stream);
@@ -733,6 +1026,7 @@ cute_b200_status lora_tn_backward(const cute_b200_lora_desc &d, const uint64_t p
 
 cute_b200_status lora_init(DeviceState &dev) {
     CB_CUDA(cudaFuncSetAttribute(lora_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
+    CB_CUDA(cudaFuncSetAttribute(lora_one_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
     for (int c = 0; c < 4; c++) CB_TRY(max_clusters(lora_few_kernel, FEW_THREADS, FEW_SMEM, 1 << c, &dev.few_clusters[c]));
     CB_TRY(lora_tiled_init(dev));
     CB_TRY(lora_grad_init());

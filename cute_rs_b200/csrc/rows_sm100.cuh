@@ -169,10 +169,10 @@ cute_b200_status max_clusters(void (*kernel)(P...), int threads, size_t smem, in
     return CUTE_B200_OK;
 }
 
-// k blocks per ring stage of a product that streams `bn` rows of a weight past `rows` rows: about 28 KB of the weight, but at
-// least four stages in a ring of `ring` bytes.
-inline int stream_blocks(int bn, int rows, uint32_t ring) {
-    int blocks = bn >= 160 ? 1 : (bn >= 80 ? 2 : 4);
+// k blocks per ring stage of a product that streams `bn` rows of a weight past `rows` rows: 10 to 40 KB of the weight (more or
+// less with another `wide`, the rows that make a stage alone), but at least four stages in a ring of `ring` bytes.
+inline int stream_blocks(int bn, int rows, uint32_t ring, int wide = 160) {
+    int blocks = bn >= wide ? 1 : (2 * bn >= wide ? 2 : 4);
     while (blocks > 1 && ring / (uint32_t(blocks * (rows + bn)) * 128u) < 4) blocks /= 2;
     return blocks;
 }
@@ -180,17 +180,19 @@ inline int stream_blocks(int bn, int rows, uint32_t ring) {
 // How a product that streams an (n, k) weight past a few rows is cut: bn rows of the weight per tile, a cluster of kc CTAs per tile.  The launch is one wave
 // where it can be; the cut with the least time for the slowest CTA wins.  A CTA streams at most what an even share of
 // HBM gives it, and no faster than its MMAs are issued (per k block four of 65 clocks or bn / 2 each, and some 80 of loop).
-inline void stream_cut(int n, int k_blocks, const int (&max_clusters)[4], int *bn, int *kc) {
+// `more`: rows of another matrix that every tile streams beside its own.
+inline void stream_cut(int n, int k_blocks, const int (&max_clusters)[4], int *bn, int *kc, int more = 0) {
     double best = 1e300;
     for (int c = 0; c < 4; c++) {
         const int parts = 1 << c, ctas_at_once = max_clusters[c] * parts;
         if (parts > k_blocks || max_clusters[c] < 1) continue;
-        for (int b = 16; b <= 256; b += 16) {
+        for (int b = 16; b + more <= 256; b += 16) {
             const int64_t ctas = int64_t((n + b - 1) / b) * parts;
             const int64_t waves = (ctas + ctas_at_once - 1) / ctas_at_once;
             const double share = 6.5e12 / double(ctas < ctas_at_once ? ctas : ctas_at_once);
             const double rate = share < 7.0e10 ? share : 7.0e10;
-            const double load = b * 128.0 / rate, math = (4.0 * (b / 2 > 65 ? b / 2 : 65) + 80.0) / 1.8e9;
+            const int cols = b + more;
+            const double load = cols * 128.0 / rate, math = (4.0 * (cols / 2 > 65 ? cols / 2 : 65) + 80.0) / 1.8e9;
             const double t = double(waves) * (((k_blocks + parts - 1) / parts) * (load > math ? load : math) + 2.0e-6) + (parts > 1 ? 1.0e-6 : 0.0);
             if (t < best * 0.999) best = t, *bn = b, *kc = parts;
         }

@@ -199,6 +199,17 @@ def test_lora_ids_outside_the_table_mean_none(lib, gpu, m):
     p.check_back(*p.back())
 
 
+@pytest.mark.parametrize("ab,c", [(BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("rank", [8, 16, 24])
+@pytest.mark.parametrize("n,k", [(4104, 4104), (40, 64), (20000, 520), (8, 8)])
+def test_lora_of_a_single_row(lib, gpu, n, k, rank, ab, c):
+    for id in (0, 4, -1, 5):
+        p = Lora(lib, 1, n, k, rank, 5, ab, c, torch.tensor([id]), seed=id + 1)
+        p.a[2], p.b[3] = float("nan"), float("inf")  # adapters that the row does not name
+        p.check(p.run())
+        p.check_back(*p.back())
+
+
 @pytest.mark.parametrize("m", [3, 100, 128, 1000])
 def test_lora_rows_do_not_touch_one_another(lib, gpu, m):
     # Infinities and NaNs in a row, or in another row's adapter, stay there: every other row has the same bits as without.
@@ -572,14 +583,16 @@ def test_moe_on_two_streams_at_once(lib, gpu):
 def test_waits_that_run_out_are_reported(lib, gpu):
     """The producers issue nothing (a test knob): every wait gives up after 20 ms, the kernels return, the report names it,
     and the next call on the same device is right."""
+    one = Lora(lib, 1, 264, 520, 16, 6, BF16, F32)
     few, tiled, moe = Lora(lib, 20, 264, 136, 72, 6, BF16, F32), Lora(lib, 700, 264, 136, 16, 6, BF16, F32), Moe(lib, 12, 24, 4, 256, 136, BF16)
-    calls = [lambda: few.run((1, 12))] + [lambda c=c: tiled.run((c, 12)) for c in (3, 4, 5, 6)] + [lambda: moe.run(tuning=12)]
+    calls = [lambda: one.run((1, 12)), lambda: few.run((1, 12))] + [lambda c=c: tiled.run((c, 12)) for c in (3, 4, 5, 6)] + [lambda: moe.run(tuning=12)]
     for call in calls:
         call()
         with pytest.raises(lib.CuteB200Error) as e:
             lib.synchronize()
         assert e.value.status == lib.ERR_DEVICE_TIMEOUT
         assert lib.device_status() == (0, 0, 0, 0)
+    one.check(one.run())
     few.check(few.run())
     tiled.check(tiled.run())
     d = tiled.desc((0, 12))
