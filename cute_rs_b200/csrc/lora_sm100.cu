@@ -375,9 +375,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
         __syncwarp();
     } else {
-        // The adapters the rows name, in the order of their first row.
+        // The adapters the rows name, in the order of their first row.  The ids, like W, are older than the kernel that
+        // computes T.
         const int row = threadIdx.x - 64;
-        ptx::griddep_wait();
         int id = row < p.m ? p.ids[row] : -1;
         if (id < 0 || id >= p.adapters) id = -1;
         h.id[row] = id;
@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
         ptx::named_barrier(1, 128);
         if (row == 0) ptx::mbar_arrive(bar(h.plan));
+        ptx::griddep_wait();
         if (b_blocks == 0) {
             float *t = reinterpret_cast<float *>(smem_raw + (low - raw)), *dots = t + (p.m + p.kc - 1) / p.kc * p.rp;
             if (p.bf16) few_dots<true>(p, h.id, t, dots, int(rank), n0, row);
