@@ -180,6 +180,15 @@ def test_lora_integers_are_exact(lib, gpu, m, n, k, rank, adapters, ids):
         assert torch.equal(p.run(tuning)[:m].double(), want)
 
 
+@pytest.mark.parametrize("ab,c", [(BF16, F16), (F16, BF16)])
+@pytest.mark.parametrize("m", [1, 20, 200])
+def test_lora_result_in_the_other_16_bit_type(lib, gpu, m, ab, c):
+    p = Lora(lib, m, 264, 520, 16, 5, ab, c)
+    for tuning in variants(m):
+        p.check(p.run(tuning))
+    p.check_back(*p.back())
+
+
 def test_lora_no_rows(lib, gpu):
     p = Lora(lib, 0, 64, 64, 16, 2, BF16, BF16)
     assert (p.run() == 7).all()
@@ -332,7 +341,7 @@ def test_gradients_against_differences(lib, gpu):
 
 
 def test_lora_captured_and_replayed_with_other_rows(lib, gpu):
-    for m in (24, 300):
+    for m in (1, 24, 300):
         p, q = (Lora(lib, m, 264, 136, 16, 6, BF16, F32, seed=s) for s in (1, 2))
         d = p.desc()
         y, work = torch.zeros(m, p.n, device="cuda"), p.workspace(lib.lora_workspace(d))
@@ -361,12 +370,12 @@ def test_lora_captured_and_replayed_with_other_rows(lib, gpu):
             assert torch.equal(y, want) and torch.equal(y2, want)
 
 
-def test_lora_on_two_streams_at_once(lib, gpu):
-    ps = [Lora(lib, 40 + 300 * i, 520, 264, 16, 6, BF16, F32, seed=i) for i in range(2)]
+def test_lora_on_several_streams_at_once(lib, gpu):
+    ps = [Lora(lib, m, 520, 264, 16, 6, BF16, F32, seed=i) for i, m in enumerate((40, 340, 1))]
     want = [p.run() for p in ps]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in ps]
-    got = [[], []]
+    got = [[] for _ in ps]
     for _ in range(20):
         for i, (p, s) in enumerate(zip(ps, streams)):
             with torch.cuda.stream(s):
