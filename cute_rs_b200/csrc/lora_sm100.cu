@@ -150,55 +150,76 @@ __device__ __forceinline__ int low_blocks(int entries, int rank, int kc, int b_b
 }
 
 // The adapters' part of columns n0.. of Y for rows rank, rank + kc, .. (row r of `t` and `out` is row rank + r kc of Y), by
-// 128 threads; id[row] < 0 = no adapter.  V: 16-byte pieces of a row of B; R: rows whose B is fetched at once, so that
-// eight or more loads are on their way (one row at a time took 0.7 us each, the latency of its loads).
-template <bool BF16, int V, int R>
-__device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, const float *t, float *out, int rank, int rows, int n0, int thread) {
-    for (int c = thread; c < p.bn && n0 + c < p.n; c += 128)
-        for (int r0 = 0; r0 < rows; r0 += R) {
-            uint4 b[R][V];
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                const int a = r0 + r < rows ? id[rank + (r0 + r) * p.kc] : -1;
-                const uint4 *src = reinterpret_cast<const uint4 *>(p.b + (int64_t(a) * p.n + n0 + c) * p.rank);
-#pragma unroll
-                for (int v = 0; v < V; v++) b[r][v] = a >= 0 ? __ldg(src + v) : make_uint4(0u, 0u, 0u, 0u);
-            }
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                if (r0 + r >= rows) break;
-                const float *tv = t + (r0 + r) * p.rp;  // zeros where the row has no adapter
-                float sum = 0.0f;
-#pragma unroll
-                for (int v = 0; v < V; v++) {
-                    const uint32_t w[4] = {b[r][v].x, b[r][v].y, b[r][v].z, b[r][v].w};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float2 f = pair_f32<BF16>(w[i]);
-                        sum = fmaf(f.y, tv[8 * v + 2 * i + 1], fmaf(f.x, tv[8 * v + 2 * i], sum));
-                    }
-                }
-                out[(r0 + r) * p.bn + c] = sum;
-            }
-        }
-}
-
-template <bool BF16>
+// 128 threads; id[row] < 0 = no adapter.  V: 16-byte pieces of a row of B; R: rows of a batch, whose B is fetched at once.
+// Of ranks up to 16 two batches are on their way (one row at a time took 0.7 us each, the latency of its loads; a batch at a
+// time, behind W's stream, 2.5), the first two while T is still being computed: 48 rows of 64 adapters, 8192 x 4096, rank 16:
+// 21.2 us, 22.1 a batch at a time; of higher ranks their traffic holds T up (16 rows, rank 32, 11008 x 4096: 25.4 us, 22.7 a batch at
+// a time).
+template <bool BF16, int V, int R, int AHEAD>
 __device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, float *t, float *out, int rank, int n0, int thread) {
-    const int rows = (p.m - rank + p.kc - 1) / p.kc;
+    const int rows = (p.m - rank + p.kc - 1) / p.kc, cols = min(p.bn, p.n - n0), groups = (rows + R - 1) / R, batches = groups * ((cols + 127) / 128);
+    uint4 b[AHEAD][R][V];
+    auto load = [&](int q, uint4 (&to)[R][V]) {
+        const int pass = q / groups, r0 = (q - pass * groups) * R, c = 128 * pass + thread;
+        if (c >= cols) return;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int a = r0 + r < rows ? id[rank + (r0 + r) * p.kc] : -1;
+            const uint4 *src = reinterpret_cast<const uint4 *>(p.b + (int64_t(a) * p.n + n0 + c) * p.rank);
+#pragma unroll
+            for (int v = 0; v < V; v++) to[r][v] = a >= 0 ? __ldg(src + v) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    auto multiply = [&](int q, const uint4 (&from)[R][V]) {
+        const int pass = q / groups, r0 = (q - pass * groups) * R, c = 128 * pass + thread;
+        if (c >= cols) return;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if (r0 + r >= rows) break;
+            const float *tv = t + (r0 + r) * p.rp;  // zeros where the row has no adapter
+            float sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const uint32_t w[4] = {from[r][v].x, from[r][v].y, from[r][v].z, from[r][v].w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 f = pair_f32<BF16>(w[i]);
+                    sum = fmaf(f.y, tv[8 * v + 2 * i + 1], fmaf(f.x, tv[8 * v + 2 * i], sum));
+                }
+            }
+            out[(r0 + r) * p.bn + c] = sum;
+        }
+    };
+    if (AHEAD == 2 && batches > 0) load(0, b[0]);
+    if (AHEAD == 2 && batches > 1) load(1, b[1]);
+    ptx::griddep_wait();
     for (int i = thread; i < rows * p.rp; i += 128) {
         const int r = i / p.rp, j = i - r * p.rp;
         const uint16_t *src = p.t + int64_t(rank + r * p.kc) * 2 * p.rp + j;
         t[i] = id[rank + r * p.kc] >= 0 ? to_f32<BF16>(src[0]) + to_f32<BF16>(src[p.rp]) : 0.0f;
     }
     ptx::named_barrier(1, 128);
-    if (p.rank == 8) few_dots<BF16, 1, 8>(p, id, t, out, rank, rows, n0, thread);
-    else if (p.rank == 16) few_dots<BF16, 2, 8>(p, id, t, out, rank, rows, n0, thread);
-    else if (p.rank == 24) few_dots<BF16, 3, 4>(p, id, t, out, rank, rows, n0, thread);
-    else few_dots<BF16, 4, 4>(p, id, t, out, rank, rows, n0, thread);
+    for (int q = 0; q < batches; q += AHEAD) {
+        if constexpr (AHEAD == 1) load(q, b[0]);
+        multiply(q, b[0]);
+        if constexpr (AHEAD == 2) {
+            if (q + 2 < batches) load(q + 2, b[0]);
+            if (q + 1 < batches) multiply(q + 1, b[1]);
+            if (q + 3 < batches) load(q + 3, b[1]);
+        }
+    }
 }
 
-__global__ void __launch_bounds__(FEW_THREADS, 1)
+template <bool BF16>
+__device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, float *t, float *out, int rank, int n0, int thread) {
+    if (p.rank == 8) few_dots<BF16, 1, 8, 2>(p, id, t, out, rank, n0, thread);
+    else if (p.rank == 16) few_dots<BF16, 2, 8, 2>(p, id, t, out, rank, n0, thread);
+    else if (p.rank == 24) few_dots<BF16, 3, 4, 1>(p, id, t, out, rank, n0, thread);
+    else few_dots<BF16, 4, 4, 1>(p, id, t, out, rank, n0, thread);
+}
+
+// 168 registers at most (what two CTAs per SM would allow; shared memory holds one), so that a CTA fits beside one of T's kernel.
+__global__ void __launch_bounds__(FEW_THREADS, 2)
     lora_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmT,
                     const __grid_constant__ CUtensorMap tmB, const FewParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -391,11 +412,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
         ptx::named_barrier(1, 128);
         if (row == 0) ptx::mbar_arrive(bar(h.plan));
-        ptx::griddep_wait();
         if (b_blocks == 0) {
             float *t = reinterpret_cast<float *>(smem_raw + (low - raw)), *dots = t + (p.m + p.kc - 1) / p.kc * p.rp;
             if (p.bf16) few_dots<true>(p, h.id, t, dots, int(rank), n0, row);
             else few_dots<false>(p, h.id, t, dots, int(rank), n0, row);
+        } else {
+            ptx::griddep_wait();
         }
 
         // The accumulator's rows to shared memory (the ring is idle: every load has been consumed).
