@@ -803,10 +803,10 @@ cute_b200_status forward_one(const LoraParams &p, bool bf16, const DeviceState &
 
 // How the few-row kernels would run a problem, and in what time.  The terms are fitted to measurements of both ways (graphs of
 // 60 calls, us, few / tiled; rows with one of a adapters each):
-//   n 4096 k 4096 rank 16 a 64: 8 rows 12 / 24, 64 rows 18 / 41, 128 rows 24 / 51
-//   n 8192 k 4096 rank 16 a 4: 8 rows 18 / 32, 32 rows 20 / 22, 64 rows 23 / 23, 128 rows 28 / 23
-//   n 16384 k 2048 rank 32 a 8: 8 rows 17 / 22, 32 rows 21 / 18, 128 rows 29 / 19
-//   n 1000 k 8192 rank 128 a 4: 8 rows 14 / 32, 128 rows 29 / 34
+//   n 4096 k 4096 rank 16 a 64: 8 rows 12 / 22, 64 rows 17 / 39, 128 rows 22 / 49
+//   n 8192 k 4096 rank 16 a 4: 8 rows 17 / 33, 32 rows 19 / 22, 64 rows 23 / 23, 128 rows 26 / 23
+//   n 16384 k 2048 rank 32 a 8: 8 rows 17 / 25, 32 rows 20 / 19, 128 rows 28 / 19
+//   n 1000 k 8192 rank 128 a 4: 8 rows 15 / 33, 128 rows 30 / 35
 // The tiled kernels read every adapter's weights tile by tile and do not cut k; the few-row kernels pay for every row: its
 // part of X per k block, its dot products (or its adapter's masked product), its place in the final sum.
 struct FewPlan {
