@@ -2,7 +2,8 @@
 //     dA[a] = sum over rows i of adapter a of U[i] x[i]^T        (rank, k)
 //     dB[a] = sum over rows i of adapter a of dY[i] T[i]^T       (n, rank)
 // Both are products over the rows of one adapter of a wide matrix V (X or dY)
-// with a narrow one L (U or T, each value the sum of two 16-bit numbers).
+// with a narrow one L (U or T, each value the sum of two 16-bit numbers, of
+// which f16's second is scaled, see store_t).
 //
 // A row list per adapter comes first (rows in ascending order).  Then one CTA
 // takes 128 columns of V for one adapter: M = the columns, N = the 2 rp columns
@@ -82,6 +83,8 @@ struct GradParams {
     const int32_t *first, *list;
     int cols[2], tiles[2], m, rank, rp, halves, kc, stages, vec;
     uint32_t stage_bytes, idesc, tmem_cols;
+    int low_col;      // of L: where the two planes begin
+    float low_scale;  // of the second plane's sums
     uint32_t *status;
     int debug;
 };
@@ -164,12 +167,12 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
             __syncwarp();
             if (run) {  // a lane per box
                 if (lane < wide_boxes) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.wide[job], full, c0 + 64 * lane, first_row);
-                else if (lane < wide_boxes + low_boxes) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.low[job], full, 64 * (lane - wide_boxes), first_row);
+                else if (lane < wide_boxes + low_boxes) ptx::tma_load_2d(dst + lane * GRAD_BOX, &maps.low[job], full, p.low_col + 64 * (lane - wide_boxes), first_row);
             } else if (lane < 16) {
                 for (int x = 0; x < wide_boxes; x++)
                     ptx::tma_gather4(dst + x * GRAD_BOX + 512u * lane, &maps.wide_rows[job], full, c0 + 64 * x, row[0], row[1], row[2], row[3]);
                 for (int x = 0; x < low_boxes; x++)
-                    ptx::tma_gather4(dst + (wide_boxes + x) * GRAD_BOX + 512u * lane, &maps.low_rows[job], full, 64 * x, row[0], row[1], row[2], row[3]);
+                    ptx::tma_gather4(dst + (wide_boxes + x) * GRAD_BOX + 512u * lane, &maps.low_rows[job], full, p.low_col + 64 * x, row[0], row[1], row[2], row[3]);
             }
             __syncwarp();
             filled |= 1u << s, filled_parity = (filled_parity & ~(1u << s)) | (ph << s);
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
                     ptx::pin16(hi);
                     ptx::pin16(lo);
 #pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] = __uint_as_float(hi[j]) + __uint_as_float(lo[j]);
+                    for (int j = 0; j < 16; j++) v[j] = fmaf(__uint_as_float(lo[j]), p.low_scale, __uint_as_float(hi[j]));
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; j++) v[j] = 0.0f;
@@ -302,6 +305,7 @@ cute_b200_status lora_row_lists(const int32_t *ids, int m, int adapters, int32_t
 cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const DeviceState &dev, cudaStream_t stream) {
     GradParams p = {};
     GradMaps maps;
+    const int low_cols = t_planes(bf16) * g.rp;
     for (int i = 0; i < 2; i++) {
         p.out[i] = g.out[i];
         p.cols[i] = g.cols[i];
@@ -309,8 +313,8 @@ cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const Devi
         const uint64_t wide = reinterpret_cast<uint64_t>(g.wide[i]), low = reinterpret_cast<uint64_t>(g.low[i]);
         CB_TRY(rows_tensor_map(&maps.wide[i], wide, bf16, g.m, g.cols[i], g.pitch[i], GRAD_ROWS));
         CB_TRY(rows_tensor_map(&maps.wide_rows[i], wide, bf16, g.m, g.cols[i], g.pitch[i], 1));
-        CB_TRY(rows_tensor_map(&maps.low[i], low, bf16, g.m, 2 * g.rp, 2 * g.rp, GRAD_ROWS));
-        CB_TRY(rows_tensor_map(&maps.low_rows[i], low, bf16, g.m, 2 * g.rp, 2 * g.rp, 1));
+        CB_TRY(rows_tensor_map(&maps.low[i], low, bf16, g.m, low_cols, low_cols, GRAD_ROWS));
+        CB_TRY(rows_tensor_map(&maps.low_rows[i], low, bf16, g.m, low_cols, low_cols, 1));
     }
     p.first = g.first, p.list = g.list;
     p.vec = reinterpret_cast<uint64_t>(g.out[1]) % 16 == 0;
@@ -320,6 +324,8 @@ cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const Devi
     if (p.stages > GRAD_STAGES) p.stages = GRAD_STAGES;
     p.idesc = make_idesc(bf16, GRAD_M, 2 * g.rp) | IDESC_A_MN | IDESC_B_MN;
     p.tmem_cols = uint32_t(2 * g.rp * p.halves);
+    p.low_col = t_hi(g.rp, bf16);
+    p.low_scale = bf16 ? 1.0f : 1.0f / LOW_SCALE;
     p.status = dev.status_word;
     p.debug = debug;
     // The rows of a tile are shared by a cluster of kc CTAs: the least time for whole waves of CTAs, each the blocks of an

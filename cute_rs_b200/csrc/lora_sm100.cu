@@ -1,9 +1,9 @@
 // A projection shared by all rows with a low-rank adapter chosen row by row:
 //     y[i] = W x[i] + scale[a] * B[a] (A[a] x[i]),   a = ids[i]
 // and its gradients.  The inner product T[i] = scale[a] * A[a] x[i] (`rank`
-// values per row) goes to the workspace as two 16-bit numbers per value, their
-// sum: the second product can then run on 16-bit operands and still carry 16
-// (bf16) or 22 (f16) bits of T.
+// values per row) goes to the workspace as 16-bit numbers whose sum is the
+// value (store_t): the second product can then run on 16-bit operands and still
+// carry 16 (bf16) or 22 (f16, but no finer than 2^-25) bits of T.
 #include "lora_sm100.cuh"
 
 namespace cb {
@@ -85,10 +85,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS) shrink_rows_kernel(const LoraP
         float sum = 0.0f;
         for (int w = 0; w < SHRINK_THREADS / 32; w++) sum += part[w][tid];
         sum = live ? sum * scale : 0.0f;
-        const uint16_t hi = from_f32<BF16>(sum);
-        uint16_t *t = p.t + int64_t(rows[tid / J]) * 2 * p.rp + j0 + tid % J;
-        t[0] = hi;
-        t[p.rp] = from_f32<BF16>(sum - to_f32<BF16>(hi));
+        store_t<BF16>(p.t + int64_t(rows[tid / J]) * t_planes(BF16) * p.rp + j0 + tid % J, p.rp, sum);
     }
 }
 
@@ -195,7 +192,7 @@ __device__ __forceinline__ void few_dots(const FewParams &p, const int32_t *id, 
     ptx::griddep_wait();
     for (int i = thread; i < rows * p.rp; i += 128) {
         const int r = i / p.rp, j = i - r * p.rp;
-        const uint16_t *src = p.t + int64_t(rank + r * p.kc) * 2 * p.rp + j;
+        const uint16_t *src = p.t + int64_t(rank + r * p.kc) * t_planes(BF16) * p.rp + j;
         t[i] = id[rank + r * p.kc] >= 0 ? to_f32<BF16>(src[0]) + to_f32<BF16>(src[p.rp]) : 0.0f;
     }
     ptx::named_barrier(1, 128);
@@ -302,7 +299,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
         if (has_low) {
             if (lane == 0) ptx::mbar_arrive_expect_tx(bar(h.low), uint32_t(t_blocks) * p.x_bytes);
             __syncwarp();
-            if (lane < t_blocks) ptx::tma_load_2d(low + uint32_t(lane) * p.x_bytes, &tmT, bar(h.low), ext_block(lane, p.rp, p.rank, whole).t_col, 0);
+            if (lane < t_blocks) ptx::tma_load_2d(low + uint32_t(lane) * p.x_bytes, &tmT, bar(h.low), ext_block(lane, p.rp, p.rank, whole, p.bf16).t_col, 0);
         }
         for (int i = 0; i < mine && ok; i += p.kps) {
             const int nk = min(p.kps, mine - i);
@@ -375,7 +372,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2)
                 // The blocks of T that go with this block of B.
                 const int parts = t_blocks / b_blocks;
                 for (int part = 0; part < parts; part++) {
-                    const ExtBlock x = ext_block(parts * q + part, p.rp, p.rank, whole);
+                    const ExtBlock x = ext_block(parts * q + part, p.rp, p.rank, whole, p.bf16);
                     const uint64_t a = sw128_desc(low + uint32_t(parts * q + part) * p.x_bytes);
                     if (leader)
                         for (int j = 0; j < x.steps; j++) ptx::umma_f16_lanes(tmem, a + 2u * j, b + 2u * (j & x.b_mask), p.idesc, 1u, o0, o1, o2, o3);
@@ -716,15 +713,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         const float s = h.scale;
         const bool has = h.id >= 0 && j < p.rank;  // past the rank may lie another adapter's sums
         const float4 w = has ? make_float4(v.x * s, v.y * s, v.z * s, v.w * s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const uint32_t h0 = pack_16(w.x, w.y, p.bf16), h1 = pack_16(w.z, w.w, p.bf16);
-        const float2 f0 = p.bf16 ? pair_f32<true>(h0) : pair_f32<false>(h0), f1 = p.bf16 ? pair_f32<true>(h1) : pair_f32<false>(h1);
-        const uint32_t l0 = pack_16(w.x - f0.x, w.y - f0.y, p.bf16), l1 = pack_16(w.z - f1.x, w.w - f1.y, p.bf16);
-        const float2 g0 = p.bf16 ? pair_f32<true>(l0) : pair_f32<false>(l0), g1 = p.bf16 ? pair_f32<true>(l1) : pair_f32<false>(l1);
-        h.t[j] = f0.x + g0.x, h.t[j + 1] = f0.y + g0.y, h.t[j + 2] = f1.x + g1.x, h.t[j + 3] = f1.y + g1.y;
-        if (blockIdx.x == 0) {
-            *reinterpret_cast<uint2 *>(p.t + j) = make_uint2(h0, h1);
-            *reinterpret_cast<uint2 *>(p.t + ONE_RANK + j) = make_uint2(l0, l1);
-        }
+        const float4 t = store_t4(p.t + j, ONE_RANK, w, p.bf16, blockIdx.x == 0);
+        h.t[j] = t.x, h.t[j + 1] = t.y, h.t[j + 2] = t.z, h.t[j + 3] = t.w;
     }
     __syncthreads();
     const int i = int(threadIdx.x);  // four columns; bn / 4 is less than the CTA's threads
@@ -871,7 +861,7 @@ cute_b200_status forward_few(const LoraParams &p, const FewPlan &plan, const Dev
     CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), BF16, p.m, p.k, p.ldx, f.xr));
     CB_TRY(rows_tensor_map(&tmW, reinterpret_cast<uint64_t>(p.w), BF16, p.n, p.k, p.k, f.bn));
     if (f.b_blocks > 0) {
-        CB_TRY(rows_tensor_map(&tmT, reinterpret_cast<uint64_t>(p.t), BF16, p.m, 2 * p.rp, 2 * p.rp, f.xr));
+        CB_TRY(rows_tensor_map(&tmT, reinterpret_cast<uint64_t>(p.t), BF16, p.m, t_planes(BF16) * p.rp, t_planes(BF16) * p.rp, f.xr));
         CB_TRY(rows_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), BF16, uint64_t(p.adapters) * p.n, p.rank, p.rank, f.bn));
     }
     const unsigned grid = unsigned((p.n + f.bn - 1) / f.bn) * unsigned(f.kc);
@@ -880,7 +870,7 @@ cute_b200_status forward_few(const LoraParams &p, const FewPlan &plan, const Dev
 
 constexpr uint64_t kAlign = 256;
 uint64_t round_up(uint64_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
-uint64_t t_bytes(const cute_b200_lora_desc &d) { return round_up(uint64_t(d.m) * padded_rank(d.rank) * 4); }
+uint64_t t_bytes(const cute_b200_lora_desc &d) { return round_up(uint64_t(d.m) * padded_rank(d.rank) * 2 * t_planes(d.ab_dtype == CUTE_B200_BF16)); }
 
 uint64_t plan_bytes(const cute_b200_lora_desc &d) { return round_up(lora_plan_bytes(d.m, d.adapters)) + kAlign; }
 

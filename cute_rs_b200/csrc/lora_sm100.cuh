@@ -10,7 +10,7 @@ struct LoraParams {
     const int32_t *ids;
     const float *scale;
     void *y;
-    uint16_t *t;    // (m, 2 rp): the rounded inner products, then their remainders
+    uint16_t *t;    // (m, t_planes() rp): the inner products, see store_t
     uint32_t *plan; // which adapters each tile of rows names (tiled kernels)
     int m, n, k, rank, rp, adapters, c_dtype;
     int64_t ldx, ldy;
@@ -46,6 +46,40 @@ __device__ __forceinline__ void store_c(void *c, int dtype, size_t i, float v) {
 
 // Width of the rank in T: 16, 32, 64 or 128.
 __host__ __device__ constexpr int padded_rank(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
+
+// How T is stored: per row `t_planes` planes of rp numbers.  A value v is split into its rounding and a remainder, v = hi + lo.
+//   bf16  hi, lo:           16 bits of v at any magnitude.
+//   f16   lo, hi, lo 2^11:  the remainder of a value below 1/4 falls below f16's smallest step, so hi + lo is off by up to
+//         2^-25 whatever v is.  Towards Y, whose accumulator takes hi and lo as they are, that is f16's own resolution.  A gradient
+//         has no such floor: its kernel sums the scaled remainders in columns of their own and scales them back in f32, which
+//         keeps 22 bits down to 2^-14 and is off by 2^-36 below.  (2^12 would overflow for values above 2^15.)
+// Y reads planes 0 and 1, or hi alone; the gradients two planes from hi on.
+__host__ __device__ constexpr int t_planes(bool bf16) { return bf16 ? 2 : 3; }
+__host__ __device__ constexpr int t_hi(int rp, bool bf16) { return bf16 ? 0 : rp; }
+constexpr float LOW_SCALE = 2048.0f;
+template <bool BF16>
+__device__ __forceinline__ void store_t(uint16_t *t, int rp, float v) {
+    const uint16_t hi = from_f32<BF16>(v);
+    const float lo = v - to_f32<BF16>(hi);
+    t[t_hi(rp, BF16)] = hi;
+    t[BF16 ? rp : 0] = from_f32<BF16>(lo);
+    if constexpr (!BF16) t[2 * rp] = from_f32<BF16>(lo * LOW_SCALE);
+}
+// Four of them, 8-byte aligned.  Returns hi + lo.
+__device__ __forceinline__ float4 store_t4(uint16_t *t, int rp, const float4 &v, bool bf16, bool store = true) {
+    const uint32_t h0 = pack_16(v.x, v.y, bf16), h1 = pack_16(v.z, v.w, bf16);
+    const float2 f0 = bf16 ? pair_f32<true>(h0) : pair_f32<false>(h0), f1 = bf16 ? pair_f32<true>(h1) : pair_f32<false>(h1);
+    const float4 lo = make_float4(v.x - f0.x, v.y - f0.y, v.z - f1.x, v.w - f1.y);
+    const uint32_t l0 = pack_16(lo.x, lo.y, bf16), l1 = pack_16(lo.z, lo.w, bf16);
+    if (store) {
+        *reinterpret_cast<uint2 *>(t + t_hi(rp, bf16)) = make_uint2(h0, h1);
+        *reinterpret_cast<uint2 *>(t + (bf16 ? rp : 0)) = make_uint2(l0, l1);
+        if (!bf16)
+            *reinterpret_cast<uint2 *>(t + 2 * rp) = make_uint2(pack_16(lo.x * LOW_SCALE, lo.y * LOW_SCALE, bf16), pack_16(lo.z * LOW_SCALE, lo.w * LOW_SCALE, bf16));
+    }
+    const float2 g0 = bf16 ? pair_f32<true>(l0) : pair_f32<false>(l0), g1 = bf16 ? pair_f32<true>(l1) : pair_f32<false>(l1);
+    return make_float4(f0.x + g0.x, f0.y + g0.y, f1.x + g1.x, f1.y + g1.y);
+}
 
 // First occurrences of ids by a hash table in shared memory.
 template <int ROWS>
@@ -111,10 +145,11 @@ struct ExtBlock {
 };
 __host__ __device__ __forceinline__ bool whole_t(int c_dtype) { return c_dtype == CUTE_B200_F32; }
 __host__ __device__ __forceinline__ int ext_blocks(int rp, bool whole) { return rp <= 32 ? 1 : (whole ? rp / 32 : rp / 64); }
-__device__ __forceinline__ ExtBlock ext_block(int q, int rp, int rank, bool whole) {
-    if (rp <= 32) return {0, 0, whole ? rp / 8 : rp / 16, rp / 16 - 1};
+__device__ __forceinline__ ExtBlock ext_block(int q, int rp, int rank, bool whole, bool bf16) {
+    const int first = whole ? 0 : t_hi(rp, bf16);
+    if (rp <= 32) return {first, 0, whole ? rp / 8 : rp / 16, rp / 16 - 1};
     const int half = whole ? q >> 1 : q, left = (rank - 64 * half + 15) / 16;  // at least 1: rank > rp / 2
-    return {(whole ? (q & 1) * rp : 0) + 64 * half, 64 * half, left < 4 ? left : 4, 3};
+    return {first + (whole ? (q & 1) * rp : 0) + 64 * half, 64 * half, left < 4 ? left : 4, 3};
 }
 
 }  // namespace

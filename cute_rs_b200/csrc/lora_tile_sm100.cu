@@ -29,7 +29,7 @@ __host__ __device__ constexpr uint64_t plan_stride(int P, int adapters) {
 //           or four stages deep, as the rank allows: the shorter one is what keeps X coming.
 //   warp 1  MMA.   warps 2-5  the adapters the rows name (and, by the cluster's first CTA,
 //           the plan of the GEMM's tile that starts at its rows), then the sum over the
-//           cluster, scale, split into two 16-bit numbers.
+//           cluster, scale, split into 16-bit numbers.
 // On the way back A is B[a] as it lies, (n, rank): rank is the fast index, so it is an MN-major operand.
 // A CTA's k range goes to 1, 2 or 4 accumulators in turn, added in f32 at the end: the tensor core cuts its sums off instead
 // of rounding them, an error of the same sign that grows with the products added into one accumulator (256 MMAs of 16: 5e-6
@@ -335,11 +335,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1)
                 const float s = h.scale[row];
                 const bool has = h.id[row] >= 0 && col < p.rank;
                 const float4 w = has ? make_float4(v.x * s, v.y * s, v.z * s, v.w * s) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const uint32_t h0 = pack_16(w.x, w.y, p.bf16), h1 = pack_16(w.z, w.w, p.bf16);
-                const float2 f0 = p.bf16 ? pair_f32<true>(h0) : pair_f32<false>(h0), f1 = p.bf16 ? pair_f32<true>(h1) : pair_f32<false>(h1);
-                uint16_t *t = p.t + int64_t(row0 + row) * 2 * p.rp + col;
-                *reinterpret_cast<uint2 *>(t) = make_uint2(h0, h1);
-                *reinterpret_cast<uint2 *>(t + p.rp) = make_uint2(pack_16(w.x - f0.x, w.y - f0.y, p.bf16), pack_16(w.z - f1.x, w.w - f1.y, p.bf16));
+                store_t4(p.t + int64_t(row0 + row) * t_planes(p.bf16) * p.rp + col, p.rp, w, p.bf16);
             });
     }
     if (p.early) ptx::griddep_wait();
@@ -392,6 +388,7 @@ struct TileParams {
     int m, n, rank, rp, adapters, c_dtype, vec;
     int k_blocks, m_tiles, n_tiles, group_m, parts;
     uint32_t idesc, low_idesc, low_box;  // low_box: bytes of an MN-major box of B, 0 = B is K-major
+    bool bf16;
     uint32_t *status;
     int debug;
 };
@@ -563,7 +560,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             }
             const int boxes = p.low_box ? C::B_ROWS / 64 : 1;  // of B per adapter
             for (int q = 0; q < q_blocks && entries > 0 && ok; q += t_blocks) {
-                const ExtBlock b = ext_block(q, p.rp, p.rank, whole);
+                const ExtBlock b = ext_block(q, p.rp, p.rank, whole, p.bf16);
                 if (q > 0 && entries > 32) read_ids(0);
                 bool head = true;  // this stage begins with T
                 for (int e = 0; e < entries && ok; head = false) {
@@ -688,7 +685,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 }
                 const uint32_t k_step = p.low_box ? MN_K_STEP : 2u;
                 for (int q = 0; q < q_blocks && entries > 0 && ok; q += t_blocks) {
-                    const ExtBlock x = ext_block(q, p.rp, p.rank, whole);
+                    const ExtBlock x = ext_block(q, p.rp, p.rank, whole, p.bf16);
                     uint32_t words = 0, t_block = 0, b_block = 0;
                     uint32_t step[4];
 #pragma unroll
@@ -901,12 +898,13 @@ cute_b200_status launch_tile(const LoraParams &p, bool bf16, int debug, const De
     const int low_rows = p.rp < 64 ? p.rp : 64;  // ranks per box of an MN-major B
     t.low_idesc = t.idesc | (p.low_mn ? IDESC_B_MN : 0u);
     t.low_box = p.low_mn ? uint32_t(low_rows) * 128u : 0u;
+    t.bf16 = bf16;
     t.status = dev.status_word;
     t.debug = debug;
     CUtensorMap tmX, tmW, tmT, tmB;
     CB_TRY(rows_tensor_map(&tmX, reinterpret_cast<uint64_t>(p.x), bf16, p.m, p.k, p.ldx, C::CTA_ROWS));
     CB_TRY(rows_tensor_map(&tmW, reinterpret_cast<uint64_t>(p.w), bf16, p.n, p.k, p.k, C::B_ROWS));
-    CB_TRY(rows_tensor_map(&tmT, reinterpret_cast<uint64_t>(p.t), bf16, p.m, 2 * p.rp, 2 * p.rp, C::CTA_ROWS));
+    CB_TRY(rows_tensor_map(&tmT, reinterpret_cast<uint64_t>(p.t), bf16, p.m, t_planes(bf16) * p.rp, t_planes(bf16) * p.rp, C::CTA_ROWS));
     if (p.low_mn) CB_TRY(stack_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), bf16, p.adapters, p.rank, p.n, low_rows));
     else CB_TRY(rows_tensor_map(&tmB, reinterpret_cast<uint64_t>(p.b), bf16, uint64_t(p.adapters) * p.n, p.rank, p.rank, C::B_ROWS));
     return launch_dependent(lora_tile_kernel<G, BN, MH>, dim3(unsigned(clusters * G)), TILE_THREADS, C::SMEM_BYTES, G, stream, tmX, tmW, tmT, tmB, t);

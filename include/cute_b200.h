@@ -195,9 +195,10 @@ cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint6
  *   (an adapter of a smaller rank is padded with zeros); adapters >= 1 with
  *   adapters * n, adapters * k and adapters * rank below 2^31.
  *   Before it is multiplied by B, scale[a] * A[a] x is rounded to the operands'
- *   type for a 16-bit Y, and to the sum of two such numbers (16 significant bits
- *   for bf16, 22 for f16) for an f32 Y and for the gradients; where an f16 value
- *   passes +-65504 its row of Y is not finite.
+ *   type for a 16-bit Y, and to the sum of two such numbers for an f32 Y: 16
+ *   significant bits for bf16; 22 for f16, but with an error of up to 2^-25
+ *   whatever the value (f16 has no smaller numbers), which is more where it is
+ *   below 1/4.  Where an f16 value passes +-65504 its row of Y is not finite.
  *   The workspace begins with these numbers, which the backward pass reads.
  *
  * cute_b200_lora_tn_backward: the gradients for dY (m, n) in the operands' type
@@ -211,6 +212,10 @@ cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint6
  *   same X, A, ids and scale, unchanged since.  dX may be null (no gradient of
  *   the input wanted), dA and dB may both be null; adapters no row names get
  *   zeros.  The sums run in a fixed order: the same call gives the same bits.
+ *   Towards dX, scale[a] * B[a]^T dY is rounded as the inner products are towards
+ *   a Y of dX's type.  In dA and dB it and scale[a] * A[a] x carry 16 significant
+ *   bits for bf16 and 22 for f16, there with an error of up to 2^-36 that shows
+ *   in values below 2^-14.
  *
  * No buffer that a call writes may overlap another of its buffers. */
 typedef struct {

@@ -1,0 +1,45 @@
+"""The gradients of lora_tn where a loose bound would hide an error: small inner products, many rows, exact sums.
+
+Tolerances are derived beside each test.
+"""
+import pytest
+import torch
+
+from tests.test_gpu_rows import BF16, F16, F32, Lora
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("size", [1e3, 1.0, 1e-2, 1e-3, 1e-4, 1e-5, 1e-6])
+@pytest.mark.parametrize("rank", [8, 24, 64, 128])
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_f16_gradients_of_small_inner_products(lib, gpu, m, rank, size):
+    """Every row has an adapter of its own, and each of its inner products is a single product of two f16 numbers, so that U
+    and T are exact in f32 and dA = U x^T, dB = dY T^T are products of two numbers.  What is left is how U and T are carried:
+    22 bits, half a step 2^-22, down to 2^-14 and 2^-36 below (half the smallest step of a remainder times 2^11); the two
+    products' sum in f32 adds 2 steps of 2^-23, the scaling back none."""
+    n, k = 136, 264
+    p = Lora(lib, m, n, k, rank, m, F16, F32, torch.arange(m))
+    p.scale.fill_(1.0)
+    part = size ** 0.5
+    one = lambda *s: torch.where(torch.rand(*s, device="cuda", generator=p.gen) < 0.5, -1.0, 1.0) * (torch.rand(*s, device="cuda", generator=p.gen) + 0.5)
+    p.a.zero_()
+    p.b.zero_()
+    j = torch.arange(rank, device="cuda")
+    p.a[:, j, j * 2] = (one(m, rank) * part).to(F16)
+    p.b[:, j, j] = (one(m, rank) * part).to(F16)
+    p.x.copy_((one(m, k) * part).to(F16))
+    p.dy.copy_((one(m, n) * part).to(F16))
+    for tuning in [(0, 0), (2, 0)] + ([(1, 0)] if m <= 128 else []):
+        p.run(tuning)
+        _, da, db = p.back()
+        x, dy = p.x.double(), p.dy.double()
+        t = torch.einsum("irk,ik->ir", p.a.double(), x)
+        u = torch.einsum("inr,in->ir", p.b.double(), dy)
+        assert torch.equal(t, t.float().double()) and torch.equal(u, u.float().double())
+        carried = lambda v: v.abs() * 2.0 ** -22 + 2.0 ** -36
+        for name, got, low, v in (("dA", da, u, x), ("dB", db.transpose(1, 2), t, dy)):
+            want = low[:, :, None] * v[:, None, :]
+            bound = carried(low)[:, :, None] * v.abs()[:, None, :] + want.abs() * 2.0 ** -22
+            off = (got.double() - want).abs()
+            assert (off <= bound).all(), f"{name} off by {(off / bound).max():.3g} of the bound"
