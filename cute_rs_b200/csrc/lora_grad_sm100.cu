@@ -14,6 +14,15 @@
 // another adapter's row, not even a NaN, takes part.  A cluster shares the rows
 // of a tile and adds its partial sums in order: the result does not depend on
 // timing.  Bound by reading X and dY once.
+//
+// The tensor core cuts its f32 sums off instead of rounding them, an error of
+// one sign that grows with the MMAs added into one accumulator.  An accumulator
+// therefore takes a few blocks only; the epilogue warps then add it to sums in
+// their registers while the next one is filled.  The error then does not grow
+// with the rows: sums of one sign over 16 k to 256 k rows are off by 1.1e-6 up to
+// rank 32 and 2.2e-6 above (8 and 16 blocks; all blocks of a CTA in one
+// accumulator: 5e-6 to 1.7e-4), at the same speed (65,536 rows, rank 128, 1024 +
+// 1024 columns, with the products: 505 us, was 505; half the blocks: 508).
 #include "lora_sm100.cuh"
 
 namespace cb {
@@ -63,13 +72,18 @@ __global__ void __launch_bounds__(LIST_THREADS) row_list_kernel(const int32_t *i
     }
 }
 
-constexpr int GRAD_THREADS = 192, GRAD_M = 128, GRAD_ROWS = 64, GRAD_STAGES = 4;
+constexpr int GRAD_M = 128, GRAD_ROWS = 64, GRAD_STAGES = 4, GRAD_BUFS = 4;
 constexpr uint32_t GRAD_BOX = GRAD_ROWS * 128, GRAD_HEAD = 1024;
 
 // How a tile is cut by rank.  What bounds the kernel beside HBM is the way from L2 to the SMs (some 100 GB/s each): per 64
 // rows a tile fetches 8 KB per 64 columns of V and 8 KB per 64 columns of L, so a high rank takes two accumulators of 128
 // columns of V (rank 128, 8192 rows, 8192 + 2048 columns: 491 MB with one, 335 MB with two), and the SM to itself.
 __host__ __device__ constexpr int grad_halves(int rp) { return rp >= 64 ? 2 : 1; }
+__host__ __device__ constexpr int grad_threads(int rp) { return 64 + 128 * grad_halves(rp); }  // an epilogue thread's sums: rp of them, of one column
+// Two CTAs share an SM up to rank 64 and have 256 columns of TMEM each: four accumulators of up to 64, or one of 256; above, one
+// of 512.  Where there is one, the MMAs wait while it is read: it takes more blocks.
+__host__ __device__ constexpr int grad_bufs(int rp) { return rp <= 32 ? GRAD_BUFS : 1; }
+__host__ __device__ constexpr int grad_depth(int rp) { return rp <= 32 ? 8 : 16; }
 __host__ __device__ constexpr int grad_low_boxes(int rp) { return (2 * rp + 63) / 64; }
 constexpr uint32_t grad_ring(int rp) { return (rp == 128 ? 192u : 96u) * 1024; }
 constexpr uint32_t grad_smem(int rp) { return 1024 + GRAD_HEAD + grad_ring(rp); }
@@ -81,8 +95,8 @@ struct GradMaps {
 struct GradParams {
     float *out[2];
     const int32_t *first, *list;
-    int cols[2], tiles[2], m, rank, rp, halves, kc, stages, vec;
-    uint32_t stage_bytes, idesc, tmem_cols;
+    int cols[2], tiles[2], m, rank, kc, stages, vec;
+    uint32_t stage_bytes, idesc;
     int low_col;      // of L: where the two planes begin
     float low_scale;  // of the second plane's sums
     uint32_t *status;
@@ -90,11 +104,15 @@ struct GradParams {
 };
 
 struct GradHead {
-    uint64_t full[GRAD_STAGES], empty[GRAD_STAGES], done, drain;
+    uint64_t full[GRAD_STAGES], empty[GRAD_STAGES], tfull[GRAD_BUFS], tempty[GRAD_BUFS], drain;
     uint32_t tmem, abort;
 };
 
-__global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
+template <int RP>
+__global__ void __launch_bounds__(grad_threads(RP), RP == 128 ? 1 : 2) lora_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
+    constexpr int HALVES = grad_halves(RP), THREADS = grad_threads(RP), BUFS = grad_bufs(RP), DEPTH = grad_depth(RP);
+    constexpr uint32_t ACC_COLS = 2 * RP * HALVES, TMEM_COLS = BUFS * ACC_COLS;
+    static_assert(TMEM_COLS >= 32 && TMEM_COLS <= (RP == 128 ? 512 : 256) && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "TMEM");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     GradHead &h = *reinterpret_cast<GradHead *>(smem_raw + (base - raw));
@@ -107,7 +125,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
     int tile = unit - a * per;
     const int job = tile >= p.tiles[0] ? 1 : 0;
     if (job) tile -= p.tiles[0];
-    const int c0 = tile * GRAD_M * p.halves, wide_boxes = 2 * p.halves, low_boxes = grad_low_boxes(p.rp);
+    const int c0 = tile * GRAD_M * HALVES, wide_boxes = 2 * HALVES, low_boxes = grad_low_boxes(RP);
     const uint64_t limit = (p.debug & 8) ? 20ull * 1000 * 1000 : WAIT_LIMIT_NS;
 
     if (threadIdx.x == 0) {
@@ -115,13 +133,16 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
             ptx::mbar_init(bar(h.full[s]), 1);
             ptx::mbar_init(bar(h.empty[s]), 1);
         }
-        ptx::mbar_init(bar(h.done), 1);
+        for (int b = 0; b < BUFS; b++) {
+            ptx::mbar_init(bar(h.tfull[b]), 1);
+            ptx::mbar_init(bar(h.tempty[b]), 4 * HALVES);
+        }
         ptx::mbar_init(bar(h.drain), 1);
         h.abort = 0u;
         ptx::fence_mbar_init();
     }
     if (warp == 1) {
-        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), p.tmem_cols);
+        ptx::tmem_alloc<1>(ptx::smem_u32(&h.tmem), TMEM_COLS);
         ptx::tmem_relinquish<1>();
     }
     ptx::tc_fence_before();
@@ -192,67 +213,72 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
         uint32_t ph = 0;
         bool ok = true, issued = false;
         for (int b = b0; b < b1; b++) {
+            const int at = (b - b0) % DEPTH, turn = (b - b0) / DEPTH, buf = turn % BUFS;
+            if (at == 0) {  // the epilogue must have read this accumulator
+                ok = __all_sync(0xffffffffu, wait_bar(bar(h.tempty[buf]), (uint32_t(turn / BUFS) & 1u) ^ 1u, abort_flag, p.status, WHERE_MMA_TMEM, uint32_t(buf), limit));
+                if (!ok) break;
+            }
             ok = __all_sync(0xffffffffu, wait_bar(bar(h.full[s]), ph, abort_flag, p.status, WHERE_MMA_FULL, uint32_t(s), limit));
             if (!ok) break;
             ptx::tc_fence_after();
             const uint32_t src = ring + uint32_t(s) * p.stage_bytes;
             const uint64_t low = mn_desc(src + uint32_t(wide_boxes) * GRAD_BOX, GRAD_BOX);
-            const uint32_t more = b > b0 ? 1u : 0u;
+            const uint32_t more = at > 0 ? 1u : 0u, d = tmem + uint32_t(buf) * ACC_COLS;
             if (leader) {
-                for (int x = 0; x < p.halves; x++) {
+#pragma unroll
+                for (int x = 0; x < HALVES; x++) {
                     const uint64_t wide = mn_desc(src + uint32_t(2 * x) * GRAD_BOX, GRAD_BOX);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        ptx::umma_f16<1>(tmem + uint32_t(2 * x * p.rp), wide + MN_K_STEP * j, low + MN_K_STEP * j, p.idesc, j > 0 ? 1u : more);
+                        ptx::umma_f16<1>(d + uint32_t(2 * x * RP), wide + MN_K_STEP * j, low + MN_K_STEP * j, p.idesc, j > 0 ? 1u : more);
                 }
                 ptx::umma_commit<1>(bar(h.empty[s]));
+                if (at == DEPTH - 1 || b + 1 == b1) ptx::umma_commit<1>(bar(h.tfull[buf]));
             }
             __syncwarp();
             issued = true;
             if (++s == p.stages) s = 0, ph ^= 1u;
         }
-        if (leader) {
-            if (ok) {
-                ptx::umma_commit<1>(bar(h.done));
-            } else if (issued) {
-                ptx::umma_commit<1>(bar(h.drain));
-                const uint64_t t0 = ptx::globaltimer_ns();
-                while (!ptx::mbar_try_wait(bar(h.drain), 0u))
-                    if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
-            }
+        if (leader && !ok && issued) {
+            ptx::umma_commit<1>(bar(h.drain));
+            const uint64_t t0 = ptx::globaltimer_ns();
+            while (!ptx::mbar_try_wait(bar(h.drain), 0u))
+                if (ptx::globaltimer_ns() - t0 > WAIT_LIMIT_NS / 4) break;
         }
         __syncwarp();
     } else {
-        const bool ok = __all_sync(0xffffffffu, wait_bar(bar(h.done), 0, abort_flag, p.status, WHERE_EPILOGUE, 0u, limit));
-        const int q = warp & 3;
-        const uint32_t pitch = uint32_t(p.rp + 4) * 4u;
-        if (ok) {
+        // A thread holds the sums of one column of V: row 32 q + lane of accumulator half x.
+        const int q = warp & 3, x = HALVES == 1 ? 0 : (warp - 2) >> 2;
+        float sum[RP] = {};
+        bool ok = true;
+        for (int b = b0, turn = 0; b < b1; b += DEPTH, turn++) {
+            const int buf = turn % BUFS;
+            ok = __all_sync(0xffffffffu, wait_bar(bar(h.tfull[buf]), uint32_t(turn / BUFS) & 1u, abort_flag, p.status, WHERE_EPILOGUE, uint32_t(buf), limit));
+            if (!ok) break;
             ptx::tc_fence_after();
-            ptx::fence_proxy_async_shared();
-            // Columns j and rp + j belong to the two numbers of value j: their sum is the gradient's part.
-            for (int i = 0; i < p.halves * p.rp; i += 16) {
-                const int x = i / p.rp, c = i - x * p.rp;
-                const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(2 * x * p.rp + c);
-                const uint32_t dst = ring + uint32_t(GRAD_M * x + 32 * q + lane) * pitch;
-                float v[16];
-                if (b0 < b1) {
-                    uint32_t hi[16], lo[16];
-                    ptx::tmem_ld_32x16(from, hi);
-                    ptx::tmem_ld_32x16(from + uint32_t(p.rp), lo);
-                    ptx::tmem_ld_wait_all();
-                    ptx::pin16(hi);
-                    ptx::pin16(lo);
+            // Columns j and RP + j belong to the two numbers of value j: their sum is the gradient's part.
+            const uint32_t from = tmem + (uint32_t(32 * q) << 16) + uint32_t(buf) * ACC_COLS + uint32_t(2 * x * RP);
 #pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] = fmaf(__uint_as_float(lo[j]), p.low_scale, __uint_as_float(hi[j]));
-                } else {
+            for (int c = 0; c < RP; c += 16) {
+                uint32_t hi[16], lo[16];
+                ptx::tmem_ld_32x16(from + uint32_t(c), hi);
+                ptx::tmem_ld_32x16(from + uint32_t(RP + c), lo);
+                ptx::tmem_ld_wait_all();
+                ptx::pin16(hi);
+                ptx::pin16(lo);
 #pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] = 0.0f;
-                }
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-                    ptx::st_shared_v4(dst + uint32_t(c + 4 * g) * 4u, __float_as_uint(v[4 * g]), __float_as_uint(v[4 * g + 1]),
-                                      __float_as_uint(v[4 * g + 2]), __float_as_uint(v[4 * g + 3]));
+                for (int j = 0; j < 16; j++) sum[c + j] += fmaf(__uint_as_float(lo[j]), p.low_scale, __uint_as_float(hi[j]));
             }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(h.tempty[buf]));
+        }
+        if (ok) {  // the ring is idle: every block has been multiplied
+            ptx::fence_proxy_async_shared();
+            const uint32_t dst = ring + uint32_t(GRAD_M * x + 32 * q + lane) * uint32_t(RP + 4) * 4u;
+#pragma unroll
+            for (int c = 0; c < RP; c += 4)
+                ptx::st_shared_v4(dst + uint32_t(c) * 4u, __float_as_uint(sum[c]), __float_as_uint(sum[c + 1]), __float_as_uint(sum[c + 2]), __float_as_uint(sum[c + 3]));
         }
         __syncwarp();
     }
@@ -264,17 +290,17 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
         ptx::cluster_wait();
     }
     if (!*abort_flag) {
-        const uint32_t pitch = uint32_t(p.rp + 4) * 4u;
+        const uint32_t pitch = uint32_t(RP + 4) * 4u;
         // Four ranks of one column of V per step.  Neighbouring threads write neighbouring addresses: of dA the columns, of dB
         // the ranks, 16 bytes at once.
-        const int cols = p.cols[job], columns = GRAD_M * p.halves, wide = min(columns, cols - c0), quads = p.rank / 4, items = columns * quads;
+        const int cols = p.cols[job], columns = GRAD_M * HALVES, wide = min(columns, cols - c0), quads = p.rank / 4, items = columns * quads;
         float *out = p.out[job] + int64_t(a) * p.rank * cols;
         const Divider by_quads(quads);
         const int shift = __ffs(columns) - 1;  // a power of two
         auto column = [&](int i) { return job ? by_quads(i) : i & (columns - 1); };
         auto first_rank = [&](int i) { return 4 * (job ? i - by_quads(i) * quads : i >> shift); };
         cluster_sums<2>(
-            items, int(rank), p.kc, GRAD_THREADS, [&](int i) { return ring + uint32_t(column(i)) * pitch + uint32_t(first_rank(i)) * 4u; },
+            items, int(rank), p.kc, THREADS, [&](int i) { return ring + uint32_t(column(i)) * pitch + uint32_t(first_rank(i)) * 4u; },
             [&](int i, const float4 &v) {
                 const int c = column(i), j = first_rank(i);
                 if (c >= wide) return;
@@ -293,7 +319,7 @@ __global__ void __launch_bounds__(GRAD_THREADS, 2) lora_grad_kernel(const __grid
         ptx::cluster_arrive();
         ptx::cluster_wait();
     }
-    if (warp == 1) ptx::tmem_dealloc<1>(tmem, p.tmem_cols);
+    if (warp == 1) ptx::tmem_dealloc<1>(tmem, TMEM_COLS);
 }
 
 }  // namespace
@@ -318,12 +344,11 @@ cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const Devi
     }
     p.first = g.first, p.list = g.list;
     p.vec = reinterpret_cast<uint64_t>(g.out[1]) % 16 == 0;
-    p.m = g.m, p.rank = g.rank, p.rp = g.rp, p.halves = grad_halves(g.rp);
-    p.stage_bytes = uint32_t(2 * p.halves + grad_low_boxes(g.rp)) * GRAD_BOX;
+    p.m = g.m, p.rank = g.rank;
+    p.stage_bytes = uint32_t(2 * grad_halves(g.rp) + grad_low_boxes(g.rp)) * GRAD_BOX;
     p.stages = int(grad_ring(g.rp) / p.stage_bytes);
     if (p.stages > GRAD_STAGES) p.stages = GRAD_STAGES;
     p.idesc = make_idesc(bf16, GRAD_M, 2 * g.rp) | IDESC_A_MN | IDESC_B_MN;
-    p.tmem_cols = uint32_t(2 * g.rp * p.halves);
     p.low_col = t_hi(g.rp, bf16);
     p.low_scale = bf16 ? 1.0f : 1.0f / LOW_SCALE;
     p.status = dev.status_word;
@@ -339,11 +364,18 @@ cute_b200_status lora_grads(const LoraGrads &g, bool bf16, int debug, const Devi
         if (t < best) best = t, p.kc = kc;
     }
     if (units * p.kc > 0x7fffffff) return fail(CUTE_B200_ERR_INVALID_ARGUMENT, "lora_tn_backward: the adapters are too large");
-    return launch_dependent(lora_grad_kernel, dim3(unsigned(units * p.kc)), GRAD_THREADS, grad_smem(g.rp), p.kc, stream, maps, p);
+    auto launch = [&](auto kernel) { return launch_dependent(kernel, dim3(unsigned(units * p.kc)), grad_threads(g.rp), grad_smem(g.rp), p.kc, stream, maps, p); };
+    if (g.rp == 16) return launch(lora_grad_kernel<16>);
+    if (g.rp == 32) return launch(lora_grad_kernel<32>);
+    if (g.rp == 64) return launch(lora_grad_kernel<64>);
+    return launch(lora_grad_kernel<128>);
 }
 
 cute_b200_status lora_grad_init() {
-    CB_CUDA(cudaFuncSetAttribute(lora_grad_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, grad_smem(128)));
+    CB_CUDA(cudaFuncSetAttribute(lora_grad_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, grad_smem(16)));
+    CB_CUDA(cudaFuncSetAttribute(lora_grad_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, grad_smem(32)));
+    CB_CUDA(cudaFuncSetAttribute(lora_grad_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, grad_smem(64)));
+    CB_CUDA(cudaFuncSetAttribute(lora_grad_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, grad_smem(128)));
     return CUTE_B200_OK;
 }
 

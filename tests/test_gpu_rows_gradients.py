@@ -43,3 +43,41 @@ def test_f16_gradients_of_small_inner_products(lib, gpu, m, rank, size):
             bound = carried(low)[:, :, None] * v.abs()[:, None, :] + want.abs() * 2.0 ** -22
             off = (got.double() - want).abs()
             assert (off <= bound).all(), f"{name} off by {(off / bound).max():.3g} of the bound"
+
+
+@pytest.mark.parametrize("rank", [16, 24, 64, 128])
+@pytest.mark.parametrize("m,adapters,share", [(262144, 1, 1.0), (131072, 16, 0.9)])
+def test_gradients_of_long_row_lists(lib, gpu, m, adapters, share, rank):
+    """All operands are small integers of one sign, U and T exact as their two numbers, and the sum over any 4096 rows of
+    an adapter stays below 2^24, where f32 is exact (asserted below), while the sum over all of them passes it.  Sums of 4096
+    rows can thus be taken in one accumulator, and adding them up in f32 costs half a step, 2^-24 of the total, per
+    addition that is added on: m / 4096 of them, and within 4096 rows up to 8 CTAs, 4 accumulators and 2 numbers."""
+    n, k = 256, 64
+    ids = torch.zeros(m, dtype=torch.int64)
+    if adapters > 1:
+        gen = torch.Generator().manual_seed(rank)
+        ids = torch.where(torch.rand(m, generator=gen) < share, 3, torch.randint(0, adapters, (m,), generator=gen))
+    p = Lora(lib, m, n, k, rank, adapters, BF16, BF16, ids)
+    draw = lambda t, lo, hi: t.copy_(torch.randint(lo, hi, t.shape, device="cuda", generator=p.gen))
+    p.scale.fill_(1.0)
+    draw(p.x, 0, 65)
+    draw(p.dy, 0, 2)
+    draw(p.a, 0, 4)
+    draw(p.b, 0, 2)
+    p.run()
+    _, da, db = p.back()
+    allowed = (m / 4096 + 8 + 4 + 2) * 2.0 ** -24
+    past = False
+    for i in range(adapters):
+        r = p.rows(i)
+        x, dy = p.x[r].double(), p.dy[r].double()
+        t, u = x @ p.a[i].double().t(), dy @ p.b[i].double()
+        assert u.max() <= 256 and t.max() < 2 ** 16
+        for name, got, low, v in (("dA", da[i], u, x), ("dB", db[i].t(), t, dy)):
+            for piece in range(0, r.numel(), 4096):
+                assert (low[piece:piece + 4096].t() @ v[piece:piece + 4096]).max() < 2 ** 24
+            want = low.t() @ v
+            past |= bool(want.max() > 2 ** 25)
+            off = (got.double() - want).abs()
+            assert (off <= allowed * want).all(), f"{name}[{i}] off by {(off / want).max():.3g}, {allowed:.3g} allowed"
+    assert past
