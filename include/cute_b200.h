@@ -189,16 +189,20 @@ cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint6
  *   B: (adapters, n, rank); ids: (m) i32; scale: (adapters) f32;
  *   Y: (m, n) f32, f16 or bf16, rows ldy apart.
  *   Rows may come in any order: packed sequences, single tokens of many
- *   requests, both mixed.  A row's result depends on its own X row and its own
- *   adapter alone, whatever infinities or NaNs other rows or adapters hold.
+ *   requests, both mixed.  Nothing of another row or of an adapter that the row
+ *   does not name reaches its result, no infinity and no NaN either.  How the
+ *   sums are cut follows m, n, k and rank, so the same row may come out with
+ *   other last bits in a batch of another size; the same call gives the same bits.
  *   m >= 0; n >= 1; k >= 8 and a multiple of 8; none above 2^30; rank a multiple of 8 in 8..128
  *   (an adapter of a smaller rank is padded with zeros); adapters >= 1 with
  *   adapters * n, adapters * k and adapters * rank below 2^31.
- *   Before it is multiplied by B, scale[a] * A[a] x is rounded to the operands'
- *   type for a 16-bit Y, and to the sum of two such numbers for an f32 Y: 16
- *   significant bits for bf16; 22 for f16, but with an error of up to 2^-25
- *   whatever the value (f16 has no smaller numbers), which is more where it is
- *   below 1/4.  Where an f16 value passes +-65504 its row of Y is not finite.
+ *   Before it is multiplied by B, scale[a] * A[a] x is rounded at least as finely
+ *   as this.  For a 16-bit Y: to the operands' type; which of the kernels that
+ *   serve few rows keep more follows the sizes.  For an f32 Y: to the sum of two
+ *   such numbers, 16 significant bits for bf16; 22 for f16, but with an error of
+ *   up to 2^-25 whatever the value (f16 has no smaller numbers), which is more
+ *   where it is below 1/4.  Where an f16 value passes +-65504 its row of Y is not
+ *   finite.
  *   The workspace begins with these numbers, which the backward pass reads.
  *
  * cute_b200_lora_tn_backward: the gradients for dY (m, n) in the operands' type
@@ -245,8 +249,9 @@ cute_b200_status cute_b200_lora_tn_backward(const cute_b200_lora_desc *desc, uin
  *   X, Y: (tokens, d); R: (experts, d); G, U: (experts, f, d); D: (experts, d, f); all in one 16-bit type.
  *   0 <= tokens <= 64; 1 <= top <= 16, top <= experts <= 512; d and f multiples of 8, experts * f and experts * d
  *   below 2^31.  The router's product, the softmax and the choice are f32; w_e * silu * up is rounded to the operands'
- *   type once, before the last product.  A token whose logits are not all finite gets a valid but unspecified choice
- *   and NaNs; other tokens are not affected. */
+ *   type once, before the last product (f16: with an error of up to 2^-25 however small, and infinite past +-65504).  A
+ *   logit of -infinity is a probability of 0.  A token with a logit that is NaN or +infinity, or with none that is finite,
+ *   gets a valid but unspecified choice and NaNs; other tokens are not affected. */
 typedef struct {
     int32_t tokens, experts, top;
     int32_t d, f;
