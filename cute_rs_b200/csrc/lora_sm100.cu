@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS) shrink_rows_kernel(const LoraP
 //           then T, once, and per adapter blocks of B[a].  A stage costs the
 //           issuing warp about 0.3 us whatever it holds (measured: 32 x 64 blocks, one per
 //           stage, stream at 1.9 TB/s, four per stage at 4.4 when lanes issue side by side),
-//           so a stage is made to hold about 28 KB and every block is another lane's.
+//           so a stage is made to hold 10 to 40 KB of W (stream_blocks) and every block is another lane's.
 //   warp 1  MMA: M 128, N bn.  The MMA always reads 128 rows of X; those past
 //           the loaded xr rows are whatever lies behind them in shared memory (in
 //           bounds, see forward_few), and end up in lanes that nothing reads.  An
@@ -828,7 +828,6 @@ template <bool BF16>
 cute_b200_status forward_few(const LoraParams &p, const FewPlan &plan, const DeviceState &dev, int debug, cudaStream_t stream) {
     if (p.rank >= 64) CB_TRY(launch_dependent(shrink_rows_kernel<BF16, 8>, dim3(unsigned(p.m), unsigned(p.rp / 8)), SHRINK_THREADS, 0, 1, stream, p));
     else CB_TRY(launch_dependent(shrink_rows_kernel<BF16, 4>, dim3(unsigned(p.m), unsigned(p.rp / 4)), SHRINK_THREADS, 0, 1, stream, p));
-    if (!p.y) return CUTE_B200_OK;
     FewParams f = {};
     f.ids = p.ids, f.y = p.y, f.ldy = p.ldy;
     f.m = p.m, f.n = p.n, f.rank = p.rank, f.rp = p.rp, f.adapters = p.adapters, f.c_dtype = p.c_dtype;

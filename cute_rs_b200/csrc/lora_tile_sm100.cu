@@ -370,7 +370,6 @@ struct Tile {
     static constexpr int ACC_COLS = MH * BN, ACC_BUFS = 2 * ACC_COLS <= 512 ? 2 : 1;
     static constexpr uint32_t TMEM_COLS = MH == 1 ? 512 : ACC_COLS * ACC_BUFS;
     static constexpr uint32_t SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 512 + 8 * 32 * TURN_PITCH * 4;
-    static constexpr uint32_t EXPECT = G * KB_BYTES;
     static constexpr int CH = BN / 64;  // 32-column chunks of an accumulator per epilogue warp
     // Blocks of B in a stage that holds one or two blocks of T, and in one without.  Two of them, the values' two numbers,
     // where they fit: they are multiplied by the same block of B.

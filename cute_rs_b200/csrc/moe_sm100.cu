@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(ROUTER_THREADS) moe_router_kernel(const MoePar
 
 // ---- which experts are chosen, and by whom ----------------------------------------
 struct MoeHead {
-    uint64_t full[16], empty[16], tfull[2], tempty[2], plan, zeroed, done, drain;
+    uint64_t full[16], empty[16], tfull[2], tempty[2], plan, done, drain;
     uint32_t tmem, abort, stop;
     int32_t active, before[4];
     int32_t expert[MAX_EXPERTS];                     // the chosen experts, ascending
