@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     } else {
         const int t = threadIdx.x - 64, named = __ldcg(p.ids), id = named >= 0 && named < p.adapters ? named : -1;
         if (t == 0) h.id = id, h.scale = id >= 0 ? __ldcg(p.scale + id) : 0.0f;
-        if (id >= 0) {  // the tile's rows of B lie one after another
+        if (id >= 0 && rank == 0) {  // the tile's rows of B lie one after another; the first CTA of a cluster multiplies them
             const int pieces = min(p.bn, p.n - n0) * p.rank / 8;
             const uint4 *src = reinterpret_cast<const uint4 *>(p.b + (int64_t(id) * p.n + n0) * p.rank);
 #pragma unroll 4
