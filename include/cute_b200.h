@@ -219,7 +219,8 @@ cute_b200_status cute_b200_gemm_tn_static(const cute_b200_gemm_desc *desc, uint6
  *   Towards dX, scale[a] * B[a]^T dY is rounded as the inner products are towards
  *   a Y of dX's type.  In dA and dB it and scale[a] * A[a] x carry 16 significant
  *   bits for bf16 and 22 for f16, there with an error of up to 2^-36 that shows
- *   in values below 2^-14.
+ *   in values below 2^-14.  The sums over the rows are f32 and taken in pieces, so
+ *   that their error does not grow with m.
  *
  * No buffer that a call writes may overlap another of its buffers. */
 typedef struct {
